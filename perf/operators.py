@@ -176,7 +176,6 @@ def prepare(case, seed):
             st["k_out"] = torch.zeros((B, case["keep"], Hkv, D), dtype=T, device=DEV)
             st["v_out"] = torch.zeros_like(st["k_out"])
             st["scores_out"] = torch.zeros((B, Hkv, case["keep"]), device=DEV)
-            st["workspace"] = st["context"].EvictWorkspace(B, Hkv, R)
         return st
     H, P = case["heads"], case["prefix"]
     st["q"] = normal(B, H, D, dtype=T, std=1.5)
@@ -274,7 +273,7 @@ def run(st):
         return [q, st["k_cache"], st["v_cache"]]
     if c["kind"] == "evict":
         kept, lens = ctx.kv_evict(st["k"], st["v"], st["scores"], st["lens"], c["keep"], sink=c["sink"], recent=c["recent"],
-                                  out=(st["k_out"], st["v_out"], st["scores_out"]), workspace=st["workspace"])
+                                  out=(st["k_out"], st["v_out"], st["scores_out"]))
         return [st["k_out"], st["v_out"], st["scores_out"], kept, lens]
     if c["kind"] == "scored":
         out = ctx.attn_decode_shared(st["q"], st["kp"], st["vp"], st["k"], st["v"], st["lens"], out_dtype=_T[c["out"]],
