@@ -467,6 +467,111 @@ typedef struct AttnMergeArgs {
 
 int attn_merge(const AttnMergeArgs* args, void* stream);
 
+/* ---- Long contexts: scaled rotary positions, a prefix shared by a batch, eviction from the caches ---------------------
+ * Operators of a server whose sequences run long. The engine has no counterpart of them: its rotary embedding is the
+ * interleaved, unscaled one (include/kernels_cpu.hpp:82-100), every sequence has a cache of its own, and a full cache slides
+ * (src/model/model.cpp:65-68). Layouts are the engine's. */
+
+enum { ATTN_ROPE_INTERLEAVED = 0, /* pairs (x[2i], x[2i+1]) */
+       ATTN_ROPE_HALF = 1 };      /* pairs (x[i], x[i + rotary_dim/2]) */
+
+/* Rotary embedding of any tokens' q and k, and the insert of k and v into the caches: token i turns by the angles
+ * pos[i] * inv_freq[] and its k and v go to row row[i] of sequence seq[i]. Position and cache row are independent (rows
+ * behind a shared prefix, rows of a cache that evicted some). Scaled contexts are a table of frequencies and a factor. */
+typedef struct AttnRopePositionsArgs {
+    void* q_out;           /* out: [tokens][n_heads][head_dim], q_out_dtype; may be q when type and stride are the same */
+    const void* q;         /* in : [tokens][n_heads][head_dim], in_dtype; the heads of a token lie side by side */
+    const void* k;         /* in : [tokens][n_kv_heads][head_dim], in_dtype */
+    const void* v;         /* in : the same */
+    void* k_cache;         /* kv_dtype, sequence s at + s*kv_batch_stride, row t at + t*kv_row_stride (elements) */
+    void* v_cache;
+    const float* inv_freq; /* device [rotary_dim/2]: radians per position of each pair, scaled as the model wants */
+    const uint32_t* pos;   /* device [tokens]: position (rotation angle) */
+    const uint32_t* row;   /* device [tokens]: cache row; one that does not exist (>= cache_rows, or seq >= n_seqs) is not
+                              written, and ATTN_STATUS_BAD_SHAPE is ORed into *status. No two tokens share a row. */
+    const uint32_t* seq;   /* device [tokens]: sequence; NULL = token i belongs to sequence i */
+    uint64_t q_stride, k_stride, v_stride; /* elements between tokens; 0 = dense. Stacked q, k, v: the stack's width */
+    uint64_t q_out_stride;
+    uint64_t kv_row_stride;   /* 0 = n_kv_heads*head_dim */
+    uint64_t kv_batch_stride; /* may be 0 only when n_seqs == 1 */
+    uint32_t tokens, n_heads, n_kv_heads, head_dim; /* head_dim even, up to 1024 */
+    uint32_t rotary_dim;      /* even; the first rotary_dim values of a head turn, the others are copied. 0 = head_dim */
+    uint32_t n_seqs, cache_rows;
+    float factor;             /* multiplies cos and sin (attention factor of a scaled context); 0 = 1 */
+    int32_t in_dtype, q_out_dtype; /* ATTN_DTYPE_F32 | F16 | BF16 */
+    int32_t kv_dtype;              /* ATTN_DTYPE_F16 | BF16 */
+    int32_t layout;                /* ATTN_ROPE_* */
+    uint32_t* status;
+} AttnRopePositionsArgs;
+int attn_rope_positions(const AttnRopePositionsArgs* args, void* stream);
+
+/* Single-token attention of a batch over a prefix that all sequences share (one copy of its K and V) and each sequence's
+ * own rows: what attn_decode would give over caches that each hold the prefix's rows followed by the own ones, reading the
+ * prefix once for the batch. With scores_out, the weight (softmax probability, summed over the query heads of a kv head) that
+ * each own row received is added to an accumulator, which attn_kv_evict reads. No own rows and no prefix: zeros. */
+typedef struct AttnDecodeSharedArgs {
+    void* o;              /* out: [batch][n_heads][head_dim], o_dtype */
+    const void* q;        /* in : [batch][n_heads][head_dim], dtype */
+    const void* k_prefix; /* in : [prefix_len][n_kv_heads][head_dim], row t at + t*prefix_row_stride; NULL when prefix_len is 0 */
+    const void* v_prefix;
+    const void* k;        /* in : own caches, sequence b at + b*kv_batch_stride, row t at + t*kv_row_stride; NULL when
+                             kv_capacity is 0 */
+    const void* v;
+    float* lse;           /* optional out: [batch][n_heads] natural-log sum-exp over prefix and own rows */
+    int32_t o_dtype;      /* dtype or ATTN_DTYPE_F32 */
+    int32_t dtype;        /* ATTN_DTYPE_F16 | BF16, of q, the prefix and the caches */
+    uint32_t batch, n_heads, n_kv_heads;
+    uint32_t head_dim;       /* 64 or 128; at most 64 query heads per kv head */
+    uint32_t prefix_len;
+    uint32_t kv_capacity;    /* rows an own cache holds; 0 = no own rows */
+    const uint32_t* kv_len;  /* device [batch], valid own rows; NULL = kv_len_uniform. A length beyond the capacity is clamped and
+                                ATTN_STATUS_BAD_SHAPE is ORed into *status */
+    uint32_t kv_len_uniform;
+    float scale;             /* 0 = 1/sqrt(head_dim) */
+    uint64_t prefix_row_stride, kv_row_stride; /* elements; 0 = n_kv_heads*head_dim */
+    uint64_t kv_batch_stride;                  /* may be 0 only when batch == 1 */
+    const float* scores;  /* optional in : accumulated weights so far, (sequence b, kv head h) at + (b*n_kv_heads + h)*score_stride;
+                             NULL = start from zero */
+    float* scores_out;    /* optional out: scores + this token's weights, for the valid rows (others are left alone); may be
+                             scores */
+    uint64_t score_stride, score_out_stride; /* floats; 0 = kv_capacity */
+    void* workspace;      /* device scratch, >= attn_decode_shared_workspace_bytes(), 16-byte aligned */
+    size_t workspace_bytes;
+    uint32_t* status;     /* optional device word for ATTN_STATUS_* bits */
+} AttnDecodeSharedArgs;
+
+/* Scratch size of attn_decode_shared on the current device; scored_rows = kv_capacity when scores_out is given, else 0.
+ * 0 = no kernel for these dimensions. */
+size_t attn_decode_shared_workspace_bytes(uint32_t batch, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                                          uint32_t scored_rows);
+int attn_decode_shared(const AttnDecodeSharedArgs* args, void* stream);
+
+/* Eviction from the caches by accumulated attention weight. Of every (sequence, kv head) with more than `keep` rows these
+ * stay: the first `sink`, the last `recent`, and of the others those with the largest scores, `keep` in all; among equal scores the
+ * lowest rows (NaN counts as less than any number). Kept rows keep their order and move to rows 0, 1, ...; shorter sequences keep
+ * all. Into other caches, or in place when k_out == k, v_out == v and scores_out == scores (same strides, out_rows == rows);
+ * any other overlap is refused. */
+typedef struct AttnKvEvictArgs {
+    const void* k;        /* in : 16-bit caches of any type, sequence b at + b*kv_batch_stride, row t at + t*kv_row_stride */
+    const void* v;
+    void* k_out;          /* out: the same geometry with out_* strides; rows behind the new length are left alone */
+    void* v_out;
+    const float* scores;  /* in : [batch][n_kv_heads] runs of score_stride floats; entries behind a length are not read */
+    float* scores_out;    /* out: scores of the kept rows; 0 from the new length up to out_rows (rows to come start at zero) */
+    uint32_t* kept;       /* out: [batch][n_kv_heads][keep] source row of each kept row, 0xffffffff behind the new length */
+    const uint32_t* kv_len;  /* device [batch]; NULL = rows. Beyond rows: clamped, ATTN_STATUS_BAD_SHAPE is ORed into *status */
+    uint32_t* kv_len_out;    /* out: [batch] min(length, keep); may be kv_len */
+    uint32_t batch, n_kv_heads, head_dim; /* head_dim a multiple of 8 up to 1024 */
+    uint32_t rows;        /* rows the caches hold */
+    uint32_t out_rows;    /* rows the output caches hold, >= keep */
+    uint32_t keep, sink, recent; /* sink + recent <= keep */
+    uint64_t kv_row_stride, out_row_stride;     /* elements, multiples of 8; 0 = n_kv_heads*head_dim */
+    uint64_t kv_batch_stride, out_batch_stride; /* may be 0 only when batch == 1 */
+    uint64_t score_stride, score_out_stride;    /* floats; 0 = rows, out_rows */
+    uint32_t* status;
+} AttnKvEvictArgs;
+int attn_kv_evict(const AttnKvEvictArgs* args, void* stream);
+
 /* Human-readable text for an ATTN_ERR_* code. */
 const char* attn_status_string(int code);
 
@@ -479,7 +584,8 @@ uint64_t attn_kernel_launch_count(void);
 /* sizeof() of an argument structure as this library was compiled, so that a foreign-function binding can check its own
  * mirror of the layout: 0 AttnDecodeArgs, 1 AttnDecodeShardedArgs, 2 AttnPrefillArgs, 3 AttnRopeInsertArgs,
  * 4 AttnGemvArgs, 5 AttnMergeArgs, 6 AttnGemmArgs, 7 AttnRopePromptArgs,
- * 8 AttnGemmPairArgs, 9 AttnGemmQ8Args; 0 for any other index. */
+ * 8 AttnGemmPairArgs, 9 AttnGemmQ8Args, 10 AttnRopePositionsArgs, 11 AttnDecodeSharedArgs, 12 AttnKvEvictArgs; 0 for any
+ * other index. */
 size_t attn_abi_struct_size(int which);
 
 #ifdef __cplusplus

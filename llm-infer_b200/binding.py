@@ -19,6 +19,7 @@ STATIC_SCRATCH_BYTES = 8 << 20
 STATUS_WAIT_TIMEOUT = 1
 STATUS_BAD_SHAPE = 2
 PREFILL_P_RESIDUAL, PREFILL_P_INPUT_TYPE = 0, 1
+ROPE_INTERLEAVED, ROPE_HALF = 0, 1
 
 # every symbol include/llm_infer_attn.h declares
 EXPORTED_SYMBOLS = (
@@ -53,6 +54,10 @@ EXPORTED_SYMBOLS = (
     "attn_rmsnorm_residual_split",
     "attn_swiglu",
     "attn_argmax",
+    "attn_rope_positions",
+    "attn_decode_shared_workspace_bytes",
+    "attn_decode_shared",
+    "attn_kv_evict",
     "attn_status_string",
     "attn_last_cuda_error",
     "attn_kernel_launch_count",
@@ -293,6 +298,102 @@ class AttnRopePromptArgs(C.Structure):
     ]
 
 
+class AttnRopePositionsArgs(C.Structure):
+    _fields_ = [
+        ("q_out", C.c_void_p),
+        ("q", C.c_void_p),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("k_cache", C.c_void_p),
+        ("v_cache", C.c_void_p),
+        ("inv_freq", C.c_void_p),
+        ("pos", C.c_void_p),
+        ("row", C.c_void_p),
+        ("seq", C.c_void_p),
+        ("q_stride", C.c_uint64),
+        ("k_stride", C.c_uint64),
+        ("v_stride", C.c_uint64),
+        ("q_out_stride", C.c_uint64),
+        ("kv_row_stride", C.c_uint64),
+        ("kv_batch_stride", C.c_uint64),
+        ("tokens", C.c_uint32),
+        ("n_heads", C.c_uint32),
+        ("n_kv_heads", C.c_uint32),
+        ("head_dim", C.c_uint32),
+        ("rotary_dim", C.c_uint32),
+        ("n_seqs", C.c_uint32),
+        ("cache_rows", C.c_uint32),
+        ("factor", C.c_float),
+        ("in_dtype", C.c_int32),
+        ("q_out_dtype", C.c_int32),
+        ("kv_dtype", C.c_int32),
+        ("layout", C.c_int32),
+        ("status", C.c_void_p),
+    ]
+
+
+class AttnDecodeSharedArgs(C.Structure):
+    _fields_ = [
+        ("o", C.c_void_p),
+        ("q", C.c_void_p),
+        ("k_prefix", C.c_void_p),
+        ("v_prefix", C.c_void_p),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("lse", C.c_void_p),
+        ("o_dtype", C.c_int32),
+        ("dtype", C.c_int32),
+        ("batch", C.c_uint32),
+        ("n_heads", C.c_uint32),
+        ("n_kv_heads", C.c_uint32),
+        ("head_dim", C.c_uint32),
+        ("prefix_len", C.c_uint32),
+        ("kv_capacity", C.c_uint32),
+        ("kv_len", C.c_void_p),
+        ("kv_len_uniform", C.c_uint32),
+        ("scale", C.c_float),
+        ("prefix_row_stride", C.c_uint64),
+        ("kv_row_stride", C.c_uint64),
+        ("kv_batch_stride", C.c_uint64),
+        ("scores", C.c_void_p),
+        ("scores_out", C.c_void_p),
+        ("score_stride", C.c_uint64),
+        ("score_out_stride", C.c_uint64),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+        ("status", C.c_void_p),
+    ]
+
+
+class AttnKvEvictArgs(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("k_out", C.c_void_p),
+        ("v_out", C.c_void_p),
+        ("scores", C.c_void_p),
+        ("scores_out", C.c_void_p),
+        ("kept", C.c_void_p),
+        ("kv_len", C.c_void_p),
+        ("kv_len_out", C.c_void_p),
+        ("batch", C.c_uint32),
+        ("n_kv_heads", C.c_uint32),
+        ("head_dim", C.c_uint32),
+        ("rows", C.c_uint32),
+        ("out_rows", C.c_uint32),
+        ("keep", C.c_uint32),
+        ("sink", C.c_uint32),
+        ("recent", C.c_uint32),
+        ("kv_row_stride", C.c_uint64),
+        ("out_row_stride", C.c_uint64),
+        ("kv_batch_stride", C.c_uint64),
+        ("out_batch_stride", C.c_uint64),
+        ("score_stride", C.c_uint64),
+        ("score_out_stride", C.c_uint64),
+        ("status", C.c_void_p),
+    ]
+
+
 class AttnError(RuntimeError):
     def __init__(self, code: int, what: str, cuda_error: int = 0):
         self.code = code
@@ -379,6 +480,14 @@ def load() -> C.CDLL:
     lib.attn_rope_prompt.argtypes = [C.POINTER(AttnRopePromptArgs), C.c_void_p]
     lib.attn_gather_rows.restype = C.c_int
     lib.attn_gather_rows.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.c_void_p]
+    lib.attn_rope_positions.restype = C.c_int
+    lib.attn_rope_positions.argtypes = [C.POINTER(AttnRopePositionsArgs), C.c_void_p]
+    lib.attn_decode_shared_workspace_bytes.restype = C.c_size_t
+    lib.attn_decode_shared_workspace_bytes.argtypes = [C.c_uint32] * 5
+    lib.attn_decode_shared.restype = C.c_int
+    lib.attn_decode_shared.argtypes = [C.POINTER(AttnDecodeSharedArgs), C.c_void_p]
+    lib.attn_kv_evict.restype = C.c_int
+    lib.attn_kv_evict.argtypes = [C.POINTER(AttnKvEvictArgs), C.c_void_p]
     lib.attn_status_string.restype = C.c_char_p
     lib.attn_status_string.argtypes = [C.c_int]
     lib.attn_last_cuda_error.restype = C.c_int
@@ -386,7 +495,8 @@ def load() -> C.CDLL:
     lib.attn_abi_struct_size.restype = C.c_size_t
     lib.attn_abi_struct_size.argtypes = [C.c_int]
     mirrors = (AttnDecodeArgs, AttnDecodeShardedArgs, AttnPrefillArgs, AttnRopeInsertArgs, AttnGemvArgs, AttnMergeArgs,
-               AttnGemmArgs, AttnRopePromptArgs, AttnGemmPairArgs, AttnGemmQ8Args)
+               AttnGemmArgs, AttnRopePromptArgs, AttnGemmPairArgs, AttnGemmQ8Args, AttnRopePositionsArgs, AttnDecodeSharedArgs,
+               AttnKvEvictArgs)
     for index, mirror in enumerate(mirrors):
         if lib.attn_abi_struct_size(index) != C.sizeof(mirror):
             raise RuntimeError(f"{mirror.__name__}: the ctypes mirror ({C.sizeof(mirror)} bytes) does not match the "

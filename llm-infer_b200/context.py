@@ -1,0 +1,280 @@
+"""Long contexts: scaled rotary positions, decode over a prefix that a batch shares, accumulated attention weights and eviction
+from the caches. Torch tensors in, the C ABI underneath, in the manner of ``attention``.
+
+The three belong to one generation path. ``rope_positions`` puts a token at any position into any cache row: behind a shared
+prefix, or into a cache that evicted rows. ``attn_decode_shared`` attends the prefix and the own rows and adds up the weight each
+own row received. ``kv_evict`` keeps the rows that matter when a cache is over its budget. ``model.Llama.generate_shared`` runs
+them together.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import torch
+
+from . import binding as _b
+from .attention import _call, _dense, _dtype_code, _require_cuda
+
+_LAYOUTS = {"interleaved": _b.ROPE_INTERLEAVED, "half": _b.ROPE_HALF}
+_INDEX = (torch.int32, torch.uint32)
+_CACHE = (torch.float16, torch.bfloat16)
+
+
+def rope_frequencies(rotary_dim: int, theta: float, scaling: dict | None = None):
+    """Radians per position of every pair (fp32, on the host) and the factor on cos and sin, for ``rope_positions``. ``scaling``
+    is None or a dict with "type" and the fields its formula uses, under the names that model files give them:
+
+    linear  factor                             every frequency / factor
+    ntk     factor                             theta * factor ** (R / (R - 2)): the lowest frequency / factor, the highest kept
+    yarn    factor, original (trained length), beta_fast = 32, beta_slow = 1, attention_factor = 0.1 ln(factor) + 1:
+            frequencies that turn fewer than beta_slow times in the trained length / factor, more than beta_fast kept, a linear
+            ramp over the pairs between
+    llama3  factor, original, low_freq_factor = 1, high_freq_factor = 4: wavelengths longer than original / low_freq_factor
+            / factor, shorter than original / high_freq_factor kept, a ramp over the turns between
+    """
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError("rotary_dim must be even and positive")
+    i = torch.arange(rotary_dim // 2, dtype=torch.float64)
+    freq = float(theta) ** (-2.0 * i / rotary_dim)
+    if scaling is None:
+        return freq.float(), 1.0
+    kind, attention = scaling.get("type"), 1.0
+    if kind not in ("linear", "ntk", "yarn", "llama3"):
+        raise ValueError(f"unknown rotary scaling {kind!r}")
+    factor = float(scaling["factor"])
+    if not factor >= 1.0:
+        raise ValueError("the scaling factor must be at least 1")
+    if kind == "linear":
+        freq = freq / factor
+    elif kind == "ntk":
+        if rotary_dim < 4:
+            raise ValueError("ntk scaling needs at least two pairs")
+        freq = (float(theta) * factor ** (rotary_dim / (rotary_dim - 2))) ** (-2.0 * i / rotary_dim)
+    elif kind == "yarn":
+        trained = float(scaling["original"])
+
+        def pair_that_turns(n):
+            return rotary_dim * math.log(trained / (n * 2 * math.pi)) / (2 * math.log(float(theta)))
+
+        low = max(math.floor(pair_that_turns(scaling.get("beta_fast", 32.0))), 0)
+        high = min(math.ceil(pair_that_turns(scaling.get("beta_slow", 1.0))), rotary_dim - 1)
+        ramp = ((i - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
+        freq = freq / factor * ramp + freq * (1.0 - ramp)
+        attention = float(scaling.get("attention_factor", 0.1 * math.log(factor) + 1.0))
+    else:
+        turns = float(scaling["original"]) * freq / (2 * math.pi)
+        low, high = float(scaling.get("low_freq_factor", 1.0)), float(scaling.get("high_freq_factor", 4.0))
+        if not high > low:
+            raise ValueError("high_freq_factor must be larger than low_freq_factor")
+        smooth = ((turns - low) / (high - low)).clamp(0.0, 1.0)
+        freq = (1.0 - smooth) * freq / factor + smooth * freq
+    return freq.float(), attention
+
+
+def _index(t, shape, what):
+    if t.dtype not in _INDEX or t.shape != shape or not t.is_cuda or not t.is_contiguous():
+        raise ValueError(f"{what} must be a dense 32-bit integer CUDA tensor of shape {tuple(shape)}")
+    return t.data_ptr()
+
+
+def _same_device(device, *tensors):
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError("all operands must be on one device")
+
+
+def _heads(t: torch.Tensor, stream, what: str) -> torch.Tensor:
+    """``t`` [tokens, heads, dim] with the heads of a token side by side (tokens may be strided), or a dense copy."""
+    if t.stride(2) == 1 and t.stride(1) == t.shape[2] and (t.shape[0] == 1 or t.stride(0) > 0):
+        return t
+    return _dense(t, stream, what)
+
+
+def rope_positions(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   pos: torch.Tensor, row: torch.Tensor, *, inv_freq: torch.Tensor, seq=None, layout: str = "interleaved",
+                   factor: float = 1.0, q_out=None, q_out_dtype=None, status=None, stream=None) -> torch.Tensor:
+    """Rotates every token's q and k by ``pos * inv_freq`` and writes k and v into row ``row`` of sequence ``seq``'s caches.
+
+    q [N, H, D], k / v [N, Hkv, D] fp32 / fp16 / bf16 (one type; views into a stacked projection are taken as they are);
+    k_cache / v_cache fp16 / bf16 [B, T, Hkv, D]; pos, row, seq int32 CUDA tensors [N] (seq None: token i is of sequence i);
+    inv_freq fp32 [rotary_dim / 2] on the device and factor as rope_frequencies gives them, values behind rotary_dim are copied.
+    layout "interleaved" pairs (2i, 2i + 1), "half" pairs (i, i + rotary_dim / 2). Returns the rotated q [N, H, D] (``q_out``, or a
+    new tensor of q_out_dtype, default q's). A row that does not exist is not written and sets ATTN_STATUS_BAD_SHAPE in status."""
+    _require_cuda(q, k, v, k_cache, v_cache, pos, row, inv_freq, seq)
+    if q.dim() != 3 or k.dim() != 3 or k_cache.dim() != 4:
+        raise ValueError("q must be [N, H, D], k and v [N, Hkv, D], the caches [B, T, Hkv, D]")
+    N, H, D = q.shape
+    B, T, Hkv, Dk = k_cache.shape
+    if k.shape != (N, Hkv, D) or v.shape != k.shape or Dk != D or v_cache.shape != k_cache.shape:
+        raise ValueError("shape mismatch between q, k, v and the caches")
+    if not (q.dtype == k.dtype == v.dtype) or k_cache.dtype not in _CACHE or v_cache.dtype != k_cache.dtype:
+        raise TypeError("q, k, v must share a dtype, and the caches be both fp16 or both bf16")
+    if k_cache.stride() != v_cache.stride() or k_cache.stride(3) != 1 or k_cache.stride(2) != D:
+        raise ValueError("the caches must be [B, row, kv_head, head_dim] with dense heads and share their strides")
+    if layout not in _LAYOUTS:
+        raise ValueError(f"layout must be one of {sorted(_LAYOUTS)}")
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or not 0 < 2 * inv_freq.numel() <= D:
+        raise ValueError("inv_freq must be a dense fp32 tensor of rotary_dim / 2 values, rotary_dim <= head_dim")
+    if seq is None and N > B:
+        raise ValueError("more tokens than sequences need seq")
+    _same_device(q.device, k, v, k_cache, v_cache, pos, row, inv_freq, seq, q_out, status)
+    pos_ptr, row_ptr = _index(pos, (N,), "pos"), _index(row, (N,), "row")
+    seq_ptr = None if seq is None else _index(seq, (N,), "seq")
+    q, k, v = _heads(q, stream, "q"), _heads(k, stream, "k"), _heads(v, stream, "v")
+    if q_out is None:
+        q_out = torch.empty((N, H, D), dtype=q_out_dtype or q.dtype, device=q.device)
+    elif q_out.shape != (N, H, D) or q_out.stride(2) != 1 or q_out.stride(1) != D or (N > 1 and q_out.stride(0) < H * D):
+        raise ValueError("q_out must be [N, H, D] with dense heads")
+    if N == 0:
+        return q_out
+    a = _b.AttnRopePositionsArgs(
+        q_out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), inv_freq.data_ptr(),
+        pos_ptr, row_ptr, seq_ptr, q.stride(0) if N > 1 else 0, k.stride(0) if N > 1 else 0, v.stride(0) if N > 1 else 0,
+        q_out.stride(0) if N > 1 else 0, k_cache.stride(1) if T > 1 else 0, k_cache.stride(0) if B > 1 else 0,
+        N, H, Hkv, D, 2 * inv_freq.numel(), B, T, float(factor), _dtype_code(q), _dtype_code(q_out), _dtype_code(k_cache),
+        _LAYOUTS[layout], status.data_ptr() if status is not None else None)
+    _call("attn_rope_positions", q.device, stream, C.byref(a))
+    return q_out
+
+
+class SharedWorkspace:
+    """Scratch of attn_decode_shared, reusable across calls of one shape on one stream; ``rows`` > 0 makes room for the scores
+    of caches of that many rows."""
+
+    def __init__(self, batch: int, n_heads: int, n_kv_heads: int, head_dim: int, rows: int = 0, device=None):
+        device = torch.device("cuda" if device is None else device)
+        if device.index is None:
+            device = torch.device(device.type, torch.cuda.current_device())
+        with torch.cuda.device(device):
+            nbytes = _b.load().attn_decode_shared_workspace_bytes(batch, n_heads, n_kv_heads, head_dim, rows)
+        if nbytes == 0:
+            raise _b.AttnError(-2, f"no shared-prefix decode kernel for batch={batch} heads={n_heads}/{n_kv_heads} dim={head_dim}")
+        self.key, self.rows = (batch, n_heads, n_kv_heads, head_dim, device.index), rows
+        self.nbytes = int(nbytes)
+        self.buf = torch.empty(self.nbytes, dtype=torch.uint8, device=device)
+        self.status = torch.zeros(1, dtype=torch.int32, device=device)
+
+
+def attn_decode_shared(q: torch.Tensor, k_prefix, v_prefix, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_len=None, *,
+                       out=None, lse=None, out_dtype=None, scale: float = 0.0, scores=None, scores_out=None,
+                       workspace: SharedWorkspace | None = None, stream=None) -> torch.Tensor:
+    """Single-token attention of a batch over a shared prefix and each sequence's own cache rows.
+
+    q          [B, H, D]        fp16 / bf16, already rotated
+    k_prefix   [P, Hkv, D]      q's type, or None (no prefix); rows may be strided. v_prefix the same
+    k_cache    [B, T, Hkv, D]   q's type; rows and sequences may be strided (T may be 0). v_cache the same
+    kv_len     None (all T rows), an int, or an int32 CUDA tensor [B] of valid own rows (0 is allowed)
+    scores     [B, Hkv, T] fp32 accumulated weights, rows dense; scores_out receives scores + this token's weights of the valid
+               rows (default: scores itself, in place). scores_out alone starts from zero
+    returns    out [B, H, D] in out_dtype (q's type, the default, or fp32); fills ``lse`` [B, H] (fp32) when given
+    """
+    _require_cuda(q, k_prefix, v_prefix, k_cache, v_cache, out, lse, scores, scores_out)
+    if q.dim() != 3 or k_cache.dim() != 4:
+        raise ValueError("q must be [B, H, D] and the caches [B, T, Hkv, D]")
+    B, H, D = q.shape
+    Bk, T, Hkv, Dk = k_cache.shape
+    if (Bk, Dk) != (B, D) or v_cache.shape != k_cache.shape or Hkv == 0 or H % Hkv:
+        raise ValueError("shape mismatch between q and the caches")
+    if q.dtype not in _CACHE or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise TypeError("q and the caches must be fp16 or bf16, of one type")
+    if k_cache.stride() != v_cache.stride() or (T and (k_cache.stride(3) != 1 or k_cache.stride(2) != D)):
+        raise ValueError("the caches must be [B, row, kv_head, head_dim] with dense heads and share their strides")
+    _same_device(q.device, k_prefix, v_prefix, k_cache, v_cache, out, lse, scores, scores_out)
+    P, kp, vp, prefix_stride = 0, None, None, 0
+    if (k_prefix is None) != (v_prefix is None):
+        raise ValueError("k_prefix without v_prefix")
+    if k_prefix is not None:
+        if k_prefix.dim() != 3 or k_prefix.shape[1:] != (Hkv, D) or v_prefix.shape != k_prefix.shape:
+            raise ValueError("the prefix must be [P, Hkv, D]")
+        if k_prefix.dtype != q.dtype or v_prefix.dtype != q.dtype:
+            raise TypeError("the prefix must have q's type")
+        P = k_prefix.shape[0]
+        if P:
+            if k_prefix.stride() != v_prefix.stride() or k_prefix.stride(2) != 1 or k_prefix.stride(1) != D:
+                raise ValueError("the prefix must be [row, kv_head, head_dim] with dense heads; K and V share their strides")
+            kp, vp, prefix_stride = k_prefix.data_ptr(), v_prefix.data_ptr(), k_prefix.stride(0) if P > 1 else 0
+    len_ptr, uniform = None, T
+    if isinstance(kv_len, int):
+        if not 0 <= kv_len <= T:
+            raise ValueError("kv_len exceeds the cache")
+        uniform = kv_len
+    elif kv_len is not None:
+        len_ptr = _index(kv_len, (B,), "kv_len")
+    if scores is not None and scores_out is None:
+        scores_out = scores
+    for t in (scores, scores_out):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (B, Hkv, T) or (T > 1 and t.stride(2) != 1) or
+                              (B > 1 and t.stride(0) != Hkv * t.stride(1))):
+            raise ValueError("scores must be fp32 [B, Hkv, T] with dense rows at one distance")
+    if T == 0:
+        scores = scores_out = None  # no rows: nothing to add up
+    q = _dense(q, stream, "q")
+    if out is None:
+        out = torch.empty((B, H, D), dtype=out_dtype or q.dtype, device=q.device)
+    elif out.shape != (B, H, D) or not out.is_contiguous():
+        raise ValueError("out must be a contiguous [B, H, D] tensor")
+    if out.dtype not in (q.dtype, torch.float32):
+        raise TypeError("out must have q's type or be fp32")
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (B, H) or not lse.is_contiguous()):
+        raise ValueError("lse must be a contiguous fp32 [B, H] tensor")
+    if B == 0:
+        return out
+    need_rows = T if scores_out is not None else 0
+    if workspace is None or workspace.key != (B, H, Hkv, D, q.device.index) or workspace.rows < need_rows:
+        workspace = SharedWorkspace(B, H, Hkv, D, need_rows, q.device)
+    a = _b.AttnDecodeSharedArgs(
+        out.data_ptr(), q.data_ptr(), kp, vp, k_cache.data_ptr() if T else None, v_cache.data_ptr() if T else None,
+        lse.data_ptr() if lse is not None else None, _dtype_code(out), _dtype_code(q), B, H, Hkv, D, P, T, len_ptr, uniform,
+        float(scale), prefix_stride, k_cache.stride(1) if T > 1 else 0, k_cache.stride(0) if B > 1 else 0,
+        scores.data_ptr() if scores is not None else None, scores_out.data_ptr() if scores_out is not None else None,
+        scores.stride(1) if scores is not None and B * Hkv > 1 else 0,
+        scores_out.stride(1) if scores_out is not None and B * Hkv > 1 else 0, workspace.buf.data_ptr(), workspace.nbytes,
+        workspace.status.data_ptr())
+    _call("attn_decode_shared", q.device, stream, C.byref(a))
+    return out
+
+
+def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor, kv_len, keep: int, *, sink: int = 0,
+             recent: int = 0, out=None, kept=None, kv_len_out=None, status=None, stream=None):
+    """Keeps, per sequence and kv head, the first ``sink`` rows, the last ``recent`` rows and those with the largest scores up to
+    ``keep`` rows, in their order.
+
+    k_cache, v_cache [B, T, Hkv, D] 16-bit, scores [B, Hkv, T] fp32 with dense rows, kv_len an int32 CUDA tensor [B] or None (T).
+    out  None: in place; or (k_out, v_out, scores_out) with [B, T2, Hkv, D] and [B, Hkv, T2], T2 >= keep, sharing no memory with
+         the inputs. K and V rows behind a new length are left alone, scores there become 0.
+    Returns (kept [B, Hkv, keep] int32: the source row of each kept row, -1 behind the new length; kv_len_out [B] int32:
+    min(length, keep); it may be given as kv_len itself)."""
+    k_out, v_out, scores_out = (k_cache, v_cache, scores) if out is None else out
+    _require_cuda(k_cache, v_cache, scores, k_out, v_out, scores_out, kv_len, kept, kv_len_out)
+    if k_cache.dim() != 4 or k_out.dim() != 4:
+        raise ValueError("the caches must be [B, T, Hkv, D]")
+    B, T, Hkv, D = k_cache.shape
+    T2 = k_out.shape[1]
+    for a, b, n in ((k_cache, v_cache, T), (k_out, v_out, T2)):
+        if a.shape != (B, n, Hkv, D) or b.shape != a.shape or a.stride() != b.stride() or a.stride(3) != 1 or a.stride(2) != D:
+            raise ValueError("the caches must be [B, row, kv_head, head_dim] with dense heads; K and V share their strides")
+        if a.dtype not in _CACHE or b.dtype != a.dtype or a.dtype != k_cache.dtype:
+            raise TypeError("the caches must be fp16 or bf16, of one type")
+    for t, n in ((scores, T), (scores_out, T2)):
+        if t.dtype != torch.float32 or t.shape != (B, Hkv, n) or (n > 1 and t.stride(2) != 1) or (B > 1 and t.stride(0) != Hkv * t.stride(1)):
+            raise ValueError("scores must be fp32 [B, Hkv, rows] with dense rows at one distance")
+    if keep < 1 or keep > T2 or sink < 0 or recent < 0 or sink + recent > keep:
+        raise ValueError("keep must be at least 1, fit the output caches and hold the sink and the recent rows")
+    _same_device(k_cache.device, v_cache, scores, k_out, v_out, scores_out, kv_len, kept, kv_len_out, status)
+    if kept is None:
+        kept = torch.empty((B, Hkv, keep), dtype=torch.int32, device=k_cache.device)
+    kept_ptr = _index(kept, (B, Hkv, keep), "kept")
+    if kv_len_out is None:
+        kv_len_out = torch.empty((B,), dtype=torch.int32, device=k_cache.device)
+    len_out_ptr = _index(kv_len_out, (B,), "kv_len_out")
+    if B == 0:
+        return kept, kv_len_out
+    a = _b.AttnKvEvictArgs(
+        k_cache.data_ptr(), v_cache.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), scores.data_ptr(), scores_out.data_ptr(), kept_ptr,
+        _index(kv_len, (B,), "kv_len") if kv_len is not None else None, len_out_ptr, B, Hkv, D, T, T2, keep, sink, recent,
+        k_cache.stride(1) if T > 1 else 0, k_out.stride(1) if T2 > 1 else 0, k_cache.stride(0) if B > 1 else 0,
+        k_out.stride(0) if B > 1 else 0, scores.stride(1) if B * Hkv > 1 else 0, scores_out.stride(1) if B * Hkv > 1 else 0,
+        status.data_ptr() if status is not None else None)
+    _call("attn_kv_evict", k_cache.device, stream, C.byref(a))
+    return kept, kv_len_out

@@ -302,6 +302,9 @@ size_t attn_abi_struct_size(int which) {
         case 7: return sizeof(AttnRopePromptArgs);
         case 8: return sizeof(AttnGemmPairArgs);
         case 9: return sizeof(AttnGemmQ8Args);
+        case 10: return sizeof(AttnRopePositionsArgs);
+        case 11: return sizeof(AttnDecodeSharedArgs);
+        case 12: return sizeof(AttnKvEvictArgs);
         default: return 0;
     }
 }

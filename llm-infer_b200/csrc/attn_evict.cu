@@ -1,0 +1,395 @@
+// Eviction from a KV cache by accumulated attention weight: of every (sequence, kv head), the first `sink` rows, the last
+// `recent` rows and the rows with the largest scores, `keep` in all, stay; their order stays too. Ties go to the lowest row.
+//
+// Two launches. (1) Which rows: a cluster of CTAs per (sequence, kv head) finds the keep-th largest key by a radix selection
+// (digits of 11, 11 and 10 bits, a histogram in shared memory per CTA, summed over the cluster), then counts and writes the
+// kept rows in order. A score's key is its bit pattern mapped so that unsigned order is the order of the numbers (NaN below
+// everything, -0 = +0); always-kept rows carry the largest key. (2) The copy, bound by memory: kept K and V rows and scores are
+// read once and written once. Into another cache it is a plain gather with as many blocks as it has work for. In place, a row only
+// moves down, so one CTA per (head, slice of the row) goes through the rows in order: everything it still has to read lies
+// behind what it writes.
+#include "attn_internal.cuh"
+#include "ptx_sm100.cuh"
+
+#include <cooperative_groups.h>
+
+namespace b200 {
+namespace {
+
+namespace cg = cooperative_groups;
+
+struct EvictParams {
+    const uint16_t* k;
+    const uint16_t* v;
+    uint16_t* k_out;
+    uint16_t* v_out;
+    const float* scores;
+    float* scores_out;
+    uint32_t* kept;
+    const uint32_t* kv_len;
+    uint32_t* kv_len_out;
+    uint64_t row_stride, batch_stride, out_row_stride, out_batch_stride;
+    uint64_t score_stride, score_out_stride;  // floats between the rows of (sequence, kv head)
+    uint32_t batch, n_kv_heads, head_dim, rows, out_rows, keep, sink, recent;
+    uint32_t* status;
+    uint32_t staged;  // keys of a CTA's slice that its shared memory holds
+    uint32_t slices;  // in place: pieces of a head's row
+    uint32_t in_place;
+};
+
+constexpr int kSelThreads = 512;
+constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kBins = 2048;
+constexpr uint32_t kSelWords = 2 * kBins + 2 * kSelWarps + 4;  // shared memory in front of the keys
+constexpr uint32_t kAlways = 0xffffffffu;
+
+// Unsigned order of the keys = order of the scores; NaN gets 0, below -inf. No score maps to kAlways (that pattern would be a NaN).
+__device__ __forceinline__ uint32_t score_key(float x) {
+    if (x != x) return 0u;
+    const uint32_t u = __float_as_uint(x + 0.f);  // -0 + 0 = +0
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+// A sequence's rows; a length beyond the cache is clamped to it (and reported by the selection). kv_len_out may be kv_len: the
+// selection reads it, and the copy, whose first CTA of a sequence writes the new length, needs only min(length, keep), which is
+// the same from either value.
+__device__ __forceinline__ uint32_t rows_of(const EvictParams& p, uint32_t b) { return min(p.kv_len ? p.kv_len[b] : p.rows, p.rows); }
+
+// One cluster per (sequence, kv head) = blockIdx.y, gridDim.x CTAs.
+__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_constant__ EvictParams p) {
+    extern __shared__ uint32_t s_all[];
+    uint32_t* s_hist = s_all;               // [kBins]
+    uint32_t* s_total = s_hist + kBins;     // [kBins], summed over the cluster
+    uint32_t* s_gt = s_total + kBins;       // [kSelWarps]
+    uint32_t* s_eq = s_gt + kSelWarps;      // [kSelWarps]
+    uint32_t* s_pick = s_eq + kSelWarps;    // digit, keys above it
+    uint32_t* s_counts = s_pick + 2;        // this CTA's keys above the threshold, equal to it
+    uint32_t* s_keys = s_counts + 2;        // [staged]
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t n_cta = gridDim.x, rank = blockIdx.x;
+    const uint32_t seg = blockIdx.y, b = seg / p.n_kv_heads;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    grid_dep_launch_dependents();
+    grid_dep_wait();
+    const uint32_t len = rows_of(p, b);
+    uint32_t* kept = p.kept + static_cast<size_t>(seg) * p.keep;
+    if (rank == 0 && tid == 0 && p.kv_len && p.kv_len[b] > p.rows && p.status) atomicOr(p.status, ATTN_STATUS_BAD_SHAPE);
+    if (len <= p.keep) {  // the same for the whole cluster
+        for (uint32_t j = rank * kSelThreads + tid; j < p.keep; j += n_cta * kSelThreads) kept[j] = j < len ? j : 0xffffffffu;
+        return;
+    }
+    // this CTA's rows: a contiguous slice, cut into one contiguous piece per warp
+    const uint32_t per_warp = ((len + n_cta * kSelWarps - 1) / (n_cta * kSelWarps) + 31) / 32 * 32;
+    const uint32_t per_cta = per_warp * kSelWarps;
+    const uint32_t begin = min(len, rank * per_cta), end = min(len, begin + per_cta);
+    const float* scores = p.scores + static_cast<size_t>(seg) * p.score_stride;
+    const uint32_t tail = len - min(len, p.recent);
+    auto make_key = [&](uint32_t i) { return (i < p.sink || i >= tail) ? kAlways : score_key(scores[i]); };
+    for (uint32_t i = tid; i < min(end - begin, p.staged); i += kSelThreads) s_keys[i] = make_key(begin + i);
+    auto key_at = [&](uint32_t i) { return i - begin < p.staged ? s_keys[i - begin] : make_key(i); };
+
+    // ---- the keep-th largest key, a digit at a time from the top
+    uint32_t prefix = 0, mask = 0, need = p.keep;  // keys with (key & mask) == prefix are still candidates for the need-th largest
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const uint32_t digit_mask = pass == 2 ? 1023u : 2047u;
+        for (int i = tid; i < kBins; i += kSelThreads) s_hist[i] = 0;
+        __syncthreads();
+        for (uint32_t i = begin + tid; i < end; i += kSelThreads) {
+            const uint32_t key = key_at(i);
+            if ((key & mask) == prefix) atomicAdd(&s_hist[(key >> shift) & digit_mask], 1u);
+        }
+        cluster.sync();
+        for (int i = tid; i < kBins; i += kSelThreads) {
+            uint32_t t = 0;
+            for (uint32_t c = 0; c < n_cta; ++c) t += *cluster.map_shared_rank(&s_hist[i], c);
+            s_total[i] = t;
+        }
+        __syncthreads();
+        // thread t owns bins kBins-1-4t .. kBins-4-4t, from the top: the bin in which the count from above reaches `need`
+        uint32_t mine[4], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum += mine[i] = s_total[kBins - 1 - 4 * tid - i];
+        uint32_t incl = sum;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const uint32_t o = __shfl_up_sync(0xffffffffu, incl, d);
+            if (lane >= d) incl += o;
+        }
+        if (lane == 31) s_gt[warp] = incl;
+        __syncthreads();
+        uint32_t above = incl - sum;
+        for (int w = 0; w < warp; ++w) above += s_gt[w];
+        if (above < need && above + sum >= need) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (above < need && above + mine[i] >= need) {
+                    s_pick[0] = kBins - 1 - 4 * tid - i;
+                    s_pick[1] = above;
+                    break;
+                }
+                above += mine[i];
+            }
+        }
+        cluster.sync();  // (also: no CTA clears its histogram while another still reads it)
+        prefix |= s_pick[0] << shift;
+        mask |= digit_mask << shift;
+        need -= s_pick[1];
+    }
+    // every key above `prefix` stays, and the first `need` rows of those equal to it
+    // ---- counts per warp, in order
+    const uint32_t wb = min(end, begin + warp * per_warp), we = min(end, wb + per_warp);
+    uint32_t n_gt = 0, n_eq = 0;
+    for (uint32_t i0 = wb; i0 < we; i0 += 32) {
+        const uint32_t i = i0 + lane;
+        const uint32_t key = i < we ? key_at(i) : 0u;
+        n_gt += __popc(__ballot_sync(0xffffffffu, i < we && key > prefix));
+        n_eq += __popc(__ballot_sync(0xffffffffu, i < we && key == prefix));
+    }
+    if (lane == 0) {
+        s_gt[warp] = n_gt;
+        s_eq[warp] = n_eq;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        uint32_t g = 0, e = 0;
+        for (int w = 0; w < kSelWarps; ++w) g += s_gt[w], e += s_eq[w];
+        s_counts[0] = g;
+        s_counts[1] = e;
+    }
+    cluster.sync();
+    uint32_t gt = 0, eq = 0;  // in front of this warp's piece
+    for (uint32_t c = 0; c < rank; ++c) {
+        const uint32_t* other = cluster.map_shared_rank(s_counts, c);
+        gt += other[0];
+        eq += other[1];
+    }
+    for (int w = 0; w < warp; ++w) gt += s_gt[w], eq += s_eq[w];
+    cluster.sync();  // no CTA leaves while another reads its counts
+    // ---- the kept rows, in order: row i goes to place (kept rows in front of it)
+    const uint32_t below = (1u << lane) - 1u;
+    for (uint32_t i0 = wb; i0 < we; i0 += 32) {
+        const uint32_t i = i0 + lane;
+        const uint32_t key = i < we ? key_at(i) : 0u;
+        const uint32_t m_gt = __ballot_sync(0xffffffffu, i < we && key > prefix), m_eq = __ballot_sync(0xffffffffu, i < we && key == prefix);
+        const uint32_t my_eq = eq + __popc(m_eq & below);
+        const uint32_t place = gt + __popc(m_gt & below) + min(my_eq, need);
+        if (i < we && (key > prefix || (key == prefix && my_eq < need))) kept[place] = i;
+        gt += __popc(m_gt);
+        eq += __popc(m_eq);
+    }
+}
+
+// ---- (2a) into another cache: grid (tiles of kept rows, sequences)
+constexpr int kGatherThreads = 256;
+constexpr int kTileRows = 16;
+__global__ void __launch_bounds__(kGatherThreads) evict_gather_kernel(const __grid_constant__ EvictParams p) {
+    extern __shared__ uint32_t s_from[];  // [n_kv_heads][kTileRows]
+    const uint32_t b = blockIdx.y, j0 = blockIdx.x * kTileRows;
+    const uint32_t D16 = p.head_dim / 8;  // 16-byte pieces of a head's row
+    grid_dep_launch_dependents();
+    grid_dep_wait();
+    for (uint32_t i = threadIdx.x; i < p.n_kv_heads * kTileRows; i += kGatherThreads) {
+        const uint32_t h = i / kTileRows, j = j0 + i % kTileRows;
+        const size_t seg = static_cast<size_t>(b) * p.n_kv_heads + h;
+        const uint32_t from = j < p.keep ? p.kept[seg * p.keep + j] : 0xffffffffu;
+        s_from[i] = from;
+        if (j < p.out_rows) p.scores_out[seg * p.score_out_stride + j] = from != 0xffffffffu ? p.scores[seg * p.score_stride + from] : 0.f;
+    }
+    __syncthreads();
+    const uint32_t width = p.n_kv_heads * D16, total = kTileRows * width;
+    const uint16_t* k = p.k + b * p.batch_stride;
+    const uint16_t* v = p.v + b * p.batch_stride;
+    uint16_t* ko = p.k_out + b * p.out_batch_stride;
+    uint16_t* vo = p.v_out + b * p.out_batch_stride;
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.kv_len_out[b] = min(rows_of(p, b), p.keep);
+    constexpr int kAhead = 4;
+    for (uint32_t u0 = threadIdx.x; u0 < total; u0 += kGatherThreads * kAhead) {
+        uint4 xk[kAhead], xv[kAhead];
+        uint64_t to[kAhead];
+        bool move[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            const uint32_t u = u0 + a * kGatherThreads;
+            const uint32_t r = u / width, c = u - r * width;
+            const uint32_t from = u < total ? s_from[(c / D16) * kTileRows + r] : 0xffffffffu;
+            move[a] = from != 0xffffffffu;
+            to[a] = (j0 + r) * p.out_row_stride + c * 8;
+            if (move[a]) {
+                xk[a] = __ldcs(reinterpret_cast<const uint4*>(k + from * p.row_stride + c * 8));
+                xv[a] = __ldcs(reinterpret_cast<const uint4*>(v + from * p.row_stride + c * 8));
+            }
+        }
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            if (move[a]) {
+                *reinterpret_cast<uint4*>(ko + to[a]) = xk[a];
+                *reinterpret_cast<uint4*>(vo + to[a]) = xv[a];
+            }
+        }
+    }
+}
+
+// ---- (2b) in place: grid (slices of a head's row, (sequence, kv head), K | V). Rows in rising order, a batch of them at a time:
+// all loads of a batch, a barrier, its stores. A row's place is never behind the row itself and the rows rise, so a store can
+// only hit rows whose loads lie in this batch or an earlier one, and the loads of later batches may be under way already.
+constexpr int kMoveThreads = 512;
+__global__ void __launch_bounds__(kMoveThreads) evict_compact_kernel(const __grid_constant__ EvictParams p) {
+    const uint32_t seg = blockIdx.y, b = seg / p.n_kv_heads, h = seg - b * p.n_kv_heads;
+    grid_dep_launch_dependents();
+    grid_dep_wait();
+    const uint32_t after = min(rows_of(p, b), p.keep);
+    const uint32_t* kept = p.kept + static_cast<size_t>(seg) * p.keep;
+    const uint32_t pieces = p.head_dim / 8 / p.slices;  // 16-byte pieces of a slice
+    const uint32_t rows_at_once = kMoveThreads / pieces;
+    const uint32_t my_row = threadIdx.x / pieces, my_piece = threadIdx.x - my_row * pieces;
+    uint16_t* base = (blockIdx.z ? p.v_out : p.k_out) + b * p.out_batch_stride + static_cast<size_t>(h) * p.head_dim +
+                     (blockIdx.x * pieces + my_piece) * 8;
+    constexpr int kAhead = 4;
+    const uint32_t step = rows_at_once * kAhead;
+    for (uint32_t j0 = 0; j0 < after; j0 += step) {
+        uint4 x[kAhead];
+        bool move[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            const uint32_t j = j0 + a * rows_at_once + my_row;
+            move[a] = my_row < rows_at_once && j < after;
+            if (move[a]) {
+                const uint32_t from = kept[j];
+                move[a] = from != j;  // rows in front of the first evicted one stay where they are
+                if (move[a]) x[a] = *reinterpret_cast<const uint4*>(base + from * p.row_stride);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a)
+            if (move[a]) *reinterpret_cast<uint4*>(base + (j0 + a * rows_at_once + my_row) * p.out_row_stride) = x[a];
+    }
+    // the scores of the rows, by one CTA per (sequence, kv head), the same way
+    if (blockIdx.x != 0 || blockIdx.z != 0) return;
+    if (h == 0 && threadIdx.x == 0) p.kv_len_out[b] = after;
+    float* s = p.scores_out + static_cast<size_t>(seg) * p.score_out_stride;
+    for (uint32_t j0 = 0; j0 < after; j0 += kMoveThreads) {
+        const uint32_t j = j0 + threadIdx.x;
+        const float x = j < after ? s[kept[j]] : 0.f;
+        __syncthreads();
+        if (j < after) s[j] = x;
+    }
+    __syncthreads();
+    for (uint32_t j = after + threadIdx.x; j < p.out_rows; j += kMoveThreads) s[j] = 0.f;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Whether two regions of `an` and `bn` bytes share a byte.
+bool overlap(const void* a, uint64_t an, const void* b, uint64_t bn) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + bn && y < x + an;
+}
+
+}  // namespace
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" int attn_kv_evict(const AttnKvEvictArgs* a, void* stream_v) {
+    if (!a || !a->k || !a->v || !a->k_out || !a->v_out || !a->scores || !a->scores_out || !a->kept || !a->kv_len_out)
+        return ATTN_ERR_INVALID_ARG;
+    if (a->batch == 0 || a->n_kv_heads == 0 || a->head_dim == 0 || a->rows == 0 || a->keep == 0 || a->out_rows < a->keep)
+        return ATTN_ERR_INVALID_ARG;
+    if (static_cast<uint64_t>(a->sink) + a->recent > a->keep) return ATTN_ERR_INVALID_ARG;  // the always-kept rows must fit
+    if (a->head_dim % 8 != 0 || a->head_dim > 1024) return ATTN_ERR_UNSUPPORTED;
+    const uint64_t segments = static_cast<uint64_t>(a->batch) * a->n_kv_heads;
+    if (segments > 65535 || a->n_kv_heads > 256 || a->rows > 0x7fffffffu || a->out_rows > 0x7fffffffu) return ATTN_ERR_UNSUPPORTED;
+    EvictParams p{};
+    const uint64_t width = static_cast<uint64_t>(a->n_kv_heads) * a->head_dim;
+    p.row_stride = a->kv_row_stride ? a->kv_row_stride : width;
+    p.out_row_stride = a->out_row_stride ? a->out_row_stride : width;
+    p.batch_stride = a->kv_batch_stride;
+    p.out_batch_stride = a->out_batch_stride;
+    p.score_stride = a->score_stride ? a->score_stride : a->rows;
+    p.score_out_stride = a->score_out_stride ? a->score_out_stride : a->out_rows;
+    if (p.row_stride < width || p.out_row_stride < width || p.score_stride < a->rows || p.score_out_stride < a->out_rows)
+        return ATTN_ERR_INVALID_ARG;
+    if (a->batch > 1 && (p.batch_stride == 0 || p.out_batch_stride < (a->out_rows - 1) * p.out_row_stride + width)) return ATTN_ERR_INVALID_ARG;
+    if (!aligned16(a->k) || !aligned16(a->v) || !aligned16(a->k_out) || !aligned16(a->v_out) ||
+        (p.row_stride | p.batch_stride | p.out_row_stride | p.out_batch_stride) % 8 != 0)
+        return ATTN_ERR_ALIGNMENT;
+    // In place means all three: the same caches with the same strides, and the same scores. Any other overlap would be read
+    // after it was overwritten.
+    p.in_place = a->k == a->k_out && a->v == a->v_out && a->scores == a->scores_out;
+    if (p.in_place) {
+        if (p.row_stride != p.out_row_stride || p.batch_stride != p.out_batch_stride || p.score_stride != p.score_out_stride ||
+            a->out_rows != a->rows)
+            return ATTN_ERR_INVALID_ARG;
+    } else {
+        const uint64_t in_bytes = 2 * ((a->batch - 1) * p.batch_stride + (a->rows - 1) * p.row_stride + width);
+        const uint64_t out_bytes = 2 * ((a->batch - 1) * p.out_batch_stride + (a->out_rows - 1) * p.out_row_stride + width);
+        const uint64_t s_in = 4 * ((segments - 1) * p.score_stride + a->rows), s_out = 4 * ((segments - 1) * p.score_out_stride + a->out_rows);
+        if (overlap(a->k, in_bytes, a->k_out, out_bytes) || overlap(a->v, in_bytes, a->v_out, out_bytes) ||
+            overlap(a->k, in_bytes, a->v_out, out_bytes) || overlap(a->v, in_bytes, a->k_out, out_bytes) ||
+            overlap(a->scores, s_in, a->scores_out, s_out))
+            return ATTN_ERR_INVALID_ARG;
+    }
+    DeviceInfo dev{};
+    const int rc = current_device_info(&dev);
+    if (rc != ATTN_OK) return rc;
+    if (dev.cc_major != 10) return ATTN_ERR_DEVICE;
+    p.k = static_cast<const uint16_t*>(a->k);
+    p.v = static_cast<const uint16_t*>(a->v);
+    p.k_out = static_cast<uint16_t*>(a->k_out);
+    p.v_out = static_cast<uint16_t*>(a->v_out);
+    p.scores = a->scores;
+    p.scores_out = a->scores_out;
+    p.kept = a->kept;
+    p.kv_len = a->kv_len;
+    p.kv_len_out = a->kv_len_out;
+    p.batch = a->batch;
+    p.n_kv_heads = a->n_kv_heads;
+    p.head_dim = a->head_dim;
+    p.rows = a->rows;
+    p.out_rows = a->out_rows;
+    p.keep = a->keep;
+    p.sink = a->sink;
+    p.recent = a->recent;
+    p.status = a->status;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+
+    // ---- which rows: as many CTAs per cluster as give a CTA at least 2048 rows, eight at most
+    uint32_t cl = 1;
+    while (cl < 8 && a->rows > cl * 2048ull) cl *= 2;
+    const uint64_t slice = (a->rows + cl - 1) / cl + 32 * kSelWarps;
+    p.staged = static_cast<uint32_t>(slice < 40 * 1024 ? slice : 40 * 1024);
+    B200_CUDA_TRY(allow_max_smem(evict_select_kernel));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(cl, static_cast<uint32_t>(segments));
+    cfg.blockDim = dim3(kSelThreads);
+    cfg.dynamicSmemBytes = (kSelWords + p.staged) * sizeof(uint32_t);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cl;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, evict_select_kernel, p));
+    g_launch_count.fetch_add(1, std::memory_order_relaxed);
+
+    // ---- the copy
+    if (p.in_place) {
+        // slices of a row until the CTAs cover the GPU twice, a slice no narrower than 32 bytes
+        p.slices = 1;
+        while (segments * 2 * p.slices < 2ull * dev.sm_count && (p.head_dim / 8) % (p.slices * 2) == 0 && p.head_dim / 8 / (p.slices * 2) >= 2)
+            p.slices *= 2;
+        B200_CUDA_TRY(launch_dependent(evict_compact_kernel, dim3(p.slices, static_cast<uint32_t>(segments), 2), dim3(kMoveThreads), 0, stream, p));
+    } else {
+        const uint32_t tiles = (a->out_rows + kTileRows - 1) / kTileRows;
+        B200_CUDA_TRY(launch_dependent(evict_gather_kernel, dim3(tiles, a->batch), dim3(kGatherThreads),
+                                       a->n_kv_heads * kTileRows * sizeof(uint32_t), stream, p));
+    }
+    g_launch_count.fetch_add(1, std::memory_order_relaxed);
+    return ATTN_OK;
+}

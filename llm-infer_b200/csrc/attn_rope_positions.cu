@@ -1,0 +1,262 @@
+// Rotary positions of a batch's tokens, both pair layouts, any table of (scaled) frequencies: q and k of every token are
+// rotated, q goes to q_out, k and v into the token's cache row.
+//
+// Mathematics: pair i of a head's first rotary_dim values, (x[2i], x[2i+1]) interleaved or (x[i], x[i + rotary_dim/2]) in the half
+// layout, turns by a = pos * inv_freq[i] and is multiplied by `factor`; the values behind rotary_dim are copied. The angle
+// is reduced to a fraction of a turn in 64 bits: a product rounded to 32 bits is off by up to 4e-3 at position 100000. cos
+// and sin and the rotation are fp32, each result is rounded once to the output's type.
+//
+// Bound by memory: every value is read once and written once. A thread owns a unit of 2 x VEC values (both halves of VEC pairs),
+// so that loads and stores are 16 bytes wide in either layout; a block owns a few tokens and makes their cos / sin table in
+// shared memory once for all heads. One unit of one value pair (VEC = 1) serves sizes, strides and addresses that 16-byte
+// accesses cannot.
+#include "attn_internal.cuh"
+#include "ptx_sm100.cuh"
+
+namespace b200 {
+namespace {
+
+struct RopePosParams {
+    void* q_out;
+    const void* q;
+    const void* k;
+    const void* v;
+    void* k_cache;
+    void* v_cache;
+    const float* inv_freq;
+    const uint32_t* pos;
+    const uint32_t* row;
+    const uint32_t* seq;  // null: token i belongs to sequence i
+    uint64_t q_stride, k_stride, v_stride, q_out_stride, kv_row_stride, kv_batch_stride;
+    uint32_t tokens, n_heads, n_kv_heads, head_dim, rotary_dim, n_seqs, cache_rows;
+    uint32_t tokens_per_block, units_per_head, units;  // units of one token: (n_heads + 2 n_kv_heads) * units_per_head
+    uint32_t half_layout;
+    float factor;
+    uint32_t* status;
+};
+
+constexpr int kThreads = 256;
+
+// 16-bit and 32-bit floating types <-> fp32, N values at a time (N * size a power of two up to 16 bytes per access)
+template <typename T>
+__device__ __forceinline__ float to_f32(T x);
+template <>
+__device__ __forceinline__ float to_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Vec {
+    T v[N];
+};
+template <typename T, int N>
+__device__ __forceinline__ void load(float (&x)[N], const T* p) {
+    const Vec<T, N> t = *reinterpret_cast<const Vec<T, N>*>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = to_f32<T>(t.v[i]);
+}
+template <typename T, int N>
+__device__ __forceinline__ void store(T* p, const float (&x)[N]) {
+    Vec<T, N> t;
+#pragma unroll
+    for (int i = 0; i < N; ++i) t.v[i] = from_f32<T>(x[i]);
+    *reinterpret_cast<Vec<T, N>*>(p) = t;
+}
+
+// grid (token groups, slices of a token's units)
+template <typename TIn, typename TQ, typename TC, int VEC>
+__global__ void __launch_bounds__(kThreads) rope_positions_kernel(const __grid_constant__ RopePosParams p) {
+    extern __shared__ float2 s_cs[];  // [tokens_per_block][rotary_dim / 2] cos, sin (times the factor)
+    grid_dep_launch_dependents();
+    grid_dep_wait();
+    const uint32_t t0 = blockIdx.x * p.tokens_per_block;
+    const uint32_t nt = min(p.tokens_per_block, p.tokens - t0);
+    const uint32_t half = p.rotary_dim / 2;
+    for (uint32_t i = threadIdx.x; i < nt * half; i += kThreads) {
+        const uint32_t t = i / half, j = i - t * half;
+        constexpr double kTurn = 0.15915494309189533577;  // 1 / (2 pi)
+        double turns = static_cast<double>(p.pos[t0 + t]) * (static_cast<double>(p.inv_freq[j]) * kTurn);
+        turns -= rint(turns);
+        float s, c;
+        sincospif(2.f * static_cast<float>(turns), &s, &c);
+        s_cs[i] = make_float2(c * p.factor, s * p.factor);
+    }
+    __syncthreads();
+
+    const uint32_t q_units = p.n_heads * p.units_per_head, k_units = p.n_kv_heads * p.units_per_head;
+    const uint32_t rot_units = half / VEC;  // of a head
+    for (uint32_t u = blockIdx.y * kThreads + threadIdx.x; u < nt * p.units; u += gridDim.y * kThreads) {
+        const uint32_t t = u / p.units, w = u - t * p.units, tok = t0 + t;
+        const bool is_q = w < q_units, is_v = w >= q_units + k_units;
+        const uint32_t in_kind = is_q ? w : is_v ? w - q_units - k_units : w - q_units;
+        const uint32_t head = in_kind / p.units_per_head, part = in_kind - head * p.units_per_head;
+        // offsets of the unit's two runs of VEC values in the head
+        const bool turn = part < rot_units;
+        uint32_t at0 = part * 2 * VEC, at1 = at0 + VEC;
+        if (turn && p.half_layout) at0 = part * VEC, at1 = at0 + half;
+        const TIn* src = (is_q ? static_cast<const TIn*>(p.q) + tok * p.q_stride
+                          : is_v ? static_cast<const TIn*>(p.v) + tok * p.v_stride
+                                 : static_cast<const TIn*>(p.k) + tok * p.k_stride) + static_cast<size_t>(head) * p.head_dim;
+        float a[VEC], b[VEC];
+        load<TIn, VEC>(a, src + at0);
+        load<TIn, VEC>(b, src + at1);
+        if (turn && !is_v) {
+            const float2* cs = s_cs + t * half + part * VEC;
+            if (p.half_layout) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const float x = a[i], y = b[i];
+                    a[i] = x * cs[i].x - y * cs[i].y;
+                    b[i] = x * cs[i].y + y * cs[i].x;
+                }
+            } else if constexpr (VEC == 1) {
+                const float x = a[0], y = b[0];
+                a[0] = x * cs[0].x - y * cs[0].y;
+                b[0] = x * cs[0].y + y * cs[0].x;
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; i += 2) {
+                    const float x0 = a[i], y0 = a[i + 1], x1 = b[i], y1 = b[i + 1];
+                    const float2 c0 = cs[i / 2], c1 = cs[VEC / 2 + i / 2];
+                    a[i] = x0 * c0.x - y0 * c0.y;
+                    a[i + 1] = x0 * c0.y + y0 * c0.x;
+                    b[i] = x1 * c1.x - y1 * c1.y;
+                    b[i + 1] = x1 * c1.y + y1 * c1.x;
+                }
+            }
+        }
+        if (is_q) {
+            TQ* dst = static_cast<TQ*>(p.q_out) + tok * p.q_out_stride + static_cast<size_t>(head) * p.head_dim;
+            store<TQ, VEC>(dst + at0, a);
+            store<TQ, VEC>(dst + at1, b);
+        } else {
+            const uint32_t seq = p.seq ? p.seq[tok] : tok, row = p.row[tok];
+            if (seq >= p.n_seqs || row >= p.cache_rows) {  // no such cache row: nothing is written
+                if (part == 0 && p.status) atomicOr(p.status, ATTN_STATUS_BAD_SHAPE);
+                continue;
+            }
+            TC* dst = static_cast<TC*>(is_v ? p.v_cache : p.k_cache) + seq * p.kv_batch_stride + row * p.kv_row_stride +
+                      static_cast<size_t>(head) * p.head_dim;
+            store<TC, VEC>(dst + at0, a);
+            store<TC, VEC>(dst + at1, b);
+        }
+    }
+}
+
+template <typename TIn, typename TQ, typename TC, int VEC>
+int launch(RopePosParams p, const DeviceInfo& dev, cudaStream_t stream) {
+    p.units_per_head = p.head_dim / (2 * VEC);
+    const uint64_t units = static_cast<uint64_t>(p.n_heads + 2ull * p.n_kv_heads) * p.units_per_head;
+    if (units > (1u << 24)) return ATTN_ERR_UNSUPPORTED;
+    p.units = static_cast<uint32_t>(units);
+    // A block takes up to four tokens when there are enough of them to fill the GPU (one evaluation of a table entry per thread
+    // at a rotary dimension of 128); fewer tokens are cut over blocks instead, a unit per thread.
+    uint32_t tb = 4;
+    while (tb > 1 && (p.tokens + tb - 1) / tb < 4u * dev.sm_count) tb /= 2;
+    while (tb > 1 && tb * p.rotary_dim / 2 * sizeof(float2) > 32 * 1024) tb /= 2;
+    p.tokens_per_block = tb;
+    const uint32_t groups = (p.tokens + tb - 1) / tb;
+    const uint32_t slices_max = (tb * p.units + kThreads - 1) / kThreads;
+    uint32_t slices = 1;
+    while (slices < slices_max && static_cast<uint64_t>(groups) * slices < 4ull * dev.sm_count) ++slices;
+    const size_t smem = static_cast<size_t>(tb) * (p.rotary_dim / 2) * sizeof(float2);
+    auto kernel = rope_positions_kernel<TIn, TQ, TC, VEC>;
+    B200_CUDA_TRY(launch_dependent(kernel, dim3(groups, slices), dim3(kThreads), smem, stream, p));
+    g_launch_count.fetch_add(1, std::memory_order_relaxed);
+    return ATTN_OK;
+}
+
+template <typename TIn, typename TQ, typename TC>
+int launch_width(const RopePosParams& p, bool wide, const DeviceInfo& dev, cudaStream_t stream) {
+    constexpr int kVec = 16 / sizeof(TIn);  // 16-byte loads
+    return wide ? launch<TIn, TQ, TC, kVec>(p, dev, stream) : launch<TIn, TQ, TC, 1>(p, dev, stream);
+}
+template <typename TIn, typename TQ>
+int launch_cache(const RopePosParams& p, int32_t kv_dtype, bool wide, const DeviceInfo& dev, cudaStream_t stream) {
+    if (kv_dtype == ATTN_DTYPE_F16) return launch_width<TIn, TQ, __half>(p, wide, dev, stream);
+    return launch_width<TIn, TQ, __nv_bfloat16>(p, wide, dev, stream);
+}
+template <typename TIn>
+int launch_q(const RopePosParams& p, int32_t q_dtype, int32_t kv_dtype, bool wide, const DeviceInfo& dev, cudaStream_t stream) {
+    if (q_dtype == ATTN_DTYPE_F32) return launch_cache<TIn, float>(p, kv_dtype, wide, dev, stream);
+    if (q_dtype == ATTN_DTYPE_F16) return launch_cache<TIn, __half>(p, kv_dtype, wide, dev, stream);
+    return launch_cache<TIn, __nv_bfloat16>(p, kv_dtype, wide, dev, stream);
+}
+
+bool float_dtype(int32_t d) { return d == ATTN_DTYPE_F32 || d == ATTN_DTYPE_F16 || d == ATTN_DTYPE_BF16; }
+uintptr_t bits(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+
+}  // namespace
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" int attn_rope_positions(const AttnRopePositionsArgs* a, void* stream_v) {
+    if (!a || !a->q_out || !a->q || !a->k || !a->v || !a->k_cache || !a->v_cache || !a->inv_freq || !a->pos || !a->row)
+        return ATTN_ERR_INVALID_ARG;
+    if (a->tokens == 0 || a->n_heads == 0 || a->n_kv_heads == 0 || a->head_dim == 0 || a->n_seqs == 0 || a->cache_rows == 0)
+        return ATTN_ERR_INVALID_ARG;
+    if (a->head_dim % 2 != 0 || a->rotary_dim % 2 != 0 || a->rotary_dim > a->head_dim) return ATTN_ERR_INVALID_ARG;
+    if (!float_dtype(a->in_dtype) || !float_dtype(a->q_out_dtype)) return ATTN_ERR_INVALID_ARG;
+    if (a->kv_dtype != ATTN_DTYPE_F16 && a->kv_dtype != ATTN_DTYPE_BF16) return ATTN_ERR_UNSUPPORTED;
+    if (a->layout != ATTN_ROPE_INTERLEAVED && a->layout != ATTN_ROPE_HALF) return ATTN_ERR_INVALID_ARG;
+    if (a->n_seqs > 1 && a->kv_batch_stride == 0) return ATTN_ERR_INVALID_ARG;
+    if (!a->seq && a->tokens > a->n_seqs) return ATTN_ERR_INVALID_ARG;
+    if (a->head_dim > 1024 || a->n_heads > 65536 || a->n_kv_heads > 65536) return ATTN_ERR_UNSUPPORTED;
+    RopePosParams p{};
+    p.q_out = a->q_out;
+    p.q = a->q;
+    p.k = a->k;
+    p.v = a->v;
+    p.k_cache = a->k_cache;
+    p.v_cache = a->v_cache;
+    p.inv_freq = a->inv_freq;
+    p.pos = a->pos;
+    p.row = a->row;
+    p.seq = a->seq;
+    const uint64_t q_width = static_cast<uint64_t>(a->n_heads) * a->head_dim, kv_width = static_cast<uint64_t>(a->n_kv_heads) * a->head_dim;
+    p.q_stride = a->q_stride ? a->q_stride : q_width;
+    p.k_stride = a->k_stride ? a->k_stride : kv_width;
+    p.v_stride = a->v_stride ? a->v_stride : kv_width;
+    p.q_out_stride = a->q_out_stride ? a->q_out_stride : q_width;
+    p.kv_row_stride = a->kv_row_stride ? a->kv_row_stride : kv_width;
+    p.kv_batch_stride = a->kv_batch_stride;
+    if (p.kv_row_stride < kv_width || p.q_out_stride < q_width) return ATTN_ERR_INVALID_ARG;  // outputs would overlap
+    p.tokens = a->tokens;
+    p.n_heads = a->n_heads;
+    p.n_kv_heads = a->n_kv_heads;
+    p.head_dim = a->head_dim;
+    p.rotary_dim = a->rotary_dim ? a->rotary_dim : a->head_dim;
+    p.n_seqs = a->n_seqs;
+    p.cache_rows = a->cache_rows;
+    p.half_layout = a->layout == ATTN_ROPE_HALF ? 1u : 0u;
+    p.factor = a->factor != 0.f ? a->factor : 1.f;
+    p.status = a->status;
+    const uint32_t in_size = a->in_dtype == ATTN_DTYPE_F32 ? 4 : 2, q_size = a->q_out_dtype == ATTN_DTYPE_F32 ? 4 : 2;
+    if ((bits(a->q) | bits(a->k) | bits(a->v)) % in_size || bits(a->q_out) % q_size || (bits(a->k_cache) | bits(a->v_cache)) % 2 ||
+        (bits(a->inv_freq) | bits(a->pos) | bits(a->row) | bits(a->seq)) % 4)
+        return ATTN_ERR_ALIGNMENT;
+    // 16-byte accesses need units of whole vectors, and strides and addresses in 16 bytes (fp32: 4 values, else 8)
+    const uint32_t vec = 16 / in_size;
+    const bool wide = p.rotary_dim % (2 * vec) == 0 && p.head_dim % (2 * vec) == 0 &&
+                      (p.q_stride | p.k_stride | p.v_stride | p.q_out_stride | p.kv_row_stride | p.kv_batch_stride) % 8 == 0 &&
+                      (bits(a->q) | bits(a->k) | bits(a->v) | bits(a->q_out) | bits(a->k_cache) | bits(a->v_cache)) % 16 == 0;
+    DeviceInfo dev{};
+    const int rc = current_device_info(&dev);
+    if (rc != ATTN_OK) return rc;
+    if (dev.cc_major != 10) return ATTN_ERR_DEVICE;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+    if (a->in_dtype == ATTN_DTYPE_F32) return launch_q<float>(p, a->q_out_dtype, a->kv_dtype, wide, dev, stream);
+    if (a->in_dtype == ATTN_DTYPE_F16) return launch_q<__half>(p, a->q_out_dtype, a->kv_dtype, wide, dev, stream);
+    return launch_q<__nv_bfloat16>(p, a->q_out_dtype, a->kv_dtype, wide, dev, stream);
+}

@@ -1,0 +1,689 @@
+// Decode attention of a batch whose sequences share a prefix: one token per sequence attends the prefix's rows (one copy for the
+// batch) and the rows of its own cache. Optionally the weight that each own row received, summed over the query heads of its
+// kv head, is added to an accumulator (what an eviction by attention weight looks at).
+//
+// Mathematics: o = sum_t p_t v_t with p the softmax over prefix and own rows. The rows are cut into pieces; each gives its own
+// softmax-normalised sum and log-sum-exp, and the pieces merge by weights exp(lse_i - LSE). All B * G query rows of a kv head meet the
+// prefix together as one matrix, so a prefix row is read once for the batch and not once per sequence.
+//
+// Two launches:
+//   split   tiles of 64 (row, head) pairs of K and V, prefix tiles first, then the own rows of sequence after sequence, are dealt to the
+//           CTAs in equal contiguous runs (two CTAs per SM). A tile streams through a ring in shared memory by 16-byte asynchronous
+//           copies; four warps multiply by mma.sync (16 query rows x 16 keys x 8 at a time). A warp owns 16 query rows of one
+//           kv head and a share of the tile's keys: with few query rows the four warps take four heads (whose slices of a cache row
+//           are contiguous) or four shares of the keys, with many rows of the prefix product four blocks of 16 rows.
+//   merge   one CTA per output row folds that row's pieces; further CTAs turn the scaled scores that the split pass left
+//           in the workspace into weights (exp2(s - LSE)), sum them over the heads and add them to the accumulators.
+// The scores of own rows cost 4 bytes per query head and row each way through L2, next to 4 * head_dim bytes of K and V per kv head.
+// P enters the second product rounded once to the caches' type when the output is 16 bits wide too (an error below the
+// output's own rounding), and as value + rounding residual for fp32 outputs.
+#include <algorithm>
+
+#include "attn_internal.cuh"
+#include "ptx_sm100.cuh"
+
+namespace b200 {
+namespace {
+
+constexpr int kThreads = 128;
+constexpr int kTilePairs = 64;  // (row, head) pairs of a tile
+constexpr uint32_t kMaxBatch = 2048;
+
+// How the four warps share a tile of one kind of segment: hpc heads x wm blocks of 16 query rows x ts shares of the keys = 4.
+struct Shape {
+    uint32_t hpc, wm, ts;
+    uint32_t keys;    // of a tile: 64 / hpc
+    uint32_t groups;  // n_kv_heads / hpc
+    uint32_t rec_rows;  // query rows per (piece, share of keys, head): 16 * wm for the prefix, G for own rows
+};
+
+struct SharedParams {
+    const uint16_t* q;
+    const uint16_t* kp;
+    const uint16_t* vp;
+    const uint16_t* k;
+    const uint16_t* v;
+    const uint32_t* kv_len;
+    uint32_t kv_len_uniform;
+    uint32_t batch, n_heads, n_kv_heads, group;
+    uint32_t prefix, rows;
+    uint64_t prefix_row_stride, row_stride, batch_stride;
+    float scale_log2;
+    Shape pre, own;
+    uint32_t row_blocks;    // blocks of 16 * pre.wm query rows against the prefix
+    uint32_t prefix_segs;   // pre.groups * row_blocks
+    uint32_t prefix_tiles;  // of one such segment
+    float* part_pre;        // [(grid + prefix_segs) * ts * hpc][rec_rows][D]
+    float* lse_pre;
+    float* part_own;        // [(grid + batch * groups) * ts * hpc][rec_rows][D]
+    float* lse_own;
+    uint32_t* seg_ctas;     // [prefix_segs + batch * own.groups]
+    float* raw;             // [batch][n_heads][raw_stride] scaled scores in log2 units, or null
+    uint64_t raw_stride;
+    uint32_t* status;
+    // merge
+    void* o;
+    float* lse;
+    int32_t o_dtype;
+    const float* scores;
+    float* scores_out;
+    uint64_t score_stride, score_out_stride;
+    uint32_t out_ctas, score_chunks;
+};
+
+constexpr uint32_t kScoreRows = 1024;  // rows of a CTA that adds up weights
+
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ uint32_t own_len(const SharedParams& p, uint32_t b) {
+    return min(p.kv_len ? p.kv_len[b] : p.kv_len_uniform, p.rows);
+}
+
+// One run of tiles of one segment: where its K and V lie and which query rows meet it.
+struct Cursor {
+    const uint16_t* k;
+    const uint16_t* v;
+    uint64_t stride;
+    uint32_t own, seg;        // kind; index among the segments of its kind
+    uint32_t b, hg, rb;       // own: sequence; head group; prefix: block of query rows
+    uint32_t tile, tiles, len;
+};
+
+template <int D, bool BF16, bool RES>
+__global__ void __launch_bounds__(kThreads, 2) shared_split_kernel(const __grid_constant__ SharedParams p) {
+    constexpr int kChunks = D / 8;                         // 16-byte pieces of a head's row
+    constexpr int kStages = D == 128 ? 3 : 6;
+    constexpr uint32_t kOperandBytes = kTilePairs * D * 2;
+    constexpr uint32_t kStageBytes = 2 * kOperandBytes;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    uint32_t* s_cum = reinterpret_cast<uint32_t*>(smem_raw + kStages * kStageBytes);  // [batch + 1] tiles of own rows, one head group
+    uint32_t* s_warp = s_cum + p.batch + 1;                                           // [4]
+    const uint32_t ring = smem_u32(smem_raw);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    grid_dep_launch_dependents();
+    grid_dep_wait();
+
+    // ---- tiles of each sequence, summed up: a batch of 128 sequences at a time
+    {
+        uint32_t base = 0;
+        if (tid == 0) s_cum[0] = 0;
+        for (uint32_t b0 = 0; b0 < p.batch; b0 += kThreads) {
+            const uint32_t b = b0 + tid;
+            uint32_t n = b < p.batch ? (own_len(p, b) + p.own.keys - 1) / p.own.keys : 0u;
+            if (b < p.batch && p.kv_len && p.kv_len[b] > p.rows && p.status && blockIdx.x == 0) atomicOr(p.status, ATTN_STATUS_BAD_SHAPE);
+            uint32_t incl = n;
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) {
+                const uint32_t o = __shfl_up_sync(0xffffffffu, incl, d);
+                if (lane >= d) incl += o;
+            }
+            if (lane == 31) s_warp[warp] = incl;
+            __syncthreads();
+            uint32_t before = base;
+            for (int w = 0; w < warp; ++w) before += s_warp[w];
+            if (b < p.batch) s_cum[b + 1] = before + incl;
+            base += s_warp[0] + s_warp[1] + s_warp[2] + s_warp[3];
+            __syncthreads();
+        }
+    }
+    const uint32_t pre_total = p.prefix_segs * p.prefix_tiles;
+    const uint32_t total = pre_total + s_cum[p.batch] * p.own.groups;
+    const uint32_t active = active_ctas(gridDim.x, 0, 1, total);
+    // ---- which CTAs share each segment, for the merge pass
+    const uint32_t own_segs = p.batch * p.own.groups;
+    for (uint32_t s = blockIdx.x * kThreads + tid; s < p.prefix_segs + own_segs; s += gridDim.x * kThreads) {
+        uint32_t first, n;
+        if (s < p.prefix_segs) {
+            first = s * p.prefix_tiles;
+            n = p.prefix_tiles;
+        } else {
+            const uint32_t b = (s - p.prefix_segs) / p.own.groups, hg = (s - p.prefix_segs) - b * p.own.groups;
+            n = s_cum[b + 1] - s_cum[b];
+            first = pre_total + s_cum[b] * p.own.groups + hg * n;
+        }
+        p.seg_ctas[s] = segment_ctas(first, static_cast<uint64_t>(first) + n, total, active);
+    }
+    if (blockIdx.x >= active) return;
+    const uint32_t t0 = static_cast<uint32_t>(static_cast<uint64_t>(blockIdx.x) * total / active);
+    const uint32_t t1 = static_cast<uint32_t>((blockIdx.x + 1ull) * total / active);
+
+    if (t0 >= t1) return;
+
+    auto locate = [&](uint32_t flat, Cursor& c) {
+        if (flat < pre_total) {
+            c.own = 0;
+            c.seg = flat / p.prefix_tiles;
+            c.tile = flat - c.seg * p.prefix_tiles;
+            c.tiles = p.prefix_tiles;
+            c.hg = c.seg / p.row_blocks;
+            c.rb = c.seg - c.hg * p.row_blocks;
+            c.b = 0;
+            c.len = p.prefix;
+            c.stride = p.prefix_row_stride;
+            c.k = p.kp + static_cast<size_t>(c.hg) * p.pre.hpc * D;
+            c.v = p.vp + static_cast<size_t>(c.hg) * p.pre.hpc * D;
+            return;
+        }
+        const uint32_t f = flat - pre_total;
+        uint32_t lo = 0, hi = p.batch;  // the last sequence whose tiles start at or before f
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (s_cum[mid] * p.own.groups <= f) lo = mid;
+            else hi = mid;
+        }
+        c.own = 1;
+        c.b = lo;
+        c.tiles = s_cum[lo + 1] - s_cum[lo];
+        const uint32_t r = f - s_cum[lo] * p.own.groups;
+        c.hg = r / c.tiles;
+        c.tile = r - c.hg * c.tiles;
+        c.seg = lo * p.own.groups + c.hg;
+        c.rb = 0;
+        c.len = own_len(p, lo);
+        c.stride = p.row_stride;
+        const size_t at = lo * p.batch_stride + static_cast<size_t>(c.hg) * p.own.hpc * D;
+        c.k = p.k + at;
+        c.v = p.v + at;
+    };
+    // the next tile of the list
+    auto advance = [&](uint32_t flat, Cursor& c) {
+        if (++c.tile == c.tiles && flat < t1) locate(flat, c);
+    };
+    auto load_tile = [&](const Cursor& c, uint32_t stage) {
+        const uint32_t hpc = c.own ? p.own.hpc : p.pre.hpc, keys = c.own ? p.own.keys : p.pre.keys;
+        const uint32_t width = hpc * kChunks;  // both powers of two
+        const uint32_t shift = 31 - __clz(width), row0 = c.tile * keys;
+        const uint32_t kdst = ring + stage * kStageBytes, vdst = kdst + kOperandBytes;
+#pragma unroll
+        for (int i = 0; i < kTilePairs * kChunks / kThreads; ++i) {
+            const uint32_t id = tid + i * kThreads;
+            const uint32_t key = id >> shift, in_row = id & (width - 1);
+            const uint32_t hs = in_row / kChunks, ch = in_row % kChunks;
+            const uint32_t row = row0 + key, r = hs * keys + key;
+            const bool there = row < c.len;
+            const size_t at = there ? row * c.stride + in_row * 8 : 0;  // (nothing is read where `there` is false: zeros are stored)
+            const uint32_t dst = r * (D * 2) + ((ch ^ (r & 7)) << 4);
+            cp_async16(kdst + dst, c.k + at, there ? 16u : 0u);
+            cp_async16(vdst + dst, c.v + at, there ? 16u : 0u);
+        }
+    };
+
+    Cursor ld, cur;
+    locate(t0, ld);
+    cur = ld;
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) {
+        if (t0 + s < t1) {
+            load_tile(ld, s);
+            advance(t0 + s + 1, ld);
+        }
+        cp_async_commit();
+    }
+
+    uint32_t qa[D / 16][4];
+    float o[D / 8][4];
+    float m[2], l[2];
+    bool fresh = true;  // the next tile begins a run of a segment
+    uint32_t stage = 0;
+    for (uint32_t t = t0; t < t1; ++t) {
+        const Shape& sh = cur.own ? p.own : p.pre;
+        // this warp's place: head hs of the group, block wr of query rows, share wk of the keys
+        const uint32_t hs = warp % sh.hpc, wr = (warp / sh.hpc) % sh.wm, wk = warp / (sh.hpc * sh.wm);
+        const uint32_t kvh = cur.hg * sh.hpc + hs;
+        if (fresh) {
+            fresh = false;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const uint32_t r = wr * 16 + half * 8 + lane / 4;
+                uint32_t b, g;
+                bool there;
+                if (cur.own) {
+                    b = cur.b;
+                    g = r;
+                    there = r < p.group;
+                } else {
+                    const uint32_t row = cur.rb * sh.wm * 16 + r;
+                    b = row / p.group;
+                    g = row - b * p.group;
+                    there = b < p.batch;
+                }
+                const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + ((static_cast<size_t>(b) * p.n_heads) + kvh * p.group + g) * D) + lane % 4;
+#pragma unroll
+                for (int kc = 0; kc < D / 16; ++kc) {
+                    qa[kc][half] = there ? src[kc * 8] : 0u;
+                    qa[kc][2 + half] = there ? src[kc * 8 + 4] : 0u;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+            m[0] = m[1] = -INFINITY;
+            l[0] = l[1] = 0.f;
+        }
+        cp_async_wait<kStages - 2>();
+        __syncthreads();
+        if (t + kStages - 1 < t1) {
+            load_tile(ld, stage == 0 ? kStages - 1 : stage - 1);
+            advance(t + kStages, ld);
+        }
+        cp_async_commit();
+        const uint32_t kbase = ring + stage * kStageBytes, vbase = kbase + kOperandBytes;
+        const uint32_t steps = sh.wm;  // 16 keys each: 64 / hpc / ts = 16 wm
+#pragma unroll 1
+        for (uint32_t st = 0; st < steps; ++st) {
+            const uint32_t key0 = (wk * steps + st) * 16;          // in the tile
+            const uint32_t row0 = hs * sh.keys + key0;             // in shared memory
+            const uint32_t first = cur.tile * sh.keys + key0;      // in the cache
+            if (first >= cur.len) break;
+            float s[2][4] = {};
+#pragma unroll
+            for (int kc = 0; kc < D / 16; ++kc) {
+                const uint32_t r = row0 + (lane >> 4) * 8 + (lane & 7), ch = kc * 2 + ((lane >> 3) & 1);
+                uint32_t b0, b1, b2, b3;
+                ldmatrix_x4(b0, b1, b2, b3, kbase + r * (D * 2) + ((ch ^ (r & 7)) << 4));
+                mma_16816<BF16>(s[0], qa[kc], b0, b1);
+                mma_16816<BF16>(s[1], qa[kc], b2, b3);
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t key = first + n * 8 + (lane & 3) * 2 + (i & 1);
+                    s[n][i] = key < cur.len ? s[n][i] * p.scale_log2 : -INFINITY;
+                }
+            if (cur.own && p.raw) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t g = wr * 16 + half * 8 + lane / 4;
+                    if (g < p.group) {
+                        float* dst = p.raw + (static_cast<size_t>(cur.b) * p.n_heads + kvh * p.group + g) * p.raw_stride + first + (lane & 3) * 2;
+                        *reinterpret_cast<float2*>(dst) = make_float2(s[0][2 * half], s[0][2 * half + 1]);
+                        *reinterpret_cast<float2*>(dst + 8) = make_float2(s[1][2 * half], s[1][2 * half + 1]);
+                    }
+                }
+            }
+            float mx[2], safe[2];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                float x = fmaxf(fmaxf(s[0][2 * half], s[0][2 * half + 1]), fmaxf(s[1][2 * half], s[1][2 * half + 1]));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+                mx[half] = fmaxf(m[half], x);
+                safe[half] = mx[half] == -INFINITY ? 0.f : mx[half];
+            }
+            if (__any_sync(0xffffffffu, mx[0] != m[0] || mx[1] != m[1])) {
+                const float f0 = fast_exp2(m[0] - safe[0]), f1 = fast_exp2(m[1] - safe[1]);
+                l[0] *= f0;
+                l[1] *= f1;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    o[i][0] *= f0;
+                    o[i][1] *= f0;
+                    o[i][2] *= f1;
+                    o[i][3] *= f1;
+                }
+                m[0] = mx[0];
+                m[1] = mx[1];
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[n][i] = fast_exp2(s[n][i] - safe[i >> 1]);
+                    l[i >> 1] += s[n][i];
+                }
+            uint32_t pa[4], pr[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = s[i >> 1][(i & 1) * 2], y = s[i >> 1][(i & 1) * 2 + 1];
+                pa[i] = pack2<BF16>(x, y);
+                if constexpr (RES) pr[i] = pack2<BF16>(x - round16<BF16>(x), y - round16<BF16>(y));
+            }
+#pragma unroll
+            for (int dc = 0; dc < D / 16; ++dc) {
+                const uint32_t r = row0 + ((lane >> 3) & 1) * 8 + (lane & 7), ch = dc * 2 + (lane >> 4);
+                uint32_t b0, b1, b2, b3;
+                ldmatrix_x4_trans(b0, b1, b2, b3, vbase + r * (D * 2) + ((ch ^ (r & 7)) << 4));
+                mma_16816<BF16>(o[2 * dc], pa, b0, b1);
+                mma_16816<BF16>(o[2 * dc + 1], pa, b2, b3);
+                if constexpr (RES) {
+                    mma_16816<BF16>(o[2 * dc], pr, b0, b1);
+                    mma_16816<BF16>(o[2 * dc + 1], pr, b2, b3);
+                }
+            }
+        }
+        if (cur.tile + 1 == cur.tiles || t + 1 == t1) {
+            // ---- the run's piece: normalised sum and log-sum-exp (log2 units) of this warp's rows and keys
+            const size_t rec = (static_cast<size_t>(blockIdx.x + cur.seg) * sh.ts + wk) * sh.hpc + hs;
+            float* po = cur.own ? p.part_own : p.part_pre;
+            float* pl = cur.own ? p.lse_own : p.lse_pre;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                float sum = l[half];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                const float inv = sum > 0.f ? 1.f / sum : 0.f;
+                const uint32_t r = wr * 16 + half * 8 + lane / 4;
+                const bool there = cur.own ? r < p.group : cur.rb * sh.wm * 16 + r < p.batch * p.group;
+                if (there) {
+                    float* dst = po + (rec * sh.rec_rows + r) * D + (lane & 3) * 2;
+#pragma unroll
+                    for (int i = 0; i < D / 8; ++i)
+                        *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[i][2 * half] * inv, o[i][2 * half + 1] * inv);
+                    if ((lane & 3) == 0) pl[rec * sh.rec_rows + r] = sum > 0.f ? m[half] + __log2f(sum) : -INFINITY;
+                }
+            }
+            fresh = true;
+        }
+        advance(t + 1, cur);
+        if (++stage == kStages) stage = 0;
+    }
+}
+
+// The pieces of one query row: of the prefix, then of its own cache.
+struct Pieces {
+    const float* o[2];
+    const float* lse[2];
+    uint32_t first[2], ts[2], count[2];
+    uint64_t step[2];  // rows between consecutive records of one CTA
+};
+template <int D>
+__device__ __forceinline__ void find_pieces(const SharedParams& p, uint32_t b, uint32_t h, Pieces& x) {
+    const uint32_t kvh = h / p.group, g = h - kvh * p.group;
+    x.count[0] = 0;
+    if (p.prefix_segs) {
+        const Shape& sh = p.pre;
+        const uint32_t row = b * p.group + g, rb = row / sh.rec_rows, r = row - rb * sh.rec_rows;
+        const uint32_t hg = kvh / sh.hpc, hs = kvh - hg * sh.hpc, seg = hg * p.row_blocks + rb;
+        const uint32_t w = p.seg_ctas[seg];
+        const uint64_t at = (static_cast<uint64_t>((w & 0xffffu) + seg) * sh.ts * sh.hpc + hs) * sh.rec_rows + r;
+        x.step[0] = static_cast<uint64_t>(sh.hpc) * sh.rec_rows;
+        x.count[0] = (w >> 16) * sh.ts;
+        x.o[0] = p.part_pre + at * D;
+        x.lse[0] = p.lse_pre + at;
+    }
+    const Shape& sh = p.own;
+    const uint32_t hg = kvh / sh.hpc, hs = kvh - hg * sh.hpc, seg = b * sh.groups + hg;
+    const uint32_t w = p.seg_ctas[p.prefix_segs + seg];
+    const uint64_t at = (static_cast<uint64_t>((w & 0xffffu) + seg) * sh.ts * sh.hpc + hs) * sh.rec_rows + g;
+    x.step[1] = static_cast<uint64_t>(sh.hpc) * sh.rec_rows;
+    x.count[1] = (w >> 16) * sh.ts;
+    x.o[1] = p.part_own + at * D;
+    x.lse[1] = p.lse_own + at;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads) shared_merge_kernel(const __grid_constant__ SharedParams p) {
+    constexpr int kPer = D / 32;  // floats of a lane
+    __shared__ float s_o[4][D];
+    __shared__ float s_ml[4][2];
+    __shared__ float s_lse[64];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    grid_dep_wait();
+    if (blockIdx.x < p.out_ctas) {
+        const uint32_t b = blockIdx.x / p.n_heads, h = blockIdx.x - b * p.n_heads;
+        Pieces x;
+        find_pieces<D>(p, b, h, x);
+        float m = -INFINITY, l = 0.f, acc[kPer] = {};
+#pragma unroll
+        for (int kind = 0; kind < 2; ++kind) {
+            constexpr int kAhead = 4;
+            for (uint32_t i0 = warp; i0 < x.count[kind]; i0 += 4 * kAhead) {
+                float ls[kAhead], v[kAhead][kPer];
+#pragma unroll
+                for (int a = 0; a < kAhead; ++a) {
+                    const uint32_t i = i0 + 4 * a;
+                    ls[a] = -INFINITY;
+                    if (i < x.count[kind]) {
+                        ls[a] = x.lse[kind][i * x.step[kind]];
+                        const float* src = x.o[kind] + i * x.step[kind] * D + lane * kPer;
+#pragma unroll
+                        for (int c = 0; c < kPer; ++c) v[a][c] = src[c];
+                    }
+                }
+#pragma unroll
+                for (int a = 0; a < kAhead; ++a) {
+                    if (ls[a] == -INFINITY) continue;
+                    const float mn = fmaxf(m, ls[a]);
+                    const float f = fast_exp2(m - mn), w = fast_exp2(ls[a] - mn);
+                    l = l * f + w;
+#pragma unroll
+                    for (int c = 0; c < kPer; ++c) acc[c] = acc[c] * f + w * v[a][c];
+                    m = mn;
+                }
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < kPer; ++c) s_o[warp][lane * kPer + c] = acc[c];
+        if (lane == 0) {
+            s_ml[warp][0] = m;
+            s_ml[warp][1] = l;
+        }
+        __syncthreads();
+        if (tid < D) {
+            const float mm = fmaxf(fmaxf(s_ml[0][0], s_ml[1][0]), fmaxf(s_ml[2][0], s_ml[3][0]));
+            const float safe = mm == -INFINITY ? 0.f : mm;
+            float sum = 0.f, val = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float f = fast_exp2(s_ml[w][0] - safe);
+                sum += f * s_ml[w][1];
+                val += f * s_o[w][tid];
+            }
+            val = sum > 0.f ? val / sum : 0.f;
+            const size_t at = static_cast<size_t>(blockIdx.x) * D + tid;
+            if (p.o_dtype == ATTN_DTYPE_F32) static_cast<float*>(p.o)[at] = val;
+            else if (p.o_dtype == ATTN_DTYPE_F16) static_cast<__half*>(p.o)[at] = __float2half_rn(val);
+            else static_cast<__nv_bfloat16*>(p.o)[at] = __float2bfloat16_rn(val);
+            if (tid == 0 && p.lse) p.lse[blockIdx.x] = sum > 0.f ? (mm + __log2f(sum)) * 0.69314718055994531f : -INFINITY;
+        }
+        return;
+    }
+    // ---- weights of the own rows of one (sequence, kv head)
+    const uint32_t idx = blockIdx.x - p.out_ctas;
+    const uint32_t seg = idx / p.score_chunks, chunk = idx - seg * p.score_chunks;
+    const uint32_t b = seg / p.n_kv_heads, kvh = seg - b * p.n_kv_heads;
+    const uint32_t len = own_len(p, b);
+    const uint32_t begin = chunk * kScoreRows, end = min(len, begin + kScoreRows);
+    if (begin >= end) return;
+    for (uint32_t g = warp; g < p.group; g += 4) {
+        Pieces x;
+        find_pieces<D>(p, b, kvh * p.group + g, x);
+        float m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int kind = 0; kind < 2; ++kind)
+            for (uint32_t i = lane; i < x.count[kind]; i += 32) {
+                const float ls = x.lse[kind][i * x.step[kind]];
+                if (ls == -INFINITY) continue;
+                const float mn = fmaxf(m, ls);
+                l = l * fast_exp2(m - mn) + fast_exp2(ls - mn);
+                m = mn;
+            }
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const float om = __shfl_xor_sync(0xffffffffu, m, d), ol = __shfl_xor_sync(0xffffffffu, l, d);
+            const float mn = fmaxf(m, om), safe = mn == -INFINITY ? 0.f : mn;
+            l = l * fast_exp2(m - safe) + ol * fast_exp2(om - safe);
+            m = mn;
+        }
+        if (lane == 0) s_lse[g] = m + __log2f(l);
+    }
+    __syncthreads();
+    const float* raw = p.raw + (static_cast<size_t>(b) * p.n_heads + kvh * p.group) * p.raw_stride;
+    for (uint32_t t = begin + tid; t < end; t += kThreads) {
+        float w = 0.f;
+        for (uint32_t g = 0; g < p.group; ++g) w += fast_exp2(raw[g * p.raw_stride + t] - s_lse[g]);
+        const float before = p.scores ? p.scores[seg * p.score_stride + t] : 0.f;
+        p.scores_out[seg * p.score_out_stride + t] = before + w;
+    }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Dimensions -> how the warps share the tiles, and the pieces of the workspace (in 32-bit words).
+struct SharedPlan {
+    Shape pre, own;
+    uint32_t row_blocks, prefix_segs, own_segs, grid;
+    size_t lse_pre, part_own, lse_own, seg_ctas, raw, words;
+    uint64_t raw_stride;
+};
+void set_shape(Shape* s, uint32_t query_rows, uint32_t n_kv_heads) {
+    s->wm = query_rows <= 16 ? 1 : query_rows <= 32 ? 2 : 4;
+    s->hpc = 4 / s->wm;
+    while (n_kv_heads % s->hpc) s->hpc /= 2;
+    s->ts = 4 / (s->wm * s->hpc);
+    s->keys = kTilePairs / s->hpc;
+    s->groups = n_kv_heads / s->hpc;
+}
+int make_shared_plan(uint32_t batch, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t scored_rows, const DeviceInfo& dev,
+                     SharedPlan* plan) {
+    if (batch == 0 || n_heads == 0 || n_kv_heads == 0 || n_heads % n_kv_heads != 0) return ATTN_ERR_INVALID_ARG;
+    const uint32_t group = n_heads / n_kv_heads;
+    if ((head_dim != 64 && head_dim != 128) || group > 64 || batch > kMaxBatch || n_heads > 4096) return ATTN_ERR_UNSUPPORTED;
+    SharedPlan& s = *plan;
+    set_shape(&s.own, group, n_kv_heads);
+    s.own.rec_rows = group;
+    set_shape(&s.pre, batch * group, n_kv_heads);
+    s.pre.rec_rows = 16 * s.pre.wm;
+    s.row_blocks = (batch * group + s.pre.rec_rows - 1) / s.pre.rec_rows;
+    s.prefix_segs = s.pre.groups * s.row_blocks;
+    s.own_segs = batch * s.own.groups;
+    s.grid = 2 * dev.sm_count;
+    const size_t pre_rows = static_cast<size_t>(s.grid + s.prefix_segs) * s.pre.ts * s.pre.hpc * s.pre.rec_rows;
+    const size_t own_rows = static_cast<size_t>(s.grid + s.own_segs) * s.own.ts * s.own.hpc * s.own.rec_rows;
+    auto round4 = [](size_t n) { return (n + 3) / 4 * 4; };
+    s.lse_pre = pre_rows * head_dim;
+    s.part_own = s.lse_pre + round4(pre_rows);
+    s.lse_own = s.part_own + own_rows * head_dim;
+    s.seg_ctas = s.lse_own + round4(own_rows);
+    s.raw = s.seg_ctas + round4(s.prefix_segs + s.own_segs);
+    s.raw_stride = (static_cast<uint64_t>(scored_rows) + 63) / 64 * 64;
+    s.words = s.raw + static_cast<size_t>(batch) * n_heads * s.raw_stride;
+    return ATTN_OK;
+}
+
+}  // namespace
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" size_t attn_decode_shared_workspace_bytes(uint32_t batch, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                                                     uint32_t scored_rows) {
+    DeviceInfo dev{};
+    if (current_device_info(&dev) != ATTN_OK) return 0;
+    SharedPlan plan{};
+    if (make_shared_plan(batch, n_heads, n_kv_heads, head_dim, scored_rows, dev, &plan) != ATTN_OK) return 0;
+    return plan.words * 4;
+}
+
+extern "C" int attn_decode_shared(const AttnDecodeSharedArgs* a, void* stream_v) {
+    if (!a || !a->o || !a->q) return ATTN_ERR_INVALID_ARG;
+    if ((a->prefix_len && (!a->k_prefix || !a->v_prefix)) || (a->kv_capacity && (!a->k || !a->v))) return ATTN_ERR_INVALID_ARG;
+    if (a->dtype != ATTN_DTYPE_F16 && a->dtype != ATTN_DTYPE_BF16) return ATTN_ERR_UNSUPPORTED;
+    if (a->o_dtype != ATTN_DTYPE_F32 && a->o_dtype != a->dtype) return ATTN_ERR_UNSUPPORTED;
+    if (a->batch == 0 || a->n_heads == 0 || a->n_kv_heads == 0 || a->n_heads % a->n_kv_heads != 0) return ATTN_ERR_INVALID_ARG;
+    if (a->batch > 1 && a->kv_capacity && a->kv_batch_stride == 0) return ATTN_ERR_INVALID_ARG;
+    if (a->scores && !a->scores_out) return ATTN_ERR_INVALID_ARG;
+    if (a->scores_out && a->kv_capacity == 0) return ATTN_ERR_INVALID_ARG;
+    const uint64_t width = static_cast<uint64_t>(a->n_kv_heads) * a->head_dim;
+    SharedParams p{};
+    p.prefix_row_stride = a->prefix_row_stride ? a->prefix_row_stride : width;
+    p.row_stride = a->kv_row_stride ? a->kv_row_stride : width;
+    p.batch_stride = a->kv_batch_stride;
+    p.score_stride = a->score_stride ? a->score_stride : a->kv_capacity;
+    p.score_out_stride = a->score_out_stride ? a->score_out_stride : a->kv_capacity;
+    if (p.prefix_row_stride < width || p.row_stride < width || p.score_stride < a->kv_capacity || p.score_out_stride < a->kv_capacity)
+        return ATTN_ERR_INVALID_ARG;
+    if (!aligned16(a->q) || !aligned16(a->k_prefix) || !aligned16(a->v_prefix) || !aligned16(a->k) || !aligned16(a->v) ||
+        (p.prefix_row_stride | p.row_stride | p.batch_stride) % 8 != 0)
+        return ATTN_ERR_ALIGNMENT;
+    DeviceInfo dev{};
+    int rc = current_device_info(&dev);
+    if (rc != ATTN_OK) return rc;
+    if (dev.cc_major != 10) return ATTN_ERR_DEVICE;
+    const bool scored = a->scores_out != nullptr;
+    SharedPlan plan{};
+    rc = make_shared_plan(a->batch, a->n_heads, a->n_kv_heads, a->head_dim, scored ? a->kv_capacity : 0, dev, &plan);
+    if (rc != ATTN_OK) return rc;
+    if (!a->workspace || a->workspace_bytes < plan.words * 4) return ATTN_ERR_WORKSPACE;
+    if (!aligned16(a->workspace)) return ATTN_ERR_ALIGNMENT;
+
+    p.q = static_cast<const uint16_t*>(a->q);
+    p.kp = static_cast<const uint16_t*>(a->k_prefix);
+    p.vp = static_cast<const uint16_t*>(a->v_prefix);
+    p.k = static_cast<const uint16_t*>(a->k);
+    p.v = static_cast<const uint16_t*>(a->v);
+    p.kv_len = a->kv_capacity ? a->kv_len : nullptr;
+    p.kv_len_uniform = a->kv_len_uniform;
+    p.batch = a->batch;
+    p.n_heads = a->n_heads;
+    p.n_kv_heads = a->n_kv_heads;
+    p.group = a->n_heads / a->n_kv_heads;
+    p.prefix = a->prefix_len;
+    p.rows = a->kv_capacity;
+    const float scale = a->scale != 0.f ? a->scale : 1.0f / sqrtf(static_cast<float>(a->head_dim));
+    p.scale_log2 = scale * 1.4426950408889634f;
+    p.pre = plan.pre;
+    p.own = plan.own;
+    p.row_blocks = plan.row_blocks;
+    p.prefix_segs = a->prefix_len ? plan.prefix_segs : 0;
+    const uint64_t prefix_tiles = (static_cast<uint64_t>(a->prefix_len) + plan.pre.keys - 1) / plan.pre.keys;
+    const uint64_t own_tiles = (static_cast<uint64_t>(a->kv_capacity) + plan.own.keys - 1) / plan.own.keys;
+    if (prefix_tiles * plan.prefix_segs + own_tiles * plan.own_segs > 0x7fffffffull) return ATTN_ERR_UNSUPPORTED;  // 32-bit tile numbers
+    p.prefix_tiles = static_cast<uint32_t>(prefix_tiles);
+    float* ws = static_cast<float*>(a->workspace);
+    p.part_pre = ws;
+    p.lse_pre = ws + plan.lse_pre;
+    p.part_own = ws + plan.part_own;
+    p.lse_own = ws + plan.lse_own;
+    p.seg_ctas = reinterpret_cast<uint32_t*>(ws + plan.seg_ctas);
+    p.raw = scored ? ws + plan.raw : nullptr;
+    p.raw_stride = plan.raw_stride;
+    p.status = a->status;
+    p.o = a->o;
+    p.lse = a->lse;
+    p.o_dtype = a->o_dtype;
+    p.scores = a->scores;
+    p.scores_out = a->scores_out;
+    p.out_ctas = a->batch * a->n_heads;
+    p.score_chunks = (a->kv_capacity + kScoreRows - 1) / kScoreRows;
+    const uint64_t merge_ctas = p.out_ctas + (scored ? static_cast<uint64_t>(a->batch) * a->n_kv_heads * p.score_chunks : 0);
+    if (merge_ctas > 0x7fffffffull) return ATTN_ERR_UNSUPPORTED;
+
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+    const uint64_t most = prefix_tiles * p.prefix_segs + own_tiles * plan.own_segs;
+    const uint32_t grid = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(plan.grid, most)));
+    auto split = [&](auto kernel) -> int {
+        B200_CUDA_TRY(allow_max_smem(kernel));
+        const size_t smem = 96 * 1024 + (a->batch + 5) * 4;  // the ring, s_cum, s_warp
+        B200_CUDA_TRY(launch_dependent(kernel, dim3(grid), dim3(kThreads), smem, stream, p));
+        g_launch_count.fetch_add(1, std::memory_order_relaxed);
+        return ATTN_OK;
+    };
+    const bool bf16 = a->dtype == ATTN_DTYPE_BF16, res = a->o_dtype == ATTN_DTYPE_F32;
+    if (a->head_dim == 128) {
+        rc = bf16 ? (res ? split(shared_split_kernel<128, true, true>) : split(shared_split_kernel<128, true, false>))
+                  : (res ? split(shared_split_kernel<128, false, true>) : split(shared_split_kernel<128, false, false>));
+    } else {
+        rc = bf16 ? (res ? split(shared_split_kernel<64, true, true>) : split(shared_split_kernel<64, true, false>))
+                  : (res ? split(shared_split_kernel<64, false, true>) : split(shared_split_kernel<64, false, false>));
+    }
+    if (rc != ATTN_OK) return rc;
+    auto merge = [&](auto kernel) -> int {
+        B200_CUDA_TRY(launch_dependent(kernel, dim3(static_cast<uint32_t>(merge_ctas)), dim3(kThreads), 0, stream, p));
+        g_launch_count.fetch_add(1, std::memory_order_relaxed);
+        return ATTN_OK;
+    };
+    return a->head_dim == 128 ? merge(shared_merge_kernel<128>) : merge(shared_merge_kernel<64>);
+}
