@@ -40,7 +40,7 @@ struct EvictParams {
 constexpr int kSelThreads = 512;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kBins = 2048;
-constexpr uint32_t kSelWords = 2 * kBins + 2 * kSelWarps + 4;  // shared memory in front of the keys
+constexpr uint32_t kSelWords = 3 * kBins + 2 * kSelWarps + 4;  // shared memory in front of the keys
 constexpr uint32_t kAlways = 0xffffffffu;
 
 // Unsigned order of the keys = order of the scores; NaN gets 0, below -inf. No score maps to kAlways (that pattern would be a NaN).
@@ -55,62 +55,90 @@ __device__ __forceinline__ uint32_t score_key(float x) {
 // the same from either value.
 __device__ __forceinline__ uint32_t rows_of(const EvictParams& p, uint32_t b) { return min(p.kv_len ? p.kv_len[b] : p.rows, p.rows); }
 
-// One cluster per (sequence, kv head) = blockIdx.y, gridDim.x CTAs.
+// One cluster of kCtas per (sequence, kv head) = blockIdx.y.
+template <int kCtas>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_constant__ EvictParams p) {
-    extern __shared__ uint32_t s_all[];
-    uint32_t* s_hist = s_all;               // [kBins]
-    uint32_t* s_total = s_hist + kBins;     // [kBins], summed over the cluster
-    uint32_t* s_gt = s_total + kBins;       // [kSelWarps]
-    uint32_t* s_eq = s_gt + kSelWarps;      // [kSelWarps]
-    uint32_t* s_pick = s_eq + kSelWarps;    // digit, keys above it
-    uint32_t* s_counts = s_pick + 2;        // this CTA's keys above the threshold, equal to it
-    uint32_t* s_keys = s_counts + 2;        // [staged]
+    extern __shared__ __align__(16) uint32_t s_all[];
+    uint32_t* s_hist = s_all;                   // [3][kBins], one histogram per digit
+    uint32_t* s_gt = s_hist + 3 * kBins;        // [kSelWarps]
+    uint32_t* s_eq = s_gt + kSelWarps;          // [kSelWarps]
+    uint32_t* s_pick = s_eq + kSelWarps;        // digit, keys above it
+    uint32_t* s_counts = s_pick + 2;            // this CTA's keys above the threshold, equal to it
+    uint32_t* s_keys = s_counts + 2;            // [staged]
     cg::cluster_group cluster = cg::this_cluster();
-    const uint32_t n_cta = gridDim.x, rank = blockIdx.x;
+    auto meet = [&]() {
+        if constexpr (kCtas > 1) cluster.sync();
+        else __syncthreads();
+    };
+    const uint32_t rank = blockIdx.x;
     const uint32_t seg = blockIdx.y, b = seg / p.n_kv_heads;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     grid_dep_launch_dependents();
+    for (int i = tid; i < 3 * kBins / 4; i += kSelThreads) reinterpret_cast<uint4*>(s_hist)[i] = make_uint4(0, 0, 0, 0);
     grid_dep_wait();
     const uint32_t len = rows_of(p, b);
     uint32_t* kept = p.kept + static_cast<size_t>(seg) * p.keep;
     if (rank == 0 && tid == 0 && p.kv_len && p.kv_len[b] > p.rows && p.status) atomicOr(p.status, ATTN_STATUS_BAD_SHAPE);
     if (len <= p.keep) {  // the same for the whole cluster
-        for (uint32_t j = rank * kSelThreads + tid; j < p.keep; j += n_cta * kSelThreads) kept[j] = j < len ? j : 0xffffffffu;
+        for (uint32_t j = rank * kSelThreads + tid; j < p.keep; j += kCtas * kSelThreads) kept[j] = j < len ? j : 0xffffffffu;
         return;
     }
     // this CTA's rows: a contiguous slice, cut into one contiguous piece per warp
-    const uint32_t per_warp = ((len + n_cta * kSelWarps - 1) / (n_cta * kSelWarps) + 31) / 32 * 32;
+    const uint32_t per_warp = ((len + kCtas * kSelWarps - 1) / (kCtas * kSelWarps) + 31) / 32 * 32;
     const uint32_t per_cta = per_warp * kSelWarps;
     const uint32_t begin = min(len, rank * per_cta), end = min(len, begin + per_cta);
     const float* scores = p.scores + static_cast<size_t>(seg) * p.score_stride;
     const uint32_t tail = len - min(len, p.recent);
-    auto make_key = [&](uint32_t i) { return (i < p.sink || i >= tail) ? kAlways : score_key(scores[i]); };
-    for (uint32_t i = tid; i < min(end - begin, p.staged); i += kSelThreads) s_keys[i] = make_key(begin + i);
-    auto key_at = [&](uint32_t i) { return i - begin < p.staged ? s_keys[i - begin] : make_key(i); };
+    auto make_key = [&](uint32_t i, float x) { return (i < p.sink || i >= tail) ? kAlways : score_key(x); };
+    const uint32_t n_staged = min(end - begin, p.staged);
+    __syncthreads();  // the histograms are clear
+    // ---- keys into shared memory, and the top digit's histogram on the way (eight loads of a thread in flight)
+    constexpr int kAhead = 8;
+    for (uint32_t i0 = begin + tid; i0 < end; i0 += kAhead * kSelThreads) {
+        float x[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            const uint32_t i = i0 + a * kSelThreads;
+            x[a] = i < end ? scores[i] : 0.f;
+        }
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            const uint32_t i = i0 + a * kSelThreads;
+            if (i < end) {
+                const uint32_t key = make_key(i, x[a]);
+                if (i - begin < n_staged) s_keys[i - begin] = key;
+                atomicAdd(&s_hist[key >> 21], 1u);
+            }
+        }
+    }
+    auto key_at = [&](uint32_t i) { return i - begin < n_staged ? s_keys[i - begin] : make_key(i, scores[i]); };
 
     // ---- the keep-th largest key, a digit at a time from the top
-    uint32_t prefix = 0, mask = 0, need = p.keep;  // keys with (key & mask) == prefix are still candidates for the need-th largest
-#pragma unroll 1
+    uint32_t prefix = 0, need = p.keep;  // keys whose upper digits are those of prefix are still candidates for the need-th largest
+#pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
         const uint32_t digit_mask = pass == 2 ? 1023u : 2047u;
-        for (int i = tid; i < kBins; i += kSelThreads) s_hist[i] = 0;
-        __syncthreads();
-        for (uint32_t i = begin + tid; i < end; i += kSelThreads) {
-            const uint32_t key = key_at(i);
-            if ((key & mask) == prefix) atomicAdd(&s_hist[(key >> shift) & digit_mask], 1u);
+        uint32_t* hist = s_hist + pass * kBins;
+        if (pass > 0) {
+            const uint32_t mask = pass == 1 ? 0xffe00000u : 0xfffffc00u;
+#pragma unroll 4
+            for (uint32_t i = begin + tid; i < end; i += kSelThreads) {
+                const uint32_t key = key_at(i);
+                if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & digit_mask], 1u);
+            }
         }
-        cluster.sync();
-        for (int i = tid; i < kBins; i += kSelThreads) {
-            uint32_t t = 0;
-            for (uint32_t c = 0; c < n_cta; ++c) t += *cluster.map_shared_rank(&s_hist[i], c);
-            s_total[i] = t;
-        }
-        __syncthreads();
-        // thread t owns bins kBins-1-4t .. kBins-4-4t, from the top: the bin in which the count from above reaches `need`
-        uint32_t mine[4], sum = 0;
+        meet();
+        // thread t owns the four bins from kBins - 4 - 4t up, so that threads run from the top: it sums them over the cluster
+        const int bin0 = kBins - 4 - 4 * tid;
+        uint4 mine = make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum += mine[i] = s_total[kBins - 1 - 4 * tid - i];
+        for (int c = 0; c < kCtas; ++c) {
+            const uint4* src = reinterpret_cast<const uint4*>(hist + bin0);
+            const uint4 h = kCtas > 1 ? *cluster.map_shared_rank(src, c) : *src;
+            mine.x += h.x, mine.y += h.y, mine.z += h.z, mine.w += h.w;
+        }
+        const uint32_t sum = mine.x + mine.y + mine.z + mine.w;
         uint32_t incl = sum;
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
@@ -119,66 +147,77 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_
         }
         if (lane == 31) s_gt[warp] = incl;
         __syncthreads();
-        uint32_t above = incl - sum;
-        for (int w = 0; w < warp; ++w) above += s_gt[w];
-        if (above < need && above + sum >= need) {
+        uint32_t above = incl - sum + __reduce_add_sync(0xffffffffu, lane < warp ? s_gt[lane] : 0u);
+        if (above < need && above + sum >= need) {  // one thread
+            uint32_t digit = bin0 + 3;
+            const uint32_t counts[4] = {mine.w, mine.z, mine.y, mine.x};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (above < need && above + mine[i] >= need) {
-                    s_pick[0] = kBins - 1 - 4 * tid - i;
-                    s_pick[1] = above;
+            for (int i = 0; i < 3; ++i) {
+                if (above + counts[i] < need) {
+                    above += counts[i];
+                    --digit;
+                } else {
                     break;
                 }
-                above += mine[i];
             }
+            s_pick[0] = digit;
+            s_pick[1] = above;
         }
-        cluster.sync();  // (also: no CTA clears its histogram while another still reads it)
+        __syncthreads();
         prefix |= s_pick[0] << shift;
-        mask |= digit_mask << shift;
         need -= s_pick[1];
+        // (the next write of s_gt and s_pick comes behind another meeting, and each digit has a histogram of its own)
     }
     // every key above `prefix` stays, and the first `need` rows of those equal to it
     // ---- counts per warp, in order
     const uint32_t wb = min(end, begin + warp * per_warp), we = min(end, wb + per_warp);
-    uint32_t n_gt = 0, n_eq = 0;
-    for (uint32_t i0 = wb; i0 < we; i0 += 32) {
-        const uint32_t i = i0 + lane;
-        const uint32_t key = i < we ? key_at(i) : 0u;
-        n_gt += __popc(__ballot_sync(0xffffffffu, i < we && key > prefix));
-        n_eq += __popc(__ballot_sync(0xffffffffu, i < we && key == prefix));
+    uint32_t n_gt = 0, n_eq = 0;  // of this lane
+#pragma unroll 4
+    for (uint32_t i = wb + lane; i < we; i += 32) {
+        const uint32_t key = key_at(i);
+        n_gt += key > prefix;
+        n_eq += key == prefix;
     }
+    n_gt = __reduce_add_sync(0xffffffffu, n_gt);
+    n_eq = __reduce_add_sync(0xffffffffu, n_eq);
+    __syncthreads();  // s_gt of the last digit has been read
     if (lane == 0) {
         s_gt[warp] = n_gt;
         s_eq[warp] = n_eq;
     }
     __syncthreads();
-    if (tid == 0) {
-        uint32_t g = 0, e = 0;
-        for (int w = 0; w < kSelWarps; ++w) g += s_gt[w], e += s_eq[w];
-        s_counts[0] = g;
-        s_counts[1] = e;
+    uint32_t gt = __reduce_add_sync(0xffffffffu, lane < warp ? s_gt[lane] : 0u);  // in front of this warp's piece
+    uint32_t eq = __reduce_add_sync(0xffffffffu, lane < warp ? s_eq[lane] : 0u);
+    if constexpr (kCtas > 1) {
+        if (warp == kSelWarps - 1 && lane == 0) {
+            s_counts[0] = gt + n_gt;
+            s_counts[1] = eq + n_eq;
+        }
+        cluster.sync();
+        uint32_t og = 0, oe = 0;
+        if (lane < static_cast<int>(rank)) {
+            const uint32_t* other = cluster.map_shared_rank(s_counts, lane);
+            og = other[0];
+            oe = other[1];
+        }
+        gt += __reduce_add_sync(0xffffffffu, og);
+        eq += __reduce_add_sync(0xffffffffu, oe);
     }
-    cluster.sync();
-    uint32_t gt = 0, eq = 0;  // in front of this warp's piece
-    for (uint32_t c = 0; c < rank; ++c) {
-        const uint32_t* other = cluster.map_shared_rank(s_counts, c);
-        gt += other[0];
-        eq += other[1];
-    }
-    for (int w = 0; w < warp; ++w) gt += s_gt[w], eq += s_eq[w];
-    cluster.sync();  // no CTA leaves while another reads its counts
     // ---- the kept rows, in order: row i goes to place (kept rows in front of it)
     const uint32_t below = (1u << lane) - 1u;
+#pragma unroll 2
     for (uint32_t i0 = wb; i0 < we; i0 += 32) {
         const uint32_t i = i0 + lane;
         const uint32_t key = i < we ? key_at(i) : 0u;
-        const uint32_t m_gt = __ballot_sync(0xffffffffu, i < we && key > prefix), m_eq = __ballot_sync(0xffffffffu, i < we && key == prefix);
+        const bool is_gt = i < we && key > prefix, is_eq = i < we && key == prefix;
+        const uint32_t m_gt = __ballot_sync(0xffffffffu, is_gt), m_eq = __ballot_sync(0xffffffffu, is_eq);
         const uint32_t my_eq = eq + __popc(m_eq & below);
         const uint32_t place = gt + __popc(m_gt & below) + min(my_eq, need);
-        if (i < we && (key > prefix || (key == prefix && my_eq < need))) kept[place] = i;
+        if (is_gt || (is_eq && my_eq < need)) kept[place] = i;
         gt += __popc(m_gt);
         eq += __popc(m_eq);
     }
+    if constexpr (kCtas > 1) cluster.sync();  // no CTA leaves while another reads its counts
 }
 
 // ---- (2a) into another cache: grid (tiles of kept rows, sequences)
@@ -361,22 +400,30 @@ extern "C" int attn_kv_evict(const AttnKvEvictArgs* a, void* stream_v) {
     while (cl < 8 && a->rows > cl * 2048ull) cl *= 2;
     const uint64_t slice = (a->rows + cl - 1) / cl + 32 * kSelWarps;
     p.staged = static_cast<uint32_t>(slice < 40 * 1024 ? slice : 40 * 1024);
-    B200_CUDA_TRY(allow_max_smem(evict_select_kernel));
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(cl, static_cast<uint32_t>(segments));
-    cfg.blockDim = dim3(kSelThreads);
-    cfg.dynamicSmemBytes = (kSelWords + p.staged) * sizeof(uint32_t);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cl;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, evict_select_kernel, p));
-    g_launch_count.fetch_add(1, std::memory_order_relaxed);
+    auto select = [&](auto kernel) -> int {
+        B200_CUDA_TRY(allow_max_smem(kernel));
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(cl, static_cast<uint32_t>(segments));
+        cfg.blockDim = dim3(kSelThreads);
+        cfg.dynamicSmemBytes = (kSelWords + p.staged) * sizeof(uint32_t);
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = cl;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 2;
+        B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, p));
+        g_launch_count.fetch_add(1, std::memory_order_relaxed);
+        return ATTN_OK;
+    };
+    const int selected = cl == 1   ? select(evict_select_kernel<1>)
+                         : cl == 2 ? select(evict_select_kernel<2>)
+                         : cl == 4 ? select(evict_select_kernel<4>)
+                                   : select(evict_select_kernel<8>);
+    if (selected != ATTN_OK) return selected;
 
     // ---- the copy
     if (p.in_place) {

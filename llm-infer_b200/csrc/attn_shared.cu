@@ -12,7 +12,7 @@
 //           copies; four warps multiply by mma.sync (16 query rows x 16 keys x 8 at a time). A warp owns 16 query rows of one
 //           kv head and a share of the tile's keys: with few query rows the four warps take four heads (whose slices of a cache row
 //           are contiguous) or four shares of the keys, with many rows of the prefix product four blocks of 16 rows.
-//   merge   one CTA per output row folds that row's pieces; further CTAs turn the scaled scores that the split pass left
+//   merge   one CTA per output row (or slice of it) folds that row's pieces; further CTAs turn the scaled scores that the split pass left
 //           in the workspace into weights (exp2(s - LSE)), sum them over the heads and add them to the accumulators.
 // The scores of own rows cost 4 bytes per query head and row each way through L2, next to 4 * head_dim bytes of K and V per kv head.
 // P enters the second product rounded once to the caches' type when the output is 16 bits wide too (an error below the
@@ -68,10 +68,8 @@ struct SharedParams {
     const float* scores;
     float* scores_out;
     uint64_t score_stride, score_out_stride;
-    uint32_t out_ctas, score_chunks;
+    uint32_t out_ctas, score_chunks, score_rows;  // score_rows: of a CTA that adds up weights
 };
-
-constexpr uint32_t kScoreRows = 1024;  // rows of a CTA that adds up weights
 
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;
@@ -423,55 +421,72 @@ __device__ __forceinline__ void find_pieces(const SharedParams& p, uint32_t b, u
     x.lse[1] = p.lse_own + at;
 }
 
-template <int D>
+// Output CTAs: one per (query row, slice of SLICE floats). Groups of SLICE / 4 lanes take a piece each, several pieces in flight per
+// lane; the groups' results merge by shuffles, then over the warps. Score CTAs behind them.
+template <int D, int SLICE>
 __global__ void __launch_bounds__(kThreads) shared_merge_kernel(const __grid_constant__ SharedParams p) {
-    constexpr int kPer = D / 32;  // floats of a lane
-    __shared__ float s_o[4][D];
+    constexpr int kLanes = SLICE / 4;           // of a group
+    constexpr int kGroups = kThreads / kLanes;  // pieces at once
+    __shared__ __align__(16) float s_o[4][SLICE];
     __shared__ float s_ml[4][2];
     __shared__ float s_lse[64];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     grid_dep_wait();
     if (blockIdx.x < p.out_ctas) {
-        const uint32_t b = blockIdx.x / p.n_heads, h = blockIdx.x - b * p.n_heads;
+        const uint32_t row = blockIdx.x / (D / SLICE), slice = blockIdx.x % (D / SLICE);
+        const uint32_t b = row / p.n_heads, h = row - b * p.n_heads;
         Pieces x;
         find_pieces<D>(p, b, h, x);
-        float m = -INFINITY, l = 0.f, acc[kPer] = {};
+        const int in_group = lane % kLanes, group = tid / kLanes;
+        float m = -INFINITY, l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto fold = [&](float mo, float lo, float4 v) {  // another state: maximum, sum, weighted sum
+            const float mn = fmaxf(m, mo), safe = mn == -INFINITY ? 0.f : mn;
+            const float f = fast_exp2(m - safe), w = fast_exp2(mo - safe);
+            l = l * f + lo * w;
+            acc.x = acc.x * f + v.x * w;
+            acc.y = acc.y * f + v.y * w;
+            acc.z = acc.z * f + v.z * w;
+            acc.w = acc.w * f + v.w * w;
+            m = mn;
+        };
 #pragma unroll
         for (int kind = 0; kind < 2; ++kind) {
             constexpr int kAhead = 4;
-            for (uint32_t i0 = warp; i0 < x.count[kind]; i0 += 4 * kAhead) {
-                float ls[kAhead], v[kAhead][kPer];
+            for (uint32_t i0 = group; i0 < x.count[kind]; i0 += kGroups * kAhead) {
+                float ls[kAhead];
+                float4 v[kAhead];
 #pragma unroll
                 for (int a = 0; a < kAhead; ++a) {
-                    const uint32_t i = i0 + 4 * a;
+                    const uint32_t i = i0 + a * kGroups;
                     ls[a] = -INFINITY;
+                    v[a] = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (i < x.count[kind]) {
                         ls[a] = x.lse[kind][i * x.step[kind]];
-                        const float* src = x.o[kind] + i * x.step[kind] * D + lane * kPer;
-#pragma unroll
-                        for (int c = 0; c < kPer; ++c) v[a][c] = src[c];
+                        v[a] = *reinterpret_cast<const float4*>(x.o[kind] + i * x.step[kind] * D + slice * SLICE + in_group * 4);
                     }
                 }
 #pragma unroll
-                for (int a = 0; a < kAhead; ++a) {
-                    if (ls[a] == -INFINITY) continue;
-                    const float mn = fmaxf(m, ls[a]);
-                    const float f = fast_exp2(m - mn), w = fast_exp2(ls[a] - mn);
-                    l = l * f + w;
-#pragma unroll
-                    for (int c = 0; c < kPer; ++c) acc[c] = acc[c] * f + w * v[a][c];
-                    m = mn;
-                }
+                for (int a = 0; a < kAhead; ++a) fold(ls[a], 1.f, v[a]);
             }
         }
 #pragma unroll
-        for (int c = 0; c < kPer; ++c) s_o[warp][lane * kPer + c] = acc[c];
+        for (int d = kLanes; d < 32; d *= 2) {
+            const float mo = __shfl_xor_sync(0xffffffffu, m, d), lo = __shfl_xor_sync(0xffffffffu, l, d);
+            float4 v;
+            v.x = __shfl_xor_sync(0xffffffffu, acc.x, d);
+            v.y = __shfl_xor_sync(0xffffffffu, acc.y, d);
+            v.z = __shfl_xor_sync(0xffffffffu, acc.z, d);
+            v.w = __shfl_xor_sync(0xffffffffu, acc.w, d);
+            fold(mo, lo, v);
+        }
+        if (lane < kLanes) *reinterpret_cast<float4*>(&s_o[warp][lane * 4]) = acc;
         if (lane == 0) {
             s_ml[warp][0] = m;
             s_ml[warp][1] = l;
         }
         __syncthreads();
-        if (tid < D) {
+        if (tid < SLICE) {
             const float mm = fmaxf(fmaxf(s_ml[0][0], s_ml[1][0]), fmaxf(s_ml[2][0], s_ml[3][0]));
             const float safe = mm == -INFINITY ? 0.f : mm;
             float sum = 0.f, val = 0.f;
@@ -482,11 +497,11 @@ __global__ void __launch_bounds__(kThreads) shared_merge_kernel(const __grid_con
                 val += f * s_o[w][tid];
             }
             val = sum > 0.f ? val / sum : 0.f;
-            const size_t at = static_cast<size_t>(blockIdx.x) * D + tid;
+            const size_t at = static_cast<size_t>(row) * D + slice * SLICE + tid;
             if (p.o_dtype == ATTN_DTYPE_F32) static_cast<float*>(p.o)[at] = val;
             else if (p.o_dtype == ATTN_DTYPE_F16) static_cast<__half*>(p.o)[at] = __float2half_rn(val);
             else static_cast<__nv_bfloat16*>(p.o)[at] = __float2bfloat16_rn(val);
-            if (tid == 0 && p.lse) p.lse[blockIdx.x] = sum > 0.f ? (mm + __log2f(sum)) * 0.69314718055994531f : -INFINITY;
+            if (tid == 0 && slice == 0 && p.lse) p.lse[row] = sum > 0.f ? (mm + __log2f(sum)) * 0.69314718055994531f : -INFINITY;
         }
         return;
     }
@@ -495,36 +510,48 @@ __global__ void __launch_bounds__(kThreads) shared_merge_kernel(const __grid_con
     const uint32_t seg = idx / p.score_chunks, chunk = idx - seg * p.score_chunks;
     const uint32_t b = seg / p.n_kv_heads, kvh = seg - b * p.n_kv_heads;
     const uint32_t len = own_len(p, b);
-    const uint32_t begin = chunk * kScoreRows, end = min(len, begin + kScoreRows);
+    const uint32_t begin = chunk * p.score_rows, end = min(len, begin + p.score_rows);
     if (begin >= end) return;
-    for (uint32_t g = warp; g < p.group; g += 4) {
-        Pieces x;
-        find_pieces<D>(p, b, kvh * p.group + g, x);
+    // the heads' log-sum-exps: eight lanes a head
+    for (uint32_t g0 = 0; g0 < p.group; g0 += kThreads / 8) {
+        const uint32_t g = g0 + tid / 8;
         float m = -INFINITY, l = 0.f;
+        if (g < p.group) {
+            Pieces x;
+            find_pieces<D>(p, b, kvh * p.group + g, x);
 #pragma unroll
-        for (int kind = 0; kind < 2; ++kind)
-            for (uint32_t i = lane; i < x.count[kind]; i += 32) {
-                const float ls = x.lse[kind][i * x.step[kind]];
-                if (ls == -INFINITY) continue;
-                const float mn = fmaxf(m, ls);
-                l = l * fast_exp2(m - mn) + fast_exp2(ls - mn);
-                m = mn;
+            for (int kind = 0; kind < 2; ++kind) {
+                constexpr int kAhead = 4;
+                for (uint32_t i0 = tid & 7; i0 < x.count[kind]; i0 += 8 * kAhead) {
+                    float ls[kAhead];
+#pragma unroll
+                    for (int a = 0; a < kAhead; ++a) {
+                        const uint32_t i = i0 + 8 * a;
+                        ls[a] = i < x.count[kind] ? x.lse[kind][i * x.step[kind]] : -INFINITY;
+                    }
+                    const float mn = fmaxf(fmaxf(fmaxf(ls[0], ls[1]), fmaxf(ls[2], ls[3])), m), safe = mn == -INFINITY ? 0.f : mn;
+                    l = l * fast_exp2(m - safe) + fast_exp2(ls[0] - safe) + fast_exp2(ls[1] - safe) + fast_exp2(ls[2] - safe) +
+                        fast_exp2(ls[3] - safe);
+                    m = mn;
+                }
             }
+        }
 #pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
+        for (int d = 1; d < 8; d *= 2) {
             const float om = __shfl_xor_sync(0xffffffffu, m, d), ol = __shfl_xor_sync(0xffffffffu, l, d);
             const float mn = fmaxf(m, om), safe = mn == -INFINITY ? 0.f : mn;
             l = l * fast_exp2(m - safe) + ol * fast_exp2(om - safe);
             m = mn;
         }
-        if (lane == 0) s_lse[g] = m + __log2f(l);
+        if ((tid & 7) == 0 && g < p.group) s_lse[g] = m + __log2f(l);
     }
     __syncthreads();
     const float* raw = p.raw + (static_cast<size_t>(b) * p.n_heads + kvh * p.group) * p.raw_stride;
     for (uint32_t t = begin + tid; t < end; t += kThreads) {
-        float w = 0.f;
-        for (uint32_t g = 0; g < p.group; ++g) w += fast_exp2(raw[g * p.raw_stride + t] - s_lse[g]);
         const float before = p.scores ? p.scores[seg * p.score_stride + t] : 0.f;
+        float w = 0.f;
+#pragma unroll 8
+        for (uint32_t g = 0; g < p.group; ++g) w += fast_exp2(raw[g * p.raw_stride + t] - s_lse[g]);
         p.scores_out[seg * p.score_out_stride + t] = before + w;
     }
 }
@@ -656,9 +683,16 @@ extern "C" int attn_decode_shared(const AttnDecodeSharedArgs* a, void* stream_v)
     p.o_dtype = a->o_dtype;
     p.scores = a->scores;
     p.scores_out = a->scores_out;
-    p.out_ctas = a->batch * a->n_heads;
-    p.score_chunks = (a->kv_capacity + kScoreRows - 1) / kScoreRows;
-    const uint64_t merge_ctas = p.out_ctas + (scored ? static_cast<uint64_t>(a->batch) * a->n_kv_heads * p.score_chunks : 0);
+    // Few output rows: slices of 32 floats, so that more CTAs take fewer pieces each.
+    const uint64_t rows = static_cast<uint64_t>(a->batch) * a->n_heads;
+    const bool sliced = rows * (a->head_dim / 32) <= 8ull * dev.sm_count;
+    p.out_ctas = static_cast<uint32_t>(sliced ? rows * (a->head_dim / 32) : rows);
+    // A CTA adds up the weights of 128 rows or a multiple of it, so that there are about eight CTAs per SM.
+    const uint64_t segs = static_cast<uint64_t>(a->batch) * a->n_kv_heads;
+    const uint64_t per_cta = (segs * a->kv_capacity + 8ull * dev.sm_count - 1) / (8ull * dev.sm_count);
+    p.score_rows = static_cast<uint32_t>(std::max<uint64_t>(1, (per_cta + kThreads - 1) / kThreads)) * kThreads;
+    p.score_chunks = (a->kv_capacity + p.score_rows - 1) / p.score_rows;
+    const uint64_t merge_ctas = p.out_ctas + (scored ? segs * p.score_chunks : 0);
     if (merge_ctas > 0x7fffffffull) return ATTN_ERR_UNSUPPORTED;
 
     cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
@@ -685,5 +719,6 @@ extern "C" int attn_decode_shared(const AttnDecodeSharedArgs* a, void* stream_v)
         g_launch_count.fetch_add(1, std::memory_order_relaxed);
         return ATTN_OK;
     };
-    return a->head_dim == 128 ? merge(shared_merge_kernel<128>) : merge(shared_merge_kernel<64>);
+    if (sliced) return a->head_dim == 128 ? merge(shared_merge_kernel<128, 32>) : merge(shared_merge_kernel<64, 32>);
+    return a->head_dim == 128 ? merge(shared_merge_kernel<128, 128>) : merge(shared_merge_kernel<64, 64>);
 }
