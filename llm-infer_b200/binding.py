@@ -481,13 +481,13 @@ def load() -> C.CDLL:
     lib.attn_gather_rows.restype = C.c_int
     lib.attn_gather_rows.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.c_void_p]
     lib.attn_rope_positions.restype = C.c_int
-    lib.attn_rope_positions.argtypes = [C.POINTER(AttnRopePositionsArgs), C.c_void_p]
+    lib.attn_rope_positions.argtypes = [C.c_void_p, C.c_void_p]  # AttnRopePositionsArgs, by reference or packed
     lib.attn_decode_shared_workspace_bytes.restype = C.c_size_t
     lib.attn_decode_shared_workspace_bytes.argtypes = [C.c_uint32] * 5
     lib.attn_decode_shared.restype = C.c_int
-    lib.attn_decode_shared.argtypes = [C.POINTER(AttnDecodeSharedArgs), C.c_void_p]
+    lib.attn_decode_shared.argtypes = [C.c_void_p, C.c_void_p]  # AttnDecodeSharedArgs, by reference or packed
     lib.attn_kv_evict.restype = C.c_int
-    lib.attn_kv_evict.argtypes = [C.POINTER(AttnKvEvictArgs), C.c_void_p]
+    lib.attn_kv_evict.argtypes = [C.c_void_p, C.c_void_p]  # AttnKvEvictArgs, by reference or packed
     lib.attn_status_string.restype = C.c_char_p
     lib.attn_status_string.argtypes = [C.c_int]
     lib.attn_last_cuda_error.restype = C.c_int

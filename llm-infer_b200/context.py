@@ -8,13 +8,13 @@ them together.
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
+import struct
 
 import torch
 
 from . import binding as _b
-from .attention import _call, _dense, _dtype_code, _require_cuda
+from .attention import _DTYPES, _dense, _dtype_code
 
 _LAYOUTS = {"interleaved": _b.ROPE_INTERLEAVED, "half": _b.ROPE_HALF}
 _INDEX = (torch.int32, torch.uint32)
@@ -72,23 +72,50 @@ def rope_frequencies(rotary_dim: int, theta: float, scaling: dict | None = None)
     return freq.float(), attention
 
 
+# The argument structures as the library lays them out. Packing one takes about a microsecond, filling the ctypes mirror field by
+# field three, of the ten that a small call costs on the host.
+ROPE_ARGS = struct.Struct("@10P6Q7If4iP")
+SHARED_ARGS = struct.Struct("@7P2i6IPIf3Q2P2QPNP")
+EVICT_ARGS = struct.Struct("@9P8I6QP")
+
+
+def _enqueue(entry: str, index: int, stream, packed: bytes) -> None:
+    """attention._call for a packed argument structure."""
+    ptr = torch._C._cuda_getCurrentRawStream(index) if stream is None else stream.cuda_stream
+    fn = getattr(_b.load(), entry)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(packed, ptr)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(packed, ptr)
+    if rc:
+        _b.check(rc, entry)
+
+
+def _one_device(*tensors) -> int:
+    """The index of the device that all operands are on."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            index = -1
+    if index < 0:
+        raise ValueError("the operands must be CUDA tensors of one device (there is no CPU path)")
+    return index
+
+
 def _index(t, shape, what):
-    if t.dtype not in _INDEX or t.shape != shape or not t.is_cuda or not t.is_contiguous():
+    if t.dtype not in _INDEX or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{what} must be a dense 32-bit integer CUDA tensor of shape {tuple(shape)}")
     return t.data_ptr()
 
 
-def _same_device(device, *tensors):
-    for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError("all operands must be on one device")
-
-
-def _heads(t: torch.Tensor, stream, what: str) -> torch.Tensor:
-    """``t`` [tokens, heads, dim] with the heads of a token side by side (tokens may be strided), or a dense copy."""
-    if t.stride(2) == 1 and t.stride(1) == t.shape[2] and (t.shape[0] == 1 or t.stride(0) > 0):
-        return t
-    return _dense(t, stream, what)
+def _score_stride(t: torch.Tensor, batch: int, kv_heads: int, rows: int) -> int:
+    """Distance of the (sequence, kv head) runs of a [batch, kv_heads, rows] tensor of weights; 0 where there is one."""
+    stride = t.stride()
+    if t.dtype != torch.float32 or t.shape != (batch, kv_heads, rows) or (rows > 1 and stride[2] != 1) or \
+            (batch > 1 and kv_heads > 1 and stride[0] != kv_heads * stride[1]):
+        raise ValueError("scores must be fp32 [B, Hkv, rows] with dense rows at one distance")
+    return stride[1] if kv_heads > 1 else stride[0] if batch > 1 else 0
 
 
 def rope_positions(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -101,40 +128,51 @@ def rope_positions(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
     inv_freq fp32 [rotary_dim / 2] on the device and factor as rope_frequencies gives them, values behind rotary_dim are copied.
     layout "interleaved" pairs (2i, 2i + 1), "half" pairs (i, i + rotary_dim / 2). Returns the rotated q [N, H, D] (``q_out``, or a
     new tensor of q_out_dtype, default q's). A row that does not exist is not written and sets ATTN_STATUS_BAD_SHAPE in status."""
-    _require_cuda(q, k, v, k_cache, v_cache, pos, row, inv_freq, seq)
-    if q.dim() != 3 or k.dim() != 3 or k_cache.dim() != 4:
+    index = _one_device(q, k, v, k_cache, v_cache, pos, row, inv_freq, seq, q_out, status)
+    if q.dim() != 3 or k_cache.dim() != 4:
         raise ValueError("q must be [N, H, D], k and v [N, Hkv, D], the caches [B, T, Hkv, D]")
     N, H, D = q.shape
     B, T, Hkv, Dk = k_cache.shape
-    if k.shape != (N, Hkv, D) or v.shape != k.shape or Dk != D or v_cache.shape != k_cache.shape:
+    if k.shape != (N, Hkv, D) or v.shape != (N, Hkv, D) or Dk != D or v_cache.shape != (B, T, Hkv, D):
         raise ValueError("shape mismatch between q, k, v and the caches")
-    if not (q.dtype == k.dtype == v.dtype) or k_cache.dtype not in _CACHE or v_cache.dtype != k_cache.dtype:
+    dtype, cache_dtype = q.dtype, k_cache.dtype
+    if not (dtype == k.dtype == v.dtype) or cache_dtype not in _CACHE or v_cache.dtype != cache_dtype:
         raise TypeError("q, k, v must share a dtype, and the caches be both fp16 or both bf16")
-    if k_cache.stride() != v_cache.stride() or k_cache.stride(3) != 1 or k_cache.stride(2) != D:
+    c_stride = k_cache.stride()
+    if v_cache.stride() != c_stride or c_stride[3] != 1 or c_stride[2] != D:
         raise ValueError("the caches must be [B, row, kv_head, head_dim] with dense heads and share their strides")
     if layout not in _LAYOUTS:
         raise ValueError(f"layout must be one of {sorted(_LAYOUTS)}")
-    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or not 0 < 2 * inv_freq.numel() <= D:
+    half = inv_freq.numel()
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or not 0 < 2 * half <= D:
         raise ValueError("inv_freq must be a dense fp32 tensor of rotary_dim / 2 values, rotary_dim <= head_dim")
     if seq is None and N > B:
         raise ValueError("more tokens than sequences need seq")
-    _same_device(q.device, k, v, k_cache, v_cache, pos, row, inv_freq, seq, q_out, status)
     pos_ptr, row_ptr = _index(pos, (N,), "pos"), _index(row, (N,), "row")
-    seq_ptr = None if seq is None else _index(seq, (N,), "seq")
-    q, k, v = _heads(q, stream, "q"), _heads(k, stream, "k"), _heads(v, stream, "v")
+    seq_ptr = 0 if seq is None else _index(seq, (N,), "seq")
+    taken = []
+    for t, what in ((q, "q"), (k, "k"), (v, "v")):
+        stride = t.stride()
+        if stride[2] != 1 or stride[1] != D or (N > 1 and stride[0] <= 0):
+            t = _dense(t, stream, what)  # a token's heads must lie side by side; tokens may be strided
+            stride = t.stride()
+        taken += (t, stride[0] if N > 1 else 0)
+    q, q_stride, k, k_stride, v, v_stride = taken
+    out_stride = 0
     if q_out is None:
-        q_out = torch.empty((N, H, D), dtype=q_out_dtype or q.dtype, device=q.device)
-    elif q_out.shape != (N, H, D) or q_out.stride(2) != 1 or q_out.stride(1) != D or (N > 1 and q_out.stride(0) < H * D):
-        raise ValueError("q_out must be [N, H, D] with dense heads")
+        q_out = torch.empty((N, H, D), dtype=q_out_dtype or dtype, device=q.device)
+    else:
+        stride = q_out.stride()
+        if q_out.shape != (N, H, D) or stride[2] != 1 or stride[1] != D or (N > 1 and stride[0] < H * D):
+            raise ValueError("q_out must be [N, H, D] with dense heads")
+        out_stride = stride[0] if N > 1 else 0
     if N == 0:
         return q_out
-    a = _b.AttnRopePositionsArgs(
+    _enqueue("attn_rope_positions", index, stream, ROPE_ARGS.pack(
         q_out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), inv_freq.data_ptr(),
-        pos_ptr, row_ptr, seq_ptr, q.stride(0) if N > 1 else 0, k.stride(0) if N > 1 else 0, v.stride(0) if N > 1 else 0,
-        q_out.stride(0) if N > 1 else 0, k_cache.stride(1) if T > 1 else 0, k_cache.stride(0) if B > 1 else 0,
-        N, H, Hkv, D, 2 * inv_freq.numel(), B, T, float(factor), _dtype_code(q), _dtype_code(q_out), _dtype_code(k_cache),
-        _LAYOUTS[layout], status.data_ptr() if status is not None else None)
-    _call("attn_rope_positions", q.device, stream, C.byref(a))
+        pos_ptr, row_ptr, seq_ptr, q_stride, k_stride, v_stride, out_stride, c_stride[1] if T > 1 else 0, c_stride[0] if B > 1 else 0,
+        N, H, Hkv, D, 2 * half, B, T, factor, _DTYPES[dtype], _dtype_code(q_out), _DTYPES[cache_dtype], _LAYOUTS[layout],
+        0 if status is None else status.data_ptr()))
     return q_out
 
 
@@ -154,6 +192,7 @@ class SharedWorkspace:
         self.nbytes = int(nbytes)
         self.buf = torch.empty(self.nbytes, dtype=torch.uint8, device=device)
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
+        self.ptr, self.status_ptr = self.buf.data_ptr(), self.status.data_ptr()
 
 
 def attn_decode_shared(q: torch.Tensor, k_prefix, v_prefix, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_len=None, *,
@@ -169,32 +208,35 @@ def attn_decode_shared(q: torch.Tensor, k_prefix, v_prefix, k_cache: torch.Tenso
                rows (default: scores itself, in place). scores_out alone starts from zero
     returns    out [B, H, D] in out_dtype (q's type, the default, or fp32); fills ``lse`` [B, H] (fp32) when given
     """
-    _require_cuda(q, k_prefix, v_prefix, k_cache, v_cache, out, lse, scores, scores_out)
+    index = _one_device(q, k_prefix, v_prefix, k_cache, v_cache, kv_len if isinstance(kv_len, torch.Tensor) else None, out, lse, scores,
+                        scores_out)
     if q.dim() != 3 or k_cache.dim() != 4:
         raise ValueError("q must be [B, H, D] and the caches [B, T, Hkv, D]")
     B, H, D = q.shape
     Bk, T, Hkv, Dk = k_cache.shape
-    if (Bk, Dk) != (B, D) or v_cache.shape != k_cache.shape or Hkv == 0 or H % Hkv:
+    if Bk != B or Dk != D or v_cache.shape != (B, T, Hkv, D) or Hkv == 0 or H % Hkv:
         raise ValueError("shape mismatch between q and the caches")
-    if q.dtype not in _CACHE or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+    dtype = q.dtype
+    if dtype not in _CACHE or k_cache.dtype != dtype or v_cache.dtype != dtype:
         raise TypeError("q and the caches must be fp16 or bf16, of one type")
-    if k_cache.stride() != v_cache.stride() or (T and (k_cache.stride(3) != 1 or k_cache.stride(2) != D)):
+    stride = k_cache.stride()
+    if v_cache.stride() != stride or (T and (stride[3] != 1 or stride[2] != D)):
         raise ValueError("the caches must be [B, row, kv_head, head_dim] with dense heads and share their strides")
-    _same_device(q.device, k_prefix, v_prefix, k_cache, v_cache, out, lse, scores, scores_out)
-    P, kp, vp, prefix_stride = 0, None, None, 0
+    P = kp = vp = prefix_stride = 0
     if (k_prefix is None) != (v_prefix is None):
         raise ValueError("k_prefix without v_prefix")
     if k_prefix is not None:
         if k_prefix.dim() != 3 or k_prefix.shape[1:] != (Hkv, D) or v_prefix.shape != k_prefix.shape:
             raise ValueError("the prefix must be [P, Hkv, D]")
-        if k_prefix.dtype != q.dtype or v_prefix.dtype != q.dtype:
+        if k_prefix.dtype != dtype or v_prefix.dtype != dtype:
             raise TypeError("the prefix must have q's type")
         P = k_prefix.shape[0]
         if P:
-            if k_prefix.stride() != v_prefix.stride() or k_prefix.stride(2) != 1 or k_prefix.stride(1) != D:
+            p_stride = k_prefix.stride()
+            if v_prefix.stride() != p_stride or p_stride[2] != 1 or p_stride[1] != D:
                 raise ValueError("the prefix must be [row, kv_head, head_dim] with dense heads; K and V share their strides")
-            kp, vp, prefix_stride = k_prefix.data_ptr(), v_prefix.data_ptr(), k_prefix.stride(0) if P > 1 else 0
-    len_ptr, uniform = None, T
+            kp, vp, prefix_stride = k_prefix.data_ptr(), v_prefix.data_ptr(), p_stride[0] if P > 1 else 0
+    len_ptr, uniform = 0, T
     if isinstance(kv_len, int):
         if not 0 <= kv_len <= T:
             raise ValueError("kv_len exceeds the cache")
@@ -203,35 +245,34 @@ def attn_decode_shared(q: torch.Tensor, k_prefix, v_prefix, k_cache: torch.Tenso
         len_ptr = _index(kv_len, (B,), "kv_len")
     if scores is not None and scores_out is None:
         scores_out = scores
-    for t in (scores, scores_out):
-        if t is not None and (t.dtype != torch.float32 or t.shape != (B, Hkv, T) or (T > 1 and t.stride(2) != 1) or
-                              (B > 1 and t.stride(0) != Hkv * t.stride(1))):
-            raise ValueError("scores must be fp32 [B, Hkv, T] with dense rows at one distance")
-    if T == 0:
-        scores = scores_out = None  # no rows: nothing to add up
-    q = _dense(q, stream, "q")
+    scores_ptr = scores_out_ptr = score_stride = score_out_stride = 0
+    if scores_out is not None:
+        score_out_stride = _score_stride(scores_out, B, Hkv, T)
+        if scores is not None:
+            score_stride = _score_stride(scores, B, Hkv, T)
+        if T:  # (without rows there is nothing to add up)
+            scores_out_ptr, scores_ptr = scores_out.data_ptr(), 0 if scores is None else scores.data_ptr()
+    if not q.is_contiguous():
+        q = _dense(q, stream, "q")
     if out is None:
-        out = torch.empty((B, H, D), dtype=out_dtype or q.dtype, device=q.device)
+        out = torch.empty((B, H, D), dtype=out_dtype or dtype, device=q.device)
     elif out.shape != (B, H, D) or not out.is_contiguous():
         raise ValueError("out must be a contiguous [B, H, D] tensor")
-    if out.dtype not in (q.dtype, torch.float32):
+    o_dtype = out.dtype
+    if o_dtype != dtype and o_dtype != torch.float32:
         raise TypeError("out must have q's type or be fp32")
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (B, H) or not lse.is_contiguous()):
         raise ValueError("lse must be a contiguous fp32 [B, H] tensor")
     if B == 0:
         return out
-    need_rows = T if scores_out is not None else 0
-    if workspace is None or workspace.key != (B, H, Hkv, D, q.device.index) or workspace.rows < need_rows:
+    need_rows = T if scores_out_ptr else 0
+    if workspace is None or workspace.key != (B, H, Hkv, D, index) or workspace.rows < need_rows:
         workspace = SharedWorkspace(B, H, Hkv, D, need_rows, q.device)
-    a = _b.AttnDecodeSharedArgs(
-        out.data_ptr(), q.data_ptr(), kp, vp, k_cache.data_ptr() if T else None, v_cache.data_ptr() if T else None,
-        lse.data_ptr() if lse is not None else None, _dtype_code(out), _dtype_code(q), B, H, Hkv, D, P, T, len_ptr, uniform,
-        float(scale), prefix_stride, k_cache.stride(1) if T > 1 else 0, k_cache.stride(0) if B > 1 else 0,
-        scores.data_ptr() if scores is not None else None, scores_out.data_ptr() if scores_out is not None else None,
-        scores.stride(1) if scores is not None and B * Hkv > 1 else 0,
-        scores_out.stride(1) if scores_out is not None and B * Hkv > 1 else 0, workspace.buf.data_ptr(), workspace.nbytes,
-        workspace.status.data_ptr())
-    _call("attn_decode_shared", q.device, stream, C.byref(a))
+    _enqueue("attn_decode_shared", index, stream, SHARED_ARGS.pack(
+        out.data_ptr(), q.data_ptr(), kp, vp, k_cache.data_ptr() if T else 0, v_cache.data_ptr() if T else 0,
+        0 if lse is None else lse.data_ptr(), _DTYPES[o_dtype], _DTYPES[dtype], B, H, Hkv, D, P, T, len_ptr, uniform,
+        scale, prefix_stride, stride[1] if T > 1 else 0, stride[0] if B > 1 else 0, scores_ptr, scores_out_ptr, score_stride,
+        score_out_stride, workspace.ptr, workspace.nbytes, workspace.status_ptr))
     return out
 
 
@@ -246,22 +287,23 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor,
     Returns (kept [B, Hkv, keep] int32: the source row of each kept row, -1 behind the new length; kv_len_out [B] int32:
     min(length, keep); it may be given as kv_len itself)."""
     k_out, v_out, scores_out = (k_cache, v_cache, scores) if out is None else out
-    _require_cuda(k_cache, v_cache, scores, k_out, v_out, scores_out, kv_len, kept, kv_len_out)
+    index = _one_device(k_cache, v_cache, scores, k_out, v_out, scores_out, kv_len, kept, kv_len_out, status)
     if k_cache.dim() != 4 or k_out.dim() != 4:
         raise ValueError("the caches must be [B, T, Hkv, D]")
     B, T, Hkv, D = k_cache.shape
     T2 = k_out.shape[1]
+    dtype = k_cache.dtype
+    strides = []
     for a, b, n in ((k_cache, v_cache, T), (k_out, v_out, T2)):
-        if a.shape != (B, n, Hkv, D) or b.shape != a.shape or a.stride() != b.stride() or a.stride(3) != 1 or a.stride(2) != D:
+        stride = a.stride()
+        if a.shape != (B, n, Hkv, D) or b.shape != (B, n, Hkv, D) or b.stride() != stride or stride[3] != 1 or stride[2] != D:
             raise ValueError("the caches must be [B, row, kv_head, head_dim] with dense heads; K and V share their strides")
-        if a.dtype not in _CACHE or b.dtype != a.dtype or a.dtype != k_cache.dtype:
+        if dtype not in _CACHE or a.dtype != dtype or b.dtype != dtype:
             raise TypeError("the caches must be fp16 or bf16, of one type")
-    for t, n in ((scores, T), (scores_out, T2)):
-        if t.dtype != torch.float32 or t.shape != (B, Hkv, n) or (n > 1 and t.stride(2) != 1) or (B > 1 and t.stride(0) != Hkv * t.stride(1)):
-            raise ValueError("scores must be fp32 [B, Hkv, rows] with dense rows at one distance")
+        strides.append(stride)
+    score_stride, score_out_stride = _score_stride(scores, B, Hkv, T), _score_stride(scores_out, B, Hkv, T2)
     if keep < 1 or keep > T2 or sink < 0 or recent < 0 or sink + recent > keep:
         raise ValueError("keep must be at least 1, fit the output caches and hold the sink and the recent rows")
-    _same_device(k_cache.device, v_cache, scores, k_out, v_out, scores_out, kv_len, kept, kv_len_out, status)
     if kept is None:
         kept = torch.empty((B, Hkv, keep), dtype=torch.int32, device=k_cache.device)
     kept_ptr = _index(kept, (B, Hkv, keep), "kept")
@@ -270,11 +312,10 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor,
     len_out_ptr = _index(kv_len_out, (B,), "kv_len_out")
     if B == 0:
         return kept, kv_len_out
-    a = _b.AttnKvEvictArgs(
+    s_in, s_out = strides
+    _enqueue("attn_kv_evict", index, stream, EVICT_ARGS.pack(
         k_cache.data_ptr(), v_cache.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), scores.data_ptr(), scores_out.data_ptr(), kept_ptr,
-        _index(kv_len, (B,), "kv_len") if kv_len is not None else None, len_out_ptr, B, Hkv, D, T, T2, keep, sink, recent,
-        k_cache.stride(1) if T > 1 else 0, k_out.stride(1) if T2 > 1 else 0, k_cache.stride(0) if B > 1 else 0,
-        k_out.stride(0) if B > 1 else 0, scores.stride(1) if B * Hkv > 1 else 0, scores_out.stride(1) if B * Hkv > 1 else 0,
-        status.data_ptr() if status is not None else None)
-    _call("attn_kv_evict", k_cache.device, stream, C.byref(a))
+        0 if kv_len is None else _index(kv_len, (B,), "kv_len"), len_out_ptr, B, Hkv, D, T, T2, keep, sink, recent,
+        s_in[1] if T > 1 else 0, s_out[1] if T2 > 1 else 0, s_in[0] if B > 1 else 0, s_out[0] if B > 1 else 0, score_stride,
+        score_out_stride, 0 if status is None else status.data_ptr()))
     return kept, kv_len_out

@@ -130,3 +130,13 @@ def test_the_mirrors_of_the_argument_structures_have_the_librarys_sizes(built_li
     b = pkg.binding
     for index, mirror in ((10, b.AttnRopePositionsArgs), (11, b.AttnDecodeSharedArgs), (12, b.AttnKvEvictArgs)):
         assert built_lib.attn_abi_struct_size(index) == C.sizeof(mirror)
+
+
+def test_packed_arguments_lie_where_the_mirrors_have_them(ctx, pkg):
+    b = pkg.binding
+    for packer, mirror in ((ctx.ROPE_ARGS, b.AttnRopePositionsArgs), (ctx.SHARED_ARGS, b.AttnDecodeSharedArgs), (ctx.EVICT_ARGS, b.AttnKvEvictArgs)):
+        assert packer.size == C.sizeof(mirror)
+        fields = mirror._fields_
+        values = [float(i + 1) if kind is C.c_float else i + 1 for i, (_, kind) in enumerate(fields)]
+        got = mirror.from_buffer_copy(packer.pack(*values))
+        assert [getattr(got, name) for name, _ in fields] == values
