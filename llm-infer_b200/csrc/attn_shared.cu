@@ -18,6 +18,7 @@
 // P enters the second product rounded once to the caches' type when the output is 16 bits wide too (an error below the
 // output's own rounding), and as value + rounding residual for fp32 outputs.
 #include <algorithm>
+#include <cstdlib>
 
 #include "attn_internal.cuh"
 #include "ptx_sm100.cuh"
@@ -51,13 +52,14 @@ struct SharedParams {
     float scale_log2;
     Shape pre, own;
     uint32_t row_blocks;    // blocks of 16 * pre.wm query rows against the prefix
-    uint32_t prefix_segs;   // pre.groups * row_blocks
+    uint32_t prefix_segs;   // pre.groups * row_blocks; 0 in the split pass when another kernel takes the prefix
     uint32_t prefix_tiles;  // of one such segment
     float* part_pre;        // [(grid + prefix_segs) * ts * hpc][rec_rows][D]
     float* lse_pre;
     float* part_own;        // [(grid + batch * groups) * ts * hpc][rec_rows][D]
     float* lse_own;
-    uint32_t* seg_ctas;     // [prefix_segs + batch * own.groups]
+    uint32_t* seg_pre;      // [prefix_segs] segment_ctas() words
+    uint32_t* seg_own;      // [batch * own.groups]
     float* raw;             // [batch][n_heads][raw_stride] scaled scores in log2 units, or null
     uint64_t raw_stride;
     uint32_t* status;
@@ -151,7 +153,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_split_kernel(const __grid_
             n = s_cum[b + 1] - s_cum[b];
             first = pre_total + s_cum[b] * p.own.groups + hg * n;
         }
-        p.seg_ctas[s] = segment_ctas(first, static_cast<uint64_t>(first) + n, total, active);
+        (s < p.prefix_segs ? p.seg_pre[s] : p.seg_own[s - p.prefix_segs]) = segment_ctas(first, static_cast<uint64_t>(first) + n, total, active);
     }
     if (blockIdx.x >= active) return;
     const uint32_t t0 = static_cast<uint32_t>(static_cast<uint64_t>(blockIdx.x) * total / active);
@@ -404,7 +406,7 @@ __device__ __forceinline__ void find_pieces(const SharedParams& p, uint32_t b, u
         const Shape& sh = p.pre;
         const uint32_t row = b * p.group + g, rb = row / sh.rec_rows, r = row - rb * sh.rec_rows;
         const uint32_t hg = kvh / sh.hpc, hs = kvh - hg * sh.hpc, seg = hg * p.row_blocks + rb;
-        const uint32_t w = p.seg_ctas[seg];
+        const uint32_t w = p.seg_pre[seg];
         const uint64_t at = (static_cast<uint64_t>((w & 0xffffu) + seg) * sh.ts * sh.hpc + hs) * sh.rec_rows + r;
         x.step[0] = static_cast<uint64_t>(sh.hpc) * sh.rec_rows;
         x.count[0] = (w >> 16) * sh.ts;
@@ -413,7 +415,7 @@ __device__ __forceinline__ void find_pieces(const SharedParams& p, uint32_t b, u
     }
     const Shape& sh = p.own;
     const uint32_t hg = kvh / sh.hpc, hs = kvh - hg * sh.hpc, seg = b * sh.groups + hg;
-    const uint32_t w = p.seg_ctas[p.prefix_segs + seg];
+    const uint32_t w = p.seg_own[seg];
     const uint64_t at = (static_cast<uint64_t>((w & 0xffffu) + seg) * sh.ts * sh.hpc + hs) * sh.rec_rows + g;
     x.step[1] = static_cast<uint64_t>(sh.hpc) * sh.rec_rows;
     x.count[1] = (w >> 16) * sh.ts;
@@ -562,7 +564,8 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 struct SharedPlan {
     Shape pre, own;
     uint32_t row_blocks, prefix_segs, own_segs, grid;
-    size_t lse_pre, part_own, lse_own, seg_ctas, raw, words;
+    uint32_t pairs, tensor_segs, tensor_grid;  // the prefix on the tensor cores
+    size_t lse_pre, part_own, lse_own, seg_pre, seg_own, raw, words;
     uint64_t raw_stride;
 };
 void set_shape(Shape* s, uint32_t query_rows, uint32_t n_kv_heads) {
@@ -587,17 +590,31 @@ int make_shared_plan(uint32_t batch, uint32_t n_heads, uint32_t n_kv_heads, uint
     s.prefix_segs = s.pre.groups * s.row_blocks;
     s.own_segs = batch * s.own.groups;
     s.grid = 2 * dev.sm_count;
-    const size_t pre_rows = static_cast<size_t>(s.grid + s.prefix_segs) * s.pre.ts * s.pre.hpc * s.pre.rec_rows;
+    s.pairs = (batch * group + kPrefixRows - 1) / kPrefixRows;
+    s.tensor_segs = s.pairs * n_kv_heads;
+    s.tensor_grid = dev.sm_count;
+    const size_t pre_rows = std::max(static_cast<size_t>(s.grid + s.prefix_segs) * s.pre.ts * s.pre.hpc * s.pre.rec_rows,
+                                     static_cast<size_t>(s.tensor_grid + s.tensor_segs) * kPrefixRows);
     const size_t own_rows = static_cast<size_t>(s.grid + s.own_segs) * s.own.ts * s.own.hpc * s.own.rec_rows;
     auto round4 = [](size_t n) { return (n + 3) / 4 * 4; };
     s.lse_pre = pre_rows * head_dim;
     s.part_own = s.lse_pre + round4(pre_rows);
     s.lse_own = s.part_own + own_rows * head_dim;
-    s.seg_ctas = s.lse_own + round4(own_rows);
-    s.raw = s.seg_ctas + round4(s.prefix_segs + s.own_segs);
+    s.seg_pre = s.lse_own + round4(own_rows);
+    s.seg_own = s.seg_pre + round4(std::max(s.prefix_segs, s.tensor_segs));
+    s.raw = s.seg_own + round4(s.own_segs);
     s.raw_stride = (static_cast<uint64_t>(scored_rows) + 63) / 64 * 64;
     s.words = s.raw + static_cast<size_t>(batch) * n_heads * s.raw_stride;
     return ATTN_OK;
+}
+
+// Whether the prefix goes to the tensor-core kernel, by query rows per kv head and key blocks in all.
+constexpr uint32_t kMinPrefixBlocks = 2;  // of a CTA
+bool prefix_on_tensor_cores(uint32_t prefix, uint32_t query_rows, uint64_t blocks) {
+#ifdef ATTN_TRACE
+    if (const char* e = getenv("ATTN_TRACE_PREFIX")) return prefix > 0 && atoi(e) != 0;  // profiling knob
+#endif
+    return prefix > 0 && query_rows > 16 && blocks >= 64;
 }
 
 }  // namespace
@@ -674,7 +691,8 @@ extern "C" int attn_decode_shared(const AttnDecodeSharedArgs* a, void* stream_v)
     p.lse_pre = ws + plan.lse_pre;
     p.part_own = ws + plan.part_own;
     p.lse_own = ws + plan.lse_own;
-    p.seg_ctas = reinterpret_cast<uint32_t*>(ws + plan.seg_ctas);
+    p.seg_pre = reinterpret_cast<uint32_t*>(ws + plan.seg_pre);
+    p.seg_own = reinterpret_cast<uint32_t*>(ws + plan.seg_own);
     p.raw = scored ? ws + plan.raw : nullptr;
     p.raw_stride = plan.raw_stride;
     p.status = a->status;
@@ -696,16 +714,48 @@ extern "C" int attn_decode_shared(const AttnDecodeSharedArgs* a, void* stream_v)
     if (merge_ctas > 0x7fffffffull) return ATTN_ERR_UNSUPPORTED;
 
     cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
-    const uint64_t most = prefix_tiles * p.prefix_segs + own_tiles * plan.own_segs;
+    const bool bf16 = a->dtype == ATTN_DTYPE_BF16, res = a->o_dtype == ATTN_DTYPE_F32;
+    const uint64_t blocks = (static_cast<uint64_t>(a->prefix_len) + kPrefixBlock - 1) / kPrefixBlock * plan.tensor_segs;
+    const bool tensor = prefix_on_tensor_cores(a->prefix_len, a->batch * p.group, blocks) && scale > 0.f && blocks <= 0x7fffffffull;
+    SharedParams in_split = p;
+    if (tensor) {
+        SharedPrefixParams t{};
+        t.q = a->q;
+        t.k = a->k_prefix;
+        t.v = a->v_prefix;
+        t.part = p.part_pre;
+        t.lse = p.lse_pre;
+        t.seg_ctas = p.seg_pre;
+        t.row_stride = p.prefix_row_stride;
+        t.batch = p.batch;
+        t.n_heads = p.n_heads;
+        t.n_kv_heads = p.n_kv_heads;
+        t.group = p.group;
+        t.head_dim = a->head_dim;
+        t.prefix = p.prefix;
+        t.pairs = plan.pairs;
+        t.segments = plan.tensor_segs;
+        t.grid = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(plan.tensor_grid, blocks / kMinPrefixBlocks)));
+        t.scale_log2 = p.scale_log2;
+        t.status = p.status;
+        t.bf16 = bf16;
+        t.residual = res;
+        if ((rc = launch_shared_prefix(t, stream)) != ATTN_OK) return rc;
+        in_split.prefix_segs = in_split.prefix_tiles = 0;
+        // how the merge pass finds the pieces: one record of 256 rows per CTA and segment
+        p.pre = Shape{1, 1, 1, kPrefixBlock, p.n_kv_heads, kPrefixRows};
+        p.row_blocks = plan.pairs;
+        p.prefix_segs = plan.tensor_segs;
+    }
+    const uint64_t most = prefix_tiles * in_split.prefix_segs + own_tiles * plan.own_segs;
     const uint32_t grid = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(plan.grid, most)));
     auto split = [&](auto kernel) -> int {
         B200_CUDA_TRY(allow_max_smem(kernel));
         const size_t smem = 96 * 1024 + (a->batch + 5) * 4;  // the ring, s_cum, s_warp
-        B200_CUDA_TRY(launch_dependent(kernel, dim3(grid), dim3(kThreads), smem, stream, p));
+        B200_CUDA_TRY(launch_dependent(kernel, dim3(grid), dim3(kThreads), smem, stream, in_split));
         g_launch_count.fetch_add(1, std::memory_order_relaxed);
         return ATTN_OK;
     };
-    const bool bf16 = a->dtype == ATTN_DTYPE_BF16, res = a->o_dtype == ATTN_DTYPE_F32;
     if (a->head_dim == 128) {
         rc = bf16 ? (res ? split(shared_split_kernel<128, true, true>) : split(shared_split_kernel<128, true, false>))
                   : (res ? split(shared_split_kernel<128, false, true>) : split(shared_split_kernel<128, false, false>));

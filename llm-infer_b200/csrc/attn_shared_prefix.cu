@@ -1,0 +1,461 @@
+// The shared prefix of a batch's decode step as a matrix product for each kv head, on the 5th-generation tensor cores
+// (tcgen05 + tensor memory): all B * G query rows of a kv head against the prefix's keys, cut over the GPU along the keys.
+//
+// Mathematics: for every query row the softmax-normalised sum over a run of keys and its log-sum-exp; the merge pass of
+// attn_shared.cu joins the runs (and the rows of the sequences' own caches) by weights exp(lse_i - LSE).
+//
+// Work: a segment is a kv head and two tiles of 128 query rows that share one K/V stream (a batch of up to 128 rows has one tile);
+// a segment has ceil(P / 64) blocks of 64 keys. The blocks of all segments form one list that is dealt to one CTA per SM in equal
+// contiguous runs; a CTA's part of a segment is one piece. The CTA's warps work as in the causal prefill: two softmax
+// warpgroups (a thread owns a query row, which is a tensor-memory lane), one thread that feeds K and V by TMA through a ring of
+// four stages, one thread that issues the MMAs, scores two blocks ahead of the products. Query rows of a kv head are not evenly
+// spaced (heads of one group, then the next sequence), so the softmax threads bring their own row into the swizzled tile.
+//
+// Bound by the K/V stream up to 128 rows (a block is 32 KB, 0.72 us of an SM's share of HBM; its scores take a warpgroup less),
+// by the exponentials and the MMAs' shared-memory reads from there on.
+// Every wait is bounded; on expiry the role records ATTN_STATUS_WAIT_TIMEOUT, stops, and the CTA still runs its common exit.
+#include <cuda.h>
+
+#include <algorithm>
+
+#include "attn_internal.cuh"
+#include "ptx_sm100.cuh"
+#include "tcgen05_sm100.cuh"
+#include "tma_tile.cuh"
+
+namespace b200 {
+namespace {
+
+using namespace tc;
+
+constexpr int BM = 128;  // query rows per tile
+constexpr int BN = 64;   // keys per block
+constexpr int kThreads = 384;
+constexpr uint32_t kSubTileBytes = BM * 64 * 2;     // [128 query rows][64 elements], 128-byte rows, swizzled
+constexpr uint32_t kTileBytes = 2 * kSubTileBytes;  // head_dim 128 (64 fills the first half)
+constexpr uint32_t kKvSubBytes = BN * 64 * 2;
+constexpr uint32_t kKvBytes = 2 * kKvSubBytes;
+constexpr int kStages = 4;
+constexpr uint32_t kTmemCols = 512;
+
+enum {
+    BAR_Q_FULL = 0,  // [tile]
+    BAR_K_FULL = 2,  // [kStages]
+    BAR_V_FULL = BAR_K_FULL + kStages,
+    BAR_K_EMPTY = BAR_V_FULL + kStages,
+    BAR_V_EMPTY = BAR_K_EMPTY + kStages,
+    BAR_S_FULL = BAR_V_EMPTY + kStages,  // [tile][block parity]: scores, probabilities, products of a block
+    BAR_P_FULL = BAR_S_FULL + 4,
+    BAR_O_DONE = BAR_P_FULL + 4,
+    BAR_COUNT = BAR_O_DONE + 4
+};
+
+constexpr uint32_t kSmemQ = 0;
+constexpr uint32_t kSmemK = kSmemQ + 2 * kTileBytes;
+constexpr uint32_t kSmemV = kSmemK + kStages * kKvBytes;
+constexpr uint32_t kSmemStage = kSmemV + kStages * kKvBytes;  // per tile: [128 rows][128 B] output staging
+constexpr uint32_t kStageTileBytes = 128 * 128;
+constexpr uint32_t kSmemBars = kSmemStage + 2 * kStageTileBytes;
+constexpr uint32_t kSmemTmemPtr = kSmemBars + BAR_COUNT * 8;
+constexpr uint32_t kSmemAlloc = kSmemTmemPtr + 16 + 1024;  // slack to align the base to 1024 bytes
+
+__device__ __forceinline__ void report_timeout(uint32_t* status) {
+    if (status) atomicOr(status, ATTN_STATUS_WAIT_TIMEOUT);
+}
+
+// One CTA's part of a segment.
+struct Item {
+    uint32_t seg, kvh, m0, block, blocks;  // first query row; first key block and their number
+    bool tile[2];
+};
+
+template <bool BF16, bool RES, int HD>
+__global__ void __launch_bounds__(kThreads, 1)
+shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                     const __grid_constant__ CUtensorMap tm_o, const __grid_constant__ SharedPrefixParams p) {
+    extern __shared__ unsigned char smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    unsigned char* smem = smem_raw + (base - raw);
+    const uint32_t bars = base + kSmemBars;
+    auto bar = [&](int i) { return bars + 8u * i; };
+    volatile uint32_t* tmem_ptr_smem = reinterpret_cast<volatile uint32_t*>(smem + kSmemTmemPtr);
+    const int tid = threadIdx.x;
+    const int warp = uniform_warp();
+    const int lane = tid & 31;
+    constexpr uint32_t kLoadKv = (HD / 64) * kKvSubBytes;  // bytes of a block actually loaded
+
+    // ---- the CTA's run of the block list
+    const uint32_t blocks = (p.prefix + BN - 1) / BN;
+    const uint32_t query_rows = p.batch * p.group;
+    const uint64_t total = static_cast<uint64_t>(p.segments) * blocks;
+    const uint32_t t0 = static_cast<uint32_t>(blockIdx.x * total / gridDim.x), t1 = static_cast<uint32_t>((blockIdx.x + 1) * total / gridDim.x);
+    auto item_at = [&](uint32_t t, Item& w) {  // the item that starts at block t of the list; false behind the run
+        if (t >= t1) return false;
+        w.seg = t / blocks;
+        w.block = t - w.seg * blocks;
+        w.blocks = min(blocks - w.block, t1 - t);
+        w.kvh = w.seg / p.pairs;
+        w.m0 = (w.seg - w.kvh * p.pairs) * 2 * BM;
+        w.tile[0] = true;
+        w.tile[1] = w.m0 + BM < query_rows;
+        return true;
+    };
+
+    // ---- set-up: barriers, tensor memory
+    if (tid == 0) {
+        mbar_init(bar(BAR_Q_FULL), 128);
+        mbar_init(bar(BAR_Q_FULL + 1), 128);
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(bar(BAR_K_FULL + s), 1);
+            mbar_init(bar(BAR_V_FULL + s), 1);
+            mbar_init(bar(BAR_K_EMPTY + s), 1);
+            mbar_init(bar(BAR_V_EMPTY + s), 1);
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(bar(BAR_S_FULL + i), 1);
+            mbar_init(bar(BAR_P_FULL + i), 128);
+            mbar_init(bar(BAR_O_DONE + i), 1);
+        }
+        mbar_init_fence();
+    }
+    if (warp == 8) {
+        tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_ptr_smem)), kTmemCols);
+        tmem_relinquish();
+    }
+    grid_dep_wait();
+    grid_dep_launch_dependents();
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem_base = *tmem_ptr_smem;
+    auto tmem_s = [&](int t, uint32_t buf) { return tmem_base + static_cast<uint32_t>(t) * 128u + buf * 64u; };
+    auto tmem_o = [&](int t) { return tmem_base + 256u + static_cast<uint32_t>(t) * 128u; };
+
+    if (warp < 8) {
+        // =============================== softmax warpgroups ===============================
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int t = warp >> 2;                 // tile
+        const int r = ((warp & 3) << 5) | lane;  // row inside the tile = tensor-memory lane
+        const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) << 5) << 16;
+        // which CTAs share each segment, for the merge pass
+        for (uint32_t s = blockIdx.x * 256 + tid; s < p.segments; s += gridDim.x * 256)
+            p.seg_ctas[s] = segment_ctas(static_cast<uint64_t>(s) * blocks, (s + 1ull) * blocks, total, gridDim.x);
+        bool ok = true;
+        uint32_t g0 = 0;  // key blocks of this tile before the current item: buffer and barrier phases run on over the items
+        Item w;
+        for (uint32_t at = t0; ok && item_at(at, w); at += w.blocks) {
+            if (!w.tile[t]) continue;
+            // ---- this thread's query row into the tile (the previous item's MMAs are over: its result has been read)
+            const uint32_t m = w.m0 + t * BM + r;
+            {
+                const uint32_t b = m / p.group, g = m - b * p.group;
+                const bool there = m < query_rows;
+                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) +
+                                                                  (static_cast<size_t>(there ? b : 0) * p.n_heads + w.kvh * p.group + (there ? g : 0)) * HD);
+                const uint32_t dst = base + kSmemQ + t * kTileBytes + r * 128;
+#pragma unroll
+                for (int half = 0; half < HD / 64; ++half) {
+                    uint4 x[8];
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) x[c] = there ? src[half * 8 + c] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + half * kSubTileBytes + ((c ^ (r & 7)) << 4)),
+                                     "r"(x[c].x), "r"(x[c].y), "r"(x[c].z), "r"(x[c].w)
+                                     : "memory");
+                }
+                fence_async_smem();
+                mbar_arrive(bar(BAR_Q_FULL + t));
+            }
+            float m_used = -INFINITY;  // maximum the stored probabilities are relative to (log2 units)
+            float l = 0.f;
+            for (uint32_t j = 0; j < w.blocks && ok; ++j) {
+                const uint32_t g = g0 + j, buf = g & 1, par = (g >> 1) & 1;
+                const uint32_t s_tmem = tmem_s(t, buf) + lane_addr;
+                if (!mbar_wait(bar(BAR_S_FULL + 2 * t + buf), par)) { report_timeout(p.status); ok = false; break; }
+                fence_after();
+                float s[BN];
+#pragma unroll
+                for (int c = 0; c < BN / 32; ++c) tmem_ld32(s_tmem + c * 32, *reinterpret_cast<float(*)[32]>(&s[c * 32]));
+                tmem_wait_ld();
+                const uint32_t left = p.prefix - (w.block + j) * BN;  // keys from this block on
+                if (left < BN) {
+#pragma unroll
+                    for (int c = 0; c < BN; ++c) {
+                        if (c >= left) s[c] = -INFINITY;
+                    }
+                }
+                // four independent chains of three-input maxima
+                float mx4[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mx4[i] = max3(s[i], s[4 + i], s[8 + i]);
+#pragma unroll
+                for (int c = 12; c + 8 <= BN; c += 8) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mx4[i] = max3(mx4[i], s[c + i], s[c + 4 + i]);
+                }
+                float mx = max3(fmaxf(mx4[0], mx4[1]), mx4[2], mx4[3]);
+#pragma unroll
+                for (int c = 12 + (BN - 12) / 8 * 8; c < BN; ++c) mx = fmaxf(mx, s[c]);
+                mx *= p.scale_log2;
+                // Rescale only when the maximum grew by more than 8 (probabilities stay below 2^8).
+                float factor = 1.f;
+                if (mx > m_used + 8.f) {
+                    factor = fast_exp2(m_used - mx);  // 0 on the first block (m_used = -inf)
+                    m_used = mx;
+                }
+                if (g >= 2 && !mbar_wait(bar(BAR_O_DONE + 2 * t + buf), par ^ 1)) { report_timeout(p.status); ok = false; break; }
+                if (j > 0 && __any_sync(0xffffffffu, factor != 1.f)) {
+                    if (!mbar_wait(bar(BAR_O_DONE + 2 * t + (buf ^ 1)), ((g - 1) >> 1) & 1)) { report_timeout(p.status); ok = false; break; }
+                    fence_after();
+#pragma unroll
+                    for (int c = 0; c < HD / 32; ++c) {
+                        float o[32];
+                        tmem_ld32(tmem_o(t) + lane_addr + c * 32, o);
+                        tmem_wait_ld();
+                        uint32_t u[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(o[i] * factor);
+                        tmem_st32(tmem_o(t) + lane_addr + c * 32, u);
+                    }
+                }
+                l *= factor;
+                // probabilities; P overwrites S in place
+                const float m_safe = m_used == -INFINITY ? 0.f : m_used;
+                const f32x2 scale2 = pack_f32x2(p.scale_log2, p.scale_log2), m2 = pack_f32x2(-m_safe, -m_safe);
+                const f32x2 minus1 = pack_f32x2(-1.f, -1.f);
+                f32x2 sum2[2] = {pack_f32x2(0.f, 0.f), pack_f32x2(0.f, 0.f)};
+#pragma unroll
+                for (int c = 0; c < BN / 32; ++c) {
+                    uint32_t hi[16], lo[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        float p0, p1;
+                        unpack_f32x2(fma_f32x2(pack_f32x2(s[c * 32 + 2 * i], s[c * 32 + 2 * i + 1]), scale2, m2), p0, p1);
+                        p0 = fast_exp2(p0);
+                        p1 = fast_exp2(p1);
+                        const f32x2 pp = pack_f32x2(p0, p1);
+                        sum2[i & 1] = add_f32x2(sum2[i & 1], pp);
+                        hi[i] = pack2<BF16>(p0, p1);
+                        if constexpr (RES) {
+                            float h0, h1, r0, r1;
+                            unpack2<BF16>(hi[i], h0, h1);
+                            unpack_f32x2(fma_f32x2(pack_f32x2(h0, h1), minus1, pp), r0, r1);
+                            lo[i] = pack2<BF16>(r0, r1);
+                        }
+                    }
+                    // 32 keys -> 16 packed columns: rounded part at column 16c, residual at BN / 2 + 16c
+                    tmem_st16(s_tmem + c * 16, hi);
+                    if constexpr (RES) tmem_st16(s_tmem + BN / 2 + c * 16, lo);
+                }
+                float s0, s1;
+                unpack_f32x2(add_f32x2(sum2[0], sum2[1]), s0, s1);
+                l += s0 + s1;
+                tmem_wait_st();
+                fence_before();
+                mbar_arrive(bar(BAR_P_FULL + 2 * t + buf));
+            }
+            g0 += w.blocks;
+            if (!ok) break;
+            // ---- the piece: O / l and log-sum-exp (log2 units)
+            if (!mbar_wait(bar(BAR_O_DONE + 2 * t + ((g0 - 1) & 1)), ((g0 - 1) >> 1) & 1)) {
+                report_timeout(p.status);
+                ok = false;
+                break;
+            }
+            fence_after();
+            const float inv = l > 0.f ? 1.f / l : 0.f;
+            const uint32_t rec_row = (blockIdx.x + w.seg) * (2 * BM) + t * BM;
+            if (m < query_rows) p.lse[rec_row + r] = l > 0.f ? m_used + __log2f(l) : -INFINITY;
+            const uint32_t stage = base + kSmemStage + t * kStageTileBytes;
+#pragma unroll
+            for (int pass = 0; pass < HD / 32; ++pass) {
+                float o[32];
+                tmem_ld32(tmem_o(t) + lane_addr + pass * 32, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(stage + r * 128 + ((c ^ (r & 7)) << 4)),
+                                 "r"(__float_as_uint(o[c * 4] * inv)), "r"(__float_as_uint(o[c * 4 + 1] * inv)),
+                                 "r"(__float_as_uint(o[c * 4 + 2] * inv)), "r"(__float_as_uint(o[c * 4 + 3] * inv))
+                                 : "memory");
+                fence_async_smem();
+                named_bar_sync(1 + t, 128);
+                if ((warp & 3) == 0 && lane == 0) {
+                    tma_store_2d(&tm_o, stage, pass * 32, rec_row);
+                    tma_store_commit();
+                    tma_store_wait_read();  // the staging tile may be overwritten after this
+                }
+                named_bar_sync(1 + t, 128);
+            }
+            fence_before();  // the next item's first product overwrites O; its P_FULL arrival orders it behind these loads
+        }
+        if ((warp & 3) == 0 && lane == 0) tma_store_wait_all();
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 8 && elect_one()) {
+            // =============================== TMA producer ===============================
+            uint32_t st = 0, phase = 0, it = 0;
+            bool ok = true;
+            Item w;
+            for (uint32_t at = t0; ok && item_at(at, w); at += w.blocks) {
+                for (uint32_t j = 0; j < w.blocks; ++j, ++it) {
+                    const int row = static_cast<int>((w.block + j) * BN), head = static_cast<int>(w.kvh);
+                    if (it >= kStages && !mbar_wait(bar(BAR_K_EMPTY + st), phase ^ 1)) { ok = false; break; }
+                    const uint32_t kdst = base + kSmemK + st * kKvBytes;
+                    mbar_arrive_expect_tx(bar(BAR_K_FULL + st), kLoadKv);
+                    tma_load_3d(kdst, &tm_k, bar(BAR_K_FULL + st), 0, row, head);
+                    if (HD > 64) tma_load_3d(kdst + kKvSubBytes, &tm_k, bar(BAR_K_FULL + st), 64, row, head);
+                    if (it >= kStages && !mbar_wait(bar(BAR_V_EMPTY + st), phase ^ 1)) { ok = false; break; }
+                    const uint32_t vdst = base + kSmemV + st * kKvBytes;
+                    mbar_arrive_expect_tx(bar(BAR_V_FULL + st), kLoadKv);
+                    tma_load_3d(vdst, &tm_v, bar(BAR_V_FULL + st), 0, row, head);
+                    if (HD > 64) tma_load_3d(vdst + kKvSubBytes, &tm_v, bar(BAR_V_FULL + st), 64, row, head);
+                    if (++st == kStages) st = 0, phase ^= 1;
+                }
+            }
+            if (!ok) report_timeout(p.status);
+        } else if (warp == 9 && elect_one()) {
+            // =============================== MMA issuer ===============================
+            constexpr uint32_t fmt = BF16 ? 1u : 0u;
+            constexpr uint32_t idesc_qk = instr_desc(fmt, fmt, 0, BM, BN);  // S: 128 rows x 64 keys
+            constexpr uint32_t idesc_pv = instr_desc(fmt, fmt, 1, BM, HD);  // O: 128 rows x head_dim
+            const uint64_t q_desc = smem_desc(base + kSmemQ, 16, 1024), k_desc = smem_desc(base + kSmemK, 16, 1024);
+            const uint64_t v_desc = smem_desc(base + kSmemV, kKvSubBytes, 1024);
+            uint32_t g0[2] = {0, 0};  // key blocks of each tile before the current item
+            uint32_t items[2] = {0, 0};
+            auto issue_qk = [&](int t, uint32_t j, uint32_t st) {
+                const uint32_t buf = (g0[t] + j) & 1;
+                const uint64_t qa = q_desc + t * (kTileBytes / 16), ka = k_desc + st * (kKvBytes / 16);
+                const uint32_t d = tmem_s(t, buf);
+#pragma unroll
+                for (int kc = 0; kc < HD / 16; ++kc)
+                    mma_ss(d, qa + (kc >> 2) * (kSubTileBytes / 16) + (kc & 3) * 2, ka + (kc >> 2) * (kKvSubBytes / 16) + (kc & 3) * 2,
+                           idesc_qk, kc > 0);
+                commit(bar(BAR_S_FULL + 2 * t + buf));
+            };
+            auto issue_pv = [&](int t, uint32_t j, uint32_t st) {
+                const uint32_t buf = (g0[t] + j) & 1;
+                const uint64_t va = v_desc + st * (kKvBytes / 16);
+                const uint32_t pa = tmem_s(t, buf);
+#pragma unroll
+                for (int kc = 0; kc < BN / 16; ++kc) mma_ts(tmem_o(t), pa + kc * 8, va + kc * 128, idesc_pv, j > 0 || kc > 0);
+                if constexpr (RES) {
+#pragma unroll
+                    for (int kc = 0; kc < BN / 16; ++kc) mma_ts(tmem_o(t), pa + BN / 2 + kc * 8, va + kc * 128, idesc_pv, 1);
+                }
+                commit(bar(BAR_O_DONE + 2 * t + buf));
+            };
+            bool ok = true;
+            uint32_t st = 0, phase = 0, kst = 0, kphase = 0;  // ring position of the next V block, of the next K block
+            auto next_k = [&]() {
+                if (++kst == kStages) kst = 0, kphase ^= 1;
+            };
+            Item w;
+            for (uint32_t at = t0; ok && item_at(at, w); at += w.blocks) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    if (ok && w.tile[t]) {
+                        ok = mbar_wait(bar(BAR_Q_FULL + t), items[t] & 1);
+                        ++items[t];
+                    }
+                for (uint32_t j = 0; j < 2 && j < w.blocks && ok; ++j) {
+                    ok = mbar_wait(bar(BAR_K_FULL + kst), kphase);
+                    if (!ok) break;
+                    fence_after();
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+                        if (w.tile[t]) issue_qk(t, j, kst);
+                    commit(bar(BAR_K_EMPTY + kst));
+                    next_k();
+                }
+                for (uint32_t j = 0; j < w.blocks && ok; ++j) {
+                    if (!mbar_wait(bar(BAR_V_FULL + st), phase)) { ok = false; break; }
+                    const bool more = j + 2 < w.blocks;
+                    bool k_ready = false;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        if (!ok || !w.tile[t]) continue;
+                        const uint32_t g = g0[t] + j;
+                        if (!mbar_wait(bar(BAR_P_FULL + 2 * t + (g & 1)), (g >> 1) & 1)) { ok = false; break; }
+                        fence_after();
+                        issue_pv(t, j, st);
+                        if (more) {
+                            if (!k_ready) {
+                                if (!mbar_wait(bar(BAR_K_FULL + kst), kphase)) { ok = false; break; }
+                                fence_after();
+                                k_ready = true;
+                            }
+                            issue_qk(t, j + 2, kst);
+                        }
+                    }
+                    if (!ok) break;
+                    commit(bar(BAR_V_EMPTY + st));
+                    if (++st == kStages) st = 0, phase ^= 1;
+                    if (more) {
+                        commit(bar(BAR_K_EMPTY + kst));
+                        next_k();
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    if (w.tile[t]) g0[t] += w.blocks;
+            }
+            if (!ok) report_timeout(p.status);
+        }
+    }
+
+    // ---- common exit: everybody meets, then the allocating warp releases tensor memory
+    fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        fence_after();
+        tmem_dealloc(tmem_base, kTmemCols);
+    }
+}
+
+int encode(CUtensorMap* map, CUtensorMapDataType type, uint32_t rank, const void* ptr, const cuuint64_t* dims, const cuuint64_t* strides,
+           const cuuint32_t* box) {
+    EncodeTiledFn enc = encode_tiled_fn();
+    if (!enc) return ATTN_ERR_CUDA;
+    const cuuint32_t unit[3] = {1, 1, 1};
+    const CUresult r = enc(map, type, rank, const_cast<void*>(ptr), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r == CUDA_SUCCESS) return ATTN_OK;
+    g_last_cuda_error = static_cast<int>(r);
+    return ATTN_ERR_CUDA;
+}
+
+}  // namespace
+
+int launch_shared_prefix(const SharedPrefixParams& p, cudaStream_t stream) {
+    const CUtensorMapDataType type = p.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    // K, V [row][kv head][head_dim] as (dim, row, head): blocks of 64 elements x 64 rows of one head; rows behind the end read as zeros
+    const cuuint64_t kv_dims[3] = {p.head_dim, p.prefix, p.n_kv_heads};
+    const cuuint64_t kv_strides[2] = {p.row_stride * 2, p.head_dim * 2ull};
+    const cuuint32_t kv_box[3] = {64, BN, 1};
+    // pieces [records * 256 rows][head_dim] fp32, stored 32 columns x 128 rows at a time
+    const cuuint64_t o_dims[2] = {p.head_dim, (static_cast<cuuint64_t>(p.grid) + p.segments) * 2 * BM};
+    const cuuint64_t o_strides[1] = {p.head_dim * 4ull};
+    const cuuint32_t o_box[2] = {32, BM};
+    CUtensorMap tm_k, tm_v, tm_o;
+    int rc;
+    if ((rc = encode(&tm_k, type, 3, p.k, kv_dims, kv_strides, kv_box)) != ATTN_OK) return rc;
+    if ((rc = encode(&tm_v, type, 3, p.v, kv_dims, kv_strides, kv_box)) != ATTN_OK) return rc;
+    if ((rc = encode(&tm_o, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, p.part, o_dims, o_strides, o_box)) != ATTN_OK) return rc;
+    auto launch = [&](auto kernel) -> int {
+        B200_CUDA_TRY(allow_max_smem(kernel));
+        B200_CUDA_TRY(launch_dependent(kernel, dim3(p.grid), dim3(kThreads), kSmemAlloc, stream, tm_k, tm_v, tm_o, p));
+        g_launch_count.fetch_add(1, std::memory_order_relaxed);
+        return ATTN_OK;
+    };
+    if (p.head_dim == 128) {
+        if (p.bf16) return p.residual ? launch(shared_prefix_kernel<true, true, 128>) : launch(shared_prefix_kernel<true, false, 128>);
+        return p.residual ? launch(shared_prefix_kernel<false, true, 128>) : launch(shared_prefix_kernel<false, false, 128>);
+    }
+    if (p.bf16) return p.residual ? launch(shared_prefix_kernel<true, true, 64>) : launch(shared_prefix_kernel<true, false, 64>);
+    return p.residual ? launch(shared_prefix_kernel<false, true, 64>) : launch(shared_prefix_kernel<false, false, 64>);
+}
+
+}  // namespace b200

@@ -149,7 +149,7 @@ def _decode64(q, kp, vp, k, v, lens, scale):
             p = torch.softmax(s, 1)
             sl = slice(h * G, (h + 1) * G)
             out[b, sl], A[b, sl] = p @ vv, p @ vv.abs()
-            ds[b, sl, 0] = ((qq.abs() @ kk.abs().T) * scale).amax(1) * (D / 16 + 8) * 2.0 ** -23
+            ds[b, sl, 0] = ((qq.abs() @ kk.abs().T) * abs(scale)).amax(1) * (D / 16 + 8) * 2.0 ** -23
             lse[b, sl] = torch.logsumexp(s, 1)
             w[b, h, :n] = p[:, P:].sum(0)
     return out, A, ds, w, lse
@@ -217,6 +217,34 @@ SHAPES = [
 @pytest.mark.parametrize("scored", [False, True])
 def test_decode_shared(ctx, shape, dtype, out_type, scored):
     _check_decode(ctx, *shape, dtype, out_type, scored)
+
+
+# long prefixes and many query rows: the prefix as a matrix product on the tensor cores
+TENSOR_SHAPES = [
+    # B, H, Hkv, D, P, T, lens
+    (5, 32, 8, 128, 513, 20, [20, 3, 0, 7, 1]),
+    (32, 32, 8, 128, 1024, 10, [(i * 3) % 11 for i in range(32)]),       # 128 rows: exactly a tile
+    (43, 24, 8, 64, 2049, 10, [(i * 3) % 11 for i in range(43)]),        # 129 rows, one key in the last block
+    (130, 4, 2, 64, 4095, 9, [(i * 5) % 10 for i in range(130)]),        # 260 rows: two segments per kv head
+    (100, 12, 4, 128, 1999, 5, [(i * 5) % 6 for i in range(100)]),       # 300 rows: the last segment has one tile
+    (3, 24, 2, 128, 5000, 70, [70, 1, 0]),
+    (7, 40, 5, 64, 1000, 33, [33] * 7),
+    (65, 8, 1, 128, 20000, 3, [3, 0, 1] * 21 + [2, 2]),
+    (2, 64, 1, 128, 65, 129, [129, 128]),
+    (300, 8, 1, 64, 10000, 4, [i % 5 for i in range(300)]),              # 2400 rows: ten segments
+]
+
+
+@pytest.mark.parametrize("shape", TENSOR_SHAPES, ids=lambda s: "b%d_h%d_%d_d%d_p%d_t%d" % s[:6])
+@pytest.mark.parametrize("dtype,out_type,scored", [("f16", "f16", True), ("bf16", "bf16", False), ("f16", "f32", False), ("bf16", "f32", True)])
+def test_decode_shared_long_prefix(ctx, shape, dtype, out_type, scored):
+    _check_decode(ctx, *shape, dtype, out_type, scored)
+
+
+def test_decode_shared_long_prefix_large_scores(ctx):
+    _check_decode(ctx, 9, 32, 8, 128, 3000, 100, [100, 50, 1, 0, 5, 6, 7, 8, 9], "f16", "f16", True, std=20.0)
+    _check_decode(ctx, 9, 32, 8, 128, 3000, 100, [100, 50, 1, 0, 5, 6, 7, 8, 9], "bf16", "f32", True, scale=0.5)
+    _check_decode(ctx, 9, 32, 8, 128, 3000, 100, [100, 50, 1, 0, 5, 6, 7, 8, 9], "f16", "f32", True, scale=-0.1)
 
 
 def test_decode_shared_large_scores_and_a_given_scale(ctx):
