@@ -259,6 +259,7 @@ struct SharedPrefixParams {
     uint64_t row_stride;
     uint32_t batch, n_heads, n_kv_heads, group, head_dim, prefix;
     uint32_t pairs, segments, grid;
+    uint32_t ctas_per_seg;  // > 0: that many CTAs for each segment; 0: the blocks of all segments dealt equally, runs may cross segments
     float scale_log2;
     uint32_t* status;
     uint32_t bf16, residual;

@@ -63,6 +63,7 @@ struct SharedParams {
     float* raw;             // [batch][n_heads][raw_stride] scaled scores in log2 units, or null
     uint64_t raw_stride;
     uint32_t* status;
+    uint32_t wait_last;     // the split pass runs beside the prefix kernel
     // merge
     void* o;
     float* lse;
@@ -112,8 +113,10 @@ __global__ void __launch_bounds__(kThreads, 2) shared_split_kernel(const __grid_
     uint32_t* s_warp = s_cum + p.batch + 1;                                           // [4]
     const uint32_t ring = smem_u32(smem_raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // Behind the prefix kernel (which waits for everything in front of it before it lets this one start, and writes nothing that this
+    // one reads or writes) the wait comes at the end: it only has to keep the merge pass from starting before the prefix is done.
     grid_dep_launch_dependents();
-    grid_dep_wait();
+    if (!p.wait_last) grid_dep_wait();
 
     // ---- tiles of each sequence, summed up: a batch of 128 sequences at a time
     {
@@ -155,11 +158,17 @@ __global__ void __launch_bounds__(kThreads, 2) shared_split_kernel(const __grid_
         }
         (s < p.prefix_segs ? p.seg_pre[s] : p.seg_own[s - p.prefix_segs]) = segment_ctas(first, static_cast<uint64_t>(first) + n, total, active);
     }
-    if (blockIdx.x >= active) return;
+    if (blockIdx.x >= active) {
+        if (p.wait_last) grid_dep_wait();
+        return;
+    }
     const uint32_t t0 = static_cast<uint32_t>(static_cast<uint64_t>(blockIdx.x) * total / active);
     const uint32_t t1 = static_cast<uint32_t>((blockIdx.x + 1ull) * total / active);
 
-    if (t0 >= t1) return;
+    if (t0 >= t1) {
+        if (p.wait_last) grid_dep_wait();
+        return;
+    }
 
     auto locate = [&](uint32_t flat, Cursor& c) {
         if (flat < pre_total) {
@@ -389,6 +398,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_split_kernel(const __grid_
         advance(t + 1, cur);
         if (++stage == kStages) stage = 0;
     }
+    if (p.wait_last) grid_dep_wait();
 }
 
 // The pieces of one query row: of the prefix, then of its own cache.
@@ -610,6 +620,7 @@ int make_shared_plan(uint32_t batch, uint32_t n_heads, uint32_t n_kv_heads, uint
 
 // Whether the prefix goes to the tensor-core kernel, by query rows per kv head and key blocks in all.
 constexpr uint32_t kMinPrefixBlocks = 2;  // of a CTA
+constexpr uint32_t kPieceBlocks = 4;
 bool prefix_on_tensor_cores(uint32_t prefix, uint32_t query_rows, uint64_t blocks) {
 #ifdef ATTN_TRACE
     if (const char* e = getenv("ATTN_TRACE_PREFIX")) return prefix > 0 && atoi(e) != 0;  // profiling knob
@@ -736,12 +747,20 @@ extern "C" int attn_decode_shared(const AttnDecodeSharedArgs* a, void* stream_v)
         t.pairs = plan.pairs;
         t.segments = plan.tensor_segs;
         t.grid = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(plan.tensor_grid, blocks / kMinPrefixBlocks)));
+        // A run that crosses from one segment into the next pays a second set of query rows and a second piece, about as much as
+        // kPieceBlocks blocks: whole CTAs per segment unless that makes the longest run longer by more.
+        const uint64_t seg_blocks = blocks / plan.tensor_segs, per_seg = std::min<uint64_t>(t.grid / plan.tensor_segs, seg_blocks);
+        if (per_seg > 0 && (seg_blocks + per_seg - 1) / per_seg <= (blocks + t.grid - 1) / t.grid + kPieceBlocks) {
+            t.ctas_per_seg = static_cast<uint32_t>(per_seg);
+            t.grid = t.ctas_per_seg * plan.tensor_segs;
+        }
         t.scale_log2 = p.scale_log2;
         t.status = p.status;
         t.bf16 = bf16;
         t.residual = res;
         if ((rc = launch_shared_prefix(t, stream)) != ATTN_OK) return rc;
         in_split.prefix_segs = in_split.prefix_tiles = 0;
+        in_split.wait_last = 1;
         // how the merge pass finds the pieces: one record of 256 rows per CTA and segment
         p.pre = Shape{1, 1, 1, kPrefixBlock, p.n_kv_heads, kPrefixRows};
         p.row_blocks = plan.pairs;

@@ -89,7 +89,15 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     const uint32_t blocks = (p.prefix + BN - 1) / BN;
     const uint32_t query_rows = p.batch * p.group;
     const uint64_t total = static_cast<uint64_t>(p.segments) * blocks;
-    const uint32_t t0 = static_cast<uint32_t>(blockIdx.x * total / gridDim.x), t1 = static_cast<uint32_t>((blockIdx.x + 1) * total / gridDim.x);
+    uint32_t t0, t1;
+    if (p.ctas_per_seg) {  // a run inside one segment
+        const uint32_t seg = blockIdx.x / p.ctas_per_seg, i = blockIdx.x - seg * p.ctas_per_seg;
+        t0 = seg * blocks + static_cast<uint32_t>(static_cast<uint64_t>(i) * blocks / p.ctas_per_seg);
+        t1 = seg * blocks + static_cast<uint32_t>((i + 1ull) * blocks / p.ctas_per_seg);
+    } else {
+        t0 = static_cast<uint32_t>(blockIdx.x * total / gridDim.x);
+        t1 = static_cast<uint32_t>((blockIdx.x + 1) * total / gridDim.x);
+    }
     auto item_at = [&](uint32_t t, Item& w) {  // the item that starts at block t of the list; false behind the run
         if (t >= t1) return false;
         w.seg = t / blocks;
@@ -140,13 +148,19 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) << 5) << 16;
         // which CTAs share each segment, for the merge pass
         for (uint32_t s = blockIdx.x * 256 + tid; s < p.segments; s += gridDim.x * 256)
-            p.seg_ctas[s] = segment_ctas(static_cast<uint64_t>(s) * blocks, (s + 1ull) * blocks, total, gridDim.x);
+            p.seg_ctas[s] = p.ctas_per_seg ? (s * p.ctas_per_seg) | p.ctas_per_seg << 16
+                                           : segment_ctas(static_cast<uint64_t>(s) * blocks, (s + 1ull) * blocks, total, gridDim.x);
         bool ok = true;
         uint32_t g0 = 0;  // key blocks of this tile before the current item: buffer and barrier phases run on over the items
+        bool staged = false;
         Item w;
         for (uint32_t at = t0; ok && item_at(at, w); at += w.blocks) {
             if (!w.tile[t]) continue;
-            // ---- this thread's query row into the tile (the previous item's MMAs are over: its result has been read)
+            // ---- this thread's query row into the tile (the previous item's MMAs are over, its result has left)
+            if (staged) {
+                if ((warp & 3) == 0 && lane == 0) tma_store_wait_read();
+                named_bar_sync(1 + t, 128);
+            }
             const uint32_t m = w.m0 + t * BM + r;
             {
                 const uint32_t b = m / p.group, g = m - b * p.group;
@@ -268,9 +282,11 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             const float inv = l > 0.f ? 1.f / l : 0.f;
             const uint32_t rec_row = (blockIdx.x + w.seg) * (2 * BM) + t * BM;
             if (m < query_rows) p.lse[rec_row + r] = l > 0.f ? m_used + __log2f(l) : -INFINITY;
-            const uint32_t stage = base + kSmemStage + t * kStageTileBytes;
-#pragma unroll
-            for (int pass = 0; pass < HD / 32; ++pass) {
+            // The tile leaves through shared memory and the TMA engine, 128 bytes of every row at a time: the query tile, which nothing
+            // reads any more, holds the first two passes, the staging tile the third. (Each pass behind the previous one's store in a
+            // single staging tile: 3 us more per piece.)
+            const bool leader = (warp & 3) == 0 && lane == 0;
+            auto put = [&](int pass, uint32_t stage) {
                 float o[32];
                 tmem_ld32(tmem_o(t) + lane_addr + pass * 32, o);
                 tmem_wait_ld();
@@ -280,15 +296,33 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                                  "r"(__float_as_uint(o[c * 4] * inv)), "r"(__float_as_uint(o[c * 4 + 1] * inv)),
                                  "r"(__float_as_uint(o[c * 4 + 2] * inv)), "r"(__float_as_uint(o[c * 4 + 3] * inv))
                                  : "memory");
+            };
+            const uint32_t stage[3] = {base + kSmemQ + t * kTileBytes, base + kSmemQ + t * kTileBytes + kSubTileBytes,
+                                       base + kSmemStage + t * kStageTileBytes};
+            constexpr int kFirst = HD == 128 ? 3 : 2;
+#pragma unroll
+            for (int pass = 0; pass < kFirst; ++pass) put(pass, stage[pass]);
+            fence_async_smem();
+            named_bar_sync(1 + t, 128);
+            if (leader) {
+#pragma unroll
+                for (int pass = 0; pass < kFirst; ++pass) {
+                    tma_store_2d(&tm_o, stage[pass], pass * 32, rec_row);
+                    tma_store_commit();
+                }
+                if (HD == 128) asm volatile("cp.async.bulk.wait_group.read 2;" ::: "memory");  // the first has been read
+            }
+            if constexpr (HD == 128) {
+                named_bar_sync(1 + t, 128);
+                put(3, stage[0]);
                 fence_async_smem();
                 named_bar_sync(1 + t, 128);
-                if ((warp & 3) == 0 && lane == 0) {
-                    tma_store_2d(&tm_o, stage, pass * 32, rec_row);
+                if (leader) {
+                    tma_store_2d(&tm_o, stage[0], 96, rec_row);
                     tma_store_commit();
-                    tma_store_wait_read();  // the staging tile may be overwritten after this
                 }
-                named_bar_sync(1 + t, 128);
             }
+            staged = true;
             fence_before();  // the next item's first product overwrites O; its P_FULL arrival orders it behind these loads
         }
         if ((warp & 3) == 0 && lane == 0) tma_store_wait_all();
