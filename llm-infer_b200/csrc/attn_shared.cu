@@ -8,8 +8,8 @@
 //
 // Two launches:
 //   split   tiles of 64 (row, head) pairs of K and V, prefix tiles first, then the own rows of sequence after sequence, are dealt to the
-//           CTAs in equal contiguous runs (two CTAs per SM). A tile streams through a ring in shared memory by 16-byte asynchronous
-//           copies; four warps multiply by mma.sync (16 query rows x 16 keys x 8 at a time). A warp owns 16 query rows of one
+//           CTAs in equal contiguous runs (two CTAs per SM). A fifth warp streams the tiles through a ring in shared memory, one TMA
+//           box each for K and V; four warps multiply by mma.sync (16 query rows x 16 keys x 8 at a time). A warp owns 16 query rows of one
 //           kv head and a share of the tile's keys: with few query rows the four warps take four heads (whose slices of a cache row
 //           are contiguous) or four shares of the keys, with many rows of the prefix product four blocks of 16 rows.
 //   merge   one CTA per output row (or slice of it) folds that row's pieces; further CTAs turn the scaled scores that the split pass left
@@ -17,11 +17,14 @@
 // The scores of own rows cost 4 bytes per query head and row each way through L2, next to 4 * head_dim bytes of K and V per kv head.
 // P enters the second product rounded once to the caches' type when the output is 16 bits wide too (an error below the
 // output's own rounding), and as value + rounding residual for fp32 outputs.
+#include <cuda.h>
+
 #include <algorithm>
 #include <cstdlib>
 
 #include "attn_internal.cuh"
 #include "ptx_sm100.cuh"
+#include "tma_tile.cuh"
 
 namespace b200 {
 namespace {
@@ -29,6 +32,7 @@ namespace {
 constexpr int kThreads = 128;
 constexpr int kTilePairs = 64;  // (row, head) pairs of a tile
 constexpr uint32_t kMaxBatch = 2048;
+constexpr int split_stages(int head_dim) { return head_dim == 128 ? 3 : 6; }  // 96 KB of tiles, two CTAs per SM
 
 // How the four warps share a tile of one kind of segment: hpc heads x wm blocks of 16 query rows x ts shares of the keys = 4.
 struct Shape {
@@ -40,15 +44,10 @@ struct Shape {
 
 struct SharedParams {
     const uint16_t* q;
-    const uint16_t* kp;
-    const uint16_t* vp;
-    const uint16_t* k;
-    const uint16_t* v;
     const uint32_t* kv_len;
     uint32_t kv_len_uniform;
     uint32_t batch, n_heads, n_kv_heads, group;
     uint32_t prefix, rows;
-    uint64_t prefix_row_stride, row_stride, batch_stride;
     float scale_log2;
     Shape pre, own;
     uint32_t row_blocks;    // blocks of 16 * pre.wm query rows against the prefix
@@ -79,50 +78,57 @@ __device__ __forceinline__ float fast_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 __device__ __forceinline__ uint32_t own_len(const SharedParams& p, uint32_t b) {
     return min(p.kv_len ? p.kv_len[b] : p.kv_len_uniform, p.rows);
 }
 
-// One run of tiles of one segment: where its K and V lie and which query rows meet it.
+// A tile of the list and its segment.
 struct Cursor {
-    const uint16_t* k;
-    const uint16_t* v;
-    uint64_t stride;
-    uint32_t own, seg;        // kind; index among the segments of its kind
-    uint32_t b, hg, rb;       // own: sequence; head group; prefix: block of query rows
+    uint32_t own, seg;         // kind; index among the segments of its kind
+    uint32_t b, hg, rb;        // own: sequence; head group; prefix: block of query rows
     uint32_t tile, tiles, len;
 };
 
+constexpr int kSplitThreads = kThreads + 32;  // four consumer warps, one producer warp
+
 template <int D, bool BF16, bool RES>
-__global__ void __launch_bounds__(kThreads, 2) shared_split_kernel(const __grid_constant__ SharedParams p) {
-    constexpr int kChunks = D / 8;                         // 16-byte pieces of a head's row
-    constexpr int kStages = D == 128 ? 3 : 6;
+__global__ void __launch_bounds__(kSplitThreads, 2)
+shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_kp,
+                    const __grid_constant__ CUtensorMap tm_vp, const __grid_constant__ SharedParams p) {
+    constexpr int kParts = D / 64;  // 128-byte parts of a head's row
+    constexpr int kStages = split_stages(D);
     constexpr uint32_t kOperandBytes = kTilePairs * D * 2;
     constexpr uint32_t kStageBytes = 2 * kOperandBytes;
-    extern __shared__ __align__(1024) unsigned char smem_raw[];
-    uint32_t* s_cum = reinterpret_cast<uint32_t*>(smem_raw + kStages * kStageBytes);  // [batch + 1] tiles of own rows, one head group
-    uint32_t* s_warp = s_cum + p.batch + 1;                                           // [4]
-    const uint32_t ring = smem_u32(smem_raw);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);  // swizzled tiles want 1024-byte alignment
+    const uint32_t ring = smem_u32(smem);
+    const uint32_t bars = ring + kStages * kStageBytes;  // full [kStages], empty [kStages]
+    uint32_t* s_cum = reinterpret_cast<uint32_t*>(smem + kStages * kStageBytes + 2 * kStages * 8);  // [batch + 1] tiles of own rows, one head group
+    uint32_t* s_warp = s_cum + p.batch + 1;                                                         // [5]
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    if (tid == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(bars + 8 * i, 1);
+            mbar_init(bars + 8 * (kStages + i), 4);
+        }
+        mbar_init_fence();
+        prefetch_tensor_map(&tm_k);
+        prefetch_tensor_map(&tm_v);
+        if (p.prefix_segs) {
+            prefetch_tensor_map(&tm_kp);
+            prefetch_tensor_map(&tm_vp);
+        }
+    }
     // Behind the prefix kernel (which waits for everything in front of it before it lets this one start, and writes nothing that this
     // one reads or writes) the wait comes at the end: it only has to keep the merge pass from starting before the prefix is done.
     grid_dep_launch_dependents();
     if (!p.wait_last) grid_dep_wait();
 
-    // ---- tiles of each sequence, summed up: a batch of 128 sequences at a time
+    // ---- tiles of each sequence, summed up: as many sequences as threads at a time
     {
         uint32_t base = 0;
         if (tid == 0) s_cum[0] = 0;
-        for (uint32_t b0 = 0; b0 < p.batch; b0 += kThreads) {
+        for (uint32_t b0 = 0; b0 < p.batch; b0 += kSplitThreads) {
             const uint32_t b = b0 + tid;
             uint32_t n = b < p.batch ? (own_len(p, b) + p.own.keys - 1) / p.own.keys : 0u;
             if (b < p.batch && p.kv_len && p.kv_len[b] > p.rows && p.status && blockIdx.x == 0) atomicOr(p.status, ATTN_STATUS_BAD_SHAPE);
@@ -137,37 +143,17 @@ __global__ void __launch_bounds__(kThreads, 2) shared_split_kernel(const __grid_
             uint32_t before = base;
             for (int w = 0; w < warp; ++w) before += s_warp[w];
             if (b < p.batch) s_cum[b + 1] = before + incl;
-            base += s_warp[0] + s_warp[1] + s_warp[2] + s_warp[3];
+            base += s_warp[0] + s_warp[1] + s_warp[2] + s_warp[3] + s_warp[4];
             __syncthreads();
         }
     }
     const uint32_t pre_total = p.prefix_segs * p.prefix_tiles;
     const uint32_t total = pre_total + s_cum[p.batch] * p.own.groups;
     const uint32_t active = active_ctas(gridDim.x, 0, 1, total);
-    // ---- which CTAs share each segment, for the merge pass
-    const uint32_t own_segs = p.batch * p.own.groups;
-    for (uint32_t s = blockIdx.x * kThreads + tid; s < p.prefix_segs + own_segs; s += gridDim.x * kThreads) {
-        uint32_t first, n;
-        if (s < p.prefix_segs) {
-            first = s * p.prefix_tiles;
-            n = p.prefix_tiles;
-        } else {
-            const uint32_t b = (s - p.prefix_segs) / p.own.groups, hg = (s - p.prefix_segs) - b * p.own.groups;
-            n = s_cum[b + 1] - s_cum[b];
-            first = pre_total + s_cum[b] * p.own.groups + hg * n;
-        }
-        (s < p.prefix_segs ? p.seg_pre[s] : p.seg_own[s - p.prefix_segs]) = segment_ctas(first, static_cast<uint64_t>(first) + n, total, active);
-    }
-    if (blockIdx.x >= active) {
-        if (p.wait_last) grid_dep_wait();
-        return;
-    }
-    const uint32_t t0 = static_cast<uint32_t>(static_cast<uint64_t>(blockIdx.x) * total / active);
-    const uint32_t t1 = static_cast<uint32_t>((blockIdx.x + 1ull) * total / active);
-
-    if (t0 >= t1) {
-        if (p.wait_last) grid_dep_wait();
-        return;
+    uint32_t t0 = 0, t1 = 0;
+    if (blockIdx.x < active) {
+        t0 = static_cast<uint32_t>(static_cast<uint64_t>(blockIdx.x) * total / active);
+        t1 = static_cast<uint32_t>((blockIdx.x + 1ull) * total / active);
     }
 
     auto locate = [&](uint32_t flat, Cursor& c) {
@@ -180,9 +166,6 @@ __global__ void __launch_bounds__(kThreads, 2) shared_split_kernel(const __grid_
             c.rb = c.seg - c.hg * p.row_blocks;
             c.b = 0;
             c.len = p.prefix;
-            c.stride = p.prefix_row_stride;
-            c.k = p.kp + static_cast<size_t>(c.hg) * p.pre.hpc * D;
-            c.v = p.vp + static_cast<size_t>(c.hg) * p.pre.hpc * D;
             return;
         }
         const uint32_t f = flat - pre_total;
@@ -201,202 +184,233 @@ __global__ void __launch_bounds__(kThreads, 2) shared_split_kernel(const __grid_
         c.seg = lo * p.own.groups + c.hg;
         c.rb = 0;
         c.len = own_len(p, lo);
-        c.stride = p.row_stride;
-        const size_t at = lo * p.batch_stride + static_cast<size_t>(c.hg) * p.own.hpc * D;
-        c.k = p.k + at;
-        c.v = p.v + at;
     };
     // the next tile of the list
     auto advance = [&](uint32_t flat, Cursor& c) {
         if (++c.tile == c.tiles && flat < t1) locate(flat, c);
     };
-    auto load_tile = [&](const Cursor& c, uint32_t stage) {
-        const uint32_t hpc = c.own ? p.own.hpc : p.pre.hpc, keys = c.own ? p.own.keys : p.pre.keys;
-        const uint32_t width = hpc * kChunks;  // both powers of two
-        const uint32_t shift = 31 - __clz(width), row0 = c.tile * keys;
-        const uint32_t kdst = ring + stage * kStageBytes, vdst = kdst + kOperandBytes;
-#pragma unroll
-        for (int i = 0; i < kTilePairs * kChunks / kThreads; ++i) {
-            const uint32_t id = tid + i * kThreads;
-            const uint32_t key = id >> shift, in_row = id & (width - 1);
-            const uint32_t hs = in_row / kChunks, ch = in_row % kChunks;
-            const uint32_t row = row0 + key, r = hs * keys + key;
-            const bool there = row < c.len;
-            const size_t at = there ? row * c.stride + in_row * 8 : 0;  // (nothing is read where `there` is false: zeros are stored)
-            const uint32_t dst = r * (D * 2) + ((ch ^ (r & 7)) << 4);
-            cp_async16(kdst + dst, c.k + at, there ? 16u : 0u);
-            cp_async16(vdst + dst, c.v + at, there ? 16u : 0u);
-        }
-    };
 
-    Cursor ld, cur;
-    locate(t0, ld);
-    cur = ld;
-#pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) {
-        if (t0 + s < t1) {
-            load_tile(ld, s);
-            advance(t0 + s + 1, ld);
-        }
-        cp_async_commit();
-    }
-
-    uint32_t qa[D / 16][4];
-    float o[D / 8][4];
-    float m[2], l[2];
-    bool fresh = true;  // the next tile begins a run of a segment
-    uint32_t stage = 0;
-    for (uint32_t t = t0; t < t1; ++t) {
-        const Shape& sh = cur.own ? p.own : p.pre;
-        // this warp's place: head hs of the group, block wr of query rows, share wk of the keys
-        const uint32_t hs = warp % sh.hpc, wr = (warp / sh.hpc) % sh.wm, wk = warp / (sh.hpc * sh.wm);
-        const uint32_t kvh = cur.hg * sh.hpc + hs;
-        if (fresh) {
-            fresh = false;
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const uint32_t r = wr * 16 + half * 8 + lane / 4;
-                uint32_t b, g;
-                bool there;
-                if (cur.own) {
-                    b = cur.b;
-                    g = r;
-                    there = r < p.group;
+    if (warp == 4) {
+        // =============================== producer ===============================
+        if (lane == 0 && t0 < t1) {
+            const uint64_t once = l2_policy_evict_first();  // own rows are read once; the prefix's may be read by several blocks of rows
+            const uint64_t again = l2_policy_evict_last();
+            Cursor c;
+            locate(t0, c);
+            uint32_t st = 0, phase = 0, n = 0;
+            bool ok = true;
+            for (uint32_t t = t0; t < t1; ++t, ++n) {
+                if (n >= kStages && !mbar_wait(bars + 8 * (kStages + st), phase ^ 1)) { ok = false; break; }
+                const uint32_t full = bars + 8 * st, dst = ring + st * kStageBytes;
+                mbar_arrive_expect_tx(full, kStageBytes);
+                if (c.own) {
+                    const int row = static_cast<int>(c.tile * p.own.keys), head = static_cast<int>(c.hg * p.own.hpc);
+                    tma_load_5d_hint(dst, &tm_k, full, row, 0, head, static_cast<int>(c.b), once);
+                    tma_load_5d_hint(dst + kOperandBytes, &tm_v, full, row, 0, head, static_cast<int>(c.b), once);
                 } else {
-                    const uint32_t row = cur.rb * sh.wm * 16 + r;
-                    b = row / p.group;
-                    g = row - b * p.group;
-                    there = b < p.batch;
+                    const int row = static_cast<int>(c.tile * p.pre.keys), head = static_cast<int>(c.hg * p.pre.hpc);
+                    tma_load_5d_hint(dst, &tm_kp, full, row, 0, head, 0, p.row_blocks > 1 ? again : once);
+                    tma_load_5d_hint(dst + kOperandBytes, &tm_vp, full, row, 0, head, 0, p.row_blocks > 1 ? again : once);
                 }
-                const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + ((static_cast<size_t>(b) * p.n_heads) + kvh * p.group + g) * D) + lane % 4;
-#pragma unroll
-                for (int kc = 0; kc < D / 16; ++kc) {
-                    qa[kc][half] = there ? src[kc * 8] : 0u;
-                    qa[kc][2 + half] = there ? src[kc * 8 + 4] : 0u;
+                advance(t + 1, c);
+                if (++st == kStages) st = 0, phase ^= 1;
+            }
+            if (!ok) {  // report, and leave no copy in flight into this CTA's memory
+                if (p.status) atomicOr(p.status, ATTN_STATUS_WAIT_TIMEOUT);
+                for (int i = 0; i < kStages; ++i) {
+                    (void)mbar_wait(bars + 8 * st, phase ^ 1);
+                    if (++st == kStages) st = 0, phase ^= 1;
                 }
             }
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-            m[0] = m[1] = -INFINITY;
-            l[0] = l[1] = 0.f;
         }
-        cp_async_wait<kStages - 2>();
-        __syncthreads();
-        if (t + kStages - 1 < t1) {
-            load_tile(ld, stage == 0 ? kStages - 1 : stage - 1);
-            advance(t + kStages, ld);
-        }
-        cp_async_commit();
-        const uint32_t kbase = ring + stage * kStageBytes, vbase = kbase + kOperandBytes;
-        const uint32_t steps = sh.wm;  // 16 keys each: 64 / hpc / ts = 16 wm
-#pragma unroll 1
-        for (uint32_t st = 0; st < steps; ++st) {
-            const uint32_t key0 = (wk * steps + st) * 16;          // in the tile
-            const uint32_t row0 = hs * sh.keys + key0;             // in shared memory
-            const uint32_t first = cur.tile * sh.keys + key0;      // in the cache
-            if (first >= cur.len) break;
-            float s[2][4] = {};
-#pragma unroll
-            for (int kc = 0; kc < D / 16; ++kc) {
-                const uint32_t r = row0 + (lane >> 4) * 8 + (lane & 7), ch = kc * 2 + ((lane >> 3) & 1);
-                uint32_t b0, b1, b2, b3;
-                ldmatrix_x4(b0, b1, b2, b3, kbase + r * (D * 2) + ((ch ^ (r & 7)) << 4));
-                mma_16816<BF16>(s[0], qa[kc], b0, b1);
-                mma_16816<BF16>(s[1], qa[kc], b2, b3);
+        __syncwarp();
+    } else {
+        // =============================== consumers ===============================
+        // which CTAs share each segment, for the merge pass
+        const uint32_t own_segs = p.batch * p.own.groups;
+        for (uint32_t s = blockIdx.x * kThreads + tid; s < p.prefix_segs + own_segs; s += gridDim.x * kThreads) {
+            uint32_t first, n;
+            if (s < p.prefix_segs) {
+                first = s * p.prefix_tiles;
+                n = p.prefix_tiles;
+            } else {
+                const uint32_t b = (s - p.prefix_segs) / p.own.groups, hg = (s - p.prefix_segs) - b * p.own.groups;
+                n = s_cum[b + 1] - s_cum[b];
+                first = pre_total + s_cum[b] * p.own.groups + hg * n;
             }
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t key = first + n * 8 + (lane & 3) * 2 + (i & 1);
-                    s[n][i] = key < cur.len ? s[n][i] * p.scale_log2 : -INFINITY;
-                }
-            if (cur.own && p.raw) {
+            (s < p.prefix_segs ? p.seg_pre[s] : p.seg_own[s - p.prefix_segs]) = segment_ctas(first, static_cast<uint64_t>(first) + n, total, active);
+        }
+        Cursor cur;
+        if (t0 < t1) locate(t0, cur);
+        uint32_t qa[D / 16][4];
+        float o[D / 8][4];
+        float m[2], l[2];
+        bool fresh = true;  // the next tile begins a run of a segment
+        uint32_t stage = 0, phase = 0;
+        for (uint32_t t = t0; t < t1; ++t) {
+            const Shape& sh = cur.own ? p.own : p.pre;
+            // this warp's place: head hs of the group, block wr of query rows, share wk of the keys (all powers of two)
+            const uint32_t hs = warp & (sh.hpc - 1), wr = (warp >> (sh.hpc >> 1)) & (sh.wm - 1), wk = warp >> ((sh.hpc >> 1) + (sh.wm >> 1));
+            const uint32_t kvh = cur.hg * sh.hpc + hs;
+            if (fresh) {
+                fresh = false;
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const uint32_t g = wr * 16 + half * 8 + lane / 4;
-                    if (g < p.group) {
-                        float* dst = p.raw + (static_cast<size_t>(cur.b) * p.n_heads + kvh * p.group + g) * p.raw_stride + first + (lane & 3) * 2;
-                        *reinterpret_cast<float2*>(dst) = make_float2(s[0][2 * half], s[0][2 * half + 1]);
-                        *reinterpret_cast<float2*>(dst + 8) = make_float2(s[1][2 * half], s[1][2 * half + 1]);
+                    const uint32_t r = wr * 16 + half * 8 + lane / 4;
+                    uint32_t b, g;
+                    bool there;
+                    if (cur.own) {
+                        b = cur.b;
+                        g = r;
+                        there = r < p.group;
+                    } else {
+                        const uint32_t row = cur.rb * sh.wm * 16 + r;
+                        b = row / p.group;
+                        g = row - b * p.group;
+                        there = b < p.batch;
+                    }
+                    const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + ((static_cast<size_t>(b) * p.n_heads) + kvh * p.group + g) * D) + lane % 4;
+#pragma unroll
+                    for (int kc = 0; kc < D / 16; ++kc) {
+                        qa[kc][half] = there ? src[kc * 8] : 0u;
+                        qa[kc][2 + half] = there ? src[kc * 8 + 4] : 0u;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+                m[0] = m[1] = -INFINITY;
+                l[0] = l[1] = 0.f;
+            }
+            if (!mbar_wait(bars + 8 * stage, phase)) {
+                if (p.status) atomicOr(p.status, ATTN_STATUS_WAIT_TIMEOUT);
+                break;
+            }
+            const uint32_t head_base = hs * (kParts * sh.keys * 128), part_bytes = sh.keys * 128;
+            const uint32_t kbase = ring + stage * kStageBytes + head_base, vbase = kbase + kOperandBytes;
+            const uint32_t steps = sh.wm;  // 16 keys each: 64 / hpc / ts = 16 wm
+#pragma unroll 1
+            for (uint32_t st = 0; st < steps; ++st) {
+                const uint32_t key0 = (wk * steps + st) * 16;      // in the tile
+                const uint32_t first = cur.tile * sh.keys + key0;  // in the cache
+                if (first >= cur.len) break;
+                // (two chains of accumulators per eight keys: half the latency of eight dependent MMAs)
+                float s[2][4] = {}, s2[2][4] = {};
+                const uint32_t krow = kbase + (key0 + (lane >> 4) * 8 + (lane & 7)) * 128;
+#pragma unroll
+                for (int kc = 0; kc < D / 16; ++kc) {
+                    const uint32_t ch = (kc * 2 + ((lane >> 3) & 1)) & 7;
+                    uint32_t b0, b1, b2, b3;
+                    ldmatrix_x4(b0, b1, b2, b3, krow + (kc >> 2) * part_bytes + ((ch ^ (lane & 7)) << 4));
+                    mma_16816<BF16>(kc & 1 ? s2[0] : s[0], qa[kc], b0, b1);
+                    mma_16816<BF16>(kc & 1 ? s2[1] : s[1], qa[kc], b2, b3);
+                }
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[n][i] = (s[n][i] + s2[n][i]) * p.scale_log2;
+                if (first + 16 > cur.len) {  // the last rows: what lies behind them in the cache must not matter
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (first + n * 8 + (lane & 3) * 2 + (i & 1) >= cur.len) s[n][i] = -INFINITY;
+                    for (uint32_t i = lane; i < 16 * kParts * 8; i += 32) {
+                        const uint32_t r = i / (kParts * 8), in_row = i % (kParts * 8);
+                        if (first + r >= cur.len) st_shared_zero16(vbase + (in_row >> 3) * part_bytes + (key0 + r) * 128 + ((in_row & 7) << 4));
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // in front of the copy that refills the stage
+                    __syncwarp();
+                }
+                if (cur.own && p.raw) {
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const uint32_t g = wr * 16 + half * 8 + lane / 4;
+                        if (g < p.group) {
+                            float* dst = p.raw + (static_cast<size_t>(cur.b) * p.n_heads + kvh * p.group + g) * p.raw_stride + first + (lane & 3) * 2;
+                            *reinterpret_cast<float2*>(dst) = make_float2(s[0][2 * half], s[0][2 * half + 1]);
+                            *reinterpret_cast<float2*>(dst + 8) = make_float2(s[1][2 * half], s[1][2 * half + 1]);
+                        }
+                    }
+                }
+                float mx[2], safe[2];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    float x = fmaxf(fmaxf(s[0][2 * half], s[0][2 * half + 1]), fmaxf(s[1][2 * half], s[1][2 * half + 1]));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+                    mx[half] = fmaxf(m[half], x);
+                    safe[half] = mx[half] == -INFINITY ? 0.f : mx[half];
+                }
+                if (__any_sync(0xffffffffu, mx[0] != m[0] || mx[1] != m[1])) {
+                    const float f0 = fast_exp2(m[0] - safe[0]), f1 = fast_exp2(m[1] - safe[1]);
+                    l[0] *= f0;
+                    l[1] *= f1;
+#pragma unroll
+                    for (int i = 0; i < D / 8; ++i) {
+                        o[i][0] *= f0;
+                        o[i][1] *= f0;
+                        o[i][2] *= f1;
+                        o[i][3] *= f1;
+                    }
+                    m[0] = mx[0];
+                    m[1] = mx[1];
+                }
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        s[n][i] = fast_exp2(s[n][i] - safe[i >> 1]);
+                        l[i >> 1] += s[n][i];
+                    }
+                uint32_t pa[4], pr[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float x = s[i >> 1][(i & 1) * 2], y = s[i >> 1][(i & 1) * 2 + 1];
+                    pa[i] = pack2<BF16>(x, y);
+                    if constexpr (RES) pr[i] = pack2<BF16>(x - round16<BF16>(x), y - round16<BF16>(y));
+                }
+                const uint32_t vrow = vbase + (key0 + ((lane >> 3) & 1) * 8 + (lane & 7)) * 128;
+#pragma unroll
+                for (int dc = 0; dc < D / 16; ++dc) {
+                    const uint32_t ch = (dc * 2 + (lane >> 4)) & 7;
+                    uint32_t b0, b1, b2, b3;
+                    ldmatrix_x4_trans(b0, b1, b2, b3, vrow + (dc >> 2) * part_bytes + ((ch ^ (lane & 7)) << 4));
+                    mma_16816<BF16>(o[2 * dc], pa, b0, b1);
+                    mma_16816<BF16>(o[2 * dc + 1], pa, b2, b3);
+                    if constexpr (RES) {
+                        mma_16816<BF16>(o[2 * dc], pr, b0, b1);
+                        mma_16816<BF16>(o[2 * dc + 1], pr, b2, b3);
                     }
                 }
             }
-            float mx[2], safe[2];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bars + 8 * (kStages + stage));
+            if (++stage == kStages) stage = 0, phase ^= 1;
+            if (cur.tile + 1 == cur.tiles || t + 1 == t1) {
+                // ---- the run's piece: normalised sum and log-sum-exp (log2 units) of this warp's rows and keys
+                const size_t rec = (static_cast<size_t>(blockIdx.x + cur.seg) * sh.ts + wk) * sh.hpc + hs;
+                float* po = cur.own ? p.part_own : p.part_pre;
+                float* pl = cur.own ? p.lse_own : p.lse_pre;
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                float x = fmaxf(fmaxf(s[0][2 * half], s[0][2 * half + 1]), fmaxf(s[1][2 * half], s[1][2 * half + 1]));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-                mx[half] = fmaxf(m[half], x);
-                safe[half] = mx[half] == -INFINITY ? 0.f : mx[half];
-            }
-            if (__any_sync(0xffffffffu, mx[0] != m[0] || mx[1] != m[1])) {
-                const float f0 = fast_exp2(m[0] - safe[0]), f1 = fast_exp2(m[1] - safe[1]);
-                l[0] *= f0;
-                l[1] *= f1;
+                for (int half = 0; half < 2; ++half) {
+                    float sum = l[half];
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+                    const uint32_t r = wr * 16 + half * 8 + lane / 4;
+                    const bool there = cur.own ? r < p.group : cur.rb * sh.wm * 16 + r < p.batch * p.group;
+                    if (there) {
+                        float* dst = po + (rec * sh.rec_rows + r) * D + (lane & 3) * 2;
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    o[i][0] *= f0;
-                    o[i][1] *= f0;
-                    o[i][2] *= f1;
-                    o[i][3] *= f1;
+                        for (int i = 0; i < D / 8; ++i)
+                            *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[i][2 * half] * inv, o[i][2 * half + 1] * inv);
+                        if ((lane & 3) == 0) pl[rec * sh.rec_rows + r] = sum > 0.f ? m[half] + __log2f(sum) : -INFINITY;
+                    }
                 }
-                m[0] = mx[0];
-                m[1] = mx[1];
+                fresh = true;
             }
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s[n][i] = fast_exp2(s[n][i] - safe[i >> 1]);
-                    l[i >> 1] += s[n][i];
-                }
-            uint32_t pa[4], pr[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = s[i >> 1][(i & 1) * 2], y = s[i >> 1][(i & 1) * 2 + 1];
-                pa[i] = pack2<BF16>(x, y);
-                if constexpr (RES) pr[i] = pack2<BF16>(x - round16<BF16>(x), y - round16<BF16>(y));
-            }
-#pragma unroll
-            for (int dc = 0; dc < D / 16; ++dc) {
-                const uint32_t r = row0 + ((lane >> 3) & 1) * 8 + (lane & 7), ch = dc * 2 + (lane >> 4);
-                uint32_t b0, b1, b2, b3;
-                ldmatrix_x4_trans(b0, b1, b2, b3, vbase + r * (D * 2) + ((ch ^ (r & 7)) << 4));
-                mma_16816<BF16>(o[2 * dc], pa, b0, b1);
-                mma_16816<BF16>(o[2 * dc + 1], pa, b2, b3);
-                if constexpr (RES) {
-                    mma_16816<BF16>(o[2 * dc], pr, b0, b1);
-                    mma_16816<BF16>(o[2 * dc + 1], pr, b2, b3);
-                }
-            }
+            advance(t + 1, cur);
         }
-        if (cur.tile + 1 == cur.tiles || t + 1 == t1) {
-            // ---- the run's piece: normalised sum and log-sum-exp (log2 units) of this warp's rows and keys
-            const size_t rec = (static_cast<size_t>(blockIdx.x + cur.seg) * sh.ts + wk) * sh.hpc + hs;
-            float* po = cur.own ? p.part_own : p.part_pre;
-            float* pl = cur.own ? p.lse_own : p.lse_pre;
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                float sum = l[half];
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                const float inv = sum > 0.f ? 1.f / sum : 0.f;
-                const uint32_t r = wr * 16 + half * 8 + lane / 4;
-                const bool there = cur.own ? r < p.group : cur.rb * sh.wm * 16 + r < p.batch * p.group;
-                if (there) {
-                    float* dst = po + (rec * sh.rec_rows + r) * D + (lane & 3) * 2;
-#pragma unroll
-                    for (int i = 0; i < D / 8; ++i)
-                        *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[i][2 * half] * inv, o[i][2 * half + 1] * inv);
-                    if ((lane & 3) == 0) pl[rec * sh.rec_rows + r] = sum > 0.f ? m[half] + __log2f(sum) : -INFINITY;
-                }
-            }
-            fresh = true;
-        }
-        advance(t + 1, cur);
-        if (++stage == kStages) stage = 0;
     }
     if (p.wait_last) grid_dep_wait();
 }
@@ -443,6 +457,7 @@ __global__ void __launch_bounds__(kThreads) shared_merge_kernel(const __grid_con
     __shared__ float s_ml[4][2];
     __shared__ float s_lse[64];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    grid_dep_launch_dependents();
     grid_dep_wait();
     if (blockIdx.x < p.out_ctas) {
         const uint32_t row = blockIdx.x / (D / SLICE), slice = blockIdx.x % (D / SLICE);
@@ -524,6 +539,30 @@ __global__ void __launch_bounds__(kThreads) shared_merge_kernel(const __grid_con
     const uint32_t len = own_len(p, b);
     const uint32_t begin = chunk * p.score_rows, end = min(len, begin + p.score_rows);
     if (begin >= end) return;
+    // A thread takes up to kAt rows at a time, kThreads apart; the first heads' scores and the weights so far are requested ahead of the
+    // log-sum-exps.
+    constexpr int kAt = 4, kHeads = 4;
+    const float* raw = p.raw + (static_cast<size_t>(b) * p.n_heads + kvh * p.group) * p.raw_stride;
+    const float* before = p.scores ? p.scores + seg * p.score_stride : nullptr;
+    float w[kAt], x4[kHeads][kAt];
+    auto fetch_rows = [&](uint32_t t0) {
+#pragma unroll
+        for (int a = 0; a < kAt; ++a) {
+            const uint32_t t = t0 + a * kThreads;
+            w[a] = before && t < end ? before[t] : 0.f;
+        }
+    };
+    auto fetch_heads = [&](uint32_t t0, uint32_t g0) {
+#pragma unroll
+        for (int g = 0; g < kHeads; ++g)
+#pragma unroll
+            for (int a = 0; a < kAt; ++a) {
+                const uint32_t t = t0 + a * kThreads;
+                x4[g][a] = t < end && g0 + g < p.group ? raw[(g0 + g) * p.raw_stride + t] : -INFINITY;
+            }
+    };
+    fetch_rows(begin + tid);
+    fetch_heads(begin + tid, 0);
     // the heads' log-sum-exps: eight lanes a head
     for (uint32_t g0 = 0; g0 < p.group; g0 += kThreads / 8) {
         const uint32_t g = g0 + tid / 8;
@@ -558,13 +597,27 @@ __global__ void __launch_bounds__(kThreads) shared_merge_kernel(const __grid_con
         if ((tid & 7) == 0 && g < p.group) s_lse[g] = m + __log2f(l);
     }
     __syncthreads();
-    const float* raw = p.raw + (static_cast<size_t>(b) * p.n_heads + kvh * p.group) * p.raw_stride;
-    for (uint32_t t = begin + tid; t < end; t += kThreads) {
-        const float before = p.scores ? p.scores[seg * p.score_stride + t] : 0.f;
-        float w = 0.f;
-#pragma unroll 8
-        for (uint32_t g = 0; g < p.group; ++g) w += fast_exp2(raw[g * p.raw_stride + t] - s_lse[g]);
-        p.scores_out[seg * p.score_out_stride + t] = before + w;
+    float* after = p.scores_out + seg * p.score_out_stride;
+    for (uint32_t t0 = begin + tid; t0 < end; t0 += kAt * kThreads) {
+        if (t0 != begin + tid) {
+            fetch_rows(t0);
+            fetch_heads(t0, 0);
+        }
+        float sum[kAt] = {};
+        for (uint32_t g0 = 0; g0 < p.group; g0 += kHeads) {
+            if (g0) fetch_heads(t0, g0);
+#pragma unroll
+            for (int g = 0; g < kHeads; ++g) {
+                const float lse = g0 + g < p.group ? s_lse[g0 + g] : 0.f;
+#pragma unroll
+                for (int a = 0; a < kAt; ++a) sum[a] += fast_exp2(x4[g][a] - lse);
+            }
+        }
+#pragma unroll
+        for (int a = 0; a < kAt; ++a) {
+            const uint32_t t = t0 + a * kThreads;
+            if (t < end) after[t] = w[a] + sum[a];
+        }
     }
 }
 
@@ -618,6 +671,24 @@ int make_shared_plan(uint32_t batch, uint32_t n_heads, uint32_t n_kv_heads, uint
     return ATTN_OK;
 }
 
+// Cache rows as [sequence][kv head][128-byte part of a head][row][64 elements]; a box is a tile: all parts of hpc heads over its
+// rows. Rows that the cache does not have read as zeros.
+int tile_map(CUtensorMap* map, const void* cache, bool bf16, uint32_t head_dim, uint32_t rows, uint32_t kv_heads, uint32_t batch,
+             uint64_t row_stride, uint64_t batch_stride, const Shape& sh) {
+    EncodeTiledFn enc = encode_tiled_fn();
+    if (!enc) return ATTN_ERR_CUDA;
+    const cuuint64_t dims[5] = {64, rows, head_dim / 64, kv_heads, batch};
+    const cuuint64_t strides[4] = {row_stride * 2, 128, head_dim * 2ull, (batch > 1 ? batch_stride : row_stride * rows) * 2};
+    const cuuint32_t box[5] = {64, sh.keys, head_dim / 64, sh.hpc, 1};
+    const cuuint32_t unit[5] = {1, 1, 1, 1, 1};
+    const CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(cache), dims,
+                           strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r == CUDA_SUCCESS) return ATTN_OK;
+    g_last_cuda_error = static_cast<int>(r);
+    return ATTN_ERR_CUDA;
+}
+
 // Whether the prefix goes to the tensor-core kernel, by query rows per kv head and key blocks in all.
 constexpr uint32_t kMinPrefixBlocks = 2;  // of a CTA
 constexpr uint32_t kPieceBlocks = 4;
@@ -653,15 +724,14 @@ extern "C" int attn_decode_shared(const AttnDecodeSharedArgs* a, void* stream_v)
     if (a->scores_out && a->kv_capacity == 0) return ATTN_ERR_INVALID_ARG;
     const uint64_t width = static_cast<uint64_t>(a->n_kv_heads) * a->head_dim;
     SharedParams p{};
-    p.prefix_row_stride = a->prefix_row_stride ? a->prefix_row_stride : width;
-    p.row_stride = a->kv_row_stride ? a->kv_row_stride : width;
-    p.batch_stride = a->kv_batch_stride;
+    const uint64_t prefix_row_stride = a->prefix_row_stride ? a->prefix_row_stride : width;
+    const uint64_t row_stride = a->kv_row_stride ? a->kv_row_stride : width, batch_stride = a->kv_batch_stride;
     p.score_stride = a->score_stride ? a->score_stride : a->kv_capacity;
     p.score_out_stride = a->score_out_stride ? a->score_out_stride : a->kv_capacity;
-    if (p.prefix_row_stride < width || p.row_stride < width || p.score_stride < a->kv_capacity || p.score_out_stride < a->kv_capacity)
+    if (prefix_row_stride < width || row_stride < width || p.score_stride < a->kv_capacity || p.score_out_stride < a->kv_capacity)
         return ATTN_ERR_INVALID_ARG;
     if (!aligned16(a->q) || !aligned16(a->k_prefix) || !aligned16(a->v_prefix) || !aligned16(a->k) || !aligned16(a->v) ||
-        (p.prefix_row_stride | p.row_stride | p.batch_stride) % 8 != 0)
+        (prefix_row_stride | row_stride | batch_stride) % 8 != 0)
         return ATTN_ERR_ALIGNMENT;
     DeviceInfo dev{};
     int rc = current_device_info(&dev);
@@ -675,10 +745,6 @@ extern "C" int attn_decode_shared(const AttnDecodeSharedArgs* a, void* stream_v)
     if (!aligned16(a->workspace)) return ATTN_ERR_ALIGNMENT;
 
     p.q = static_cast<const uint16_t*>(a->q);
-    p.kp = static_cast<const uint16_t*>(a->k_prefix);
-    p.vp = static_cast<const uint16_t*>(a->v_prefix);
-    p.k = static_cast<const uint16_t*>(a->k);
-    p.v = static_cast<const uint16_t*>(a->v);
     p.kv_len = a->kv_capacity ? a->kv_len : nullptr;
     p.kv_len_uniform = a->kv_len_uniform;
     p.batch = a->batch;
@@ -737,7 +803,7 @@ extern "C" int attn_decode_shared(const AttnDecodeSharedArgs* a, void* stream_v)
         t.part = p.part_pre;
         t.lse = p.lse_pre;
         t.seg_ctas = p.seg_pre;
-        t.row_stride = p.prefix_row_stride;
+        t.row_stride = prefix_row_stride;
         t.batch = p.batch;
         t.n_heads = p.n_heads;
         t.n_kv_heads = p.n_kv_heads;
@@ -768,10 +834,23 @@ extern "C" int attn_decode_shared(const AttnDecodeSharedArgs* a, void* stream_v)
     }
     const uint64_t most = prefix_tiles * in_split.prefix_segs + own_tiles * plan.own_segs;
     const uint32_t grid = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(plan.grid, most)));
+    CUtensorMap tm_k{}, tm_v{}, tm_kp{}, tm_vp{};
+    if (a->kv_capacity) {
+        if ((rc = tile_map(&tm_k, a->k, bf16, a->head_dim, p.rows, p.n_kv_heads, p.batch, row_stride, batch_stride, p.own)) != ATTN_OK ||
+            (rc = tile_map(&tm_v, a->v, bf16, a->head_dim, p.rows, p.n_kv_heads, p.batch, row_stride, batch_stride, p.own)) != ATTN_OK)
+            return rc;
+    }
+    if (in_split.prefix_segs) {
+        if ((rc = tile_map(&tm_kp, a->k_prefix, bf16, a->head_dim, p.prefix, p.n_kv_heads, 1, prefix_row_stride, 0, p.pre)) != ATTN_OK ||
+            (rc = tile_map(&tm_vp, a->v_prefix, bf16, a->head_dim, p.prefix, p.n_kv_heads, 1, prefix_row_stride, 0, p.pre)) != ATTN_OK)
+            return rc;
+    }
     auto split = [&](auto kernel) -> int {
         B200_CUDA_TRY(allow_max_smem(kernel));
-        const size_t smem = 96 * 1024 + (a->batch + 5) * 4;  // the ring, s_cum, s_warp
-        B200_CUDA_TRY(launch_dependent(kernel, dim3(grid), dim3(kThreads), smem, stream, in_split));
+        // alignment, the ring, its barriers, s_cum, s_warp
+        const int stages = split_stages(static_cast<int>(a->head_dim));
+        const size_t smem = 1024 + static_cast<size_t>(stages) * (2 * kTilePairs * a->head_dim * 2 + 16) + (a->batch + 1 + 5) * 4;
+        B200_CUDA_TRY(launch_dependent(kernel, dim3(grid), dim3(kSplitThreads), smem, stream, tm_k, tm_v, tm_kp, tm_vp, in_split));
         g_launch_count.fetch_add(1, std::memory_order_relaxed);
         return ATTN_OK;
     };

@@ -126,6 +126,9 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             mbar_init(bar(BAR_O_DONE + i), 1);
         }
         mbar_init_fence();
+        prefetch_tensor_map(&tm_k);
+        prefetch_tensor_map(&tm_v);
+        prefetch_tensor_map(&tm_o);
     }
     if (warp == 8) {
         tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_ptr_smem)), kTmemCols);

@@ -26,4 +26,9 @@ inline EncodeTiledFn encode_tiled_fn() {
     return reinterpret_cast<EncodeTiledFn>(fn);
 }
 
+// A descriptor that lies in a kernel's parameters, fetched ahead of the first copy that uses it.
+__device__ __forceinline__ void prefetch_tensor_map(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
 }  // namespace b200
