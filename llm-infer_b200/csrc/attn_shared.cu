@@ -32,7 +32,8 @@ namespace {
 constexpr int kThreads = 128;
 constexpr int kTilePairs = 64;  // (row, head) pairs of a tile
 constexpr uint32_t kMaxBatch = 2048;
-constexpr int split_stages(int head_dim) { return head_dim == 128 ? 3 : 6; }  // 96 KB of tiles, two CTAs per SM
+constexpr uint32_t kMaxSlots = 12;
+constexpr size_t kSplitSmem = 113 * 1024;  // of a CTA of the split pass, two per SM
 
 // How the four warps share a tile of one kind of segment: hpc heads x wm blocks of 16 query rows x ts shares of the keys = 4.
 struct Shape {
@@ -62,6 +63,8 @@ struct SharedParams {
     float* raw;             // [batch][n_heads][raw_stride] scaled scores in log2 units, or null
     uint64_t raw_stride;
     uint32_t* status;
+    uint32_t prefix_weight; // cost of a prefix tile in own tiles
+    uint32_t slots, q_held; // ring slots (K or V of a tile each), query rows a warp keeps in shared memory
     uint32_t wait_last;     // the split pass runs beside the prefix kernel
     // merge
     void* o;
@@ -89,27 +92,28 @@ struct Cursor {
     uint32_t tile, tiles, len;
 };
 
-constexpr int kSplitThreads = kThreads + 32;  // four consumer warps, one producer warp
+constexpr int kSplitThreads = kThreads + 64;  // four consumer warps, the producer warp, one that notes which CTAs share each segment
 
 template <int D, bool BF16, bool RES>
 __global__ void __launch_bounds__(kSplitThreads, 2)
 shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_kp,
                     const __grid_constant__ CUtensorMap tm_vp, const __grid_constant__ SharedParams p) {
-    constexpr int kParts = D / 64;  // 128-byte parts of a head's row
-    constexpr int kStages = split_stages(D);
-    constexpr uint32_t kOperandBytes = kTilePairs * D * 2;
-    constexpr uint32_t kStageBytes = 2 * kOperandBytes;
+    constexpr int kParts = D / 64;                    // 128-byte parts of a head's row
+    constexpr uint32_t kSlotBytes = kTilePairs * D * 2;  // K or V of a tile
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);  // swizzled tiles want 1024-byte alignment
     const uint32_t ring = smem_u32(smem);
-    const uint32_t bars = ring + kStages * kStageBytes;  // full [kStages], empty [kStages]
-    uint32_t* s_cum = reinterpret_cast<uint32_t*>(smem + kStages * kStageBytes + 2 * kStages * 8);  // [batch + 1] tiles of own rows, one head group
-    uint32_t* s_warp = s_cum + p.batch + 1;                                                         // [5]
+    const uint32_t slots = p.slots;
+    const uint32_t bars = ring + slots * kSlotBytes;          // full [slots], empty [slots]
+    const uint32_t q_zero = bars + kMaxSlots * 16;            // a row of zeros
+    const uint32_t q_rows = q_zero + D * 2;                   // [4 warps][q_held rows], 16-byte chunks swizzled by the row
+    uint32_t* s_cum = reinterpret_cast<uint32_t*>(smem + (q_rows - ring) + 4 * p.q_held * D * 2);  // [batch + 1] tiles of own rows, one head group
+    uint32_t* s_warp = s_cum + p.batch + 1;                   // [6]
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     if (tid == 0) {
-        for (int i = 0; i < kStages; ++i) {
+        for (uint32_t i = 0; i < slots; ++i) {
             mbar_init(bars + 8 * i, 1);
-            mbar_init(bars + 8 * (kStages + i), 4);
+            mbar_init(bars + 8 * (slots + i), 4);
         }
         mbar_init_fence();
         prefetch_tensor_map(&tm_k);
@@ -119,6 +123,7 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             prefetch_tensor_map(&tm_vp);
         }
     }
+    if (tid < kParts * 8) st_shared_zero16(q_zero + tid * 16);
     // Behind the prefix kernel (which waits for everything in front of it before it lets this one start, and writes nothing that this
     // one reads or writes) the wait comes at the end: it only has to keep the merge pass from starting before the prefix is done.
     grid_dep_launch_dependents();
@@ -143,17 +148,27 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             uint32_t before = base;
             for (int w = 0; w < warp; ++w) before += s_warp[w];
             if (b < p.batch) s_cum[b + 1] = before + incl;
-            base += s_warp[0] + s_warp[1] + s_warp[2] + s_warp[3] + s_warp[4];
+            base += s_warp[0] + s_warp[1] + s_warp[2] + s_warp[3] + s_warp[4] + s_warp[5];
             __syncthreads();
         }
     }
-    const uint32_t pre_total = p.prefix_segs * p.prefix_tiles;
-    const uint32_t total = pre_total + s_cum[p.batch] * p.own.groups;
-    const uint32_t active = active_ctas(gridDim.x, 0, 1, total);
+    // The list in units: a prefix tile counts as many as its blocks of 16 query rows make it cost, an own tile one. A tile belongs to the
+    // CTA that has its first unit; with at least a prefix tile's units per CTA, every CTA of a segment's range has a tile of it.
+    const uint32_t pre_total = p.prefix_segs * p.prefix_tiles, pre_units = pre_total * p.prefix_weight;
+    const uint32_t own_total = s_cum[p.batch] * p.own.groups;
+    const uint32_t units = pre_units + own_total;
+    const uint32_t active = active_ctas(gridDim.x, 0, p.prefix_segs ? p.prefix_weight : 1, units);
+    auto tile_at = [&](uint32_t c) {  // the first tile of CTA c
+        const uint32_t u = static_cast<uint32_t>(static_cast<uint64_t>(c) * units / active);
+        return u < pre_units ? (u + p.prefix_weight - 1) / p.prefix_weight : pre_total + (u - pre_units);
+    };
+    auto cta_of = [&](uint32_t tile) {
+        return cta_of_tile(tile < pre_total ? tile * p.prefix_weight : pre_units + (tile - pre_total), units, active);
+    };
     uint32_t t0 = 0, t1 = 0;
     if (blockIdx.x < active) {
-        t0 = static_cast<uint32_t>(static_cast<uint64_t>(blockIdx.x) * total / active);
-        t1 = static_cast<uint32_t>((blockIdx.x + 1ull) * total / active);
+        t0 = tile_at(blockIdx.x);
+        t1 = tile_at(blockIdx.x + 1);
     }
 
     auto locate = [&](uint32_t flat, Cursor& c) {
@@ -197,38 +212,34 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             const uint64_t again = l2_policy_evict_last();
             Cursor c;
             locate(t0, c);
-            uint32_t st = 0, phase = 0, n = 0;
+            uint32_t st = 0, phase = 1;  // (a fresh barrier counts as past its odd phase: the first round does not wait)
             bool ok = true;
-            for (uint32_t t = t0; t < t1; ++t, ++n) {
-                if (n >= kStages && !mbar_wait(bars + 8 * (kStages + st), phase ^ 1)) { ok = false; break; }
-                const uint32_t full = bars + 8 * st, dst = ring + st * kStageBytes;
-                mbar_arrive_expect_tx(full, kStageBytes);
-                if (c.own) {
-                    const int row = static_cast<int>(c.tile * p.own.keys), head = static_cast<int>(c.hg * p.own.hpc);
-                    tma_load_5d_hint(dst, &tm_k, full, row, 0, head, static_cast<int>(c.b), once);
-                    tma_load_5d_hint(dst + kOperandBytes, &tm_v, full, row, 0, head, static_cast<int>(c.b), once);
-                } else {
-                    const int row = static_cast<int>(c.tile * p.pre.keys), head = static_cast<int>(c.hg * p.pre.hpc);
-                    tma_load_5d_hint(dst, &tm_kp, full, row, 0, head, 0, p.row_blocks > 1 ? again : once);
-                    tma_load_5d_hint(dst + kOperandBytes, &tm_vp, full, row, 0, head, 0, p.row_blocks > 1 ? again : once);
+            for (uint32_t t = t0; t < t1 && ok; ++t) {
+                const Shape& sh = c.own ? p.own : p.pre;
+                const int row = static_cast<int>(c.tile * sh.keys), head = static_cast<int>(c.hg * sh.hpc), seq = static_cast<int>(c.b);
+                const uint64_t policy = c.own || p.row_blocks == 1 ? once : again;
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    if (!mbar_wait(bars + 8 * (slots + st), phase)) { ok = false; break; }
+                    mbar_arrive_expect_tx(bars + 8 * st, kSlotBytes);
+                    tma_load_5d_hint(ring + st * kSlotBytes, c.own ? (v ? &tm_v : &tm_k) : (v ? &tm_vp : &tm_kp), bars + 8 * st, row, 0, head, seq, policy);
+                    if (++st == slots) st = 0, phase ^= 1;
                 }
                 advance(t + 1, c);
-                if (++st == kStages) st = 0, phase ^= 1;
             }
             if (!ok) {  // report, and leave no copy in flight into this CTA's memory
                 if (p.status) atomicOr(p.status, ATTN_STATUS_WAIT_TIMEOUT);
-                for (int i = 0; i < kStages; ++i) {
-                    (void)mbar_wait(bars + 8 * st, phase ^ 1);
-                    if (++st == kStages) st = 0, phase ^= 1;
+                for (uint32_t i = 0; i < slots; ++i) {
+                    (void)mbar_wait(bars + 8 * st, phase);
+                    if (++st == slots) st = 0, phase ^= 1;
                 }
             }
         }
         __syncwarp();
-    } else {
-        // =============================== consumers ===============================
+    } else if (warp == 5) {
         // which CTAs share each segment, for the merge pass
         const uint32_t own_segs = p.batch * p.own.groups;
-        for (uint32_t s = blockIdx.x * kThreads + tid; s < p.prefix_segs + own_segs; s += gridDim.x * kThreads) {
+        for (uint32_t s = blockIdx.x * 32 + lane; s < p.prefix_segs + own_segs; s += gridDim.x * 32) {
             uint32_t first, n;
             if (s < p.prefix_segs) {
                 first = s * p.prefix_tiles;
@@ -238,88 +249,92 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 n = s_cum[b + 1] - s_cum[b];
                 first = pre_total + s_cum[b] * p.own.groups + hg * n;
             }
-            (s < p.prefix_segs ? p.seg_pre[s] : p.seg_own[s - p.prefix_segs]) = segment_ctas(first, static_cast<uint64_t>(first) + n, total, active);
+            const uint32_t from = n ? cta_of(first) : 0, count = n ? cta_of(first + n - 1) - from + 1 : 0;
+            (s < p.prefix_segs ? p.seg_pre[s] : p.seg_own[s - p.prefix_segs]) = from | count << 16;
         }
+    } else {
+        // =============================== consumers ===============================
         Cursor cur;
         if (t0 < t1) locate(t0, cur);
-        uint32_t qa[D / 16][4];
+        const uint32_t my_q = q_rows + warp * p.q_held * (D * 2);
+        uint32_t q_lane = 0, q_xor = 0;  // this lane's row for ldmatrix, and its swizzle
         float o[D / 8][4];
         float m[2], l[2];
         bool fresh = true;  // the next tile begins a run of a segment
-        uint32_t stage = 0, phase = 0;
+        uint32_t slot = 0, phase = 0;
+        auto next_slot = [&]() {
+            if (++slot == slots) slot = 0, phase ^= 1;
+        };
+        bool ok = true;
         for (uint32_t t = t0; t < t1; ++t) {
             const Shape& sh = cur.own ? p.own : p.pre;
             // this warp's place: head hs of the group, block wr of query rows, share wk of the keys (all powers of two)
             const uint32_t hs = warp & (sh.hpc - 1), wr = (warp >> (sh.hpc >> 1)) & (sh.wm - 1), wk = warp >> ((sh.hpc >> 1) + (sh.wm >> 1));
             const uint32_t kvh = cur.hg * sh.hpc + hs;
             if (fresh) {
+                // ---- the warp's query rows into shared memory (its own: no other warp waits); rows that are not there are the row of zeros
                 fresh = false;
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const uint32_t r = wr * 16 + half * 8 + lane / 4;
-                    uint32_t b, g;
-                    bool there;
-                    if (cur.own) {
-                        b = cur.b;
-                        g = r;
-                        there = r < p.group;
-                    } else {
-                        const uint32_t row = cur.rb * sh.wm * 16 + r;
-                        b = row / p.group;
-                        g = row - b * p.group;
-                        there = b < p.batch;
-                    }
-                    const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + ((static_cast<size_t>(b) * p.n_heads) + kvh * p.group + g) * D) + lane % 4;
-#pragma unroll
-                    for (int kc = 0; kc < D / 16; ++kc) {
-                        qa[kc][half] = there ? src[kc * 8] : 0u;
-                        qa[kc][2 + half] = there ? src[kc * 8 + 4] : 0u;
-                    }
+                const uint32_t row0 = cur.own ? wr * 16 : cur.rb * sh.wm * 16 + wr * 16, all = cur.own ? p.group : p.batch * p.group;
+                const uint32_t n = row0 < all ? min(16u, all - row0) : 0u;
+                __syncwarp();
+                for (uint32_t i = lane; i < n * (kParts * 8); i += 32) {
+                    const uint32_t r = i / (kParts * 8), ch = i % (kParts * 8), row = row0 + r;
+                    const uint32_t b = cur.own ? cur.b : row / p.group, g = cur.own ? row : row - b * p.group;
+                    const uint4 x = *reinterpret_cast<const uint4*>(p.q + (static_cast<size_t>(b) * p.n_heads + kvh * p.group + g) * D + ch * 8);
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(my_q + r * (D * 2) + ((ch ^ (r & 7)) << 4)), "r"(x.x), "r"(x.y),
+                                 "r"(x.z), "r"(x.w)
+                                 : "memory");
                 }
+                __syncwarp();
+                const uint32_t r = lane & 15;
+                q_lane = r < n ? my_q + r * (D * 2) : q_zero;
+                q_xor = r < n ? r & 7 : 0;
 #pragma unroll
                 for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
                 m[0] = m[1] = -INFINITY;
                 l[0] = l[1] = 0.f;
             }
-            if (!mbar_wait(bars + 8 * stage, phase)) {
-                if (p.status) atomicOr(p.status, ATTN_STATUS_WAIT_TIMEOUT);
-                break;
-            }
             const uint32_t head_base = hs * (kParts * sh.keys * 128), part_bytes = sh.keys * 128;
-            const uint32_t kbase = ring + stage * kStageBytes + head_base, vbase = kbase + kOperandBytes;
             const uint32_t steps = sh.wm;  // 16 keys each: 64 / hpc / ts = 16 wm
+            const uint32_t first0 = cur.tile * sh.keys + wk * steps * 16;  // the warp's first key in the cache
+            const uint32_t live = first0 < cur.len ? min(steps, (cur.len - first0 + 15) / 16) : 0u;
+            const uint32_t k_slot = slot, k_phase = phase;
+            next_slot();
+            const uint32_t v_slot = slot, v_phase = phase;
+            next_slot();
+            const uint32_t kbase = ring + k_slot * kSlotBytes + head_base, vbase = ring + v_slot * kSlotBytes + head_base;
+            ok = mbar_wait(bars + 8 * k_slot, k_phase);
 #pragma unroll 1
-            for (uint32_t st = 0; st < steps; ++st) {
-                const uint32_t key0 = (wk * steps + st) * 16;      // in the tile
-                const uint32_t first = cur.tile * sh.keys + key0;  // in the cache
-                if (first >= cur.len) break;
+            for (uint32_t st = 0; st < live && ok; ++st) {
+                const uint32_t key0 = (wk * steps + st) * 16;  // in the tile
+                const uint32_t first = first0 + st * 16;       // in the cache
                 // (two chains of accumulators per eight keys: half the latency of eight dependent MMAs)
                 float s[2][4] = {}, s2[2][4] = {};
                 const uint32_t krow = kbase + (key0 + (lane >> 4) * 8 + (lane & 7)) * 128;
 #pragma unroll
                 for (int kc = 0; kc < D / 16; ++kc) {
                     const uint32_t ch = (kc * 2 + ((lane >> 3) & 1)) & 7;
-                    uint32_t b0, b1, b2, b3;
+                    uint32_t qa[4], b0, b1, b2, b3;
+                    ldmatrix_x4(qa[0], qa[1], qa[2], qa[3], q_lane + (((kc * 2 + (lane >> 4)) ^ q_xor) << 4));
                     ldmatrix_x4(b0, b1, b2, b3, krow + (kc >> 2) * part_bytes + ((ch ^ (lane & 7)) << 4));
-                    mma_16816<BF16>(kc & 1 ? s2[0] : s[0], qa[kc], b0, b1);
-                    mma_16816<BF16>(kc & 1 ? s2[1] : s[1], qa[kc], b2, b3);
+                    mma_16816<BF16>(kc & 1 ? s2[0] : s[0], qa, b0, b1);
+                    mma_16816<BF16>(kc & 1 ? s2[1] : s[1], qa, b2, b3);
+                }
+                if (st + 1 == live) {  // the keys' slot can be filled again
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bars + 8 * (slots + k_slot));
                 }
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) s[n][i] = (s[n][i] + s2[n][i]) * p.scale_log2;
-                if (first + 16 > cur.len) {  // the last rows: what lies behind them in the cache must not matter
+                const bool tail = first + 16 > cur.len;  // the last rows: what lies behind them in the cache must not matter
+                if (tail) {
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             if (first + n * 8 + (lane & 3) * 2 + (i & 1) >= cur.len) s[n][i] = -INFINITY;
-                    for (uint32_t i = lane; i < 16 * kParts * 8; i += 32) {
-                        const uint32_t r = i / (kParts * 8), in_row = i % (kParts * 8);
-                        if (first + r >= cur.len) st_shared_zero16(vbase + (in_row >> 3) * part_bytes + (key0 + r) * 128 + ((in_row & 7) << 4));
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // in front of the copy that refills the stage
-                    __syncwarp();
                 }
                 if (cur.own && p.raw) {
 #pragma unroll
@@ -369,6 +384,16 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                     pa[i] = pack2<BF16>(x, y);
                     if constexpr (RES) pr[i] = pack2<BF16>(x - round16<BF16>(x), y - round16<BF16>(y));
                 }
+                if (st == 0) ok = mbar_wait(bars + 8 * v_slot, v_phase);
+                if (!ok) break;
+                if (tail) {
+                    for (uint32_t i = lane; i < 16 * kParts * 8; i += 32) {
+                        const uint32_t r = i / (kParts * 8), in_row = i % (kParts * 8);
+                        if (first + r >= cur.len) st_shared_zero16(vbase + (in_row >> 3) * part_bytes + (key0 + r) * 128 + ((in_row & 7) << 4));
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // in front of the copy that refills the slot
+                    __syncwarp();
+                }
                 const uint32_t vrow = vbase + (key0 + ((lane >> 3) & 1) * 8 + (lane & 7)) * 128;
 #pragma unroll
                 for (int dc = 0; dc < D / 16; ++dc) {
@@ -383,9 +408,16 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                     }
                 }
             }
+            if (live == 0 && ok) ok = mbar_wait(bars + 8 * v_slot, v_phase);  // (every consumer follows every phase of every slot)
+            if (!ok) {
+                if (p.status) atomicOr(p.status, ATTN_STATUS_WAIT_TIMEOUT);
+                break;
+            }
             __syncwarp();
-            if (lane == 0) mbar_arrive(bars + 8 * (kStages + stage));
-            if (++stage == kStages) stage = 0, phase ^= 1;
+            if (lane == 0) {
+                if (live == 0) mbar_arrive(bars + 8 * (slots + k_slot));
+                mbar_arrive(bars + 8 * (slots + v_slot));
+            }
             if (cur.tile + 1 == cur.tiles || t + 1 == t1) {
                 // ---- the run's piece: normalised sum and log-sum-exp (log2 units) of this warp's rows and keys
                 const size_t rec = (static_cast<size_t>(blockIdx.x + cur.seg) * sh.ts + wk) * sh.hpc + hs;
@@ -845,11 +877,16 @@ extern "C" int attn_decode_shared(const AttnDecodeSharedArgs* a, void* stream_v)
             (rc = tile_map(&tm_vp, a->v_prefix, bf16, a->head_dim, p.prefix, p.n_kv_heads, 1, prefix_row_stride, 0, p.pre)) != ATTN_OK)
             return rc;
     }
+    // Shared memory: alignment, the ring, its barriers, the row of zeros, four warps' query rows, s_cum, s_warp; as many slots as fit.
+    const size_t slot_bytes = static_cast<size_t>(kTilePairs) * a->head_dim * 2;
+    in_split.q_held = in_split.prefix_segs ? 16 : std::min<uint32_t>(16, p.group);
+    const size_t fixed = 1024 + kMaxSlots * 16 + (1 + 4 * in_split.q_held) * a->head_dim * 2 + (a->batch + 1 + 6) * 4;
+    in_split.slots = static_cast<uint32_t>(std::min<size_t>(kMaxSlots, (kSplitSmem - fixed) / slot_bytes));
+    const size_t smem = fixed + in_split.slots * slot_bytes;
+    in_split.prefix_weight = std::max(1u, p.pre.wm / p.own.wm);
+    if (most * in_split.prefix_weight > 0x7fffffffull) return ATTN_ERR_UNSUPPORTED;  // 32-bit units
     auto split = [&](auto kernel) -> int {
         B200_CUDA_TRY(allow_max_smem(kernel));
-        // alignment, the ring, its barriers, s_cum, s_warp
-        const int stages = split_stages(static_cast<int>(a->head_dim));
-        const size_t smem = 1024 + static_cast<size_t>(stages) * (2 * kTilePairs * a->head_dim * 2 + 16) + (a->batch + 1 + 5) * 4;
         B200_CUDA_TRY(launch_dependent(kernel, dim3(grid), dim3(kSplitThreads), smem, stream, tm_k, tm_v, tm_kp, tm_vp, in_split));
         g_launch_count.fetch_add(1, std::memory_order_relaxed);
         return ATTN_OK;
