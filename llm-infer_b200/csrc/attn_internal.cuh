@@ -260,7 +260,8 @@ struct SharedPrefixParams {
     uint32_t batch, n_heads, n_kv_heads, group, head_dim, prefix;
     uint32_t pairs, segments, grid;
     uint32_t ctas_per_seg;  // > 0: that many CTAs for each segment; 0: the blocks of all segments dealt equally, runs may cross segments
-    float scale_log2;
+    float scale_log2;    // of the scale's magnitude; q_sign flips the query's sign for a negative one
+    uint32_t q_sign;
     uint32_t* status;
     uint32_t bf16, residual;
 };

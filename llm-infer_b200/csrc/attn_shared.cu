@@ -20,7 +20,9 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdlib>
+#include <type_traits>
 
 #include "attn_internal.cuh"
 #include "ptx_sm100.cuh"
@@ -49,7 +51,8 @@ struct SharedParams {
     uint32_t kv_len_uniform;
     uint32_t batch, n_heads, n_kv_heads, group;
     uint32_t prefix, rows;
-    float scale_log2;
+    float scale_log2;       // of the scale's magnitude
+    uint32_t q_sign;        // 0x80008000 for a negative scale: flips the query's sign instead
     Shape pre, own;
     uint32_t row_blocks;    // blocks of 16 * pre.wm query rows against the prefix
     uint32_t prefix_segs;   // pre.groups * row_blocks; 0 in the split pass when another kernel takes the prefix
@@ -99,7 +102,8 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
 shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_kp,
                     const __grid_constant__ CUtensorMap tm_vp, const __grid_constant__ SharedParams p) {
     constexpr int kParts = D / 64;                    // 128-byte parts of a head's row
-    constexpr uint32_t kSlotBytes = kTilePairs * D * 2;  // K or V of a tile
+    constexpr uint32_t kPartBytes = kTilePairs * 128;    // of all heads and keys of a tile
+    constexpr uint32_t kSlotBytes = kParts * kPartBytes; // K or V of a tile
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);  // swizzled tiles want 1024-byte alignment
     const uint32_t ring = smem_u32(smem);
@@ -222,7 +226,7 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 for (int v = 0; v < 2; ++v) {
                     if (!mbar_wait(bars + 8 * (slots + st), phase)) { ok = false; break; }
                     mbar_arrive_expect_tx(bars + 8 * st, kSlotBytes);
-                    tma_load_5d_hint(ring + st * kSlotBytes, c.own ? (v ? &tm_v : &tm_k) : (v ? &tm_vp : &tm_kp), bars + 8 * st, row, 0, head, seq, policy);
+                    tma_load_5d_hint(ring + st * kSlotBytes, c.own ? (v ? &tm_v : &tm_k) : (v ? &tm_vp : &tm_kp), bars + 8 * st, row, head, 0, seq, policy);
                     if (++st == slots) st = 0, phase ^= 1;
                 }
                 advance(t + 1, c);
@@ -257,7 +261,14 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         Cursor cur;
         if (t0 < t1) locate(t0, cur);
         const uint32_t my_q = q_rows + warp * p.q_held * (D * 2);
-        uint32_t q_lane = 0, q_xor = 0;  // this lane's row for ldmatrix, and its swizzle
+        // Offsets of the 16-byte chunks that this lane hands to ldmatrix, four of them in a 128-byte part: keys, values, query row.
+        uint32_t k_off[4], v_off[4], q_off[4], q_lane = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            k_off[i] = ((i * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4;
+            v_off[i] = ((i * 2 + (lane >> 4)) ^ (lane & 7)) << 4;
+            q_off[i] = 0;
+        }
         float o[D / 8][4];
         float m[2], l[2];
         bool fresh = true;  // the next tile begins a run of a segment
@@ -280,7 +291,8 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 for (uint32_t i = lane; i < n * (kParts * 8); i += 32) {
                     const uint32_t r = i / (kParts * 8), ch = i % (kParts * 8), row = row0 + r;
                     const uint32_t b = cur.own ? cur.b : row / p.group, g = cur.own ? row : row - b * p.group;
-                    const uint4 x = *reinterpret_cast<const uint4*>(p.q + (static_cast<size_t>(b) * p.n_heads + kvh * p.group + g) * D + ch * 8);
+                    uint4 x = *reinterpret_cast<const uint4*>(p.q + (static_cast<size_t>(b) * p.n_heads + kvh * p.group + g) * D + ch * 8);
+                    x.x ^= p.q_sign, x.y ^= p.q_sign, x.z ^= p.q_sign, x.w ^= p.q_sign;  // a negative scale's sign
                     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(my_q + r * (D * 2) + ((ch ^ (r & 7)) << 4)), "r"(x.x), "r"(x.y),
                                  "r"(x.z), "r"(x.w)
                                  : "memory");
@@ -288,13 +300,21 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 __syncwarp();
                 const uint32_t r = lane & 15;
                 q_lane = r < n ? my_q + r * (D * 2) : q_zero;
-                q_xor = r < n ? r & 7 : 0;
+                // the next segment's rows, on their way into L1 (rows of the list's own segments follow one another in q)
+                if (cur.own && t + (cur.tiles - cur.tile) < t1) {
+                    const uint64_t next = static_cast<uint64_t>(cur.b) * p.n_heads + (kvh + sh.hpc) * p.group + row0;
+                    for (uint32_t i = lane; i < n * (kParts * 8); i += 32)
+                        if (i % 8 == 0 && next + i / (kParts * 8) < static_cast<uint64_t>(p.batch) * p.n_heads)
+                            asm volatile("prefetch.global.L1 [%0];" ::"l"(p.q + next * D + i * 8));
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) q_off[i] = ((i * 2 + (lane >> 4)) ^ (r < n ? r & 7 : 0)) << 4;
 #pragma unroll
                 for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
                 m[0] = m[1] = -INFINITY;
                 l[0] = l[1] = 0.f;
             }
-            const uint32_t head_base = hs * (kParts * sh.keys * 128), part_bytes = sh.keys * 128;
+            const uint32_t head_base = hs * (sh.keys * 128);
             const uint32_t steps = sh.wm;  // 16 keys each: 64 / hpc / ts = 16 wm
             const uint32_t first0 = cur.tile * sh.keys + wk * steps * 16;  // the warp's first key in the cache
             const uint32_t live = first0 < cur.len ? min(steps, (cur.len - first0 + 15) / 16) : 0u;
@@ -304,34 +324,43 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             next_slot();
             const uint32_t kbase = ring + k_slot * kSlotBytes + head_base, vbase = ring + v_slot * kSlotBytes + head_base;
             ok = mbar_wait(bars + 8 * k_slot, k_phase);
-#pragma unroll 1
-            for (uint32_t st = 0; st < live && ok; ++st) {
+            // Scores, probabilities and products of NB blocks of 16 keys.
+            auto blocks = [&](auto nb, uint32_t st) {
+                constexpr int NB = decltype(nb)::value;
                 const uint32_t key0 = (wk * steps + st) * 16;  // in the tile
                 const uint32_t first = first0 + st * 16;       // in the cache
-                // (two chains of accumulators per eight keys: half the latency of eight dependent MMAs)
-                float s[2][4] = {}, s2[2][4] = {};
-                const uint32_t krow = kbase + (key0 + (lane >> 4) * 8 + (lane & 7)) * 128;
+                float s[2 * NB][4] = {};
+                {
+                    // (one block: two chains of accumulators, half the latency of eight dependent MMAs)
+                    float s2[2][4] = {};
+                    const uint32_t krow = kbase + (key0 + (lane >> 4) * 8 + (lane & 7)) * 128;
 #pragma unroll
-                for (int kc = 0; kc < D / 16; ++kc) {
-                    const uint32_t ch = (kc * 2 + ((lane >> 3) & 1)) & 7;
-                    uint32_t qa[4], b0, b1, b2, b3;
-                    ldmatrix_x4(qa[0], qa[1], qa[2], qa[3], q_lane + (((kc * 2 + (lane >> 4)) ^ q_xor) << 4));
-                    ldmatrix_x4(b0, b1, b2, b3, krow + (kc >> 2) * part_bytes + ((ch ^ (lane & 7)) << 4));
-                    mma_16816<BF16>(kc & 1 ? s2[0] : s[0], qa, b0, b1);
-                    mma_16816<BF16>(kc & 1 ? s2[1] : s[1], qa, b2, b3);
+                    for (int kc = 0; kc < D / 16; ++kc) {
+                        uint32_t qa[4];
+                        ldmatrix_x4(qa[0], qa[1], qa[2], qa[3], q_lane + q_off[kc & 3] + (kc >> 2) * 128);
+#pragma unroll
+                        for (int n = 0; n < NB; ++n) {
+                            uint32_t b0, b1, b2, b3;
+                            ldmatrix_x4(b0, b1, b2, b3, krow + k_off[kc & 3] + (kc >> 2) * kPartBytes + n * 2048);
+                            mma_16816<BF16>(NB == 1 && (kc & 1) ? s2[0] : s[2 * n], qa, b0, b1);
+                            mma_16816<BF16>(NB == 1 && (kc & 1) ? s2[1] : s[2 * n + 1], qa, b2, b3);
+                        }
+                    }
+                    if constexpr (NB == 1) {
+#pragma unroll
+                        for (int n = 0; n < 2; ++n)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) s[n][i] += s2[n][i];
+                    }
                 }
-                if (st + 1 == live) {  // the keys' slot can be filled again
+                if (st + NB >= live) {  // the keys' slot can be filled again
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bars + 8 * (slots + k_slot));
                 }
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[n][i] = (s[n][i] + s2[n][i]) * p.scale_log2;
-                const bool tail = first + 16 > cur.len;  // the last rows: what lies behind them in the cache must not matter
+                const bool tail = first + 16 * NB > cur.len;  // the last rows: what lies behind them in the cache must not matter
                 if (tail) {
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
+                    for (int n = 0; n < 2 * NB; ++n)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             if (first + n * 8 + (lane & 3) * 2 + (i & 1) >= cur.len) s[n][i] = -INFINITY;
@@ -342,22 +371,30 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                         const uint32_t g = wr * 16 + half * 8 + lane / 4;
                         if (g < p.group) {
                             float* dst = p.raw + (static_cast<size_t>(cur.b) * p.n_heads + kvh * p.group + g) * p.raw_stride + first + (lane & 3) * 2;
-                            *reinterpret_cast<float2*>(dst) = make_float2(s[0][2 * half], s[0][2 * half + 1]);
-                            *reinterpret_cast<float2*>(dst + 8) = make_float2(s[1][2 * half], s[1][2 * half + 1]);
+#pragma unroll
+                            for (int n = 0; n < 2 * NB; ++n)
+                                if (n < 2 || first + n * 8 < cur.len)  // (the row of scores is a multiple of 16 keys long)
+                                    *reinterpret_cast<float2*>(dst + n * 8) = make_float2(s[n][2 * half] * p.scale_log2, s[n][2 * half + 1] * p.scale_log2);
                         }
                     }
                 }
-                float mx[2], safe[2];
+                // The maximum that the probabilities are relative to moves only when it grew by more than 2^8: the true sum
+                // normalises at the end, and probabilities stay below 2^8.
+                float mx[2];
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    float x = fmaxf(fmaxf(s[0][2 * half], s[0][2 * half + 1]), fmaxf(s[1][2 * half], s[1][2 * half + 1]));
+                    float x = fmaxf(s[0][2 * half], s[0][2 * half + 1]);
+#pragma unroll
+                    for (int n = 1; n < 2 * NB; ++n) x = fmaxf(x, fmaxf(s[n][2 * half], s[n][2 * half + 1]));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-                    mx[half] = fmaxf(m[half], x);
-                    safe[half] = mx[half] == -INFINITY ? 0.f : mx[half];
+                    mx[half] = x * p.scale_log2;
                 }
-                if (__any_sync(0xffffffffu, mx[0] != m[0] || mx[1] != m[1])) {
-                    const float f0 = fast_exp2(m[0] - safe[0]), f1 = fast_exp2(m[1] - safe[1]);
+                const bool grow0 = mx[0] > m[0] + 8.f, grow1 = mx[1] > m[1] + 8.f;
+                if (__any_sync(0xffffffffu, grow0 || grow1)) {
+                    const float f0 = grow0 ? fast_exp2(m[0] - mx[0]) : 1.f, f1 = grow1 ? fast_exp2(m[1] - mx[1]) : 1.f;
+                    if (grow0) m[0] = mx[0];
+                    if (grow1) m[1] = mx[1];
                     l[0] *= f0;
                     l[1] *= f1;
 #pragma unroll
@@ -367,46 +404,54 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                         o[i][2] *= f1;
                         o[i][3] *= f1;
                     }
-                    m[0] = mx[0];
-                    m[1] = mx[1];
                 }
+                const float ref[2] = {m[0] == -INFINITY ? 0.f : -m[0], m[1] == -INFINITY ? 0.f : -m[1]};
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                for (int n = 0; n < 2 * NB; ++n)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        s[n][i] = fast_exp2(s[n][i] - safe[i >> 1]);
+                        s[n][i] = fast_exp2(fmaf(s[n][i], p.scale_log2, ref[i >> 1]));
                         l[i >> 1] += s[n][i];
                     }
-                uint32_t pa[4], pr[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float x = s[i >> 1][(i & 1) * 2], y = s[i >> 1][(i & 1) * 2 + 1];
-                    pa[i] = pack2<BF16>(x, y);
-                    if constexpr (RES) pr[i] = pack2<BF16>(x - round16<BF16>(x), y - round16<BF16>(y));
-                }
                 if (st == 0) ok = mbar_wait(bars + 8 * v_slot, v_phase);
-                if (!ok) break;
+                if (!ok) return;
                 if (tail) {
-                    for (uint32_t i = lane; i < 16 * kParts * 8; i += 32) {
+                    for (uint32_t i = lane; i < NB * 16 * kParts * 8; i += 32) {
                         const uint32_t r = i / (kParts * 8), in_row = i % (kParts * 8);
-                        if (first + r >= cur.len) st_shared_zero16(vbase + (in_row >> 3) * part_bytes + (key0 + r) * 128 + ((in_row & 7) << 4));
+                        if (first + r >= cur.len) st_shared_zero16(vbase + (in_row >> 3) * kPartBytes + (key0 + r) * 128 + ((in_row & 7) << 4));
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // in front of the copy that refills the slot
                     __syncwarp();
                 }
                 const uint32_t vrow = vbase + (key0 + ((lane >> 3) & 1) * 8 + (lane & 7)) * 128;
 #pragma unroll
-                for (int dc = 0; dc < D / 16; ++dc) {
-                    const uint32_t ch = (dc * 2 + (lane >> 4)) & 7;
-                    uint32_t b0, b1, b2, b3;
-                    ldmatrix_x4_trans(b0, b1, b2, b3, vrow + (dc >> 2) * part_bytes + ((ch ^ (lane & 7)) << 4));
-                    mma_16816<BF16>(o[2 * dc], pa, b0, b1);
-                    mma_16816<BF16>(o[2 * dc + 1], pa, b2, b3);
-                    if constexpr (RES) {
-                        mma_16816<BF16>(o[2 * dc], pr, b0, b1);
-                        mma_16816<BF16>(o[2 * dc + 1], pr, b2, b3);
+                for (int n = 0; n < NB; ++n) {
+                    uint32_t pa[4];
+                    [[maybe_unused]] uint32_t pr[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float x = s[2 * n + (i >> 1)][(i & 1) * 2], y = s[2 * n + (i >> 1)][(i & 1) * 2 + 1];
+                        pa[i] = pack2<BF16>(x, y);
+                        if constexpr (RES) pr[i] = pack2<BF16>(x - round16<BF16>(x), y - round16<BF16>(y));
+                    }
+#pragma unroll
+                    for (int dc = 0; dc < D / 16; ++dc) {
+                        uint32_t b0, b1, b2, b3;
+                        ldmatrix_x4_trans(b0, b1, b2, b3, vrow + v_off[dc & 3] + (dc >> 2) * kPartBytes + n * 2048);
+                        mma_16816<BF16>(o[2 * dc], pa, b0, b1);
+                        mma_16816<BF16>(o[2 * dc + 1], pa, b2, b3);
+                        if constexpr (RES) {
+                            mma_16816<BF16>(o[2 * dc], pr, b0, b1);
+                            mma_16816<BF16>(o[2 * dc + 1], pr, b2, b3);
+                        }
                     }
                 }
+            };
+            if (steps == 1) {
+                if (live && ok) blocks(std::integral_constant<int, 1>{}, 0);
+            } else {  // (a second block behind the last keys is masked like the rest of a last block)
+#pragma unroll 1
+                for (uint32_t st = 0; st < live && ok; st += 2) blocks(std::integral_constant<int, 2>{}, st);
             }
             if (live == 0 && ok) ok = mbar_wait(bars + 8 * v_slot, v_phase);  // (every consumer follows every phase of every slot)
             if (!ok) {
@@ -703,15 +748,15 @@ int make_shared_plan(uint32_t batch, uint32_t n_heads, uint32_t n_kv_heads, uint
     return ATTN_OK;
 }
 
-// Cache rows as [sequence][kv head][128-byte part of a head][row][64 elements]; a box is a tile: all parts of hpc heads over its
+// Cache rows as [sequence][128-byte part of a head][kv head][row][64 elements]; a box is a tile: all parts of hpc heads over its
 // rows. Rows that the cache does not have read as zeros.
 int tile_map(CUtensorMap* map, const void* cache, bool bf16, uint32_t head_dim, uint32_t rows, uint32_t kv_heads, uint32_t batch,
              uint64_t row_stride, uint64_t batch_stride, const Shape& sh) {
     EncodeTiledFn enc = encode_tiled_fn();
     if (!enc) return ATTN_ERR_CUDA;
-    const cuuint64_t dims[5] = {64, rows, head_dim / 64, kv_heads, batch};
-    const cuuint64_t strides[4] = {row_stride * 2, 128, head_dim * 2ull, (batch > 1 ? batch_stride : row_stride * rows) * 2};
-    const cuuint32_t box[5] = {64, sh.keys, head_dim / 64, sh.hpc, 1};
+    const cuuint64_t dims[5] = {64, rows, kv_heads, head_dim / 64, batch};
+    const cuuint64_t strides[4] = {row_stride * 2, head_dim * 2ull, 128, (batch > 1 ? batch_stride : row_stride * rows) * 2};
+    const cuuint32_t box[5] = {64, sh.keys, sh.hpc, head_dim / 64, 1};
     const cuuint32_t unit[5] = {1, 1, 1, 1, 1};
     const CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(cache), dims,
                            strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -721,14 +766,56 @@ int tile_map(CUtensorMap* map, const void* cache, bool bf16, uint32_t head_dim, 
     return ATTN_ERR_CUDA;
 }
 
-// Whether the prefix goes to the tensor-core kernel, by query rows per kv head and key blocks in all.
+// Which kernel takes the prefix, and how the SMs are shared. The split pass can take it along with the own rows in one launch; the
+// tensor-core kernel does many query rows or long prefixes faster, but is a launch more. Where it takes fewer CTAs than there are
+// SMs, the split pass runs beside it on the others. Times in us, measured on shapes of 64- and 128-dimension heads (graphs of calls).
+struct PrefixChoice {
+    bool tensor;
+    uint32_t prefix_ctas, split_ctas;
+};
 constexpr uint32_t kMinPrefixBlocks = 2;  // of a CTA
 constexpr uint32_t kPieceBlocks = 4;
-bool prefix_on_tensor_cores(uint32_t prefix, uint32_t query_rows, uint64_t blocks) {
+PrefixChoice choose_prefix(const SharedPlan& plan, uint32_t sms, uint32_t head_dim, uint64_t prefix_tiles, uint64_t own_tiles, uint64_t blocks,
+                           uint32_t query_rows) {
+    const uint64_t all = prefix_tiles + own_tiles;
+    PrefixChoice c{false, 0, static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(2 * sms, all)))};
+    if (prefix_tiles == 0) return c;
 #ifdef ATTN_TRACE
-    if (const char* e = getenv("ATTN_TRACE_PREFIX")) return prefix > 0 && atoi(e) != 0;  // profiling knob
+    const char* knob = getenv("ATTN_TRACE_PREFIX");  // profiling knob
+    if (knob && atoi(knob) == 0) return c;
 #endif
-    return prefix > 0 && query_rows > 16 && blocks >= 64;
+    const double dim = head_dim / 128.0;
+    const double tile_bytes = 32768.0 * dim, bandwidth = 6.2e6;  // bytes per us
+    const double own_tile = 0.55 * dim, launch = 5.0;            // us of an SM per own tile; a launch's fixed part
+    const double shared_tile = (plan.pre.wm == 4 ? 1.15 : plan.pre.wm == 2 ? 0.65 : 0.55) * dim;  // of a prefix tile in the split pass
+    const double block = (query_rows > 128 ? 1.1 : 0.8) * (0.4 + 0.6 * dim);                      // of a key block in the tensor-core kernel
+    const double block_bytes = 16384.0 * 2 * dim;
+    auto split_time = [&](double ctas) {
+        const double sm = ctas / 2;
+        return launch + std::max(own_tiles * own_tile / sm, own_tiles * tile_bytes / bandwidth);
+    };
+    auto prefix_time = [&](double ctas) { return launch + 1.0 + std::max(std::ceil(blocks / ctas) * block, blocks / plan.pairs * block_bytes / bandwidth); };
+    const double together = launch + std::max((prefix_tiles * shared_tile + own_tiles * own_tile) / sms, all * tile_bytes / bandwidth);
+    // one behind the other
+    const uint32_t most = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(sms, blocks / kMinPrefixBlocks)));
+    double best = prefix_time(most) + split_time(2.0 * sms) - 2.0;
+    c.prefix_ctas = most;
+    const uint32_t split_all = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(2 * sms, own_tiles)));
+    c.split_ctas = split_all;
+    // side by side
+    const double both = launch + (own_tiles * tile_bytes + blocks / plan.pairs * block_bytes) / bandwidth;
+    for (uint32_t n = 8; n < sms; n += 4) {
+        if (n > most) break;
+        const uint32_t m = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(2 * (sms - n), own_tiles)));
+        const double t = std::max(std::max(prefix_time(n), split_time(m)), both);
+        if (t < best) best = t, c.prefix_ctas = n, c.split_ctas = m;
+    }
+    c.tensor = best + 1.5 < together;
+#ifdef ATTN_TRACE
+    if (knob) c.tensor = true;
+#endif
+    if (!c.tensor) c.split_ctas = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(2 * sms, all)));
+    return c;
 }
 
 }  // namespace
@@ -825,7 +912,14 @@ extern "C" int attn_decode_shared(const AttnDecodeSharedArgs* a, void* stream_v)
     cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
     const bool bf16 = a->dtype == ATTN_DTYPE_BF16, res = a->o_dtype == ATTN_DTYPE_F32;
     const uint64_t blocks = (static_cast<uint64_t>(a->prefix_len) + kPrefixBlock - 1) / kPrefixBlock * plan.tensor_segs;
-    const bool tensor = prefix_on_tensor_cores(a->prefix_len, a->batch * p.group, blocks) && scale > 0.f && blocks <= 0x7fffffffull;
+    // (lengths that lie on the device are taken to be five eighths of the capacity)
+    const uint64_t own_guess = a->kv_len ? own_tiles * plan.own_segs * 5 / 8
+                                         : (std::min(a->kv_len_uniform, a->kv_capacity) + plan.own.keys - 1ull) / plan.own.keys * plan.own_segs;
+    PrefixChoice choice = choose_prefix(plan, dev.sm_count, a->head_dim, prefix_tiles * p.prefix_segs, own_guess, blocks, a->batch * p.group);
+    if (blocks > 0x7fffffffull) choice.tensor = false;
+    const bool tensor = choice.tensor;
+    p.scale_log2 = fabsf(p.scale_log2);
+    p.q_sign = scale < 0.f ? 0x80008000u : 0u;
     SharedParams in_split = p;
     if (tensor) {
         SharedPrefixParams t{};
@@ -844,7 +938,8 @@ extern "C" int attn_decode_shared(const AttnDecodeSharedArgs* a, void* stream_v)
         t.prefix = p.prefix;
         t.pairs = plan.pairs;
         t.segments = plan.tensor_segs;
-        t.grid = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(plan.tensor_grid, blocks / kMinPrefixBlocks)));
+        t.grid = choice.prefix_ctas;
+        t.q_sign = p.q_sign;
         // A run that crosses from one segment into the next pays a second set of query rows and a second piece, about as much as
         // kPieceBlocks blocks: whole CTAs per segment unless that makes the longest run longer by more.
         const uint64_t seg_blocks = blocks / plan.tensor_segs, per_seg = std::min<uint64_t>(t.grid / plan.tensor_segs, seg_blocks);
@@ -864,8 +959,7 @@ extern "C" int attn_decode_shared(const AttnDecodeSharedArgs* a, void* stream_v)
         p.row_blocks = plan.pairs;
         p.prefix_segs = plan.tensor_segs;
     }
-    const uint64_t most = prefix_tiles * in_split.prefix_segs + own_tiles * plan.own_segs;
-    const uint32_t grid = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(plan.grid, most)));
+    const uint32_t grid = choice.split_ctas;
     CUtensorMap tm_k{}, tm_v{}, tm_kp{}, tm_vp{};
     if (a->kv_capacity) {
         if ((rc = tile_map(&tm_k, a->k, bf16, a->head_dim, p.rows, p.n_kv_heads, p.batch, row_stride, batch_stride, p.own)) != ATTN_OK ||
@@ -883,8 +977,9 @@ extern "C" int attn_decode_shared(const AttnDecodeSharedArgs* a, void* stream_v)
     const size_t fixed = 1024 + kMaxSlots * 16 + (1 + 4 * in_split.q_held) * a->head_dim * 2 + (a->batch + 1 + 6) * 4;
     in_split.slots = static_cast<uint32_t>(std::min<size_t>(kMaxSlots, (kSplitSmem - fixed) / slot_bytes));
     const size_t smem = fixed + in_split.slots * slot_bytes;
-    in_split.prefix_weight = std::max(1u, p.pre.wm / p.own.wm);
-    if (most * in_split.prefix_weight > 0x7fffffffull) return ATTN_ERR_UNSUPPORTED;  // 32-bit units
+    // A prefix tile of four row blocks keeps a CTA as busy as two own tiles; others are as fast as memory in either form.
+    in_split.prefix_weight = plan.pre.wm == 4 && plan.own.wm == 1 ? 2 : 1;
+    if ((prefix_tiles * in_split.prefix_segs + own_tiles * plan.own_segs) * in_split.prefix_weight > 0x7fffffffull) return ATTN_ERR_UNSUPPORTED;  // 32-bit units
     auto split = [&](auto kernel) -> int {
         B200_CUDA_TRY(allow_max_smem(kernel));
         B200_CUDA_TRY(launch_dependent(kernel, dim3(grid), dim3(kSplitThreads), smem, stream, tm_k, tm_v, tm_kp, tm_vp, in_split));

@@ -179,7 +179,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 #pragma unroll
                     for (int c = 0; c < 8; ++c)
                         asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + half * kSubTileBytes + ((c ^ (r & 7)) << 4)),
-                                     "r"(x[c].x), "r"(x[c].y), "r"(x[c].z), "r"(x[c].w)
+                                     "r"(x[c].x ^ p.q_sign), "r"(x[c].y ^ p.q_sign), "r"(x[c].z ^ p.q_sign), "r"(x[c].w ^ p.q_sign)
                                      : "memory");
                 }
                 fence_async_smem();
