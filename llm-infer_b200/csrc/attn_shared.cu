@@ -211,6 +211,9 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 
     if (warp == 4) {
         // =============================== producer ===============================
+        // 28 MB of tiles are requested at once as soon as the CTAs know theirs, and query rows that are requested behind them came 3 to
+        // 5 us later, with no tile worked on until then: the consumers' requests go first.
+        if (t0 < t1) block_wait(1, kThreads + 32);
         if (lane == 0 && t0 < t1) {
             const uint64_t once = l2_policy_evict_first();  // own rows are read once; the prefix's may be read by several blocks of rows
             const uint64_t again = l2_policy_evict_last();
@@ -287,11 +290,18 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 fresh = false;
                 const uint32_t row0 = cur.own ? wr * 16 : cur.rb * sh.wm * 16 + wr * 16, all = cur.own ? p.group : p.batch * p.group;
                 const uint32_t n = row0 < all ? min(16u, all - row0) : 0u;
+                auto q_at = [&](uint32_t r, uint32_t ch) {  // chunk ch of the warp's row r
+                    const uint32_t row = row0 + r, b = cur.own ? cur.b : row / p.group, g = cur.own ? row : row - b * p.group;
+                    return p.q + (static_cast<size_t>(b) * p.n_heads + kvh * p.group + g) * D + ch * 8;
+                };
+                if (t == t0) {
+                    if (lane < n * kParts) touch(q_at(lane / kParts, lane % kParts * 8));
+                    block_arrive(1, kThreads + 32);
+                }
                 __syncwarp();
                 for (uint32_t i = lane; i < n * (kParts * 8); i += 32) {
-                    const uint32_t r = i / (kParts * 8), ch = i % (kParts * 8), row = row0 + r;
-                    const uint32_t b = cur.own ? cur.b : row / p.group, g = cur.own ? row : row - b * p.group;
-                    uint4 x = *reinterpret_cast<const uint4*>(p.q + (static_cast<size_t>(b) * p.n_heads + kvh * p.group + g) * D + ch * 8);
+                    const uint32_t r = i / (kParts * 8), ch = i % (kParts * 8);
+                    uint4 x = *reinterpret_cast<const uint4*>(q_at(r, ch));
                     x.x ^= p.q_sign, x.y ^= p.q_sign, x.z ^= p.q_sign, x.w ^= p.q_sign;  // a negative scale's sign
                     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(my_q + r * (D * 2) + ((ch ^ (r & 7)) << 4)), "r"(x.x), "r"(x.y),
                                  "r"(x.z), "r"(x.w)
@@ -305,7 +315,7 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                     const uint64_t next = static_cast<uint64_t>(cur.b) * p.n_heads + (kvh + sh.hpc) * p.group + row0;
                     for (uint32_t i = lane; i < n * (kParts * 8); i += 32)
                         if (i % 8 == 0 && next + i / (kParts * 8) < static_cast<uint64_t>(p.batch) * p.n_heads)
-                            asm volatile("prefetch.global.L1 [%0];" ::"l"(p.q + next * D + i * 8));
+                            prefetch_l1(p.q + next * D + i * 8);
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) q_off[i] = ((i * 2 + (lane >> 4)) ^ (r < n ? r & 7 : 0)) << 4;

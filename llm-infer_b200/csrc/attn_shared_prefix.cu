@@ -157,6 +157,17 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         uint32_t g0 = 0;  // key blocks of this tile before the current item: buffer and barrier phases run on over the items
         bool staged = false;
         Item w;
+        // The first item's query rows are requested ahead of the tiles: behind them they came 3 us later.
+        if (item_at(t0, w)) {
+            const uint32_t m = w.m0 + t * BM + r;
+            if (m < query_rows) {
+                const uint32_t b = m / p.group, g = m - b * p.group;
+                const uint16_t* src = static_cast<const uint16_t*>(p.q) + (static_cast<size_t>(b) * p.n_heads + w.kvh * p.group + g) * HD;
+#pragma unroll
+                for (int half = 0; half < HD / 64; ++half) touch(src + half * 64);
+            }
+        }
+        block_arrive(3, 288);
         for (uint32_t at = t0; ok && item_at(at, w); at += w.blocks) {
             if (!w.tile[t]) continue;
             // ---- this thread's query row into the tile (the previous item's MMAs are over, its result has left)
@@ -331,6 +342,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         if ((warp & 3) == 0 && lane == 0) tma_store_wait_all();
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 8) block_wait(3, 288);
         if (warp == 8 && elect_one()) {
             // =============================== TMA producer ===============================
             uint32_t st = 0, phase = 0, it = 0;

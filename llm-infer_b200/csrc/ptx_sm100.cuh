@@ -184,6 +184,16 @@ __device__ __forceinline__ float round16(float x) {
     }
 }
 
+__device__ __forceinline__ void prefetch_l1(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
+// Requests the line that holds *p into L1 by a load whose value nobody waits for.
+__device__ __forceinline__ void touch(const void* p) {
+    uint32_t unused;
+    asm volatile("ld.global.u32 %0, [%1];" : "=r"(unused) : "l"(p) : "memory");
+}
+// The two halves of a barrier between some warps of a block: `threads` counts those that arrive and those that wait.
+__device__ __forceinline__ void block_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ void block_wait(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
 // Programmatic dependent launch: the dependent grid may start once every CTA of
 // this grid has called this (or exited); it still has to call grid_dep_wait()
 // before it touches what this grid writes.
