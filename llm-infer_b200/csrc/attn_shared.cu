@@ -67,6 +67,7 @@ struct SharedParams {
     uint64_t raw_stride;
     uint32_t* status;
     uint32_t prefix_weight; // cost of a prefix tile in own tiles
+    uint32_t switch_units;  // cost of an own segment's start in own tiles
     uint32_t slots, q_held; // ring slots (K or V of a tile each), query rows a warp keeps in shared memory
     uint32_t wait_last;     // the split pass runs beside the prefix kernel
     // merge
@@ -93,6 +94,7 @@ struct Cursor {
     uint32_t own, seg;         // kind; index among the segments of its kind
     uint32_t b, hg, rb;        // own: sequence; head group; prefix: block of query rows
     uint32_t tile, tiles, len;
+    uint32_t unit;             // the tile's first unit of the list
 };
 
 constexpr int kSplitThreads = kThreads + 64;  // four consumer warps, the producer warp, one that notes which CTAs share each segment
@@ -111,7 +113,7 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     const uint32_t bars = ring + slots * kSlotBytes;          // full [slots], empty [slots]
     const uint32_t q_zero = bars + kMaxSlots * 16;            // a row of zeros
     const uint32_t q_rows = q_zero + D * 2;                   // [4 warps][q_held rows], 16-byte chunks swizzled by the row
-    uint32_t* s_cum = reinterpret_cast<uint32_t*>(smem + (q_rows - ring) + 4 * p.q_held * D * 2);  // [batch + 1] tiles of own rows, one head group
+    uint32_t* s_cum = reinterpret_cast<uint32_t*>(smem + (q_rows - ring) + 4 * p.q_held * D * 2);  // [batch + 1] units of own rows, one head group
     uint32_t* s_warp = s_cum + p.batch + 1;                   // [6]
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     if (tid == 0) {
@@ -133,13 +135,17 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     grid_dep_launch_dependents();
     if (!p.wait_last) grid_dep_wait();
 
-    // ---- tiles of each sequence, summed up: as many sequences as threads at a time
+    // ---- units of each sequence and head group, summed up: as many sequences as threads at a time
+    auto own_units = [&](uint32_t b) {
+        const uint32_t tiles = (own_len(p, b) + p.own.keys - 1) / p.own.keys;
+        return tiles ? tiles + p.switch_units : 0u;
+    };
     {
         uint32_t base = 0;
         if (tid == 0) s_cum[0] = 0;
         for (uint32_t b0 = 0; b0 < p.batch; b0 += kSplitThreads) {
             const uint32_t b = b0 + tid;
-            uint32_t n = b < p.batch ? (own_len(p, b) + p.own.keys - 1) / p.own.keys : 0u;
+            const uint32_t n = b < p.batch ? own_units(b) : 0u;
             if (b < p.batch && p.kv_len && p.kv_len[b] > p.rows && p.status && blockIdx.x == 0) atomicOr(p.status, ATTN_STATUS_BAD_SHAPE);
             uint32_t incl = n;
 #pragma unroll
@@ -156,72 +162,80 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             __syncthreads();
         }
     }
-    // The list in units: a prefix tile counts as many as its blocks of 16 query rows make it cost, an own tile one. A tile belongs to the
-    // CTA that has its first unit; with at least a prefix tile's units per CTA, every CTA of a segment's range has a tile of it.
-    const uint32_t pre_total = p.prefix_segs * p.prefix_tiles, pre_units = pre_total * p.prefix_weight;
-    const uint32_t own_total = s_cum[p.batch] * p.own.groups;
-    const uint32_t units = pre_units + own_total;
+    // The list in units: a prefix tile counts as many as its blocks of 16 query rows make it cost, an own tile one, the start of an own
+    // segment (its query rows, its piece) switch_units. A tile belongs to the CTA that has its first unit; with at least a prefix tile's
+    // units per CTA, every CTA between those of a segment's first and last tile has a tile of it.
+    const uint32_t pre_units = p.prefix_segs * p.prefix_tiles * p.prefix_weight;
+    const uint32_t units = pre_units + s_cum[p.batch] * p.own.groups;
     const uint32_t active = active_ctas(gridDim.x, 0, p.prefix_segs ? p.prefix_weight : 1, units);
-    auto tile_at = [&](uint32_t c) {  // the first tile of CTA c
-        const uint32_t u = static_cast<uint32_t>(static_cast<uint64_t>(c) * units / active);
-        return u < pre_units ? (u + p.prefix_weight - 1) / p.prefix_weight : pre_total + (u - pre_units);
-    };
-    auto cta_of = [&](uint32_t tile) {
-        return cta_of_tile(tile < pre_total ? tile * p.prefix_weight : pre_units + (tile - pre_total), units, active);
-    };
-    uint32_t t0 = 0, t1 = 0;
+    uint32_t u0 = 0, u1 = 0;
     if (blockIdx.x < active) {
-        t0 = tile_at(blockIdx.x);
-        t1 = tile_at(blockIdx.x + 1);
+        u0 = static_cast<uint32_t>(static_cast<uint64_t>(blockIdx.x) * units / active);
+        u1 = static_cast<uint32_t>((blockIdx.x + 1ull) * units / active);
     }
 
-    auto locate = [&](uint32_t flat, Cursor& c) {
-        if (flat < pre_total) {
-            c.own = 0;
-            c.seg = flat / p.prefix_tiles;
-            c.tile = flat - c.seg * p.prefix_tiles;
-            c.tiles = p.prefix_tiles;
-            c.hg = c.seg / p.row_blocks;
-            c.rb = c.seg - c.hg * p.row_blocks;
-            c.b = 0;
-            c.len = p.prefix;
-            return;
+    // The first tile at or behind unit u: its segment, and c.unit, the tile's first unit (which may be behind the CTA's last).
+    auto locate = [&](uint32_t u, Cursor& c) {
+        if (u < pre_units) {
+            const uint32_t tile = (u + p.prefix_weight - 1) / p.prefix_weight;
+            c.unit = tile * p.prefix_weight;
+            if (c.unit < pre_units) {
+                c.own = 0;
+                c.seg = tile / p.prefix_tiles;
+                c.tile = tile - c.seg * p.prefix_tiles;
+                c.tiles = p.prefix_tiles;
+                c.hg = c.seg / p.row_blocks;
+                c.rb = c.seg - c.hg * p.row_blocks;
+                c.b = 0;
+                c.len = p.prefix;
+                return;
+            }
+            u = pre_units;
         }
-        const uint32_t f = flat - pre_total;
-        uint32_t lo = 0, hi = p.batch;  // the last sequence whose tiles start at or before f
+        c.unit = units;
+        if (u >= units) return;
+        const uint32_t f = u - pre_units;
+        uint32_t lo = 0, hi = p.batch;  // the last sequence whose units start at or before f
         while (hi - lo > 1) {
             const uint32_t mid = (lo + hi) / 2;
             if (s_cum[mid] * p.own.groups <= f) lo = mid;
             else hi = mid;
         }
+        const uint32_t span = s_cum[lo + 1] - s_cum[lo];  // units of one head group
+        const uint32_t r = f - s_cum[lo] * p.own.groups;
         c.own = 1;
         c.b = lo;
-        c.tiles = s_cum[lo + 1] - s_cum[lo];
-        const uint32_t r = f - s_cum[lo] * p.own.groups;
-        c.hg = r / c.tiles;
-        c.tile = r - c.hg * c.tiles;
+        c.tiles = span - p.switch_units;
+        c.hg = r / span;
+        const uint32_t at = max(r - c.hg * span, p.switch_units);
+        c.tile = at - p.switch_units;
+        c.unit = pre_units + s_cum[lo] * p.own.groups + c.hg * span + at;
         c.seg = lo * p.own.groups + c.hg;
         c.rb = 0;
         c.len = own_len(p, lo);
     };
     // the next tile of the list
-    auto advance = [&](uint32_t flat, Cursor& c) {
-        if (++c.tile == c.tiles && flat < t1) locate(flat, c);
+    auto advance = [&](Cursor& c) {
+        const uint32_t next = c.unit + (c.own ? 1 : p.prefix_weight);
+        if (++c.tile < c.tiles) c.unit = next;
+        else locate(next, c);
     };
+    Cursor cur;  // of the consumers, and of the producer
+    locate(u0, cur);
+    const bool busy = cur.unit < u1;
 
     if (warp == 4) {
         // =============================== producer ===============================
         // 28 MB of tiles are requested at once as soon as the CTAs know theirs, and query rows that are requested behind them came 3 to
         // 5 us later, with no tile worked on until then: the consumers' requests go first.
-        if (t0 < t1) block_wait(1, kThreads + 32);
-        if (lane == 0 && t0 < t1) {
+        if (busy) block_wait(1, kThreads + 32);
+        if (lane == 0 && busy) {
             const uint64_t once = l2_policy_evict_first();  // own rows are read once; the prefix's may be read by several blocks of rows
             const uint64_t again = l2_policy_evict_last();
-            Cursor c;
-            locate(t0, c);
+            Cursor& c = cur;
             uint32_t st = 0, phase = 1;  // (a fresh barrier counts as past its odd phase: the first round does not wait)
             bool ok = true;
-            for (uint32_t t = t0; t < t1 && ok; ++t) {
+            while (c.unit < u1 && ok) {
                 const Shape& sh = c.own ? p.own : p.pre;
                 const int row = static_cast<int>(c.tile * sh.keys), head = static_cast<int>(c.hg * sh.hpc), seq = static_cast<int>(c.b);
                 const uint64_t policy = c.own || p.row_blocks == 1 ? once : again;
@@ -232,7 +246,7 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                     tma_load_5d_hint(ring + st * kSlotBytes, c.own ? (v ? &tm_v : &tm_k) : (v ? &tm_vp : &tm_kp), bars + 8 * st, row, head, 0, seq, policy);
                     if (++st == slots) st = 0, phase ^= 1;
                 }
-                advance(t + 1, c);
+                advance(c);
             }
             if (!ok) {  // report, and leave no copy in flight into this CTA's memory
                 if (p.status) atomicOr(p.status, ATTN_STATUS_WAIT_TIMEOUT);
@@ -247,22 +261,22 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         // which CTAs share each segment, for the merge pass
         const uint32_t own_segs = p.batch * p.own.groups;
         for (uint32_t s = blockIdx.x * 32 + lane; s < p.prefix_segs + own_segs; s += gridDim.x * 32) {
-            uint32_t first, n;
+            uint32_t first, last;  // units of the first and the last tile; no tile: last < first
             if (s < p.prefix_segs) {
-                first = s * p.prefix_tiles;
-                n = p.prefix_tiles;
+                first = s * p.prefix_tiles * p.prefix_weight;
+                last = first + (p.prefix_tiles - 1) * p.prefix_weight;
             } else {
                 const uint32_t b = (s - p.prefix_segs) / p.own.groups, hg = (s - p.prefix_segs) - b * p.own.groups;
-                n = s_cum[b + 1] - s_cum[b];
-                first = pre_total + s_cum[b] * p.own.groups + hg * n;
+                const uint32_t span = s_cum[b + 1] - s_cum[b], start = pre_units + s_cum[b] * p.own.groups + hg * span;
+                first = span ? start + p.switch_units : 1;
+                last = span ? start + span - 1 : 0;
             }
-            const uint32_t from = n ? cta_of(first) : 0, count = n ? cta_of(first + n - 1) - from + 1 : 0;
+            const uint32_t from = last < first ? 0 : cta_of_tile(first, units, active);
+            const uint32_t count = last < first ? 0 : cta_of_tile(last, units, active) - from + 1;
             (s < p.prefix_segs ? p.seg_pre[s] : p.seg_own[s - p.prefix_segs]) = from | count << 16;
         }
     } else {
         // =============================== consumers ===============================
-        Cursor cur;
-        if (t0 < t1) locate(t0, cur);
         const uint32_t my_q = q_rows + warp * p.q_held * (D * 2);
         // Offsets of the 16-byte chunks that this lane hands to ldmatrix, four of them in a 128-byte part: keys, values, query row.
         uint32_t k_off[4], v_off[4], q_off[4], q_lane = 0;
@@ -279,8 +293,8 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         auto next_slot = [&]() {
             if (++slot == slots) slot = 0, phase ^= 1;
         };
-        bool ok = true;
-        for (uint32_t t = t0; t < t1; ++t) {
+        bool ok = true, first_run = true;
+        while (cur.unit < u1) {
             const Shape& sh = cur.own ? p.own : p.pre;
             // this warp's place: head hs of the group, block wr of query rows, share wk of the keys (all powers of two)
             const uint32_t hs = warp & (sh.hpc - 1), wr = (warp >> (sh.hpc >> 1)) & (sh.wm - 1), wk = warp >> ((sh.hpc >> 1) + (sh.wm >> 1));
@@ -294,7 +308,8 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                     const uint32_t row = row0 + r, b = cur.own ? cur.b : row / p.group, g = cur.own ? row : row - b * p.group;
                     return p.q + (static_cast<size_t>(b) * p.n_heads + kvh * p.group + g) * D + ch * 8;
                 };
-                if (t == t0) {
+                if (first_run) {
+                    first_run = false;
                     if (lane < n * kParts) touch(q_at(lane / kParts, lane % kParts * 8));
                     block_arrive(1, kThreads + 32);
                 }
@@ -311,11 +326,9 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 const uint32_t r = lane & 15;
                 q_lane = r < n ? my_q + r * (D * 2) : q_zero;
                 // the next segment's rows, on their way into L1 (rows of the list's own segments follow one another in q)
-                if (cur.own && t + (cur.tiles - cur.tile) < t1) {
+                if (cur.own && cur.unit + (cur.tiles - cur.tile) < u1) {
                     const uint64_t next = static_cast<uint64_t>(cur.b) * p.n_heads + (kvh + sh.hpc) * p.group + row0;
-                    for (uint32_t i = lane; i < n * (kParts * 8); i += 32)
-                        if (i % 8 == 0 && next + i / (kParts * 8) < static_cast<uint64_t>(p.batch) * p.n_heads)
-                            prefetch_l1(p.q + next * D + i * 8);
+                    if (lane < n * kParts && next + lane / kParts < static_cast<uint64_t>(p.batch) * p.n_heads) touch(p.q + next * D + lane * 64);
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) q_off[i] = ((i * 2 + (lane >> 4)) ^ (r < n ? r & 7 : 0)) << 4;
@@ -473,7 +486,7 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 if (live == 0) mbar_arrive(bars + 8 * (slots + k_slot));
                 mbar_arrive(bars + 8 * (slots + v_slot));
             }
-            if (cur.tile + 1 == cur.tiles || t + 1 == t1) {
+            if (cur.tile + 1 == cur.tiles || cur.unit + (cur.own ? 1 : p.prefix_weight) >= u1) {
                 // ---- the run's piece: normalised sum and log-sum-exp (log2 units) of this warp's rows and keys
                 const size_t rec = (static_cast<size_t>(blockIdx.x + cur.seg) * sh.ts + wk) * sh.hpc + hs;
                 float* po = cur.own ? p.part_own : p.part_pre;
@@ -496,7 +509,7 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 }
                 fresh = true;
             }
-            advance(t + 1, cur);
+            advance(cur);
         }
     }
     if (p.wait_last) grid_dep_wait();
@@ -988,8 +1001,11 @@ extern "C" int attn_decode_shared(const AttnDecodeSharedArgs* a, void* stream_v)
     in_split.slots = static_cast<uint32_t>(std::min<size_t>(kMaxSlots, (kSplitSmem - fixed) / slot_bytes));
     const size_t smem = fixed + in_split.slots * slot_bytes;
     // A prefix tile of four row blocks keeps a CTA as busy as two own tiles; others are as fast as memory in either form.
+    // A CTA that meets a second own segment ended 2.5 us, two tiles, behind the others (16 ragged caches of up to 4096 rows). Not counted
+    // where a CTA has few tiles: there it would only keep CTAs idle.
+    in_split.switch_units = own_guess >= 8ull * grid ? 2 : 0;
     in_split.prefix_weight = plan.pre.wm == 4 && plan.own.wm == 1 ? 2 : 1;
-    if ((prefix_tiles * in_split.prefix_segs + own_tiles * plan.own_segs) * in_split.prefix_weight > 0x7fffffffull) return ATTN_ERR_UNSUPPORTED;  // 32-bit units
+    if (prefix_tiles * in_split.prefix_segs * in_split.prefix_weight + (own_tiles + in_split.switch_units) * plan.own_segs > 0x7fffffffull) return ATTN_ERR_UNSUPPORTED;  // 32-bit units
     auto split = [&](auto kernel) -> int {
         B200_CUDA_TRY(allow_max_smem(kernel));
         B200_CUDA_TRY(launch_dependent(kernel, dim3(grid), dim3(kSplitThreads), smem, stream, tm_k, tm_v, tm_kp, tm_vp, in_split));
