@@ -33,14 +33,15 @@ struct EvictParams {
     uint32_t batch, n_kv_heads, head_dim, rows, out_rows, keep, sink, recent;
     uint32_t* status;
     uint32_t staged;  // keys of a CTA's slice that its shared memory holds
+    uint32_t scores_aligned;  // every run of scores starts on 16 bytes
     uint32_t slices;  // in place: pieces of a head's row
     uint32_t in_place;
 };
 
-constexpr int kSelThreads = 512;
+constexpr int kSelThreads = 1024;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kBins = 2048;
-constexpr uint32_t kSelWords = 3 * kBins + 2 * kSelWarps + 4;  // shared memory in front of the keys
+constexpr uint32_t kSelWords = 4 * kBins + 2 * kSelWarps + 4;  // shared memory in front of the keys
 constexpr uint32_t kAlways = 0xffffffffu;
 
 // Unsigned order of the keys = order of the scores; NaN gets 0, below -inf. No score maps to kAlways (that pattern would be a NaN).
@@ -55,12 +56,13 @@ __device__ __forceinline__ uint32_t score_key(float x) {
 // the same from either value.
 __device__ __forceinline__ uint32_t rows_of(const EvictParams& p, uint32_t b) { return min(p.kv_len ? p.kv_len[b] : p.rows, p.rows); }
 
-// One cluster of kCtas per (sequence, kv head) = blockIdx.y.
+// One cluster of kCtas per (sequence, kv head) = blockIdx.y. A CTA keeps the keys of its rows in shared memory and goes through them four
+// at a time; rows beyond `staged` (more than 40960 rows a CTA) are read again from the scores.
 template <int kCtas>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_constant__ EvictParams p) {
     extern __shared__ __align__(16) uint32_t s_all[];
-    uint32_t* s_hist = s_all;                   // [3][kBins], one histogram per digit
-    uint32_t* s_gt = s_hist + 3 * kBins;        // [kSelWarps]
+    uint32_t* s_hist = s_all;                   // [4][kBins]: two for the top digit (even and odd lanes: fewer meet in a bin), one for each other
+    uint32_t* s_gt = s_hist + 4 * kBins;        // [kSelWarps]
     uint32_t* s_eq = s_gt + kSelWarps;          // [kSelWarps]
     uint32_t* s_pick = s_eq + kSelWarps;        // digit, keys above it
     uint32_t* s_counts = s_pick + 2;            // this CTA's keys above the threshold, equal to it
@@ -74,7 +76,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_
     const uint32_t seg = blockIdx.y, b = seg / p.n_kv_heads;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     grid_dep_launch_dependents();
-    for (int i = tid; i < 3 * kBins / 4; i += kSelThreads) reinterpret_cast<uint4*>(s_hist)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < 4 * kBins / 4; i += kSelThreads) reinterpret_cast<uint4*>(s_hist)[i] = make_uint4(0, 0, 0, 0);
     grid_dep_wait();
     const uint32_t len = rows_of(p, b);
     uint32_t* kept = p.kept + static_cast<size_t>(seg) * p.keep;
@@ -84,34 +86,51 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_
         return;
     }
     // this CTA's rows: a contiguous slice, cut into one contiguous piece per warp
-    const uint32_t per_warp = ((len + kCtas * kSelWarps - 1) / (kCtas * kSelWarps) + 31) / 32 * 32;
-    const uint32_t per_cta = per_warp * kSelWarps;
-    const uint32_t begin = min(len, rank * per_cta), end = min(len, begin + per_cta);
-    const float* scores = p.scores + static_cast<size_t>(seg) * p.score_stride;
-    const uint32_t tail = len - min(len, p.recent);
-    auto make_key = [&](uint32_t i, float x) { return (i < p.sink || i >= tail) ? kAlways : score_key(x); };
-    const uint32_t n_staged = min(end - begin, p.staged);
+    const uint32_t per_warp = ((len + kCtas * kSelWarps - 1) / (kCtas * kSelWarps) + 127) / 128 * 128;
+    const uint32_t begin = min(len, rank * per_warp * kSelWarps), end = min(len, begin + per_warp * kSelWarps);
+    const uint32_t n = end - begin, n_staged = min(n, p.staged);
+    const float* scores = p.scores + static_cast<size_t>(seg) * p.score_stride + begin;
+    const uint32_t sink = p.sink > begin ? p.sink - begin : 0u;                       // relative to the slice from here on
+    const uint32_t tail = len - min(len, p.recent) > begin ? len - min(len, p.recent) - begin : 0u;
+    auto make_key = [&](uint32_t i, float x) { return (i < sink || i >= tail) ? kAlways : score_key(x); };
     __syncthreads();  // the histograms are clear
-    // ---- keys into shared memory, and the top digit's histogram on the way (eight loads of a thread in flight)
-    constexpr int kAhead = 8;
-    for (uint32_t i0 = begin + tid; i0 < end; i0 += kAhead * kSelThreads) {
-        float x[kAhead];
+    uint32_t* top = s_hist + (lane & 1) * kBins;
+    // ---- keys into shared memory, and the top digit's histogram on the way (four 16-byte loads of a thread in flight)
+    const uint32_t n4 = p.scores_aligned ? n_staged / 4 : 0u;
+    constexpr int kAhead = 4;
+    for (uint32_t i0 = tid; i0 < n4; i0 += kAhead * kSelThreads) {
+        float4 x[kAhead];
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) {
             const uint32_t i = i0 + a * kSelThreads;
-            x[a] = i < end ? scores[i] : 0.f;
+            x[a] = i < n4 ? reinterpret_cast<const float4*>(scores)[i] : make_float4(0.f, 0.f, 0.f, 0.f);
         }
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) {
             const uint32_t i = i0 + a * kSelThreads;
-            if (i < end) {
-                const uint32_t key = make_key(i, x[a]);
-                if (i - begin < n_staged) s_keys[i - begin] = key;
-                atomicAdd(&s_hist[key >> 21], 1u);
+            if (i < n4) {
+                const uint4 k = make_uint4(make_key(4 * i, x[a].x), make_key(4 * i + 1, x[a].y), make_key(4 * i + 2, x[a].z), make_key(4 * i + 3, x[a].w));
+                reinterpret_cast<uint4*>(s_keys)[i] = k;
+                atomicAdd(&top[k.x >> 21], 1u);
+                atomicAdd(&top[k.y >> 21], 1u);
+                atomicAdd(&top[k.z >> 21], 1u);
+                atomicAdd(&top[k.w >> 21], 1u);
             }
         }
     }
-    auto key_at = [&](uint32_t i) { return i - begin < n_staged ? s_keys[i - begin] : make_key(i, scores[i]); };
+    for (uint32_t i = 4 * n4 + tid; i < n; i += kSelThreads) {
+        const uint32_t key = make_key(i, scores[i]);
+        if (i < n_staged) s_keys[i] = key;
+        atomicAdd(&top[key >> 21], 1u);
+    }
+    // four keys from row i (a multiple of four) on; rows behind the slice's end get key 0 and must be left out by their index
+    auto keys_at = [&](uint32_t i) {
+        if (i + 4 <= n_staged) return *reinterpret_cast<const uint4*>(s_keys + i);
+        uint32_t k[4];
+#pragma unroll
+        for (int a = 0; a < 4; ++a) k[a] = i + a < n_staged ? s_keys[i + a] : i + a < n ? make_key(i + a, scores[i + a]) : 0u;
+        return make_uint4(k[0], k[1], k[2], k[3]);
+    };
 
     // ---- the keep-th largest key, a digit at a time from the top
     uint32_t prefix = 0, need = p.keep;  // keys whose upper digits are those of prefix are still candidates for the need-th largest
@@ -119,26 +138,39 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
         const uint32_t digit_mask = pass == 2 ? 1023u : 2047u;
-        uint32_t* hist = s_hist + pass * kBins;
+        uint32_t* hist = s_hist + (pass == 0 ? 0 : (pass + 1) * kBins);
         if (pass > 0) {
-            const uint32_t mask = pass == 1 ? 0xffe00000u : 0xfffffc00u;
-#pragma unroll 4
-            for (uint32_t i = begin + tid; i < end; i += kSelThreads) {
-                const uint32_t key = key_at(i);
-                if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & digit_mask], 1u);
+            const int above = pass == 1 ? 21 : 10;
+            const uint32_t want = prefix >> above;
+            auto count = [&](uint32_t i, uint32_t key) {
+                if (key >> above == want && i < n) atomicAdd(&hist[(key >> shift) & digit_mask], 1u);
+            };
+            __syncthreads();  // (the keys are other threads')
+#pragma unroll 2
+            for (uint32_t i = 4 * tid; i < n; i += 4 * kSelThreads) {
+                const uint4 k = keys_at(i);
+                count(i, k.x);
+                count(i + 1, k.y);
+                count(i + 2, k.z);
+                count(i + 3, k.w);
             }
         }
         meet();
-        // thread t owns the four bins from kBins - 4 - 4t up, so that threads run from the top: it sums them over the cluster
-        const int bin0 = kBins - 4 - 4 * tid;
-        uint4 mine = make_uint4(0, 0, 0, 0);
+        // thread t owns the bins from kBins - kOwn - kOwn t up, so that threads run from the top: it sums them over the cluster
+        constexpr int kOwn = kBins / kSelThreads;  // two
+        const int bin0 = kBins - kOwn - kOwn * tid;
+        uint2 mine = make_uint2(0, 0);
 #pragma unroll
         for (int c = 0; c < kCtas; ++c) {
-            const uint4* src = reinterpret_cast<const uint4*>(hist + bin0);
-            const uint4 h = kCtas > 1 ? *cluster.map_shared_rank(src, c) : *src;
-            mine.x += h.x, mine.y += h.y, mine.z += h.z, mine.w += h.w;
+#pragma unroll
+            for (int copy = 0; copy < (pass == 0 ? 2 : 1); ++copy) {
+                const uint2* src = reinterpret_cast<const uint2*>(hist + copy * kBins + bin0);
+                // (each CTA starts with another one: all of them on one CTA's memory at a time took 3 us more per digit)
+                const uint2 h = kCtas > 1 ? *cluster.map_shared_rank(src, (rank + c) % kCtas) : *src;
+                mine.x += h.x, mine.y += h.y;
+            }
         }
-        const uint32_t sum = mine.x + mine.y + mine.z + mine.w;
+        const uint32_t sum = mine.x + mine.y;
         uint32_t incl = sum;
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
@@ -147,21 +179,11 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_
         }
         if (lane == 31) s_gt[warp] = incl;
         __syncthreads();
-        uint32_t above = incl - sum + __reduce_add_sync(0xffffffffu, lane < warp ? s_gt[lane] : 0u);
+        const uint32_t above = incl - sum + __reduce_add_sync(0xffffffffu, lane < warp ? s_gt[lane] : 0u);
         if (above < need && above + sum >= need) {  // one thread
-            uint32_t digit = bin0 + 3;
-            const uint32_t counts[4] = {mine.w, mine.z, mine.y, mine.x};
-#pragma unroll
-            for (int i = 0; i < 3; ++i) {
-                if (above + counts[i] < need) {
-                    above += counts[i];
-                    --digit;
-                } else {
-                    break;
-                }
-            }
-            s_pick[0] = digit;
-            s_pick[1] = above;
+            const bool upper = above + mine.y >= need;
+            s_pick[0] = bin0 + (upper ? 1 : 0);
+            s_pick[1] = above + (upper ? 0 : mine.y);
         }
         __syncthreads();
         prefix |= s_pick[0] << shift;
@@ -169,14 +191,23 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_
         // (the next write of s_gt and s_pick comes behind another meeting, and each digit has a histogram of its own)
     }
     // every key above `prefix` stays, and the first `need` rows of those equal to it
-    // ---- counts per warp, in order
-    const uint32_t wb = min(end, begin + warp * per_warp), we = min(end, wb + per_warp);
-    uint32_t n_gt = 0, n_eq = 0;  // of this lane
-#pragma unroll 4
-    for (uint32_t i = wb + lane; i < we; i += 32) {
-        const uint32_t key = key_at(i);
-        n_gt += key > prefix;
-        n_eq += key == prefix;
+    // ---- counts per warp, in order: keys above in the low half of a word, equal ones in the high half (a lane's at most 2^16)
+    const uint32_t wb = min(n, warp * per_warp), we = min(n, wb + per_warp);
+    auto tally = [&](uint32_t i, const uint4& k, uint32_t (&gt)[4], uint32_t (&eq)[4]) {
+        const uint32_t key[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            gt[a] = i + a < we && key[a] > prefix;
+            eq[a] = i + a < we && key[a] == prefix;
+        }
+    };
+    uint32_t n_gt = 0, n_eq = 0;
+#pragma unroll 2
+    for (uint32_t i = wb + 4 * lane; i < we; i += 128) {
+        uint32_t gt[4], eq[4];
+        tally(i, keys_at(i), gt, eq);
+        n_gt += gt[0] + gt[1] + gt[2] + gt[3];
+        n_eq += eq[0] + eq[1] + eq[2] + eq[3];
     }
     n_gt = __reduce_add_sync(0xffffffffu, n_gt);
     n_eq = __reduce_add_sync(0xffffffffu, n_eq);
@@ -204,18 +235,27 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_
         eq += __reduce_add_sync(0xffffffffu, oe);
     }
     // ---- the kept rows, in order: row i goes to place (kept rows in front of it)
-    const uint32_t below = (1u << lane) - 1u;
-#pragma unroll 2
-    for (uint32_t i0 = wb; i0 < we; i0 += 32) {
-        const uint32_t i = i0 + lane;
-        const uint32_t key = i < we ? key_at(i) : 0u;
-        const bool is_gt = i < we && key > prefix, is_eq = i < we && key == prefix;
-        const uint32_t m_gt = __ballot_sync(0xffffffffu, is_gt), m_eq = __ballot_sync(0xffffffffu, is_eq);
-        const uint32_t my_eq = eq + __popc(m_eq & below);
-        const uint32_t place = gt + __popc(m_gt & below) + min(my_eq, need);
-        if (is_gt || (is_eq && my_eq < need)) kept[place] = i;
-        gt += __popc(m_gt);
-        eq += __popc(m_eq);
+    for (uint32_t i0 = wb; i0 < we; i0 += 128) {  // the same number of rounds for all lanes
+        const uint32_t i = i0 + 4 * lane;
+        uint32_t is_gt[4], is_eq[4];
+        tally(i, i < we ? keys_at(i) : make_uint4(0, 0, 0, 0), is_gt, is_eq);
+        uint32_t mine = is_gt[0] + is_gt[1] + is_gt[2] + is_gt[3] + ((is_eq[0] + is_eq[1] + is_eq[2] + is_eq[3]) << 16);
+        uint32_t incl = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const uint32_t o = __shfl_up_sync(0xffffffffu, incl, d);
+            if (lane >= d) incl += o;
+        }
+        const uint32_t all = __shfl_sync(0xffffffffu, incl, 31);
+        uint32_t g = gt + ((incl - mine) & 0xffffu), e = eq + ((incl - mine) >> 16);
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            if (is_gt[a] || (is_eq[a] && e < need)) kept[g + min(e, need)] = begin + i + a;
+            g += is_gt[a];
+            e += is_eq[a];
+        }
+        gt += all & 0xffffu;
+        eq += all >> 16;
     }
     if constexpr (kCtas > 1) cluster.sync();  // no CTA leaves while another reads its counts
 }
@@ -398,7 +438,8 @@ extern "C" int attn_kv_evict(const AttnKvEvictArgs* a, void* stream_v) {
     // ---- which rows: as many CTAs per cluster as give a CTA at least 2048 rows, eight at most
     uint32_t cl = 1;
     while (cl < 8 && a->rows > cl * 2048ull) cl *= 2;
-    const uint64_t slice = (a->rows + cl - 1) / cl + 32 * kSelWarps;
+    const uint64_t slice = (a->rows + cl - 1) / cl + 128 * kSelWarps;
+    p.scores_aligned = aligned16(a->scores) && p.score_stride % 4 == 0;
     p.staged = static_cast<uint32_t>(slice < 40 * 1024 ? slice : 40 * 1024);
     auto select = [&](auto kernel) -> int {
         B200_CUDA_TRY(allow_max_smem(kernel));
