@@ -521,7 +521,7 @@ typedef struct AttnDecodeSharedArgs {
     int32_t o_dtype;      /* dtype or ATTN_DTYPE_F32 */
     int32_t dtype;        /* ATTN_DTYPE_F16 | BF16, of q, the prefix and the caches */
     uint32_t batch, n_heads, n_kv_heads;
-    uint32_t head_dim;       /* 64 or 128; at most 64 query heads per kv head */
+    uint32_t head_dim;       /* 64 or 128; at most 64 query heads per kv head, 1024 in all, 2048 sequences */
     uint32_t prefix_len;
     uint32_t kv_capacity;    /* rows an own cache holds; 0 = no own rows */
     const uint32_t* kv_len;  /* device [batch], valid own rows; NULL = kv_len_uniform. A length beyond the capacity is clamped and

@@ -150,6 +150,10 @@ __host__ __device__ inline uint64_t div_mostly_32(uint64_t a, uint64_t b) {
     return a / b;
 }
 
+// x / d for x below 2^32 / d by one multiplication (a division by a variable is a chain of ~ 100 clocks): magic from divider(d).
+__host__ __device__ inline uint32_t divider(uint32_t d) { return d == 1 ? 0u : 0xffffffffu / d + 1u; }
+__device__ __forceinline__ uint32_t fast_div(uint32_t x, uint32_t magic) { return magic ? __umulhi(x, magic) : x; }
+
 // Number of CTAs that actually take tiles, identical in the split and merge passes.
 __host__ __device__ inline uint32_t active_ctas(uint32_t grid, uint32_t max_ctas, uint32_t min_tiles, uint64_t nt) {
     uint64_t a = grid;
@@ -258,6 +262,7 @@ struct SharedPrefixParams {
     uint32_t* seg_ctas;  // [segments] segment_ctas() words
     uint64_t row_stride;
     uint32_t batch, n_heads, n_kv_heads, group, head_dim, prefix;
+    uint32_t div_group;  // divider(group)
     uint32_t pairs, segments, grid;
     uint32_t ctas_per_seg;  // > 0: that many CTAs for each segment; 0: the blocks of all segments dealt equally, runs may cross segments
     float scale_log2;    // of the scale's magnitude; q_sign flips the query's sign for a negative one

@@ -50,6 +50,7 @@ struct SharedParams {
     const uint32_t* kv_len;
     uint32_t kv_len_uniform;
     uint32_t batch, n_heads, n_kv_heads, group;
+    uint32_t div_heads, div_group;  // divider(n_heads), divider(group)
     uint32_t prefix, rows;
     float scale_log2;       // of the scale's magnitude
     uint32_t q_sign;        // 0x80008000 for a negative scale: flips the query's sign instead
@@ -170,8 +171,8 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     const uint32_t active = active_ctas(gridDim.x, 0, p.prefix_segs ? p.prefix_weight : 1, units);
     uint32_t u0 = 0, u1 = 0;
     if (blockIdx.x < active) {
-        u0 = static_cast<uint32_t>(static_cast<uint64_t>(blockIdx.x) * units / active);
-        u1 = static_cast<uint32_t>((blockIdx.x + 1ull) * units / active);
+        u0 = static_cast<uint32_t>(div_mostly_32(static_cast<uint64_t>(blockIdx.x) * units, active));
+        u1 = static_cast<uint32_t>(div_mostly_32((blockIdx.x + 1ull) * units, active));
     }
 
     // The first tile at or behind unit u: its segment, and c.unit, the tile's first unit (which may be behind the CTA's last).
@@ -305,30 +306,30 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 const uint32_t row0 = cur.own ? wr * 16 : cur.rb * sh.wm * 16 + wr * 16, all = cur.own ? p.group : p.batch * p.group;
                 const uint32_t n = row0 < all ? min(16u, all - row0) : 0u;
                 auto q_at = [&](uint32_t r, uint32_t ch) {  // chunk ch of the warp's row r
-                    const uint32_t row = row0 + r, b = cur.own ? cur.b : row / p.group, g = cur.own ? row : row - b * p.group;
+                    const uint32_t row = row0 + r, b = cur.own ? cur.b : fast_div(row, p.div_group), g = cur.own ? row : row - b * p.group;
                     return p.q + (static_cast<size_t>(b) * p.n_heads + kvh * p.group + g) * D + ch * 8;
                 };
-                if (first_run) {
-                    first_run = false;
-                    if (lane < n * kParts) touch(q_at(lane / kParts, lane % kParts * 8));
-                    block_arrive(1, kThreads + 32);
-                }
                 __syncwarp();
                 for (uint32_t i = lane; i < n * (kParts * 8); i += 32) {
                     const uint32_t r = i / (kParts * 8), ch = i % (kParts * 8);
-                    uint4 x = *reinterpret_cast<const uint4*>(q_at(r, ch));
-                    x.x ^= p.q_sign, x.y ^= p.q_sign, x.z ^= p.q_sign, x.w ^= p.q_sign;  // a negative scale's sign
-                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(my_q + r * (D * 2) + ((ch ^ (r & 7)) << 4)), "r"(x.x), "r"(x.y),
-                                 "r"(x.z), "r"(x.w)
-                                 : "memory");
+                    cp_async16(my_q + r * (D * 2) + ((ch ^ (r & 7)) << 4), q_at(r, ch));
                 }
+                if (first_run) {
+                    first_run = false;
+                    block_arrive(1, kThreads + 32);
+                }
+                cp_async_wait_all();
+                if (p.q_sign)  // a negative scale's sign; each lane its own chunks
+                    for (uint32_t i = lane; i < n * (kParts * 8); i += 32)
+                        xor_shared16(my_q + i / (kParts * 8) * (D * 2) + (((i % (kParts * 8)) ^ (i / (kParts * 8) & 7)) << 4), p.q_sign);
                 __syncwarp();
                 const uint32_t r = lane & 15;
                 q_lane = r < n ? my_q + r * (D * 2) : q_zero;
                 // the next segment's rows, on their way into L1 (rows of the list's own segments follow one another in q)
                 if (cur.own && cur.unit + (cur.tiles - cur.tile) < u1) {
                     const uint64_t next = static_cast<uint64_t>(cur.b) * p.n_heads + (kvh + sh.hpc) * p.group + row0;
-                    if (lane < n * kParts && next + lane / kParts < static_cast<uint64_t>(p.batch) * p.n_heads) touch(p.q + next * D + lane * 64);
+                    for (uint32_t i = lane; i < n * kParts * 4; i += 32)  // 32 bytes each
+                        if (next + i / (kParts * 4) < static_cast<uint64_t>(p.batch) * p.n_heads) touch(p.q + next * D + i * 16);
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) q_off[i] = ((i * 2 + (lane >> 4)) ^ (r < n ? r & 7 : 0)) << 4;
@@ -524,12 +525,13 @@ struct Pieces {
 };
 template <int D>
 __device__ __forceinline__ void find_pieces(const SharedParams& p, uint32_t b, uint32_t h, Pieces& x) {
-    const uint32_t kvh = h / p.group, g = h - kvh * p.group;
+    const uint32_t kvh = fast_div(h, p.div_group), g = h - kvh * p.group;
     x.count[0] = 0;
     if (p.prefix_segs) {
         const Shape& sh = p.pre;
-        const uint32_t row = b * p.group + g, rb = row / sh.rec_rows, r = row - rb * sh.rec_rows;
-        const uint32_t hg = kvh / sh.hpc, hs = kvh - hg * sh.hpc, seg = hg * p.row_blocks + rb;
+        // (rec_rows and hpc are powers of two here, hpc at most four)
+        const uint32_t row = b * p.group + g, rb = row >> (31 - __clz(sh.rec_rows)), r = row & (sh.rec_rows - 1);
+        const uint32_t hg = kvh >> (sh.hpc >> 1), hs = kvh & (sh.hpc - 1), seg = hg * p.row_blocks + rb;
         const uint32_t w = p.seg_pre[seg];
         const uint64_t at = (static_cast<uint64_t>((w & 0xffffu) + seg) * sh.ts * sh.hpc + hs) * sh.rec_rows + r;
         x.step[0] = static_cast<uint64_t>(sh.hpc) * sh.rec_rows;
@@ -538,7 +540,7 @@ __device__ __forceinline__ void find_pieces(const SharedParams& p, uint32_t b, u
         x.lse[0] = p.lse_pre + at;
     }
     const Shape& sh = p.own;
-    const uint32_t hg = kvh / sh.hpc, hs = kvh - hg * sh.hpc, seg = b * sh.groups + hg;
+    const uint32_t hg = kvh >> (sh.hpc >> 1), hs = kvh & (sh.hpc - 1), seg = b * sh.groups + hg;
     const uint32_t w = p.seg_own[seg];
     const uint64_t at = (static_cast<uint64_t>((w & 0xffffu) + seg) * sh.ts * sh.hpc + hs) * sh.rec_rows + g;
     x.step[1] = static_cast<uint64_t>(sh.hpc) * sh.rec_rows;
@@ -561,7 +563,7 @@ __global__ void __launch_bounds__(kThreads) shared_merge_kernel(const __grid_con
     grid_dep_wait();
     if (blockIdx.x < p.out_ctas) {
         const uint32_t row = blockIdx.x / (D / SLICE), slice = blockIdx.x % (D / SLICE);
-        const uint32_t b = row / p.n_heads, h = row - b * p.n_heads;
+        const uint32_t b = fast_div(row, p.div_heads), h = row - b * p.n_heads;
         Pieces x;
         find_pieces<D>(p, b, h, x);
         const int in_group = lane % kLanes, group = tid / kLanes;
@@ -743,7 +745,7 @@ int make_shared_plan(uint32_t batch, uint32_t n_heads, uint32_t n_kv_heads, uint
                      SharedPlan* plan) {
     if (batch == 0 || n_heads == 0 || n_kv_heads == 0 || n_heads % n_kv_heads != 0) return ATTN_ERR_INVALID_ARG;
     const uint32_t group = n_heads / n_kv_heads;
-    if ((head_dim != 64 && head_dim != 128) || group > 64 || batch > kMaxBatch || n_heads > 4096) return ATTN_ERR_UNSUPPORTED;
+    if ((head_dim != 64 && head_dim != 128) || group > 64 || batch > kMaxBatch || n_heads > 1024) return ATTN_ERR_UNSUPPORTED;
     SharedPlan& s = *plan;
     set_shape(&s.own, group, n_kv_heads);
     s.own.rec_rows = group;
@@ -893,6 +895,8 @@ extern "C" int attn_decode_shared(const AttnDecodeSharedArgs* a, void* stream_v)
     p.n_heads = a->n_heads;
     p.n_kv_heads = a->n_kv_heads;
     p.group = a->n_heads / a->n_kv_heads;
+    p.div_heads = divider(p.n_heads);
+    p.div_group = divider(p.group);
     p.prefix = a->prefix_len;
     p.rows = a->kv_capacity;
     const float scale = a->scale != 0.f ? a->scale : 1.0f / sqrtf(static_cast<float>(a->head_dim));
@@ -957,6 +961,7 @@ extern "C" int attn_decode_shared(const AttnDecodeSharedArgs* a, void* stream_v)
         t.n_heads = p.n_heads;
         t.n_kv_heads = p.n_kv_heads;
         t.group = p.group;
+        t.div_group = p.div_group;
         t.head_dim = a->head_dim;
         t.prefix = p.prefix;
         t.pairs = plan.pairs;

@@ -92,11 +92,11 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     uint32_t t0, t1;
     if (p.ctas_per_seg) {  // a run inside one segment
         const uint32_t seg = blockIdx.x / p.ctas_per_seg, i = blockIdx.x - seg * p.ctas_per_seg;
-        t0 = seg * blocks + static_cast<uint32_t>(static_cast<uint64_t>(i) * blocks / p.ctas_per_seg);
-        t1 = seg * blocks + static_cast<uint32_t>((i + 1ull) * blocks / p.ctas_per_seg);
+        t0 = seg * blocks + static_cast<uint32_t>(div_mostly_32(static_cast<uint64_t>(i) * blocks, p.ctas_per_seg));
+        t1 = seg * blocks + static_cast<uint32_t>(div_mostly_32((i + 1ull) * blocks, p.ctas_per_seg));
     } else {
-        t0 = static_cast<uint32_t>(blockIdx.x * total / gridDim.x);
-        t1 = static_cast<uint32_t>((blockIdx.x + 1) * total / gridDim.x);
+        t0 = static_cast<uint32_t>(div_mostly_32(blockIdx.x * total, gridDim.x));
+        t1 = static_cast<uint32_t>(div_mostly_32((blockIdx.x + 1) * total, gridDim.x));
     }
     auto item_at = [&](uint32_t t, Item& w) {  // the item that starts at block t of the list; false behind the run
         if (t >= t1) return false;
@@ -157,45 +157,56 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         uint32_t g0 = 0;  // key blocks of this tile before the current item: buffer and barrier phases run on over the items
         bool staged = false;
         Item w;
-        // The first item's query rows are requested ahead of the tiles: behind them they came 3 us later.
-        if (item_at(t0, w)) {
-            const uint32_t m = w.m0 + t * BM + r;
-            if (m < query_rows) {
-                const uint32_t b = m / p.group, g = m - b * p.group;
-                const uint16_t* src = static_cast<const uint16_t*>(p.q) + (static_cast<size_t>(b) * p.n_heads + w.kvh * p.group + g) * HD;
-#pragma unroll
-                for (int half = 0; half < HD / 64; ++half) touch(src + half * 64);
+        // A warp brings its 32 query rows of an item, neighbouring lanes neighbouring 16-byte chunks (a row per thread took 2 us to
+        // request); rows that are not there are zeros.
+        constexpr int kRowChunks = HD / 8;
+        auto chunk_at = [&](int i) {  // where chunk i of this lane goes
+            const int idx = i * 32 + lane, row = ((warp & 3) << 5) + idx / kRowChunks, c = idx % kRowChunks;
+            return base + kSmemQ + t * kTileBytes + row * 128 + (c >> 3) * kSubTileBytes + (((c & 7) ^ (row & 7)) << 4);
+        };
+        auto bring_rows = [&]() {
+            uint32_t m = w.m0 + t * BM + ((warp & 3) << 5) + lane / kRowChunks;
+            uint32_t b = fast_div(m, p.div_group), g = m - b * p.group;
+#pragma unroll 1  // (run once or twice: every 128 bytes of straight code are a miss of the instruction cache)
+            for (int i = 0; i < kRowChunks; ++i) {
+                if (m < query_rows) {
+                    cp_async16(chunk_at(i), static_cast<const uint16_t*>(p.q) + (static_cast<size_t>(b) * p.n_heads + w.kvh * p.group + g) * HD +
+                                                lane % kRowChunks * 8);
+                } else {
+                    st_shared_zero16(chunk_at(i));
+                }
+                m += 32 / kRowChunks;
+                g += 32 / kRowChunks;
+                while (g >= p.group) g -= p.group, ++b;
             }
+        };
+        auto rows_there = [&]() {
+            cp_async_wait_all();
+            if (p.q_sign) {
+#pragma unroll 1
+                for (int i = 0; i < kRowChunks; ++i) xor_shared16(chunk_at(i), p.q_sign);
+            }
+            fence_async_smem();
+            mbar_arrive(bar(BAR_Q_FULL + t));
+        };
+        // The first item's query rows are requested ahead of the tiles: behind them they came 3 us later.
+        bool brought = false;
+        if (item_at(t0, w) && w.tile[t]) {
+            bring_rows();
+            brought = true;
         }
         block_arrive(3, 288);
         for (uint32_t at = t0; ok && item_at(at, w); at += w.blocks) {
             if (!w.tile[t]) continue;
-            // ---- this thread's query row into the tile (the previous item's MMAs are over, its result has left)
+            // ---- the query rows into the tile (the previous item's MMAs are over, its result has left)
+            const uint32_t m = w.m0 + t * BM + r;
             if (staged) {
                 if ((warp & 3) == 0 && lane == 0) tma_store_wait_read();
                 named_bar_sync(1 + t, 128);
             }
-            const uint32_t m = w.m0 + t * BM + r;
-            {
-                const uint32_t b = m / p.group, g = m - b * p.group;
-                const bool there = m < query_rows;
-                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) +
-                                                                  (static_cast<size_t>(there ? b : 0) * p.n_heads + w.kvh * p.group + (there ? g : 0)) * HD);
-                const uint32_t dst = base + kSmemQ + t * kTileBytes + r * 128;
-#pragma unroll
-                for (int half = 0; half < HD / 64; ++half) {
-                    uint4 x[8];
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) x[c] = there ? src[half * 8 + c] : make_uint4(0, 0, 0, 0);
-#pragma unroll
-                    for (int c = 0; c < 8; ++c)
-                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + half * kSubTileBytes + ((c ^ (r & 7)) << 4)),
-                                     "r"(x[c].x ^ p.q_sign), "r"(x[c].y ^ p.q_sign), "r"(x[c].z ^ p.q_sign), "r"(x[c].w ^ p.q_sign)
-                                     : "memory");
-                }
-                fence_async_smem();
-                mbar_arrive(bar(BAR_Q_FULL + t));
-            }
+            if (!brought) bring_rows();
+            brought = false;
+            rows_there();
             float m_used = -INFINITY;  // maximum the stored probabilities are relative to (log2 units)
             float l = 0.f;
             for (uint32_t j = 0; j < w.blocks && ok; ++j) {
@@ -297,8 +308,8 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             const uint32_t rec_row = (blockIdx.x + w.seg) * (2 * BM) + t * BM;
             if (m < query_rows) p.lse[rec_row + r] = l > 0.f ? m_used + __log2f(l) : -INFINITY;
             // The tile leaves through shared memory and the TMA engine, 128 bytes of every row at a time: the query tile, which nothing
-            // reads any more, holds the first two passes, the staging tile the third. (Each pass behind the previous one's store in a
-            // single staging tile: 3 us more per piece.)
+            // reads any more, holds the first two passes, the staging tile the third, so that only the fourth waits for a store. (Each pass
+            // behind the previous one's store in a single staging tile: 3 us more per piece.)
             const bool leader = (warp & 3) == 0 && lane == 0;
             auto put = [&](int pass, uint32_t stage) {
                 float o[32];
@@ -311,28 +322,21 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                                  "r"(__float_as_uint(o[c * 4 + 2] * inv)), "r"(__float_as_uint(o[c * 4 + 3] * inv))
                                  : "memory");
             };
-            const uint32_t stage[3] = {base + kSmemQ + t * kTileBytes, base + kSmemQ + t * kTileBytes + kSubTileBytes,
-                                       base + kSmemStage + t * kStageTileBytes};
-            constexpr int kFirst = HD == 128 ? 3 : 2;
-#pragma unroll
-            for (int pass = 0; pass < kFirst; ++pass) put(pass, stage[pass]);
-            fence_async_smem();
-            named_bar_sync(1 + t, 128);
-            if (leader) {
-#pragma unroll
-                for (int pass = 0; pass < kFirst; ++pass) {
-                    tma_store_2d(&tm_o, stage[pass], pass * 32, rec_row);
-                    tma_store_commit();
+            constexpr int kPasses = HD / 32;
+#pragma unroll 1
+            for (int pass = 0; pass < kPasses; ++pass) {
+                const uint32_t stage = pass == 2   ? base + kSmemStage + t * kStageTileBytes
+                                       : pass == 1 ? base + kSmemQ + t * kTileBytes + kSubTileBytes
+                                                   : base + kSmemQ + t * kTileBytes;
+                if (pass == 3) {  // the first pass's store has been read
+                    if (leader) asm volatile("cp.async.bulk.wait_group.read 2;" ::: "memory");
+                    named_bar_sync(1 + t, 128);
                 }
-                if (HD == 128) asm volatile("cp.async.bulk.wait_group.read 2;" ::: "memory");  // the first has been read
-            }
-            if constexpr (HD == 128) {
-                named_bar_sync(1 + t, 128);
-                put(3, stage[0]);
+                put(pass, stage);
                 fence_async_smem();
                 named_bar_sync(1 + t, 128);
                 if (leader) {
-                    tma_store_2d(&tm_o, stage[0], 96, rec_row);
+                    tma_store_2d(&tm_o, stage, pass * 32, rec_row);
                     tma_store_commit();
                 }
             }

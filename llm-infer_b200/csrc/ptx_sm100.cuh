@@ -184,11 +184,20 @@ __device__ __forceinline__ float round16(float x) {
     }
 }
 
-__device__ __forceinline__ void prefetch_l1(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
-// Requests the line that holds *p into L1 by a load whose value nobody waits for.
+// Requests the 32 bytes that hold *p into L1 by a load whose value nobody waits for.
 __device__ __forceinline__ void touch(const void* p) {
     uint32_t unused;
     asm volatile("ld.global.u32 %0, [%1];" : "=r"(unused) : "l"(p) : "memory");
+}
+// 16 bytes from global to shared memory, asynchronously; a thread waits for all of its own copies.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+__device__ __forceinline__ void xor_shared16(uint32_t addr, uint32_t mask) {
+    asm volatile(
+        "{\n\t.reg .b32 a, b, c, d;\n\tld.shared.v4.b32 {a, b, c, d}, [%0];\n\txor.b32 a, a, %1;\n\txor.b32 b, b, %1;\n\t"
+        "xor.b32 c, c, %1;\n\txor.b32 d, d, %1;\n\tst.shared.v4.b32 [%0], {a, b, c, d};\n\t}" ::"r"(addr), "r"(mask) : "memory");
 }
 // The two halves of a barrier between some warps of a block: `threads` counts those that arrive and those that wait.
 __device__ __forceinline__ void block_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
