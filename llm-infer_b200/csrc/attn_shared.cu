@@ -809,15 +809,15 @@ PrefixChoice choose_prefix(const SharedPlan& plan, uint32_t sms, uint32_t head_d
     const char* knob = getenv("ATTN_TRACE_PREFIX");  // profiling knob
     if (knob && atoi(knob) == 0) return c;
 #endif
-    const double dim = head_dim / 128.0;
-    const double tile_bytes = 32768.0 * dim, bandwidth = 6.2e6;  // bytes per us
-    const double own_tile = 0.55 * dim, launch = 5.0;            // us of an SM per own tile; a launch's fixed part
-    const double shared_tile = (plan.pre.wm == 4 ? 1.15 : plan.pre.wm == 2 ? 0.65 : 0.55) * dim;  // of a prefix tile in the split pass
+    const double dim = head_dim / 128.0, work = 0.75 + 0.25 * dim;
+    const double tile_bytes = 32768.0 * dim, bandwidth = 6.2e6;     // bytes per us
+    const double own_tile = 0.6 * work, own_seg = 2.0, launch = 5.0;  // us of an SM per own tile, of a CTA per own segment; a launch's fixed part
+    const double shared_tile = (plan.pre.wm == 4 ? 1.15 : plan.pre.wm == 2 ? 0.65 : 0.6) * work;  // of a prefix tile in the split pass
     const double block = (query_rows > 128 ? 1.1 : 0.8) * (0.4 + 0.6 * dim);                      // of a key block in the tensor-core kernel
     const double block_bytes = 16384.0 * 2 * dim;
     auto split_time = [&](double ctas) {
-        const double sm = ctas / 2;
-        return launch + std::max(own_tiles * own_tile / sm, own_tiles * tile_bytes / bandwidth);
+        const double segs = std::ceil(plan.own_segs / ctas) * (own_tiles ? own_seg : 0.0);
+        return launch + segs + std::max(own_tiles * own_tile / (ctas / 2), own_tiles * tile_bytes / bandwidth);
     };
     auto prefix_time = [&](double ctas) { return launch + 1.0 + std::max(std::ceil(blocks / ctas) * block, blocks / plan.pairs * block_bytes / bandwidth); };
     const double together = launch + std::max((prefix_tiles * shared_tile + own_tiles * own_tile) / sms, all * tile_bytes / bandwidth);
