@@ -18,6 +18,7 @@ from dataclasses import dataclass
 import torch
 
 from . import attention as A
+from . import context as X
 
 KV_SINK = 4  # attention-sink rows of the sliding window (include/model/model.hpp)
 
@@ -85,7 +86,10 @@ def random_weights(cfg: ModelConfig, seed: int, device="cpu", weight_type: str =
 class Llama:
     """Batched token-at-a-time forward, whole-prompt prefill and greedy generation on one GPU."""
 
-    def __init__(self, cfg: ModelConfig, weights: dict, batch: int, device=None, weight_type: str = "f16"):
+    def __init__(self, cfg: ModelConfig, weights: dict, batch: int, device=None, weight_type: str = "f16",
+                 rope_layout: str = "interleaved", rope_scaling: dict | None = None):
+        """``rope_layout`` and ``rope_scaling`` (context.rope_frequencies): positions of models that pair a head's halves, or whose
+        frequencies are scaled for long contexts. The defaults are the engine's positions and kernels."""
         dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         if dev.type != "cuda":
             raise ValueError("the model runs on a CUDA device only (there is no CPU path)")
@@ -95,6 +99,12 @@ class Llama:
         if weight_type not in ("f16", "q8_0"):
             raise ValueError("weight_type must be 'f16' (the engine's) or 'q8_0'")
         self.weight_type = weight_type
+        # the table of context.rope_positions, and whether every path has to use it
+        inv_freq, self._rope_factor = X.rope_frequencies(c.rotary_dim or c.head_dim, c.rope_theta, rope_scaling)
+        self._inv_freq, self._rope_layout = inv_freq.to(dev), rope_layout
+        self._own_rope = rope_layout != "interleaved" or rope_scaling is not None
+        if self._own_rope and c.qkv_clip > 0:
+            raise ValueError("scaled or half-paired positions have no clamp of q, k and v in the prompt phase")
         q8 = weight_type == "q8_0"
         self._gemv = A.gemv_q8_0 if q8 else A.gemv_f16
         self._embed = A.embed_q8_0 if q8 else A.embed_f16
@@ -188,9 +198,28 @@ class Llama:
         self._positions.copy_(host, non_blocking=True)
         return kv_sink
 
-    def _launch_step(self, kv_sink: int, want_logits: bool) -> None:
+    def _attend(self, l: int, kv_sink: int) -> torch.Tensor:
+        """Positions, cache insert and attention of layer ``l`` over every sequence's own cache."""
+        c = self.cfg
+        if self._own_rope:
+            if kv_sink:
+                raise ValueError("scaled or half-paired positions do not slide past max_seq_len")
+            X.rope_positions(self.q, self.k, self.v, self.k_cache[l], self.v_cache[l], self.pos, self.kv_pos, inv_freq=self._inv_freq,
+                             factor=self._rope_factor, layout=self._rope_layout, q_out=self.q, status=self.status)
+        else:
+            A.rope_kv_insert(self.q, self.k, self.v, self.k_cache[l], self.v_cache[l], self.pos, self.kv_pos,
+                             theta=c.rope_theta, rotary_dim=c.rotary_dim, kv_sink=kv_sink, q_out=self.q,
+                             pos_early=True)   # positions are copied in before the step's first kernel
+        # (two_pass: another order of the sums moves fp16 ties of the next layers' cache rows, so a step's results would
+        # change with max_seq_len, which the choice of the form looks at)
+        A.attn_decode(self.q, self.k_cache[l], self.v_cache[l], self.kv_len, out=self.att,
+                      workspace=self.workspace, kv_early=self.kv_early and kv_sink == 0, two_pass=True)
+        return self.att
+
+    def _launch_step(self, kv_sink: int, want_logits: bool, attend=None) -> None:
         """Every launch of one step, reading self.tokens / pos / kv_pos / kv_len. With logits the step ends with the
-        greedy pick (self.next_token) and feeds it back into self.tokens for the next step."""
+        greedy pick (self.next_token) and feeds it back into self.tokens for the next step. ``attend(l)`` stands in for
+        _attend: it reads self.q, self.k, self.v and returns the attention's output."""
         c, w, B = self.cfg, self.wg, self.batch
 
         def gemv(x, name, l=None, **kw):
@@ -199,21 +228,14 @@ class Llama:
             return self._gemv(x, w[name] if l is None else w[name][l], **kw)
 
         self._embed(w["embed"], self.tokens, out=self.x, status=self.status)
-        att_flat = self.att.view(B, self._q_dim)
         pending = None  # partial products of the previous layer's down projection, still to be added into x
         for l in range(c.n_layers):
             A.rmsnorm(self.x, w["rms_att"][l], c.norm_eps, out=self.xb, partials=pending)
             pending = None
             gemv(self.xb, "wqkv", l, out=self.q.view(B, self._q_dim), out2=self.k.view(B, self._kv_dim),
                  out3=self.v.view(B, self._kv_dim), clip=c.qkv_clip)
-            A.rope_kv_insert(self.q, self.k, self.v, self.k_cache[l], self.v_cache[l], self.pos, self.kv_pos,
-                             theta=c.rope_theta, rotary_dim=c.rotary_dim, kv_sink=kv_sink, q_out=self.q,
-                             pos_early=True)   # positions are copied in before the step's first kernel
-            # (two_pass: another order of the sums moves fp16 ties of the next layers' cache rows, so a step's results would
-            # change with max_seq_len, which the choice of the form looks at)
-            A.attn_decode(self.q, self.k_cache[l], self.v_cache[l], self.kv_len, out=self.att,
-                          workspace=self.workspace, kv_early=self.kv_early and kv_sink == 0, two_pass=True)
-            gemv(att_flat, "wo", l, out=self.x, accumulate=True)           # x += Wo att
+            att = self._attend(l, kv_sink) if attend is None else attend(l)
+            gemv(att.view(B, self._q_dim), "wo", l, out=self.x, accumulate=True)   # x += Wo att
             A.rmsnorm(self.x, w["rms_ffn"][l], c.norm_eps, out=self.xb)
             gemv(self.xb, "w13", l, out=self.hb, swiglu=True)              # hb = silu(W1 xb) * (W3 xb)
             if self._k_split > 1:
@@ -249,10 +271,22 @@ class Llama:
         ``exact`` = False drops the residual terms (activations and Q8_0 weights enter the tensor cores rounded once to
         fp16, one MMA instead of two or three): a third of the tensor work, results within about 1e-3 relative, no
         longer guaranteed to give the token-at-a-time path's greedy tokens."""
-        import numpy as np
-        c, w, B, dev = self.cfg, self.w, self.batch, self.device
-        if len(prompts) != B or not self.can_prefill(prompts):
+        if len(prompts) != self.batch or not self.can_prefill(prompts):
             raise ValueError("prefill() needs one prompt per sequence, head_dim 64 or 128 and prompts that fit the cache")
+        w, c = self.w, self.cfg
+        x, last_rows = self._prompt_rows(prompts, self.k_cache, self.v_cache, exact)
+        # the last token of every prompt: final norm, classifier, greedy pick (the decode step's own kernels)
+        A.gather_rows(x, last_rows, out=self.x)
+        A.rmsnorm(self.x, w["rms_final"], c.norm_eps, out=self.xb)
+        self._gemv(self.xb, self.wg["wcls"], out=self.logits, **({"rows": self._rows["wcls"]} if self._rows else {}))
+        A.argmax(self.logits, out=self.next_token)
+        self.tokens.copy_(self.next_token)
+
+    def _prompt_rows(self, prompts, k_cache: torch.Tensor, v_cache: torch.Tensor, exact: bool):
+        """All layers over the tokens of ``prompts``, whose keys and values go into rows 0, 1, ... of k_cache, v_cache [layers,
+        len(prompts), rows, Hkv, D]. Returns the tokens' last hidden rows and the row of each prompt's last token."""
+        import numpy as np
+        c, w, B, dev = self.cfg, self.w, len(prompts), self.device
         q8 = self.weight_type == "q8_0"
         lens = [len(p) for p in prompts]
         starts = np.concatenate([[0], np.cumsum(lens)]).astype(np.int64)
@@ -298,23 +332,24 @@ class Llama:
         for l in range(c.n_layers):
             A.rmsnorm_pair(x, w["rms_att"][l], c.norm_eps, out=pair_d)
             project(pair_d, w["wqkv"][l], qkv)
-            A.rope_prompt(qkv, q16, self.k_cache[l], self.v_cache[l], token_seq, token_pos, n_heads=H,
-                          theta=c.rope_theta, rotary_dim=c.rotary_dim, qkv_clip=c.qkv_clip)
+            if self._own_rope:
+                heads = qkv.view(T, H + 2 * c.n_kv_heads, D)
+                X.rope_positions(heads[:, :H], heads[:, H:H + c.n_kv_heads], heads[:, H + c.n_kv_heads:], k_cache[l], v_cache[l],
+                                 token_pos, token_pos, seq=token_seq, inv_freq=self._inv_freq, factor=self._rope_factor,
+                                 layout=self._rope_layout, q_out=q16, status=self.status)
+            else:
+                A.rope_prompt(qkv, q16, k_cache[l], v_cache[l], token_seq, token_pos, n_heads=H,
+                              theta=c.rope_theta, rotary_dim=c.rotary_dim, qkv_clip=c.qkv_clip)
             for b in range(B):
                 s0, s1, n = int(starts[b]), int(starts[b + 1]), lens[b]
-                A.attn_prefill_causal(q16[s0:s1].unsqueeze(0), self.k_cache[l, b, :n].unsqueeze(0),
-                                      self.v_cache[l, b, :n].unsqueeze(0), out=att[s0:s1].unsqueeze(0), status=self.status)
+                A.attn_prefill_causal(q16[s0:s1].unsqueeze(0), k_cache[l, b, :n].unsqueeze(0),
+                                      v_cache[l, b, :n].unsqueeze(0), out=att[s0:s1].unsqueeze(0), status=self.status)
             A.split_pair(att.view(T, q_dim), out=pair_q)
             project(pair_q, w["wo"][l], x, accumulate=True)               # x += Wo att
             A.rmsnorm_pair(x, w["rms_ffn"][l], c.norm_eps, out=pair_d)
             project(pair_d, w["w13"][l], pair_h, swiglu=True)             # silu(gate) * up
             project(pair_h, w["w2"][l], x, accumulate=True)               # x += W2 (silu(gate) * up)
-        # the last token of every prompt: final norm, classifier, greedy pick (the decode step's own kernels)
-        A.gather_rows(x, last_rows, out=self.x)
-        A.rmsnorm(self.x, w["rms_final"], c.norm_eps, out=self.xb)
-        self._gemv(self.xb, self.wg["wcls"], out=self.logits, **({"rows": self._rows["wcls"]} if self._rows else {}))
-        A.argmax(self.logits, out=self.next_token)
-        self.tokens.copy_(self.next_token)
+        return x, last_rows
 
     def capture(self) -> None:
         """Record the step once per mode (prefill: no classifier; decode: classifier + greedy pick + feedback) as CUDA
@@ -401,4 +436,76 @@ class Llama:
                           else "token-at-a-time")
         if int(self.status.item()) != 0 or int(self.workspace.status.item()) != 0:
             raise RuntimeError("a kernel reported a status bit (token id out of range or a wait that ran out)")
+        return (out.cpu(), out_logits.cpu()) if want_logits else out.cpu()
+
+    def encode_prefix(self, tokens, exact: bool = True):
+        """Keys and values of a prefix that sequences will share: (k, v) fp16 [layers, P, Hkv, D], computed once by the prompt
+        phase (prefill)."""
+        c = self.cfg
+        P = len(tokens)
+        if not self.can_prefill([tokens[:1]]) or P == 0:
+            raise ValueError("a prefix needs at least one token and a model that prefill() takes")
+        k = torch.empty((c.n_layers, 1, P, c.n_kv_heads, c.head_dim), dtype=torch.float16, device=self.device)
+        v = torch.empty_like(k)
+        self._prompt_rows([list(tokens)], k, v, exact)
+        return k[:, 0], v[:, 0]
+
+    def generate_shared(self, prefix, prompts, n_new: int, *, budget: int = 0, sink: int = KV_SINK, recent: int = 0,
+                        evict_every: int = 32, want_logits: bool = False):
+        """Greedy generation of a ragged batch behind a shared prefix: what generate() gives for prefix + prompt of every sequence, with
+        the prefix computed and kept once. ``prefix`` is a list of token ids or what encode_prefix() returned for one. The own caches
+        hold the prompts' and the generated tokens' rows only; the prompts are fed one token per step.
+        ``budget`` > 0 bounds them: whenever a cache holds budget + evict_every rows, every layer and kv head keeps budget of them -
+        the first ``sink``, the last ``recent`` (0: half of the budget) and those that received the most attention weight so far
+        (context.kv_evict). Returns int32 [B, n_new] on the host (and the logits, when asked)."""
+        c, B, dev = self.cfg, self.batch, self.device
+        if len(prompts) != B or any(len(p) == 0 for p in prompts):
+            raise ValueError("one non-empty prompt per sequence of the batch")
+        kp, vp = prefix if isinstance(prefix, tuple) else self.encode_prefix(prefix)
+        P, longest = kp.shape[1], max(len(p) for p in prompts)
+        rows = longest + n_new if budget <= 0 else min(longest + n_new, budget + evict_every)
+        recent = recent or budget // 2
+        if rows > c.max_seq_len or (budget > 0 and (evict_every < 1 or sink + recent > budget)):
+            raise ValueError("the own rows must fit max_seq_len, and the sink and recent rows the budget")
+        kc, vc = self.k_cache[:, :, :rows], self.v_cache[:, :, :rows]
+        evicts = budget > 0 and longest + n_new > rows
+        scores = torch.zeros((c.n_layers, B, c.n_kv_heads, rows), device=dev) if evicts else None
+        workspace = X.SharedWorkspace(B, c.n_heads, c.n_kv_heads, c.head_dim, rows=rows if evicts else 0, device=dev)
+        q16 = torch.empty((B, c.n_heads, c.head_dim), dtype=torch.float16, device=dev)
+        att = torch.empty((B, c.n_heads, c.head_dim), dtype=torch.float32, device=dev)
+
+        def attend(l):
+            X.rope_positions(self.q, self.k, self.v, kc[l], vc[l], self.pos, self.kv_pos, inv_freq=self._inv_freq,
+                             factor=self._rope_factor, layout=self._rope_layout, q_out=q16, status=self.status)
+            return X.attn_decode_shared(q16, kp[l], vp[l], kc[l], vc[l], self.kv_len, out=att,
+                                        scores=None if scores is None else scores[l], workspace=workspace)
+
+        delay = [longest - len(p) for p in prompts]  # sequences start late, so that all prompts end at the same step
+        held = [0] * B                               # rows of each cache
+        out = torch.zeros((B, n_new), dtype=torch.int32, device=dev)
+        out_logits = torch.zeros((B, n_new, c.vocab_size), device=dev) if want_logits else None
+        for step in range(longest + n_new - 1):
+            at = [max(step - d, 0) for d in delay]   # index of the token in its sequence; one that waits feeds its first again
+            if evicts and max(held) == rows:
+                for l in range(c.n_layers):          # (self.kv_len still holds the last step's lengths)
+                    X.kv_evict(kc[l], vc[l], scores[l], self.kv_len, budget, sink=sink, recent=recent, status=self.status)
+                held = [min(n, budget) for n in held]
+            for b, d in enumerate(delay):
+                if step <= d:                        # its first token: row 0 of an empty cache
+                    held[b] = 0
+                    if scores is not None:
+                        scores[:, b].zero_()
+            positions = torch.tensor([[P + a for a in at], held, [n + 1 for n in held]], dtype=torch.int32).pin_memory()
+            self._positions.copy_(positions, non_blocking=True)
+            held = [n + 1 for n in held]
+            if step < longest:
+                self.tokens.copy_(torch.tensor([p[a] for p, a in zip(prompts, at)], dtype=torch.int32).pin_memory(), non_blocking=True)
+            self._launch_step(0, step + 1 >= longest, attend)
+            if step + 1 >= longest:
+                out[:, step + 1 - longest] = self.next_token
+                if want_logits:
+                    out_logits[:, step + 1 - longest] = self.logits
+        torch.cuda.synchronize(dev)
+        if int(self.status.item()) != 0 or int(workspace.status.item()) != 0:
+            raise RuntimeError("a kernel reported a status bit (token id or cache row out of range, or a wait that ran out)")
         return (out.cpu(), out_logits.cpu()) if want_logits else out.cpu()
