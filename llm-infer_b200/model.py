@@ -86,6 +86,8 @@ def random_weights(cfg: ModelConfig, seed: int, device="cpu", weight_type: str =
 class Llama:
     """Batched token-at-a-time forward, whole-prompt prefill and greedy generation on one GPU."""
 
+    _own_rope = False  # the engine's rotary kernels, unless the model asks for other positions
+
     def __init__(self, cfg: ModelConfig, weights: dict, batch: int, device=None, weight_type: str = "f16",
                  rope_layout: str = "interleaved", rope_scaling: dict | None = None):
         """``rope_layout`` and ``rope_scaling`` (context.rope_frequencies): positions of models that pair a head's halves, or whose
