@@ -155,22 +155,29 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_
                 count(i + 3, k.w);
             }
         }
-        meet();
-        // thread t owns the bins from kBins - kOwn - kOwn t up, so that threads run from the top: it sums them over the cluster
-        constexpr int kOwn = kBins / kSelThreads;  // two
-        const int bin0 = kBins - kOwn - kOwn * tid;
-        uint2 mine = make_uint2(0, 0);
-#pragma unroll
-        for (int c = 0; c < kCtas; ++c) {
-#pragma unroll
-            for (int copy = 0; copy < (pass == 0 ? 2 : 1); ++copy) {
-                const uint2* src = reinterpret_cast<const uint2*>(hist + copy * kBins + bin0);
-                // (each CTA starts with another one: all of them on one CTA's memory at a time took 3 us more per digit)
-                const uint2 h = kCtas > 1 ? *cluster.map_shared_rank(src, (rank + c) % kCtas) : *src;
-                mine.x += h.x, mine.y += h.y;
+        if (pass == 0) {  // the two copies into one
+            __syncthreads();
+            for (int i = tid; i < kBins / 4; i += kSelThreads) {
+                uint4* x = reinterpret_cast<uint4*>(hist) + i;
+                const uint4 y = x[kBins / 4];
+                *x = make_uint4(x->x + y.x, x->y + y.y, x->z + y.z, x->w + y.w);
             }
         }
-        const uint32_t sum = mine.x + mine.y;
+        meet();
+        // thread t of the first 512 owns the four bins from kBins - 4 - 4 t up, so that threads run from the top: it sums them over the
+        // cluster, 16 bytes at a time
+        const int bin0 = kBins - 4 - 4 * tid;
+        uint4 mine = make_uint4(0, 0, 0, 0);
+        if (tid < kBins / 4) {
+            const uint4* src = reinterpret_cast<const uint4*>(hist + bin0);
+#pragma unroll
+            for (int c = 0; c < kCtas; ++c) {
+                // (each CTA starts with another one: all of them on one CTA's memory at a time took 1 us more per digit)
+                const uint4 h = kCtas > 1 ? *cluster.map_shared_rank(src, (rank + c) % kCtas) : *src;
+                mine.x += h.x, mine.y += h.y, mine.z += h.z, mine.w += h.w;
+            }
+        }
+        const uint32_t sum = mine.x + mine.y + mine.z + mine.w;
         uint32_t incl = sum;
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
@@ -181,9 +188,9 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_
         __syncthreads();
         const uint32_t above = incl - sum + __reduce_add_sync(0xffffffffu, lane < warp ? s_gt[lane] : 0u);
         if (above < need && above + sum >= need) {  // one thread
-            const bool upper = above + mine.y >= need;
-            s_pick[0] = bin0 + (upper ? 1 : 0);
-            s_pick[1] = above + (upper ? 0 : mine.y);
+            const uint32_t a1 = above + mine.w, a2 = a1 + mine.z, a3 = a2 + mine.y;  // keys in and above the upper one, two, three bins
+            s_pick[0] = bin0 + (a1 >= need ? 3 : a2 >= need ? 2 : a3 >= need ? 1 : 0);
+            s_pick[1] = a1 >= need ? above : a2 >= need ? a1 : a3 >= need ? a2 : a3;
         }
         __syncthreads();
         prefix |= s_pick[0] << shift;
@@ -234,28 +241,29 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_
         gt += __reduce_add_sync(0xffffffffu, og);
         eq += __reduce_add_sync(0xffffffffu, oe);
     }
-    // ---- the kept rows, in order: row i goes to place (kept rows in front of it)
-    for (uint32_t i0 = wb; i0 < we; i0 += 128) {  // the same number of rounds for all lanes
-        const uint32_t i = i0 + 4 * lane;
-        uint32_t is_gt[4], is_eq[4];
-        tally(i, i < we ? keys_at(i) : make_uint4(0, 0, 0, 0), is_gt, is_eq);
-        uint32_t mine = is_gt[0] + is_gt[1] + is_gt[2] + is_gt[3] + ((is_eq[0] + is_eq[1] + is_eq[2] + is_eq[3]) << 16);
-        uint32_t incl = mine;
-#pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-            const uint32_t o = __shfl_up_sync(0xffffffffu, incl, d);
-            if (lane >= d) incl += o;
+    // ---- the kept rows, in order: row i goes to place (kept rows in front of it). A row of keys per lane; equal keys are rare, and
+    // rows without one take the short way.
+    const uint32_t below = (1u << lane) - 1u;
+    auto emit = [&](uint32_t i, bool in, uint32_t key) {
+        const bool is_gt = in && key > prefix, is_eq = in && key == prefix;
+        const uint32_t m_gt = __ballot_sync(0xffffffffu, is_gt), m_eq = __ballot_sync(0xffffffffu, is_eq);
+        uint32_t place = gt + min(eq, need) + __popc(m_gt & below);
+        bool stays = is_gt;
+        if (m_eq) {
+            const uint32_t my_eq = eq + __popc(m_eq & below);
+            place += min(my_eq, need) - min(eq, need);
+            stays = is_gt || (is_eq && my_eq < need);
         }
-        const uint32_t all = __shfl_sync(0xffffffffu, incl, 31);
-        uint32_t g = gt + ((incl - mine) & 0xffffu), e = eq + ((incl - mine) >> 16);
-#pragma unroll
-        for (int a = 0; a < 4; ++a) {
-            if (is_gt[a] || (is_eq[a] && e < need)) kept[g + min(e, need)] = begin + i + a;
-            g += is_gt[a];
-            e += is_eq[a];
-        }
-        gt += all & 0xffffu;
-        eq += all >> 16;
+        if (stays) kept[place] = begin + i;
+        gt += __popc(m_gt);
+        eq += __popc(m_eq);
+    };
+    const uint32_t whole = wb + (min(we, n_staged) > wb ? (min(we, n_staged) - wb) / 32 * 32 : 0u);  // full rounds of staged keys
+#pragma unroll 4
+    for (uint32_t i0 = wb; i0 < whole; i0 += 32) emit(i0 + lane, true, s_keys[i0 + lane]);
+    for (uint32_t i0 = whole; i0 < we; i0 += 32) {
+        const uint32_t i = i0 + lane;
+        emit(i, i < we, i < n_staged ? s_keys[i] : i < we ? make_key(i, scores[i]) : 0u);
     }
     if constexpr (kCtas > 1) cluster.sync();  // no CTA leaves while another reads its counts
 }
