@@ -443,9 +443,9 @@ extern "C" int attn_kv_evict(const AttnKvEvictArgs* a, void* stream_v) {
     p.status = a->status;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
 
-    // ---- which rows: as many CTAs per cluster as give a CTA at least 2048 rows, eight at most
+    // ---- which rows: one CTA for up to 8192 rows (meeting another one costs more than 4096 rows do), eight at most
     uint32_t cl = 1;
-    while (cl < 8 && a->rows > cl * 2048ull) cl *= 2;
+    while (cl < 8 && a->rows > cl * 8192ull) cl *= 2;
     const uint64_t slice = (a->rows + cl - 1) / cl + 128 * kSelWarps;
     p.scores_aligned = aligned16(a->scores) && p.score_stride % 4 == 0;
     p.staged = static_cast<uint32_t>(slice < 40 * 1024 ? slice : 40 * 1024);
