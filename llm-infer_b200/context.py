@@ -293,29 +293,31 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor,
     B, T, Hkv, D = k_cache.shape
     T2 = k_out.shape[1]
     dtype = k_cache.dtype
-    strides = []
-    for a, b, n in ((k_cache, v_cache, T), (k_out, v_out, T2)):
-        stride = a.stride()
-        if a.shape != (B, n, Hkv, D) or b.shape != (B, n, Hkv, D) or b.stride() != stride or stride[3] != 1 or stride[2] != D:
-            raise ValueError("the caches must be [B, row, kv_head, head_dim] with dense heads; K and V share their strides")
-        if dtype not in _CACHE or a.dtype != dtype or b.dtype != dtype:
-            raise TypeError("the caches must be fp16 or bf16, of one type")
-        strides.append(stride)
+    s_in, s_out = k_cache.stride(), k_out.stride()
+    if v_cache.shape != k_cache.shape or k_out.shape != (B, T2, Hkv, D) or v_out.shape != k_out.shape or v_cache.stride() != s_in or \
+            v_out.stride() != s_out or s_in[3] != 1 or s_in[2] != D or s_out[3] != 1 or s_out[2] != D:
+        raise ValueError("the caches must be [B, row, kv_head, head_dim] with dense heads; K and V share their strides")
+    if dtype not in _CACHE or not (v_cache.dtype == k_out.dtype == v_out.dtype == dtype):
+        raise TypeError("the caches must be fp16 or bf16, of one type")
     score_stride, score_out_stride = _score_stride(scores, B, Hkv, T), _score_stride(scores_out, B, Hkv, T2)
     if keep < 1 or keep > T2 or sink < 0 or recent < 0 or sink + recent > keep:
         raise ValueError("keep must be at least 1, fit the output caches and hold the sink and the recent rows")
     if kept is None:
         kept = torch.empty_strided((B, Hkv, keep), (Hkv * keep, keep, 1), dtype=torch.int32, device=k_cache.device)
-    kept_ptr = _index(kept, (B, Hkv, keep), "kept")
+        kept_ptr = kept.data_ptr()
+    else:
+        kept_ptr = _index(kept, (B, Hkv, keep), "kept")
+    len_ptr = 0 if kv_len is None else _index(kv_len, (B,), "kv_len")
     if kv_len_out is None:
         kv_len_out = torch.empty((B,), dtype=torch.int32, device=k_cache.device) if kv_len is None else torch.empty_like(kv_len)
-    len_out_ptr = _index(kv_len_out, (B,), "kv_len_out")
+        len_out_ptr = kv_len_out.data_ptr()
+    else:
+        len_out_ptr = _index(kv_len_out, (B,), "kv_len_out")
     if B == 0:
         return kept, kv_len_out
-    s_in, s_out = strides
     _enqueue("attn_kv_evict", index, stream, EVICT_ARGS.pack(
         k_cache.data_ptr(), v_cache.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), scores.data_ptr(), scores_out.data_ptr(), kept_ptr,
-        0 if kv_len is None else _index(kv_len, (B,), "kv_len"), len_out_ptr, B, Hkv, D, T, T2, keep, sink, recent,
+        len_ptr, len_out_ptr, B, Hkv, D, T, T2, keep, sink, recent,
         s_in[1] if T > 1 else 0, s_out[1] if T2 > 1 else 0, s_in[0] if B > 1 else 0, s_out[0] if B > 1 else 0, score_stride,
         score_out_stride, 0 if status is None else status.data_ptr()))
     return kept, kv_len_out
