@@ -550,11 +550,12 @@ __device__ __forceinline__ void find_pieces(const SharedParams& p, uint32_t b, u
 }
 
 // Output CTAs: one per (query row, slice of SLICE floats). Groups of SLICE / 4 lanes take a piece each, several pieces in flight per
-// lane; the groups' results merge by shuffles, then over the warps. Score CTAs behind them.
-template <int D, int SLICE>
+// lane; the groups' results merge by shuffles, then over the warps. WARP_ROWS: a warp takes a whole row by itself, four rows a CTA (many
+// rows of few pieces: 2048 rows of ten pieces take 11 us with four warps a row). Score CTAs behind them.
+template <int D, int SLICE, bool WARP_ROWS>
 __global__ void __launch_bounds__(kThreads) shared_merge_kernel(const __grid_constant__ SharedParams p) {
-    constexpr int kLanes = SLICE / 4;           // of a group
-    constexpr int kGroups = kThreads / kLanes;  // pieces at once
+    constexpr int kLanes = SLICE / 4;                                // of a group
+    constexpr int kGroups = (WARP_ROWS ? 32 : kThreads) / kLanes;    // pieces at once
     __shared__ __align__(16) float s_o[4][SLICE];
     __shared__ float s_ml[4][2];
     __shared__ float s_lse[64];
@@ -562,11 +563,12 @@ __global__ void __launch_bounds__(kThreads) shared_merge_kernel(const __grid_con
     grid_dep_launch_dependents();
     grid_dep_wait();
     if (blockIdx.x < p.out_ctas) {
-        const uint32_t row = blockIdx.x / (D / SLICE), slice = blockIdx.x % (D / SLICE);
+        const uint32_t row = WARP_ROWS ? blockIdx.x * 4 + warp : blockIdx.x / (D / SLICE), slice = WARP_ROWS ? 0 : blockIdx.x % (D / SLICE);
+        if (WARP_ROWS && row >= p.batch * p.n_heads) return;
         const uint32_t b = fast_div(row, p.div_heads), h = row - b * p.n_heads;
         Pieces x;
         find_pieces<D>(p, b, h, x);
-        const int in_group = lane % kLanes, group = tid / kLanes;
+        const int in_group = lane % kLanes, group = (WARP_ROWS ? lane : tid) / kLanes;
         float m = -INFINITY, l = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         auto fold = [&](float mo, float lo, float4 v) {  // another state: maximum, sum, weighted sum
@@ -608,6 +610,18 @@ __global__ void __launch_bounds__(kThreads) shared_merge_kernel(const __grid_con
             v.z = __shfl_xor_sync(0xffffffffu, acc.z, d);
             v.w = __shfl_xor_sync(0xffffffffu, acc.w, d);
             fold(mo, lo, v);
+        }
+        if constexpr (WARP_ROWS) {
+            if (lane < kLanes) {
+                const float inv = l > 0.f ? 1.f / l : 0.f;
+                const size_t at = static_cast<size_t>(row) * D + lane * 4;
+                acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
+                if (p.o_dtype == ATTN_DTYPE_F32) *reinterpret_cast<float4*>(static_cast<float*>(p.o) + at) = acc;
+                else if (p.o_dtype == ATTN_DTYPE_F16) *reinterpret_cast<uint2*>(static_cast<__half*>(p.o) + at) = make_uint2(pack2<false>(acc.x, acc.y), pack2<false>(acc.z, acc.w));
+                else *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.o) + at) = make_uint2(pack2<true>(acc.x, acc.y), pack2<true>(acc.z, acc.w));
+            }
+            if (lane == 0 && p.lse) p.lse[row] = l > 0.f ? (m + __log2f(l)) * 0.69314718055994531f : -INFINITY;
+            return;
         }
         if (lane < kLanes) *reinterpret_cast<float4*>(&s_o[warp][lane * 4]) = acc;
         if (lane == 0) {
@@ -924,17 +938,11 @@ extern "C" int attn_decode_shared(const AttnDecodeSharedArgs* a, void* stream_v)
     p.o_dtype = a->o_dtype;
     p.scores = a->scores;
     p.scores_out = a->scores_out;
-    // Few output rows: slices of 32 floats, so that more CTAs take fewer pieces each.
-    const uint64_t rows = static_cast<uint64_t>(a->batch) * a->n_heads;
-    const bool sliced = rows * (a->head_dim / 32) <= 8ull * dev.sm_count;
-    p.out_ctas = static_cast<uint32_t>(sliced ? rows * (a->head_dim / 32) : rows);
     // A CTA adds up the weights of 128 rows or a multiple of it, so that there are about eight CTAs per SM.
     const uint64_t segs = static_cast<uint64_t>(a->batch) * a->n_kv_heads;
     const uint64_t per_cta = (segs * a->kv_capacity + 8ull * dev.sm_count - 1) / (8ull * dev.sm_count);
     p.score_rows = static_cast<uint32_t>(std::max<uint64_t>(1, (per_cta + kThreads - 1) / kThreads)) * kThreads;
     p.score_chunks = (a->kv_capacity + p.score_rows - 1) / p.score_rows;
-    const uint64_t merge_ctas = p.out_ctas + (scored ? segs * p.score_chunks : 0);
-    if (merge_ctas > 0x7fffffffull) return ATTN_ERR_UNSUPPORTED;
 
     cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
     const bool bf16 = a->dtype == ATTN_DTYPE_BF16, res = a->o_dtype == ATTN_DTYPE_F32;
@@ -1025,11 +1033,21 @@ extern "C" int attn_decode_shared(const AttnDecodeSharedArgs* a, void* stream_v)
                   : (res ? split(shared_split_kernel<64, false, true>) : split(shared_split_kernel<64, false, false>));
     }
     if (rc != ATTN_OK) return rc;
+    // Few output rows: slices of 32 floats, so that more CTAs take fewer pieces each. Many rows: whole rows, by a warp each where few CTAs
+    // share a segment. (16-byte stores need an output aligned to them.)
+    const uint64_t rows = static_cast<uint64_t>(a->batch) * a->n_heads;
+    const bool sliced = rows * (a->head_dim / 32) <= 8ull * dev.sm_count;
+    const uint64_t pieces = (p.prefix_segs ? (tensor ? choice.prefix_ctas : grid) / p.prefix_segs * p.pre.ts + 1 : 0) + grid / plan.own_segs * p.own.ts + 1;
+    const bool warp_rows = !sliced && pieces <= 24 && aligned16(a->o);
+    p.out_ctas = static_cast<uint32_t>(sliced ? rows * (a->head_dim / 32) : warp_rows ? (rows + 3) / 4 : rows);
+    const uint64_t merge_ctas = p.out_ctas + (scored ? segs * p.score_chunks : 0);
+    if (merge_ctas > 0x7fffffffull) return ATTN_ERR_UNSUPPORTED;
     auto merge = [&](auto kernel) -> int {
         B200_CUDA_TRY(launch_dependent(kernel, dim3(static_cast<uint32_t>(merge_ctas)), dim3(kThreads), 0, stream, p));
         g_launch_count.fetch_add(1, std::memory_order_relaxed);
         return ATTN_OK;
     };
-    if (sliced) return a->head_dim == 128 ? merge(shared_merge_kernel<128, 32>) : merge(shared_merge_kernel<64, 32>);
-    return a->head_dim == 128 ? merge(shared_merge_kernel<128, 128>) : merge(shared_merge_kernel<64, 64>);
+    if (sliced) return a->head_dim == 128 ? merge(shared_merge_kernel<128, 32, false>) : merge(shared_merge_kernel<64, 32, false>);
+    if (warp_rows) return a->head_dim == 128 ? merge(shared_merge_kernel<128, 128, true>) : merge(shared_merge_kernel<64, 64, true>);
+    return a->head_dim == 128 ? merge(shared_merge_kernel<128, 128, false>) : merge(shared_merge_kernel<64, 64, false>);
 }
