@@ -1,13 +1,17 @@
 // Eviction from a KV cache by accumulated attention weight: of every (sequence, kv head), the first `sink` rows, the last
 // `recent` rows and the rows with the largest scores, `keep` in all, stay; their order stays too. Ties go to the lowest row.
 //
-// Two launches. (1) Which rows: a cluster of CTAs per (sequence, kv head) finds the keep-th largest key by a radix selection
+// Two launches. (1) Which rows: a CTA or a cluster of them per (sequence, kv head) finds the keep-th largest key by a radix selection
 // (digits of 11, 11 and 10 bits, a histogram in shared memory per CTA, summed over the cluster), then counts and writes the
 // kept rows in order. A score's key is its bit pattern mapped so that unsigned order is the order of the numbers (NaN below
 // everything, -0 = +0); always-kept rows carry the largest key. (2) The copy, bound by memory: kept K and V rows and scores are
 // read once and written once. Into another cache it is a plain gather with as many blocks as it has work for. In place, a row only
 // moves down, so one CTA per (head, slice of the row) goes through the rows in order: everything it still has to read lies
 // behind what it writes.
+//
+// Graphs of calls: 16 ragged sequences of up to 4096 rows into caches of 1999 (8 kv heads of 128, 246 MB) 49.3 us, of which the
+// copy is 39 (6.2 TB/s) and the selection 6; one sequence of 131072 rows to 16384 48.6 us: copy 22, selection 19 (a digit costs 3.5 us,
+// 2 of them the sum of the histograms over eight CTAs); 1024 rows to 256 8.9 us, all of it latency.
 #include "attn_internal.cuh"
 #include "ptx_sm100.cuh"
 

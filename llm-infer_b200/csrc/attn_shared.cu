@@ -6,17 +6,23 @@
 // softmax-normalised sum and log-sum-exp, and the pieces merge by weights exp(lse_i - LSE). All B * G query rows of a kv head meet the
 // prefix together as one matrix, so a prefix row is read once for the batch and not once per sequence.
 //
-// Two launches:
+// Two launches, or three with a long prefix and many query rows, whose product then has a kernel of its own (attn_shared_prefix.cu):
 //   split   tiles of 64 (row, head) pairs of K and V, prefix tiles first, then the own rows of sequence after sequence, are dealt to the
-//           CTAs in equal contiguous runs (two CTAs per SM). A fifth warp streams the tiles through a ring in shared memory, one TMA
-//           box each for K and V; four warps multiply by mma.sync (16 query rows x 16 keys x 8 at a time). A warp owns 16 query rows of one
-//           kv head and a share of the tile's keys: with few query rows the four warps take four heads (whose slices of a cache row
-//           are contiguous) or four shares of the keys, with many rows of the prefix product four blocks of 16 rows.
-//   merge   one CTA per output row (or slice of it) folds that row's pieces; further CTAs turn the scaled scores that the split pass left
-//           in the workspace into weights (exp2(s - LSE)), sum them over the heads and add them to the accumulators.
+//           CTAs in contiguous runs of equal cost (two CTAs per SM). A warp streams K and V tiles through a ring in shared memory, a TMA
+//           box each; four warps multiply by mma.sync (16 query rows x 16 keys x 8 at a time). A warp owns 16 query rows of one kv
+//           head and a share of the tile's keys: with few query rows the four warps take four heads (whose slices of a cache row are
+//           contiguous) or four shares of the keys, with many rows of the prefix product four blocks of 16 rows.
+//   merge   folds the pieces of an output row, by a warp, a CTA, or a CTA per slice of the row; further CTAs turn the scaled scores that
+//           the split pass left in the workspace into weights (exp2(s - LSE)), sum them over the heads and add them to the accumulators.
 // The scores of own rows cost 4 bytes per query head and row each way through L2, next to 4 * head_dim bytes of K and V per kv head.
 // P enters the second product rounded once to the caches' type when the output is 16 bits wide too (an error below the
 // output's own rounding), and as value + rounding residual for fp32 outputs.
+//
+// Bound by HBM where there is enough to read: 16 ragged caches of up to 4096 rows (168 MB, with weights) take 38.6 us in a graph of
+// calls, of which the streaming alone takes 30; 7 sequences over 131072 shared rows (543 MB) 95 us = 5.7 TB/s. Smaller calls are a chain
+// of latencies: lengths and dealing 1.1 us, query rows and first tile 2.5, a tile 1.2 us from barrier to barrier, pieces and merge 4.
+// What that taught: query rows requested behind the tiles' 28 MB came 3 to 5 us late, a chain of eight dependent MMAs and divisions by
+// variables show, and a tile in two slots (K is handed back before the softmax) keeps the stream going.
 #include <cuda.h>
 
 #include <algorithm>

@@ -9,10 +9,13 @@
 // contiguous runs; a CTA's part of a segment is one piece. The CTA's warps work as in the causal prefill: two softmax
 // warpgroups (a thread owns a query row, which is a tensor-memory lane), one thread that feeds K and V by TMA through a ring of
 // four stages, one thread that issues the MMAs, scores two blocks ahead of the products. Query rows of a kv head are not evenly
-// spaced (heads of one group, then the next sequence), so the softmax threads bring their own row into the swizzled tile.
+// spaced (heads of one group, then the next sequence), so the softmax warps bring them into the swizzled tile.
 //
-// Bound by the K/V stream up to 128 rows (a block is 32 KB, 0.72 us of an SM's share of HBM; its scores take a warpgroup less),
-// by the exponentials and the MMAs' shared-memory reads from there on.
+// Bound by the K/V stream up to 128 rows: a block takes 0.80 us of a CTA (32 KB, 0.72 us of an SM's share of HBM). With two tiles it
+// takes 1.1 us, in which the special-function units are busy for 0.55 and the tensor pipe for 0.6: the chain from scores to
+// probabilities of one block. A launch costs 10 us around its blocks (query rows 2, first block 2, piece and exit 4), which is why
+// short prefixes stay in the split pass of attn_shared.cu. 256 query rows x 65536 keys, 8 kv heads of 128, fp16: 79 us in all
+// (in the split pass: 355); 128 rows: 56 (185); 20 rows: 52 (51).
 // Every wait is bounded; on expiry the role records ATTN_STATUS_WAIT_TIMEOUT, stops, and the CTA still runs its common exit.
 #include <cuda.h>
 
@@ -350,7 +353,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         if (warp == 8 && elect_one()) {
             // =============================== TMA producer ===============================
             uint32_t st = 0, phase = 0, it = 0;
-            bool ok = true;
+            bool ok = true, key_ahead = false;  // key_ahead: the stage's K is under way, its V is not
             Item w;
             for (uint32_t at = t0; ok && item_at(at, w); at += w.blocks) {
                 for (uint32_t j = 0; j < w.blocks; ++j, ++it) {
@@ -360,7 +363,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                     mbar_arrive_expect_tx(bar(BAR_K_FULL + st), kLoadKv);
                     tma_load_3d(kdst, &tm_k, bar(BAR_K_FULL + st), 0, row, head);
                     if (HD > 64) tma_load_3d(kdst + kKvSubBytes, &tm_k, bar(BAR_K_FULL + st), 64, row, head);
-                    if (it >= kStages && !mbar_wait(bar(BAR_V_EMPTY + st), phase ^ 1)) { ok = false; break; }
+                    if (it >= kStages && !mbar_wait(bar(BAR_V_EMPTY + st), phase ^ 1)) { ok = false; key_ahead = true; break; }
                     const uint32_t vdst = base + kSmemV + st * kKvBytes;
                     mbar_arrive_expect_tx(bar(BAR_V_FULL + st), kLoadKv);
                     tma_load_3d(vdst, &tm_v, bar(BAR_V_FULL + st), 0, row, head);
@@ -368,7 +371,14 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                     if (++st == kStages) st = 0, phase ^= 1;
                 }
             }
-            if (!ok) report_timeout(p.status);
+            if (!ok) {  // report, and leave no copy in flight into this CTA's memory
+                report_timeout(p.status);
+                for (uint32_t s = 0; s < kStages; ++s) {
+                    const uint32_t v_phase = s < st ? phase : phase ^ 1, k_phase = s == st && key_ahead ? phase : v_phase;
+                    (void)mbar_wait(bar(BAR_K_FULL + s), k_phase);
+                    (void)mbar_wait(bar(BAR_V_FULL + s), v_phase);
+                }
+            }
         } else if (warp == 9 && elect_one()) {
             // =============================== MMA issuer ===============================
             constexpr uint32_t fmt = BF16 ? 1u : 0u;
