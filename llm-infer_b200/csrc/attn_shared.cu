@@ -558,8 +558,8 @@ __device__ __forceinline__ void find_pieces(const SharedParams& p, uint32_t b, u
 // Output CTAs: one per (query row, slice of SLICE floats). Groups of SLICE / 4 lanes take a piece each, several pieces in flight per
 // lane; the groups' results merge by shuffles, then over the warps. WARP_ROWS: a warp takes a whole row by itself, four rows a CTA (many
 // rows of few pieces: 2048 rows of ten pieces take 11 us with four warps a row). Score CTAs behind them.
-template <int D, int SLICE, bool WARP_ROWS>
-__global__ void __launch_bounds__(kThreads) shared_merge_kernel(const __grid_constant__ SharedParams p) {
+template <int D, int SLICE, bool WARP_ROWS, bool SCORED>
+__global__ void __launch_bounds__(kThreads, !SCORED ? 1 : SLICE < D ? 8 : 6) shared_merge_kernel(const __grid_constant__ SharedParams p) {
     constexpr int kLanes = SLICE / 4;                                // of a group
     constexpr int kGroups = (WARP_ROWS ? 32 : kThreads) / kLanes;    // pieces at once
     __shared__ __align__(16) float s_o[4][SLICE];
@@ -654,6 +654,7 @@ __global__ void __launch_bounds__(kThreads) shared_merge_kernel(const __grid_con
         }
         return;
     }
+    if constexpr (!SCORED) return;
     // ---- weights of the own rows of one (sequence, kv head)
     const uint32_t idx = blockIdx.x - p.out_ctas;
     const uint32_t seg = idx / p.score_chunks, chunk = idx - seg * p.score_chunks;
@@ -661,27 +662,28 @@ __global__ void __launch_bounds__(kThreads) shared_merge_kernel(const __grid_con
     const uint32_t len = own_len(p, b);
     const uint32_t begin = chunk * p.score_rows, end = min(len, begin + p.score_rows);
     if (begin >= end) return;
-    // A thread takes up to kAt rows at a time, kThreads apart; the first heads' scores and the weights so far are requested ahead of the
-    // log-sum-exps.
-    constexpr int kAt = 4, kHeads = 4;
+    // Sixteen scores of a thread are requested at once, the first ones ahead of the log-sum-exps: four heads of four rows, kThreads apart, or
+    // sixteen heads where a CTA has no more rows than threads (twelve heads per kv head, 128 rows: 5 us with four at a time).
     const float* raw = p.raw + (static_cast<size_t>(b) * p.n_heads + kvh * p.group) * p.raw_stride;
     const float* before = p.scores ? p.scores + seg * p.score_stride : nullptr;
-    float w[kAt], x4[kHeads][kAt];
+    float* after = p.scores_out + seg * p.score_out_stride;
+    const bool one_row = p.score_rows == kThreads;
+    const uint32_t heads_at_once = one_row ? 16 : 4;
+    float w[4], x[16];
     auto fetch_rows = [&](uint32_t t0) {
 #pragma unroll
-        for (int a = 0; a < kAt; ++a) {
+        for (int a = 0; a < 4; ++a) {
             const uint32_t t = t0 + a * kThreads;
             w[a] = before && t < end ? before[t] : 0.f;
         }
     };
+    // score i of a thread: row t0 + a * kThreads of head g0 + g
     auto fetch_heads = [&](uint32_t t0, uint32_t g0) {
 #pragma unroll
-        for (int g = 0; g < kHeads; ++g)
-#pragma unroll
-            for (int a = 0; a < kAt; ++a) {
-                const uint32_t t = t0 + a * kThreads;
-                x4[g][a] = t < end && g0 + g < p.group ? raw[(g0 + g) * p.raw_stride + t] : -INFINITY;
-            }
+        for (int i = 0; i < 16; ++i) {
+            const uint32_t g = g0 + (one_row ? i : i / 4), t = t0 + (one_row ? 0 : i % 4 * kThreads);
+            x[i] = t < end && g < p.group ? raw[g * p.raw_stride + t] : -INFINITY;
+        }
     };
     fetch_rows(begin + tid);
     fetch_heads(begin + tid, 0);
@@ -690,17 +692,17 @@ __global__ void __launch_bounds__(kThreads) shared_merge_kernel(const __grid_con
         const uint32_t g = g0 + tid / 8;
         float m = -INFINITY, l = 0.f;
         if (g < p.group) {
-            Pieces x;
-            find_pieces<D>(p, b, kvh * p.group + g, x);
+            Pieces pc;
+            find_pieces<D>(p, b, kvh * p.group + g, pc);
 #pragma unroll
             for (int kind = 0; kind < 2; ++kind) {
                 constexpr int kAhead = 4;
-                for (uint32_t i0 = tid & 7; i0 < x.count[kind]; i0 += 8 * kAhead) {
+                for (uint32_t i0 = tid & 7; i0 < pc.count[kind]; i0 += 8 * kAhead) {
                     float ls[kAhead];
 #pragma unroll
                     for (int a = 0; a < kAhead; ++a) {
                         const uint32_t i = i0 + 8 * a;
-                        ls[a] = i < x.count[kind] ? x.lse[kind][i * x.step[kind]] : -INFINITY;
+                        ls[a] = i < pc.count[kind] ? pc.lse[kind][i * pc.step[kind]] : -INFINITY;
                     }
                     const float mn = fmaxf(fmaxf(fmaxf(ls[0], ls[1]), fmaxf(ls[2], ls[3])), m), safe = mn == -INFINITY ? 0.f : mn;
                     l = l * fast_exp2(m - safe) + fast_exp2(ls[0] - safe) + fast_exp2(ls[1] - safe) + fast_exp2(ls[2] - safe) +
@@ -719,26 +721,28 @@ __global__ void __launch_bounds__(kThreads) shared_merge_kernel(const __grid_con
         if ((tid & 7) == 0 && g < p.group) s_lse[g] = m + __log2f(l);
     }
     __syncthreads();
-    float* after = p.scores_out + seg * p.score_out_stride;
-    for (uint32_t t0 = begin + tid; t0 < end; t0 += kAt * kThreads) {
+    for (uint32_t t0 = begin + tid; t0 < end; t0 += 4 * kThreads) {
         if (t0 != begin + tid) {
             fetch_rows(t0);
             fetch_heads(t0, 0);
         }
-        float sum[kAt] = {};
-        for (uint32_t g0 = 0; g0 < p.group; g0 += kHeads) {
+        float sum[4] = {};
+        for (uint32_t g0 = 0; g0 < p.group; g0 += heads_at_once) {
             if (g0) fetch_heads(t0, g0);
 #pragma unroll
-            for (int g = 0; g < kHeads; ++g) {
-                const float lse = g0 + g < p.group ? s_lse[g0 + g] : 0.f;
-#pragma unroll
-                for (int a = 0; a < kAt; ++a) sum[a] += fast_exp2(x4[g][a] - lse);
+            for (int i = 0; i < 16; ++i) {
+                const uint32_t g = g0 + (one_row ? i : i / 4);
+                sum[i % 4] += fast_exp2(x[i] - (g < p.group ? s_lse[g] : 0.f));
             }
         }
+        if (one_row) {
+            if (t0 < end) after[t0] = w[0] + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+        } else {
 #pragma unroll
-        for (int a = 0; a < kAt; ++a) {
-            const uint32_t t = t0 + a * kThreads;
-            if (t < end) after[t] = w[a] + sum[a];
+            for (int a = 0; a < 4; ++a) {
+                const uint32_t t = t0 + a * kThreads;
+                if (t < end) after[t] = w[a] + sum[a];
+            }
         }
     }
 }
@@ -820,10 +824,13 @@ struct PrefixChoice {
 };
 constexpr uint32_t kMinPrefixBlocks = 2;  // of a CTA
 constexpr uint32_t kPieceBlocks = 4;
-PrefixChoice choose_prefix(const SharedPlan& plan, uint32_t sms, uint32_t head_dim, uint64_t prefix_tiles, uint64_t own_tiles, uint64_t blocks,
-                           uint32_t query_rows) {
+PrefixChoice choose_prefix(const SharedPlan& plan, uint32_t sms, uint32_t head_dim, uint64_t prefix_tiles, uint64_t own_tiles, uint64_t own_most,
+                           uint64_t blocks, uint32_t query_rows) {
+    // (times go by the tiles that are expected, the number of CTAs by those that there can be)
+    auto ctas_for = [](uint64_t ctas, uint64_t tiles) { return static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(ctas, tiles))); };
     const uint64_t all = prefix_tiles + own_tiles;
-    PrefixChoice c{false, 0, static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(2 * sms, all)))};
+    const uint32_t both_ctas = ctas_for(2 * sms, prefix_tiles + own_most);
+    PrefixChoice c{false, 0, both_ctas};
     if (prefix_tiles == 0) return c;
 #ifdef ATTN_TRACE
     const char* knob = getenv("ATTN_TRACE_PREFIX");  // profiling knob
@@ -842,16 +849,15 @@ PrefixChoice choose_prefix(const SharedPlan& plan, uint32_t sms, uint32_t head_d
     auto prefix_time = [&](double ctas) { return launch + 1.0 + std::max(std::ceil(blocks / ctas) * block, blocks / plan.pairs * block_bytes / bandwidth); };
     const double together = launch + std::max((prefix_tiles * shared_tile + own_tiles * own_tile) / sms, all * tile_bytes / bandwidth);
     // one behind the other
-    const uint32_t most = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(sms, blocks / kMinPrefixBlocks)));
+    const uint32_t most = ctas_for(sms, blocks / kMinPrefixBlocks);
     double best = prefix_time(most) + split_time(2.0 * sms) - 2.0;
     c.prefix_ctas = most;
-    const uint32_t split_all = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(2 * sms, own_tiles)));
-    c.split_ctas = split_all;
+    c.split_ctas = ctas_for(2 * sms, own_most);
     // side by side
     const double both = launch + (own_tiles * tile_bytes + blocks / plan.pairs * block_bytes) / bandwidth;
     for (uint32_t n = 8; n < sms; n += 4) {
         if (n > most) break;
-        const uint32_t m = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(2 * (sms - n), own_tiles)));
+        const uint32_t m = ctas_for(2 * (sms - n), own_most);
         const double t = std::max(std::max(prefix_time(n), split_time(m)), both);
         if (t < best) best = t, c.prefix_ctas = n, c.split_ctas = m;
     }
@@ -859,7 +865,7 @@ PrefixChoice choose_prefix(const SharedPlan& plan, uint32_t sms, uint32_t head_d
 #ifdef ATTN_TRACE
     if (knob) c.tensor = true;
 #endif
-    if (!c.tensor) c.split_ctas = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(2 * sms, all)));
+    if (!c.tensor) c.split_ctas = both_ctas;
     return c;
 }
 
@@ -956,7 +962,8 @@ extern "C" int attn_decode_shared(const AttnDecodeSharedArgs* a, void* stream_v)
     // (lengths that lie on the device are taken to be five eighths of the capacity)
     const uint64_t own_guess = a->kv_len ? own_tiles * plan.own_segs * 5 / 8
                                          : (std::min(a->kv_len_uniform, a->kv_capacity) + plan.own.keys - 1ull) / plan.own.keys * plan.own_segs;
-    PrefixChoice choice = choose_prefix(plan, dev.sm_count, a->head_dim, prefix_tiles * p.prefix_segs, own_guess, blocks, a->batch * p.group);
+    PrefixChoice choice = choose_prefix(plan, dev.sm_count, a->head_dim, prefix_tiles * p.prefix_segs, own_guess, own_tiles * plan.own_segs, blocks,
+                                        a->batch * p.group);
     if (blocks > 0x7fffffffull) choice.tensor = false;
     const bool tensor = choice.tensor;
     p.scale_log2 = fabsf(p.scale_log2);
@@ -1053,7 +1060,11 @@ extern "C" int attn_decode_shared(const AttnDecodeSharedArgs* a, void* stream_v)
         g_launch_count.fetch_add(1, std::memory_order_relaxed);
         return ATTN_OK;
     };
-    if (sliced) return a->head_dim == 128 ? merge(shared_merge_kernel<128, 32, false>) : merge(shared_merge_kernel<64, 32, false>);
-    if (warp_rows) return a->head_dim == 128 ? merge(shared_merge_kernel<128, 128, true>) : merge(shared_merge_kernel<64, 64, true>);
-    return a->head_dim == 128 ? merge(shared_merge_kernel<128, 128, false>) : merge(shared_merge_kernel<64, 64, false>);
+    auto merge_rows = [&](auto scores) -> int {
+        constexpr bool S = decltype(scores)::value;
+        if (sliced) return a->head_dim == 128 ? merge(shared_merge_kernel<128, 32, false, S>) : merge(shared_merge_kernel<64, 32, false, S>);
+        if (warp_rows) return a->head_dim == 128 ? merge(shared_merge_kernel<128, 128, true, S>) : merge(shared_merge_kernel<64, 64, true, S>);
+        return a->head_dim == 128 ? merge(shared_merge_kernel<128, 128, false, S>) : merge(shared_merge_kernel<64, 64, false, S>);
+    };
+    return scored ? merge_rows(std::true_type{}) : merge_rows(std::false_type{});
 }
