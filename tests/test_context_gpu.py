@@ -434,3 +434,50 @@ def test_decode_then_evict_then_decode(ctx):
             ks[b, :, h], vs[b, :, h] = k0[b, rows, h], v0[b, rows, h]
     want, A, ds, _, _ = _decode64(q, None, None, ks, vs, [64, 64], D ** -0.5)
     assert ((got.double().cpu() - want).abs() <= U["f16"] * want.abs() + (U["f16"] + 2 * ds + 2.0 ** -20) * A).all()
+
+
+def test_decode_shared_writes_any_aligned_output(ctx):
+    """Outputs two bytes off a 16-byte boundary, over the forms of the merge: the same values."""
+    for B, H, Hkv, D, P, Tn in ((2, 8, 2, 64, 100, 30), (40, 32, 8, 128, 0, 50), (64, 32, 8, 128, 3000, 20)):
+        g = _gen(B)
+        q, k, v = (torch.randn(s, generator=g).half().cuda() for s in ((B, H, D), (B, Tn, Hkv, D), (B, Tn, Hkv, D)))
+        kp, vp = (torch.randn((P, Hkv, D), generator=g).half().cuda() for _ in range(2)) if P else (None, None)
+        want = ctx.attn_decode_shared(q, kp, vp, k, v)
+        out = torch.zeros(B * H * D + 1, dtype=torch.float16, device="cuda")[1:].view(B, H, D)
+        assert ctx.attn_decode_shared(q, kp, vp, k, v, out=out).data_ptr() == out.data_ptr()
+        assert (out.float() - want.float()).abs().max() <= 2.0 ** -9  # one fp16 step below 4: another order of the pieces
+
+
+def test_decode_shared_long_prefix_in_a_graph_and_back_to_back(ctx):
+    """Three launches per call, the second beside the first: calls that follow one another share a workspace and do not disturb
+    each other, whatever lies between them."""
+    g = _gen(11)
+    B, H, Hkv, D, P, Tn = 40, 32, 8, 128, 5000, 60
+    calls = []
+    for i in range(3):
+        q, k, v = (torch.randn(s, generator=g).half().cuda() for s in ((B, H, D), (B, Tn, Hkv, D), (B, Tn, Hkv, D)))
+        kp, vp = (torch.randn((P, Hkv, D), generator=g).half().cuda() for _ in range(2))
+        lens = torch.randint(0, Tn + 1, (B,), generator=g, dtype=torch.int32).cuda()
+        calls.append((q, kp, vp, k, v, lens))
+    scores = [torch.zeros((B, Hkv, Tn), device="cuda") for _ in calls]
+    want = []
+    for c, s in zip(calls, scores):
+        want.append(ctx.attn_decode_shared(*c, scores=s).clone())
+        torch.cuda.synchronize()
+    once = [s.clone() for s in scores]
+    ws = ctx.SharedWorkspace(B, H, Hkv, D, rows=Tn)
+    outs = [torch.empty_like(w) for w in want]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for c, s, o in zip(calls, scores, outs):
+            ctx.attn_decode_shared(*c, scores=s, out=o, workspace=ws)
+    for _ in range(4):
+        graph.replay()
+    for c, s, o in zip(calls, scores, outs):
+        for _ in range(3):
+            ctx.attn_decode_shared(*c, scores=s, out=o, workspace=ws)
+    torch.cuda.synchronize()
+    assert int(ws.status.item()) == 0
+    for o, w, s, one in zip(outs, want, scores, once):
+        assert torch.equal(o, w)
+        assert (s - 8 * one).abs().max() <= 8 * 2.0 ** -22 * 4 * 8  # eight steps of weights of at most four each, added one by one
