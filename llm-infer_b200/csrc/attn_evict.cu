@@ -45,7 +45,8 @@ struct EvictParams {
 constexpr int kSelThreads = 1024;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kBins = 2048;
-constexpr uint32_t kSelWords = 4 * kBins + 2 * kSelWarps + 4;  // shared memory in front of the keys
+constexpr int kGroups = kBins / 32;
+constexpr uint32_t kSelWords = 4 * kBins + 3 * kGroups + 2 * kSelWarps + 4;  // shared memory in front of the keys
 constexpr uint32_t kAlways = 0xffffffffu;
 
 // Unsigned order of the keys = order of the scores; NaN gets 0, below -inf. No score maps to kAlways (that pattern would be a NaN).
@@ -66,7 +67,8 @@ template <int kCtas>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_constant__ EvictParams p) {
     extern __shared__ __align__(16) uint32_t s_all[];
     uint32_t* s_hist = s_all;                   // [4][kBins]: two for the top digit (even and odd lanes: fewer meet in a bin), one for each other
-    uint32_t* s_gt = s_hist + 4 * kBins;        // [kSelWarps]
+    uint32_t* s_group = s_hist + 4 * kBins;     // [3][kGroups]: a digit's histogram in sums over 32 bins
+    uint32_t* s_gt = s_group + 3 * kGroups;     // [kSelWarps]
     uint32_t* s_eq = s_gt + kSelWarps;          // [kSelWarps]
     uint32_t* s_pick = s_eq + kSelWarps;        // digit, keys above it
     uint32_t* s_counts = s_pick + 2;            // this CTA's keys above the threshold, equal to it
@@ -159,47 +161,57 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_
                 count(i + 3, k.w);
             }
         }
-        if (pass == 0) {  // the two copies into one
-            __syncthreads();
-            for (int i = tid; i < kBins / 4; i += kSelThreads) {
-                uint4* x = reinterpret_cast<uint4*>(hist) + i;
+        __syncthreads();  // the histogram is complete
+        uint32_t* group = s_group + pass * kGroups;
+        if (tid < kBins / 4) {
+            uint4* x = reinterpret_cast<uint4*>(hist) + tid;
+            uint4 h = *x;
+            if (pass == 0) {  // the two copies into one
                 const uint4 y = x[kBins / 4];
-                *x = make_uint4(x->x + y.x, x->y + y.y, x->z + y.z, x->w + y.w);
+                h = make_uint4(h.x + y.x, h.y + y.y, h.z + y.z, h.w + y.w);
+                *x = h;
             }
+            uint32_t sum = h.x + h.y + h.z + h.w;
+#pragma unroll
+            for (int d = 1; d < 8; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            if (lane % 8 == 0) group[tid / 8] = sum;
         }
         meet();
-        // thread t of the first 512 owns the four bins from kBins - 4 - 4 t up, so that threads run from the top: it sums them over the
-        // cluster, 16 bytes at a time
-        const int bin0 = kBins - 4 - 4 * tid;
-        uint4 mine = make_uint4(0, 0, 0, 0);
-        if (tid < kBins / 4) {
-            const uint4* src = reinterpret_cast<const uint4*>(hist + bin0);
+        // One warp finds the bin, from the top: first its group of 32, then the bin in it. So a CTA reads 384 bytes of each other's
+        // memory and not 8 KB (which took 2 us a digit).
+        if (warp == 0) {
+            auto total = [&](const uint32_t* at) {  // over the cluster; each CTA starts with another one
+                uint32_t sum = 0;
 #pragma unroll
-            for (int c = 0; c < kCtas; ++c) {
-                // (each CTA starts with another one: all of them on one CTA's memory at a time took 1 us more per digit)
-                const uint4 h = kCtas > 1 ? *cluster.map_shared_rank(src, (rank + c) % kCtas) : *src;
-                mine.x += h.x, mine.y += h.y, mine.z += h.z, mine.w += h.w;
+                for (int c = 0; c < kCtas; ++c) sum += kCtas > 1 ? *cluster.map_shared_rank(at, (rank + c) % kCtas) : *at;
+                return sum;
+            };
+            auto scan = [&](uint32_t x) {
+#pragma unroll
+                for (int d = 1; d < 32; d *= 2) {
+                    const uint32_t o = __shfl_up_sync(0xffffffffu, x, d);
+                    if (lane >= d) x += o;
+                }
+                return x;
+            };
+            const uint32_t hi = total(group + kGroups - 1 - 2 * lane), lo = total(group + kGroups - 2 - 2 * lane);
+            const uint32_t incl = scan(hi + lo);
+            const int at = __ffs(__ballot_sync(0xffffffffu, incl >= need)) - 1;  // there are at least `need` candidates: some lane has it
+            const uint32_t upper = __shfl_sync(0xffffffffu, incl - lo, at), above = __shfl_sync(0xffffffffu, incl - lo - hi, at);
+            const int picked = kGroups - 1 - 2 * at - (upper >= need ? 0 : 1);
+            const uint32_t before = upper >= need ? above : upper;  // keys in the groups above
+            const uint32_t mine = total(hist + 32 * picked + 31 - lane);
+            const uint32_t upto = before + scan(mine);
+            const int bin = __ffs(__ballot_sync(0xffffffffu, upto >= need)) - 1;
+            if (lane == bin) {
+                s_pick[0] = 32 * picked + 31 - lane;
+                s_pick[1] = upto - mine;
             }
-        }
-        const uint32_t sum = mine.x + mine.y + mine.z + mine.w;
-        uint32_t incl = sum;
-#pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-            const uint32_t o = __shfl_up_sync(0xffffffffu, incl, d);
-            if (lane >= d) incl += o;
-        }
-        if (lane == 31) s_gt[warp] = incl;
-        __syncthreads();
-        const uint32_t above = incl - sum + __reduce_add_sync(0xffffffffu, lane < warp ? s_gt[lane] : 0u);
-        if (above < need && above + sum >= need) {  // one thread
-            const uint32_t a1 = above + mine.w, a2 = a1 + mine.z, a3 = a2 + mine.y;  // keys in and above the upper one, two, three bins
-            s_pick[0] = bin0 + (a1 >= need ? 3 : a2 >= need ? 2 : a3 >= need ? 1 : 0);
-            s_pick[1] = a1 >= need ? above : a2 >= need ? a1 : a3 >= need ? a2 : a3;
         }
         __syncthreads();
         prefix |= s_pick[0] << shift;
         need -= s_pick[1];
-        // (the next write of s_gt and s_pick comes behind another meeting, and each digit has a histogram of its own)
+        // (the next write of s_pick comes behind another meeting, and each digit has a histogram of its own)
     }
     // every key above `prefix` stays, and the first `need` rows of those equal to it
     // ---- counts per warp, in order: keys above in the low half of a word, equal ones in the high half (a lane's at most 2^16)
@@ -222,7 +234,6 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_
     }
     n_gt = __reduce_add_sync(0xffffffffu, n_gt);
     n_eq = __reduce_add_sync(0xffffffffu, n_eq);
-    __syncthreads();  // s_gt of the last digit has been read
     if (lane == 0) {
         s_gt[warp] = n_gt;
         s_eq[warp] = n_eq;
@@ -245,8 +256,8 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_
         gt += __reduce_add_sync(0xffffffffu, og);
         eq += __reduce_add_sync(0xffffffffu, oe);
     }
-    // ---- the kept rows, in order: row i goes to place (kept rows in front of it). A row of keys per lane; equal keys are rare, and
-    // rows without one take the short way.
+    // ---- the kept rows, in order: row i goes to place (kept rows in front of it). Four keys a lane at a time where none equals the
+    // threshold (few do, unless scores repeat), and otherwise a key a lane.
     const uint32_t below = (1u << lane) - 1u;
     auto emit = [&](uint32_t i, bool in, uint32_t key) {
         const bool is_gt = in && key > prefix, is_eq = in && key == prefix;
@@ -262,9 +273,30 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_
         gt += __popc(m_gt);
         eq += __popc(m_eq);
     };
-    const uint32_t whole = wb + (min(we, n_staged) > wb ? (min(we, n_staged) - wb) / 32 * 32 : 0u);  // full rounds of staged keys
-#pragma unroll 4
-    for (uint32_t i0 = wb; i0 < whole; i0 += 32) emit(i0 + lane, true, s_keys[i0 + lane]);
+    const uint32_t whole = wb + (min(we, n_staged) > wb ? (min(we, n_staged) - wb) / 128 * 128 : 0u);  // full rounds of staged keys
+#pragma unroll 1
+    for (uint32_t i0 = wb; i0 < whole; i0 += 128) {
+        const uint32_t i = i0 + 4 * lane;
+        const uint4 k = *reinterpret_cast<const uint4*>(s_keys + i);
+        if (__any_sync(0xffffffffu, k.x == prefix || k.y == prefix || k.z == prefix || k.w == prefix)) {
+#pragma unroll
+            for (int a = 0; a < 4; ++a) emit(i0 + 32 * a + lane, true, s_keys[i0 + 32 * a + lane]);
+            continue;
+        }
+        const uint32_t mine = (k.x > prefix) + (k.y > prefix) + (k.z > prefix) + (k.w > prefix);
+        uint32_t incl = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const uint32_t o = __shfl_up_sync(0xffffffffu, incl, d);
+            if (lane >= d) incl += o;
+        }
+        uint32_t* to = kept + (gt + min(eq, need) + incl - mine);
+        if (k.x > prefix) *to++ = begin + i;
+        if (k.y > prefix) *to++ = begin + i + 1;
+        if (k.z > prefix) *to++ = begin + i + 2;
+        if (k.w > prefix) *to = begin + i + 3;
+        gt += __shfl_sync(0xffffffffu, incl, 31);
+    }
     for (uint32_t i0 = whole; i0 < we; i0 += 32) {
         const uint32_t i = i0 + lane;
         emit(i, i < we, i < n_staged ? s_keys[i] : i < we ? make_key(i, scores[i]) : 0u);
