@@ -252,13 +252,13 @@ constexpr int kClusterNotTaken = 1;  // nothing was launched: the other form has
 int launch_decode_cluster(const DecodeParams& p, const DecodeClusterPlan& plan, uint32_t head_dim, bool qsplit, bool kv_bf16,
                           cudaStream_t stream);
 // The shared prefix of a batch's decode step on the tensor cores (attn_shared_prefix.cu): pieces of the softmax over the prefix for
-// all query rows. A segment is a kv head and up to 256 of its batch * group query rows; grid CTAs share the key blocks of all segments.
+// all query rows. A segment is a kv head and up to 256 (fp32 outputs: 128) of its batch * group query rows; grid CTAs share the key blocks of all segments.
 struct SharedPrefixParams {
     const void* q;
     const void* k;
     const void* v;
-    float* part;         // [(grid + segments) * 256][head_dim]
-    float* lse;          // [(grid + segments) * 256], log2 units
+    float* part;         // [(grid + segments) * 256 (128)][head_dim]
+    float* lse;          // [(grid + segments) * 256 (128)], log2 units
     uint32_t* seg_ctas;  // [segments] segment_ctas() words
     uint64_t row_stride;
     uint32_t batch, n_heads, n_kv_heads, group, head_dim, prefix;
@@ -270,7 +270,7 @@ struct SharedPrefixParams {
     uint32_t* status;
     uint32_t bf16, residual;
 };
-constexpr uint32_t kPrefixBlock = 64, kPrefixRows = 256;  // keys of a block, query rows of a segment
+constexpr uint32_t kPrefixBlock = 64, kPrefixRows = 256;  // keys of a block, query rows of a segment (half of them for fp32 outputs)
 int launch_shared_prefix(const SharedPrefixParams& p, cudaStream_t stream);
 // fp16-weight GEMV on the tensor cores (attn_gemv_f16mma.cu): batches and the fused forms of attn_gemv_f16.
 int launch_gemv_f16_mma(const AttnGemvArgs* a, cudaStream_t stream);

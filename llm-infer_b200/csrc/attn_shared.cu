@@ -16,7 +16,7 @@
 //           the split pass left in the workspace into weights (exp2(s - LSE)), sum them over the heads and add them to the accumulators.
 // The scores of own rows cost 4 bytes per query head and row each way through L2, next to 4 * head_dim bytes of K and V per kv head.
 // P enters the second product rounded once to the caches' type when the output is 16 bits wide too (an error below the
-// output's own rounding), and as value + rounding residual for fp32 outputs.
+// output's own rounding), and in two (fp16) or three (bf16) parts that hold its 24 bits for fp32 outputs.
 //
 // Bound by HBM where there is enough to read: 16 ragged caches of up to 4096 rows (168 MB, with weights) take 38.6 us in a graph of
 // calls, of which the streaming alone takes 30; 7 sequences over 131072 shared rows (543 MB) 95 us = 5.7 TB/s. Smaller calls are a chain
@@ -454,25 +454,55 @@ shared_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                     __syncwarp();
                 }
                 const uint32_t vrow = vbase + (key0 + ((lane >> 3) & 1) * 8 + (lane & 7)) * 128;
+if constexpr (RES) {
+                    // P in as many parts as hold its 24 bits. A matrix instruction cuts its sum off instead of rounding it, which makes long sums
+                    // small (4e-6 of them after 440 instructions): each starts from zero here and is added to the rest by an addition.
+                    constexpr int kTerms = BF16 ? 3 : 2;
+                    uint32_t pa[NB][kTerms][4];
 #pragma unroll
-                for (int n = 0; n < NB; ++n) {
-                    uint32_t pa[4];
-                    [[maybe_unused]] uint32_t pr[4];
+                    for (int n = 0; n < NB; ++n)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float x = s[2 * n + (i >> 1)][(i & 1) * 2], y = s[2 * n + (i >> 1)][(i & 1) * 2 + 1];
-                        pa[i] = pack2<BF16>(x, y);
-                        if constexpr (RES) pr[i] = pack2<BF16>(x - round16<BF16>(x), y - round16<BF16>(y));
-                    }
+                        for (int i = 0; i < 4; ++i) {
+                            float x = s[2 * n + (i >> 1)][(i & 1) * 2], y = s[2 * n + (i >> 1)][(i & 1) * 2 + 1];
+#pragma unroll
+                            for (int t = 0; t < kTerms; ++t) {
+                                pa[n][t][i] = BF16 ? pack_upper16(x, y) : pack2<BF16>(x, y);
+                                x -= BF16 ? upper16(x) : round16<BF16>(x);
+                                y -= BF16 ? upper16(y) : round16<BF16>(y);
+                            }
+                        }
 #pragma unroll
                     for (int dc = 0; dc < D / 16; ++dc) {
-                        uint32_t b0, b1, b2, b3;
-                        ldmatrix_x4_trans(b0, b1, b2, b3, vrow + v_off[dc & 3] + (dc >> 2) * kPartBytes + n * 2048);
-                        mma_16816<BF16>(o[2 * dc], pa, b0, b1);
-                        mma_16816<BF16>(o[2 * dc + 1], pa, b2, b3);
-                        if constexpr (RES) {
-                            mma_16816<BF16>(o[2 * dc], pr, b0, b1);
-                            mma_16816<BF16>(o[2 * dc + 1], pr, b2, b3);
+                        float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int n = 0; n < NB; ++n) {
+                            uint32_t b0, b1, b2, b3;
+                            ldmatrix_x4_trans(b0, b1, b2, b3, vrow + v_off[dc & 3] + (dc >> 2) * kPartBytes + n * 2048);
+#pragma unroll
+                            for (int t = kTerms - 1; t >= 0; --t) {
+                                mma_16816<BF16>(x, pa[n][t], b0, b1);
+                                mma_16816<BF16>(y, pa[n][t], b2, b3);
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            o[2 * dc][i] += x[i];
+                            o[2 * dc + 1][i] += y[i];
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) {
+                        uint32_t pa[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            pa[i] = pack2<BF16>(s[2 * n + (i >> 1)][(i & 1) * 2], s[2 * n + (i >> 1)][(i & 1) * 2 + 1]);
+#pragma unroll
+                        for (int dc = 0; dc < D / 16; ++dc) {
+                            uint32_t b0, b1, b2, b3;
+                            ldmatrix_x4_trans(b0, b1, b2, b3, vrow + v_off[dc & 3] + (dc >> 2) * kPartBytes + n * 2048);
+                            mma_16816<BF16>(o[2 * dc], pa, b0, b1);
+                            mma_16816<BF16>(o[2 * dc + 1], pa, b2, b3);
                         }
                     }
                 }
@@ -754,6 +784,7 @@ struct SharedPlan {
     Shape pre, own;
     uint32_t row_blocks, prefix_segs, own_segs, grid;
     uint32_t pairs, tensor_segs, tensor_grid;  // the prefix on the tensor cores
+    uint32_t tiles;  // as `pairs`, in half as many query rows, which is what a segment of an fp32 output has
     size_t lse_pre, part_own, lse_own, seg_pre, seg_own, raw, words;
     uint64_t raw_stride;
 };
@@ -770,7 +801,7 @@ int make_shared_plan(uint32_t batch, uint32_t n_heads, uint32_t n_kv_heads, uint
     if (batch == 0 || n_heads == 0 || n_kv_heads == 0 || n_heads % n_kv_heads != 0) return ATTN_ERR_INVALID_ARG;
     const uint32_t group = n_heads / n_kv_heads;
     if ((head_dim != 64 && head_dim != 128) || group > 64 || batch > kMaxBatch || n_heads > 1024) return ATTN_ERR_UNSUPPORTED;
-    SharedPlan& s = *plan;
+    SharedPlan& s = *plan;  // (sized for either type of output)
     set_shape(&s.own, group, n_kv_heads);
     s.own.rec_rows = group;
     set_shape(&s.pre, batch * group, n_kv_heads);
@@ -780,6 +811,7 @@ int make_shared_plan(uint32_t batch, uint32_t n_heads, uint32_t n_kv_heads, uint
     s.own_segs = batch * s.own.groups;
     s.grid = 2 * dev.sm_count;
     s.pairs = (batch * group + kPrefixRows - 1) / kPrefixRows;
+    s.tiles = (batch * group + kPrefixRows / 2 - 1) / (kPrefixRows / 2);
     s.tensor_segs = s.pairs * n_kv_heads;
     s.tensor_grid = dev.sm_count;
     const size_t pre_rows = std::max(static_cast<size_t>(s.grid + s.prefix_segs) * s.pre.ts * s.pre.hpc * s.pre.rec_rows,
@@ -790,7 +822,7 @@ int make_shared_plan(uint32_t batch, uint32_t n_heads, uint32_t n_kv_heads, uint
     s.part_own = s.lse_pre + round4(pre_rows);
     s.lse_own = s.part_own + own_rows * head_dim;
     s.seg_pre = s.lse_own + round4(own_rows);
-    s.seg_own = s.seg_pre + round4(std::max(s.prefix_segs, s.tensor_segs));
+    s.seg_own = s.seg_pre + round4(std::max(s.prefix_segs, s.tiles * n_kv_heads));
     s.raw = s.seg_own + round4(s.own_segs);
     s.raw_stride = (static_cast<uint64_t>(scored_rows) + 63) / 64 * 64;
     s.words = s.raw + static_cast<size_t>(batch) * n_heads * s.raw_stride;
@@ -825,7 +857,7 @@ struct PrefixChoice {
 constexpr uint32_t kMinPrefixBlocks = 2;  // of a CTA
 constexpr uint32_t kPieceBlocks = 4;
 PrefixChoice choose_prefix(const SharedPlan& plan, uint32_t sms, uint32_t head_dim, uint64_t prefix_tiles, uint64_t own_tiles, uint64_t own_most,
-                           uint64_t blocks, uint32_t query_rows) {
+                           uint64_t blocks, uint32_t query_rows, bool res) {
     // (times go by the tiles that are expected, the number of CTAs by those that there can be)
     auto ctas_for = [](uint64_t ctas, uint64_t tiles) { return static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(ctas, tiles))); };
     const uint64_t all = prefix_tiles + own_tiles;
@@ -836,11 +868,12 @@ PrefixChoice choose_prefix(const SharedPlan& plan, uint32_t sms, uint32_t head_d
     const char* knob = getenv("ATTN_TRACE_PREFIX");  // profiling knob
     if (knob && atoi(knob) == 0) return c;
 #endif
-    const double dim = head_dim / 128.0, work = 0.75 + 0.25 * dim;
+    const double dim = head_dim / 128.0, work = res ? 0.4 + 0.6 * dim : 0.75 + 0.25 * dim;
     const double tile_bytes = 32768.0 * dim, bandwidth = 6.2e6;     // bytes per us
-    const double own_tile = 0.6 * work, own_seg = 2.0, launch = 5.0;  // us of an SM per own tile, of a CTA per own segment; a launch's fixed part
-    const double shared_tile = (plan.pre.wm == 4 ? 1.15 : plan.pre.wm == 2 ? 0.65 : 0.6) * work;  // of a prefix tile in the split pass
-    const double block = (query_rows > 128 ? 1.1 : 0.8) * (0.4 + 0.6 * dim);                      // of a key block in the tensor-core kernel
+    const double own_tile = (res ? 0.85 : 0.6) * work, own_seg = 2.0, launch = 5.0;  // us of an SM per own tile, of a CTA per own segment; a launch's fixed part
+    // of a prefix tile in the split pass, of a key block in the tensor-core kernel; fp32 outputs take two or three times the second products
+    const double shared_tile = (plan.pre.wm == 4 ? (res ? 2.9 : 1.15) : plan.pre.wm == 2 ? (res ? 1.35 : 0.65) : res ? 0.9 : 0.6) * work;
+    const double block = res ? 1.05 : (query_rows > 128 ? 1.1 : 0.8) * (0.4 + 0.6 * dim);
     const double block_bytes = 16384.0 * 2 * dim;
     auto split_time = [&](double ctas) {
         const double segs = std::ceil(plan.own_segs / ctas) * (own_tiles ? own_seg : 0.0);
@@ -958,12 +991,17 @@ extern "C" int attn_decode_shared(const AttnDecodeSharedArgs* a, void* stream_v)
 
     cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
     const bool bf16 = a->dtype == ATTN_DTYPE_BF16, res = a->o_dtype == ATTN_DTYPE_F32;
+    const uint32_t seg_rows = res ? kPrefixRows / 2 : kPrefixRows;
+    if (res) {
+        plan.pairs = plan.tiles;
+        plan.tensor_segs = plan.tiles * a->n_kv_heads;
+    }
     const uint64_t blocks = (static_cast<uint64_t>(a->prefix_len) + kPrefixBlock - 1) / kPrefixBlock * plan.tensor_segs;
     // (lengths that lie on the device are taken to be five eighths of the capacity)
     const uint64_t own_guess = a->kv_len ? own_tiles * plan.own_segs * 5 / 8
                                          : (std::min(a->kv_len_uniform, a->kv_capacity) + plan.own.keys - 1ull) / plan.own.keys * plan.own_segs;
     PrefixChoice choice = choose_prefix(plan, dev.sm_count, a->head_dim, prefix_tiles * p.prefix_segs, own_guess, own_tiles * plan.own_segs, blocks,
-                                        a->batch * p.group);
+                                        std::min(a->batch * p.group, seg_rows), res);
     if (blocks > 0x7fffffffull) choice.tensor = false;
     const bool tensor = choice.tensor;
     p.scale_log2 = fabsf(p.scale_log2);
@@ -1003,8 +1041,8 @@ extern "C" int attn_decode_shared(const AttnDecodeSharedArgs* a, void* stream_v)
         if ((rc = launch_shared_prefix(t, stream)) != ATTN_OK) return rc;
         in_split.prefix_segs = in_split.prefix_tiles = 0;
         in_split.wait_last = 1;
-        // how the merge pass finds the pieces: one record of 256 rows per CTA and segment
-        p.pre = Shape{1, 1, 1, kPrefixBlock, p.n_kv_heads, kPrefixRows};
+        // how the merge pass finds the pieces: one record of a segment's rows per CTA and segment
+        p.pre = Shape{1, 1, 1, kPrefixBlock, p.n_kv_heads, seg_rows};
         p.row_blocks = plan.pairs;
         p.prefix_segs = plan.tensor_segs;
     }

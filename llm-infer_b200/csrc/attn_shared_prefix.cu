@@ -11,6 +11,12 @@
 // four stages, one thread that issues the MMAs, scores two blocks ahead of the products. Query rows of a kv head are not evenly
 // spaced (heads of one group, then the next sequence), so the softmax warps bring them into the swizzled tile.
 //
+// With fp32 outputs a segment is one tile, whose keys and output columns the two softmax warpgroups share; P enters the second product in
+// the two (fp16) or three (bf16) parts that hold its 24 bits, and a block's products start from zero and are added up in registers.
+// 128 query rows of 128 dimensions x 65536 keys, 8 kv heads: 67 us (fp16) and 74 (bf16), for 58 with outputs of 16 bits, all of it the
+// further MMAs (a third block of scores in tensor memory changed nothing); errors 7e-7 and 5e-7 of the output, where sums left in tensor
+// memory and two parts were off by 9e-6.
+//
 // Bound by the K/V stream up to 128 rows: a block takes 0.80 us of a CTA (32 KB, 0.72 us of an SM's share of HBM). With two tiles it
 // takes 1.1 us, in which the special-function units are busy for 0.55 and the tensor pipe for 0.6: the chain from scores to
 // probabilities of one block. A launch costs 10 us around its blocks (query rows 2, first block 2, piece and exit 4), which is why
@@ -50,7 +56,8 @@ enum {
     BAR_S_FULL = BAR_V_EMPTY + kStages,  // [tile][block parity]: scores, probabilities, products of a block
     BAR_P_FULL = BAR_S_FULL + 4,
     BAR_O_DONE = BAR_P_FULL + 4,
-    BAR_COUNT = BAR_O_DONE + 4
+    BAR_O_FREE = BAR_O_DONE + 4,  // fp32 outputs: [block parity] the block's products have been added up
+    BAR_COUNT = BAR_O_FREE + 2
 };
 
 constexpr uint32_t kSmemQ = 0;
@@ -86,6 +93,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     const int tid = threadIdx.x;
     const int warp = uniform_warp();
     const int lane = tid & 31;
+    constexpr uint32_t kRows = RES ? BM : 2 * BM;  // query rows of a segment
     constexpr uint32_t kLoadKv = (HD / 64) * kKvSubBytes;  // bytes of a block actually loaded
 
     // ---- the CTA's run of the block list
@@ -107,9 +115,9 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         w.block = t - w.seg * blocks;
         w.blocks = min(blocks - w.block, t1 - t);
         w.kvh = w.seg / p.pairs;
-        w.m0 = (w.seg - w.kvh * p.pairs) * 2 * BM;
+        w.m0 = (w.seg - w.kvh * p.pairs) * kRows;
         w.tile[0] = true;
-        w.tile[1] = w.m0 + BM < query_rows;
+        w.tile[1] = !RES && w.m0 + BM < query_rows;
         return true;
     };
 
@@ -125,9 +133,11 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(bar(BAR_S_FULL + i), 1);
-            mbar_init(bar(BAR_P_FULL + i), 128);
+            mbar_init(bar(BAR_P_FULL + i), RES ? 256 : 128);
             mbar_init(bar(BAR_O_DONE + i), 1);
         }
+        mbar_init(bar(BAR_O_FREE), 256);
+        mbar_init(bar(BAR_O_FREE + 1), 256);
         mbar_init_fence();
         prefetch_tensor_map(&tm_k);
         prefetch_tensor_map(&tm_v);
@@ -144,11 +154,12 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     fence_after();
     const uint32_t tmem_base = *tmem_ptr_smem;
     auto tmem_s = [&](int t, uint32_t buf) { return tmem_base + static_cast<uint32_t>(t) * 128u + buf * 64u; };
-    auto tmem_o = [&](int t) { return tmem_base + 256u + static_cast<uint32_t>(t) * 128u; };
+    auto tmem_o = [&](int t) { return tmem_base + 256u + static_cast<uint32_t>(t) * 128u; };  // of a tile; fp32 outputs: of a block parity
+    auto tmem_third = [&](uint32_t buf) { return tmem_base + 128u + buf * 32u; };  // fp32 outputs of bf16: the third part of P
 
     if (warp < 8) {
         // =============================== softmax warpgroups ===============================
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");  // 256 * 208 + 128 * 88 = 384 * 168
         const int t = warp >> 2;                 // tile
         const int r = ((warp & 3) << 5) | lane;  // row inside the tile = tensor-memory lane
         const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) << 5) << 16;
@@ -156,10 +167,11 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         for (uint32_t s = blockIdx.x * 256 + tid; s < p.segments; s += gridDim.x * 256)
             p.seg_ctas[s] = p.ctas_per_seg ? (s * p.ctas_per_seg) | p.ctas_per_seg << 16
                                            : segment_ctas(static_cast<uint64_t>(s) * blocks, (s + 1ull) * blocks, total, gridDim.x);
+        const bool leader = (warp & 3) == 0 && lane == 0;
         bool ok = true;
         uint32_t g0 = 0;  // key blocks of this tile before the current item: buffer and barrier phases run on over the items
         bool staged = false;
-        Item w;
+        Item w{};
         // A warp brings its 32 query rows of an item, neighbouring lanes neighbouring 16-byte chunks (a row per thread took 2 us to
         // request); rows that are not there are zeros.
         constexpr int kRowChunks = HD / 8;
@@ -199,12 +211,161 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             brought = true;
         }
         block_arrive(3, 288);
+        if constexpr (RES) {
+            // ---- fp32 outputs: the warpgroups share a tile, each takes half of a block's keys and half of O's columns. A block's products start
+            // from zero and are added up here: the tensor cores cut their sums off instead of rounding them, which over hundreds of
+            // instructions makes the result small by 8e-6 of it. P's parts hold its 24 bits.
+            constexpr int kKeys = BN / 2, kCols = HD / 2;
+            const uint32_t xch = base + kSmemStage + kStageTileBytes + r * 4;  // [block parity][warpgroup][row]: the other half's maximum, or sum
+            auto exchange = [&](uint32_t slot, float x) {
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(xch + (slot * 2 + t) * (BM * 4)), "f"(x) : "memory");
+                named_bar_sync(4, 256);
+                float y;
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(y) : "r"(xch + (slot * 2 + (t ^ 1)) * (BM * 4)) : "memory");
+                return y;
+            };
+            // (a thread that has given up waits no more but meets the others all the same: the barriers count on everybody)
+            auto wait = [&](uint32_t b, uint32_t parity) {
+                if (ok && !mbar_wait(b, parity)) {
+                    report_timeout(p.status);
+                    ok = false;
+                }
+            };
+            for (uint32_t at = t0; item_at(at, w); at += w.blocks) {
+                if (staged) {  // the memory that the last result left through is free again
+                    if (leader) tma_store_wait_read();
+                    named_bar_sync(4, 256);
+                }
+                if (t == 0) {
+                    if (!brought) bring_rows();
+                    brought = false;
+                    rows_there();
+                }
+                float o[kCols];
+#pragma unroll
+                for (int c = 0; c < kCols; ++c) o[c] = 0.f;
+                auto add_products = [&](uint32_t g, float factor) {  // of block g, which the maximum's growth makes `factor` of o
+                    wait(bar(BAR_O_DONE + (g & 1)), (g >> 1) & 1);
+                    fence_after();
+#pragma unroll
+                    for (int c = 0; c < kCols / 32; ++c) {
+                        float x[32];
+                        tmem_ld32(tmem_o(static_cast<int>(g & 1)) + lane_addr + t * kCols + c * 32, x);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[c * 32 + i] = fmaf(o[c * 32 + i], factor, x[i]);
+                    }
+                    fence_before();
+                    mbar_arrive(bar(BAR_O_FREE + (g & 1)));
+                };
+                float m_used = -INFINITY, l = 0.f, last = 1.f;
+#pragma unroll 1
+                for (uint32_t j = 0; j < w.blocks; ++j) {
+                    const uint32_t g = g0 + j, buf = g & 1;
+                    const uint32_t s_tmem = tmem_s(0, buf) + lane_addr;
+                    wait(bar(BAR_S_FULL + buf), (g >> 1) & 1);
+                    fence_after();
+                    float s[kKeys];
+                    tmem_ld32(s_tmem + t * kKeys, s);
+                    tmem_wait_ld();
+                    const uint32_t left = p.prefix - (w.block + j) * BN;  // keys from this block on
+                    if (left < BN) {
+#pragma unroll
+                        for (int c = 0; c < kKeys; ++c) {
+                            if (t * kKeys + c >= left) s[c] = -INFINITY;
+                        }
+                    }
+                    float mx4[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mx4[i] = max3(s[i], s[4 + i], s[8 + i]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mx4[i] = max3(mx4[i], s[12 + i], s[16 + i]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mx4[i] = max3(mx4[i], s[20 + i], max3(s[24 + i], s[28 + i], -INFINITY));
+                    float mx = max3(fmaxf(mx4[0], mx4[1]), mx4[2], mx4[3]);
+                    fence_before();
+                    mx = fmaxf(mx, exchange(buf, mx)) * p.scale_log2;
+                    fence_after();  // both halves have been read: P may overwrite them
+                    float factor = 1.f;
+                    if (mx > m_used + 8.f) {
+                        factor = fast_exp2(m_used - mx);
+                        m_used = mx;
+                    }
+                    const float m_safe = m_used == -INFINITY ? 0.f : m_used;
+                    const f32x2 scale2 = pack_f32x2(p.scale_log2, p.scale_log2), m2 = pack_f32x2(-m_safe, -m_safe);
+                    f32x2 sum2[2] = {pack_f32x2(0.f, 0.f), pack_f32x2(0.f, 0.f)};
+                    uint32_t hi[16], lo[16];
+                    [[maybe_unused]] uint32_t third[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        float p0, p1;
+                        unpack_f32x2(fma_f32x2(pack_f32x2(s[2 * i], s[2 * i + 1]), scale2, m2), p0, p1);
+                        p0 = fast_exp2(p0);
+                        p1 = fast_exp2(p1);
+                        const f32x2 pp = pack_f32x2(p0, p1);
+                        sum2[i & 1] = add_f32x2(sum2[i & 1], pp);
+                        if constexpr (BF16) {  // 8 bits at a time, cut off
+                            const float r0 = p0 - upper16(p0), r1 = p1 - upper16(p1);
+                            hi[i] = pack_upper16(p0, p1);
+                            lo[i] = pack_upper16(r0, r1);
+                            third[i] = pack_upper16(r0 - upper16(r0), r1 - upper16(r1));
+                        } else {
+                            float h0, h1;
+                            hi[i] = pack2<BF16>(p0, p1);
+                            unpack2<BF16>(hi[i], h0, h1);
+                            lo[i] = pack2<BF16>(p0 - h0, p1 - h1);
+                        }
+                    }
+                    // 32 keys -> 16 packed columns of each part
+                    tmem_st16(s_tmem + t * 16, hi);
+                    tmem_st16(s_tmem + BN / 2 + t * 16, lo);
+                    if constexpr (BF16) tmem_st16(tmem_third(buf) + lane_addr + t * 16, third);
+                    float s0, s1;
+                    unpack_f32x2(add_f32x2(sum2[0], sum2[1]), s0, s1);
+                    l = l * factor + (s0 + s1);
+                    tmem_wait_st();
+                    fence_before();
+                    mbar_arrive(bar(BAR_P_FULL + buf));
+                    if (j > 0) add_products(g - 1, last);
+                    last = factor;
+                }
+                g0 += w.blocks;
+                add_products(g0 - 1, last);
+                // ---- the piece: O / l and log-sum-exp (log2 units)
+                l += exchange(g0 & 1, l);
+                named_bar_sync(4, 256);  // (the exchanged values have been read)
+                const float inv = l > 0.f ? 1.f / l : 0.f;
+                const uint32_t rec_row = (blockIdx.x + w.seg) * kRows;
+                if (t == 0 && w.m0 + r < query_rows) p.lse[rec_row + r] = l > 0.f ? m_used + __log2f(l) : -INFINITY;
+                // through shared memory and the TMA engine, 32 columns at a time: the second query tile and the staging tiles are free
+#pragma unroll
+                for (int pass = 0; pass < kCols / 32; ++pass) {
+                    const uint32_t stage = t == 0 ? base + kSmemQ + kTileBytes + pass * kSubTileBytes : base + kSmemStage + pass * kStageTileBytes;
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(stage + r * 128 + ((c ^ (r & 7)) << 4)),
+                                     "r"(__float_as_uint(o[pass * 32 + c * 4] * inv)), "r"(__float_as_uint(o[pass * 32 + c * 4 + 1] * inv)),
+                                     "r"(__float_as_uint(o[pass * 32 + c * 4 + 2] * inv)), "r"(__float_as_uint(o[pass * 32 + c * 4 + 3] * inv))
+                                     : "memory");
+                }
+                fence_async_smem();
+                named_bar_sync(1 + t, 128);
+                if (leader) {
+#pragma unroll
+                    for (int pass = 0; pass < kCols / 32; ++pass)
+                        tma_store_2d(&tm_o, t == 0 ? base + kSmemQ + kTileBytes + pass * kSubTileBytes : base + kSmemStage + pass * kStageTileBytes,
+                                     t * kCols + pass * 32, rec_row);
+                    tma_store_commit();
+                }
+                staged = true;
+            }
+        } else {
         for (uint32_t at = t0; ok && item_at(at, w); at += w.blocks) {
             if (!w.tile[t]) continue;
             // ---- the query rows into the tile (the previous item's MMAs are over, its result has left)
             const uint32_t m = w.m0 + t * BM + r;
             if (staged) {
-                if ((warp & 3) == 0 && lane == 0) tma_store_wait_read();
+                if (leader) tma_store_wait_read();
                 named_bar_sync(1 + t, 128);
             }
             if (!brought) bring_rows();
@@ -266,11 +427,10 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                 // probabilities; P overwrites S in place
                 const float m_safe = m_used == -INFINITY ? 0.f : m_used;
                 const f32x2 scale2 = pack_f32x2(p.scale_log2, p.scale_log2), m2 = pack_f32x2(-m_safe, -m_safe);
-                const f32x2 minus1 = pack_f32x2(-1.f, -1.f);
                 f32x2 sum2[2] = {pack_f32x2(0.f, 0.f), pack_f32x2(0.f, 0.f)};
 #pragma unroll
                 for (int c = 0; c < BN / 32; ++c) {
-                    uint32_t hi[16], lo[16];
+                    uint32_t hi[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         float p0, p1;
@@ -280,16 +440,8 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                         const f32x2 pp = pack_f32x2(p0, p1);
                         sum2[i & 1] = add_f32x2(sum2[i & 1], pp);
                         hi[i] = pack2<BF16>(p0, p1);
-                        if constexpr (RES) {
-                            float h0, h1, r0, r1;
-                            unpack2<BF16>(hi[i], h0, h1);
-                            unpack_f32x2(fma_f32x2(pack_f32x2(h0, h1), minus1, pp), r0, r1);
-                            lo[i] = pack2<BF16>(r0, r1);
-                        }
                     }
-                    // 32 keys -> 16 packed columns: rounded part at column 16c, residual at BN / 2 + 16c
-                    tmem_st16(s_tmem + c * 16, hi);
-                    if constexpr (RES) tmem_st16(s_tmem + BN / 2 + c * 16, lo);
+                    tmem_st16(s_tmem + c * 16, hi);  // 32 keys -> 16 packed columns
                 }
                 float s0, s1;
                 unpack_f32x2(add_f32x2(sum2[0], sum2[1]), s0, s1);
@@ -308,12 +460,11 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             }
             fence_after();
             const float inv = l > 0.f ? 1.f / l : 0.f;
-            const uint32_t rec_row = (blockIdx.x + w.seg) * (2 * BM) + t * BM;
+            const uint32_t rec_row = (blockIdx.x + w.seg) * kRows + t * BM;
             if (m < query_rows) p.lse[rec_row + r] = l > 0.f ? m_used + __log2f(l) : -INFINITY;
             // The tile leaves through shared memory and the TMA engine, 128 bytes of every row at a time: the query tile, which nothing
             // reads any more, holds the first two passes, the staging tile the third, so that only the fourth waits for a store. (Each pass
             // behind the previous one's store in a single staging tile: 3 us more per piece.)
-            const bool leader = (warp & 3) == 0 && lane == 0;
             auto put = [&](int pass, uint32_t stage) {
                 float o[32];
                 tmem_ld32(tmem_o(t) + lane_addr + pass * 32, o);
@@ -346,9 +497,10 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             staged = true;
             fence_before();  // the next item's first product overwrites O; its P_FULL arrival orders it behind these loads
         }
-        if ((warp & 3) == 0 && lane == 0) tma_store_wait_all();
+        }
+        if (leader) tma_store_wait_all();
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == 8) block_wait(3, 288);
         if (warp == 8 && elect_one()) {
             // =============================== TMA producer ===============================
@@ -402,11 +554,17 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                 const uint32_t buf = (g0[t] + j) & 1;
                 const uint64_t va = v_desc + st * (kKvBytes / 16);
                 const uint32_t pa = tmem_s(t, buf);
+if constexpr (RES) {  // from zero, the small parts first
+                    const uint32_t d = tmem_o(static_cast<int>(buf));
 #pragma unroll
-                for (int kc = 0; kc < BN / 16; ++kc) mma_ts(tmem_o(t), pa + kc * 8, va + kc * 128, idesc_pv, j > 0 || kc > 0);
-                if constexpr (RES) {
+                    for (int kc = 0; kc < BN / 16 && BF16; ++kc) mma_ts(d, tmem_third(buf) + kc * 8, va + kc * 128, idesc_pv, kc > 0);
 #pragma unroll
-                    for (int kc = 0; kc < BN / 16; ++kc) mma_ts(tmem_o(t), pa + BN / 2 + kc * 8, va + kc * 128, idesc_pv, 1);
+                    for (int kc = 0; kc < BN / 16; ++kc) mma_ts(d, pa + BN / 2 + kc * 8, va + kc * 128, idesc_pv, BF16 || kc > 0);
+#pragma unroll
+                    for (int kc = 0; kc < BN / 16; ++kc) mma_ts(d, pa + kc * 8, va + kc * 128, idesc_pv, 1);
+                } else {
+#pragma unroll
+                    for (int kc = 0; kc < BN / 16; ++kc) mma_ts(tmem_o(t), pa + kc * 8, va + kc * 128, idesc_pv, j > 0 || kc > 0);
                 }
                 commit(bar(BAR_O_DONE + 2 * t + buf));
             };
@@ -442,6 +600,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                         if (!ok || !w.tile[t]) continue;
                         const uint32_t g = g0[t] + j;
                         if (!mbar_wait(bar(BAR_P_FULL + 2 * t + (g & 1)), (g >> 1) & 1)) { ok = false; break; }
+                        if (RES && g >= 2 && !mbar_wait(bar(BAR_O_FREE + (g & 1)), ((g >> 1) & 1) ^ 1)) { ok = false; break; }
                         fence_after();
                         issue_pv(t, j, st);
                         if (more) {
@@ -498,8 +657,8 @@ int launch_shared_prefix(const SharedPrefixParams& p, cudaStream_t stream) {
     const cuuint64_t kv_dims[3] = {p.head_dim, p.prefix, p.n_kv_heads};
     const cuuint64_t kv_strides[2] = {p.row_stride * 2, p.head_dim * 2ull};
     const cuuint32_t kv_box[3] = {64, BN, 1};
-    // pieces [records * 256 rows][head_dim] fp32, stored 32 columns x 128 rows at a time
-    const cuuint64_t o_dims[2] = {p.head_dim, (static_cast<cuuint64_t>(p.grid) + p.segments) * 2 * BM};
+    // pieces [records * 256 or 128 rows][head_dim] fp32, stored 32 columns x 128 rows at a time
+    const cuuint64_t o_dims[2] = {p.head_dim, (static_cast<cuuint64_t>(p.grid) + p.segments) * (p.residual ? BM : 2 * BM)};
     const cuuint64_t o_strides[1] = {p.head_dim * 4ull};
     const cuuint32_t o_box[2] = {32, BM};
     CUtensorMap tm_k, tm_v, tm_o;

@@ -175,6 +175,10 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     }
 }
 
+// The bf16 that a float starts with, as a float; those of two floats, side by side.
+__device__ __forceinline__ float upper16(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+__device__ __forceinline__ uint32_t pack_upper16(float x, float y) { return __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632); }
+
 template <bool BF16>
 __device__ __forceinline__ float round16(float x) {
     if constexpr (BF16) {

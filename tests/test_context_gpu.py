@@ -481,3 +481,49 @@ def test_decode_shared_long_prefix_in_a_graph_and_back_to_back(ctx):
     for o, w, s, one in zip(outs, want, scores, once):
         assert torch.equal(o, w)
         assert (s - 8 * one).abs().max() <= 8 * 2.0 ** -22 * 4 * 8  # eight steps of weights of at most four each, added one by one
+
+
+@pytest.mark.parametrize("dtype", (torch.float16, torch.bfloat16))
+@pytest.mark.parametrize("P, Tn", ((131072, 0), (131072, 300), (0, 4096)))
+def test_fp32_outputs_of_long_sums_are_not_small(ctx, dtype, P, Tn):
+    """Positive values: a bias of the sums shows. A matrix instruction may cut off up to one unit in the last place; a chain of them
+    over one block has at most twelve. Additions of blocks and the probabilities' own roundings average out over rows and outputs,
+    up to a common error of exp2, 2^-22. So the mean signed error is below 12 * 2^-23, that, and the few roundings of joining
+    the pieces: 18 * 2^-23."""
+    B, H, Hkv, D = 16, 8, 2, 128
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.zeros((B, H, D), dtype=dtype, device="cuda")
+    q[:, :, 0] = 1
+    k, kp = (torch.zeros(s, dtype=dtype, device="cuda") for s in ((B, Tn, Hkv, D), (P, Hkv, D)))
+    v, vp = ((1 + torch.rand(s, generator=g, device="cuda")).to(dtype) for s in ((B, Tn, Hkv, D), (P, Hkv, D)))
+    for x in (k, kp):
+        x[..., 0] = (-2 * torch.rand(x.shape[:-1], generator=g, device="cuda")).to(dtype)
+    out = ctx.attn_decode_shared(q, kp if P else None, vp if P else None, k, v, out_dtype=torch.float32, scale=1.0).double()
+    w, wp = k[..., :1].double().exp(), kp[..., :1].double().exp()
+    want = ((w * v.double()).sum(1) + (wp * vp.double()).sum(0)) / (w.sum(1) + wp.sum(0))
+    want = want.repeat_interleave(H // Hkv, dim=1)
+    assert abs(float(((out - want) / want).mean())) <= 18 * 2.0 ** -23
+
+
+@pytest.mark.parametrize("dtype", (torch.float16, torch.bfloat16))
+@pytest.mark.parametrize("D", (64, 128))
+def test_fp32_outputs_take_probabilities_in_full(ctx, dtype, D):
+    """Two rows, one of score 0 and value 0, one of score -a and value 1: the output is p / (1 + p), p = exp(-a). Relative errors:
+    of p 2^-22 (exp2) and 2^-22 (the scale's product), the sum 2^-24, the division 2^-23, three cut-off additions 2^-23 each, the
+    joining of pieces 2^-21; together 6.25 * 2^-22. (A p of 16 bits would be off by up to 2^-17.)"""
+    B, H = 4, 64
+    a = ((1 + torch.arange(B * H, dtype=torch.float64)) / 128).to(dtype).cuda()  # up to 2, exact in either type
+    q = torch.zeros((B, H, D), dtype=dtype, device="cuda")
+    q[:, :, 0] = a.view(B, H)
+    for prefix in (False, True):
+        rows = 0 if prefix else 2
+        k, v = torch.zeros((2, 1, D), dtype=dtype, device="cuda"), torch.zeros((2, 1, D), dtype=dtype, device="cuda")
+        k[1, 0, 0] = -1
+        v[1] = 1
+        own = torch.zeros((B, 0, 1, D), dtype=dtype, device="cuda") if prefix else k[None].expand(B, -1, -1, -1).contiguous()
+        own_v = own if prefix else v[None].expand(B, -1, -1, -1).contiguous()
+        out = ctx.attn_decode_shared(q, k if prefix else None, v if prefix else None, own, own_v, out_dtype=torch.float32, scale=0.75).double()
+        p = torch.exp(-0.75 * a.double()).view(B, H, 1)
+        want = (p / (1 + p)).expand(B, H, D)
+        assert own.shape[1] == rows
+        assert float(((out - want) / want).abs().max()) <= 6.25 * 2.0 ** -22
