@@ -92,6 +92,13 @@ def _enqueue(entry: str, index: int, stream, packed: bytes) -> None:
         _b.check(rc, entry)
 
 
+def _on(stream, make, *args, **kwargs):
+    """What ``make`` allocates, for a kernel that runs on ``stream``: from that stream's memory, so that nothing the current stream
+    still does, or does next, shares it."""
+    with torch.cuda.stream(stream):
+        return make(*args, **kwargs)
+
+
 def _one_device(*tensors) -> int:
     """The index of the device that all operands are on."""
     index = tensors[0].get_device()
@@ -160,7 +167,8 @@ def rope_positions(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
     q, q_stride, k, k_stride, v, v_stride = taken
     out_stride = 0
     if q_out is None:
-        q_out = torch.empty_like(q, dtype=q_out_dtype or dtype, memory_format=torch.contiguous_format)
+        form = dict(dtype=q_out_dtype or dtype, memory_format=torch.contiguous_format)
+        q_out = torch.empty_like(q, **form) if stream is None else _on(stream, torch.empty_like, q, **form)
     else:
         stride = q_out.stride()
         if q_out.shape != (N, H, D) or stride[2] != 1 or stride[1] != D or (N > 1 and stride[0] < H * D):
@@ -255,7 +263,8 @@ def attn_decode_shared(q: torch.Tensor, k_prefix, v_prefix, k_cache: torch.Tenso
     if not q.is_contiguous():
         q = _dense(q, stream, "q")
     if out is None:
-        out = torch.empty_like(q, dtype=out_dtype or dtype)  # (q is dense; half the host time of torch.empty)
+        form = dict(dtype=out_dtype or dtype)  # (q is dense; half the host time of torch.empty)
+        out = torch.empty_like(q, **form) if stream is None else _on(stream, torch.empty_like, q, **form)
     elif out.shape != (B, H, D) or not out.is_contiguous():
         raise ValueError("out must be a contiguous [B, H, D] tensor")
     o_dtype = out.dtype
@@ -267,7 +276,8 @@ def attn_decode_shared(q: torch.Tensor, k_prefix, v_prefix, k_cache: torch.Tenso
         return out
     need_rows = T if scores_out_ptr else 0
     if workspace is None or workspace.key != (B, H, Hkv, D, index) or workspace.rows < need_rows:
-        workspace = SharedWorkspace(B, H, Hkv, D, need_rows, q.device)
+        shape = (B, H, Hkv, D, need_rows, q.device)
+        workspace = SharedWorkspace(*shape) if stream is None else _on(stream, SharedWorkspace, *shape)
     _enqueue("attn_decode_shared", index, stream, SHARED_ARGS.pack(
         out.data_ptr(), q.data_ptr(), kp, vp, k_cache.data_ptr() if T else 0, v_cache.data_ptr() if T else 0,
         0 if lse is None else lse.data_ptr(), _DTYPES[o_dtype], _DTYPES[dtype], B, H, Hkv, D, P, T, len_ptr, uniform,
@@ -303,13 +313,18 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor,
     if keep < 1 or keep > T2 or sink < 0 or recent < 0 or sink + recent > keep:
         raise ValueError("keep must be at least 1, fit the output caches and hold the sink and the recent rows")
     if kept is None:
-        kept = torch.empty_strided((B, Hkv, keep), (Hkv * keep, keep, 1), dtype=torch.int32, device=k_cache.device)
+        form, where = ((B, Hkv, keep), (Hkv * keep, keep, 1)), dict(dtype=torch.int32, device=k_cache.device)
+        kept = torch.empty_strided(*form, **where) if stream is None else _on(stream, torch.empty_strided, *form, **where)
         kept_ptr = kept.data_ptr()
     else:
         kept_ptr = _index(kept, (B, Hkv, keep), "kept")
     len_ptr = 0 if kv_len is None else _index(kv_len, (B,), "kv_len")
     if kv_len_out is None:
-        kv_len_out = torch.empty((B,), dtype=torch.int32, device=k_cache.device) if kv_len is None else torch.empty_like(kv_len)
+        if kv_len is None or stream is not None:
+            where = dict(dtype=torch.int32, device=k_cache.device)
+            kv_len_out = torch.empty((B,), **where) if stream is None else _on(stream, torch.empty, (B,), **where)
+        else:
+            kv_len_out = torch.empty_like(kv_len)
         len_out_ptr = kv_len_out.data_ptr()
     else:
         len_out_ptr = _index(kv_len_out, (B,), "kv_len_out")

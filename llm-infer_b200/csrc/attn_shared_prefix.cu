@@ -13,7 +13,7 @@
 //
 // With fp32 outputs a segment is one tile, whose keys and output columns the two softmax warpgroups share; P enters the second product in
 // the two (fp16) or three (bf16) parts that hold its 24 bits, and a block's products start from zero and are added up in registers.
-// 128 query rows of 128 dimensions x 65536 keys, 8 kv heads: 67 us (fp16) and 74 (bf16), for 58 with outputs of 16 bits, all of it the
+// 64 query rows of 128 dimensions x 65536 keys, 8 kv heads: 67 us (fp16) and 74 (bf16), for 58 with outputs of 16 bits, all of it the
 // further MMAs (a third block of scores in tensor memory changed nothing); errors 7e-7 and 5e-7 of the output, where sums left in tensor
 // memory and two parts were off by 9e-6.
 //

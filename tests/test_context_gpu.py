@@ -527,3 +527,40 @@ def test_fp32_outputs_take_probabilities_in_full(ctx, dtype, D):
         want = (p / (1 + p)).expand(B, H, D)
         assert own.shape[1] == rows
         assert float(((out - want) / want).abs().max()) <= 6.25 * 2.0 ** -22
+
+
+def test_memory_of_a_call_belongs_to_its_stream(ctx):
+    """Calls on a stream that is busy, without outputs or workspaces of the caller's: what the current stream allocates and writes in
+    the meantime neither changes their results nor is changed by them."""
+    g = _gen(5)
+    B, H, Hkv, D, P, Tn = 8, 32, 8, 128, 3000, 700
+    q, k, v = (torch.randn(s, generator=g).half().cuda() for s in ((B, H, D), (B, Tn, Hkv, D), (B, Tn, Hkv, D)))
+    kp, vp = (torch.randn((P, Hkv, D), generator=g).half().cuda() for _ in range(2))
+    zero = torch.zeros((B, Hkv, Tn), device="cuda")
+    inv, _ = ctx.rope_frequencies(D, 10000.0)
+    inv, pos, new = inv.cuda(), torch.arange(B, dtype=torch.int32, device="cuda"), torch.randn((B, Hkv, D), generator=g).half().cuda()
+
+    def calls(stream):
+        scores, cache = zero.clone(), [torch.zeros((B, 8, Hkv, D), dtype=torch.float16, device="cuda") for _ in range(2)]
+        outs = [torch.zeros((B, 256, Hkv, D), dtype=torch.float16, device="cuda") for _ in range(2)] + [torch.zeros((B, Hkv, 256), device="cuda")]
+        torch.cuda.synchronize()
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                torch.cuda._sleep(50_000_000)
+        turned = ctx.rope_positions(q, new, new, *cache, pos, pos, inv_freq=inv, stream=stream)
+        out = ctx.attn_decode_shared(turned, kp, vp, k, v, scores_out=scores, stream=stream)
+        kept, lens = ctx.kv_evict(k, v, scores, None, 256, sink=4, recent=16, out=tuple(outs), stream=stream)
+        return turned, out, scores, kept, lens, *outs
+
+    want = calls(None)
+    side = torch.cuda.Stream()
+    torch.cuda.empty_cache()
+    sizes = (B * H * D * 2, B * Hkv * 256 * 4, B * 4, ctx.SharedWorkspace(B, H, Hkv, D, rows=Tn).nbytes)
+    got = calls(side)
+    assert not side.query()  # (still busy: nothing of it has run)
+    others = [torch.full((n,), 7, dtype=torch.uint8, device="cuda") for n in sizes for _ in range(4)]
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    for x in others:
+        assert bool((x == 7).all())
