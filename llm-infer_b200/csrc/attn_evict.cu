@@ -9,9 +9,9 @@
 // moves down, so one CTA per (head, slice of the row) goes through the rows in order: everything it still has to read lies
 // behind what it writes.
 //
-// Graphs of calls: 16 ragged sequences of up to 4096 rows into caches of 1999 (8 kv heads of 128, 246 MB) 49.3 us, of which the
-// copy is 39 (6.2 TB/s) and the selection 6; one sequence of 131072 rows to 16384 48.6 us: copy 22, selection 19 (a digit costs 3.5 us,
-// 2 of them the sum of the histograms over eight CTAs); 1024 rows to 256 8.9 us, all of it latency.
+// Graphs of calls: 16 ragged sequences of up to 4096 rows into caches of 1999 (8 kv heads of 128, 246 MB) 49.1 us, of which the
+// copy is 39 (6.2 TB/s) and the selection 6; one sequence of 131072 rows to 16384 39.3 us: copy 22, the rest the selection on 64 SMs (48.6
+// while every CTA read the others' histograms whole, 2 us a digit); 1024 rows to 256 9.2 us, all of it latency.
 #include "attn_internal.cuh"
 #include "ptx_sm100.cuh"
 
