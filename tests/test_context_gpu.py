@@ -550,7 +550,7 @@ def test_memory_of_a_call_belongs_to_its_stream(ctx):
         turned = ctx.rope_positions(q, new, new, *cache, pos, pos, inv_freq=inv, stream=stream)
         out = ctx.attn_decode_shared(turned, kp, vp, k, v, scores_out=scores, stream=stream)
         kept, lens = ctx.kv_evict(k, v, scores, None, 256, sink=4, recent=16, out=tuple(outs), stream=stream)
-        return turned, out, scores, kept, lens, *outs
+        return turned, out, scores, kept, lens, *outs, *cache  # (what the caller brought must live until the stream is through, the caches too)
 
     want = calls(None)
     side = torch.cuda.Stream()
