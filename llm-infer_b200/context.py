@@ -167,8 +167,9 @@ def rope_positions(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
     q, q_stride, k, k_stride, v, v_stride = taken
     out_stride = 0
     if q_out is None:
-        form = dict(dtype=q_out_dtype or dtype, memory_format=torch.contiguous_format)
-        q_out = torch.empty_like(q, **form) if stream is None else _on(stream, torch.empty_like, q, **form)
+        o_dtype = q_out_dtype or dtype
+        q_out = torch.empty_like(q, dtype=o_dtype, memory_format=torch.contiguous_format) if stream is None else \
+            _on(stream, torch.empty_like, q, dtype=o_dtype, memory_format=torch.contiguous_format)
     else:
         stride = q_out.stride()
         if q_out.shape != (N, H, D) or stride[2] != 1 or stride[1] != D or (N > 1 and stride[0] < H * D):
@@ -263,8 +264,8 @@ def attn_decode_shared(q: torch.Tensor, k_prefix, v_prefix, k_cache: torch.Tenso
     if not q.is_contiguous():
         q = _dense(q, stream, "q")
     if out is None:
-        form = dict(dtype=out_dtype or dtype)  # (q is dense; half the host time of torch.empty)
-        out = torch.empty_like(q, **form) if stream is None else _on(stream, torch.empty_like, q, **form)
+        o_dtype = out_dtype or dtype  # (q is dense: empty_like, which takes half the host time of torch.empty)
+        out = torch.empty_like(q, dtype=o_dtype) if stream is None else _on(stream, torch.empty_like, q, dtype=o_dtype)
     elif out.shape != (B, H, D) or not out.is_contiguous():
         raise ValueError("out must be a contiguous [B, H, D] tensor")
     o_dtype = out.dtype
@@ -313,18 +314,18 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor,
     if keep < 1 or keep > T2 or sink < 0 or recent < 0 or sink + recent > keep:
         raise ValueError("keep must be at least 1, fit the output caches and hold the sink and the recent rows")
     if kept is None:
-        form, where = ((B, Hkv, keep), (Hkv * keep, keep, 1)), dict(dtype=torch.int32, device=k_cache.device)
-        kept = torch.empty_strided(*form, **where) if stream is None else _on(stream, torch.empty_strided, *form, **where)
+        shape, stride, device = (B, Hkv, keep), (Hkv * keep, keep, 1), k_cache.device
+        kept = torch.empty_strided(shape, stride, dtype=torch.int32, device=device) if stream is None else \
+            _on(stream, torch.empty_strided, shape, stride, dtype=torch.int32, device=device)
         kept_ptr = kept.data_ptr()
     else:
         kept_ptr = _index(kept, (B, Hkv, keep), "kept")
     len_ptr = 0 if kv_len is None else _index(kv_len, (B,), "kv_len")
     if kv_len_out is None:
-        if kv_len is None or stream is not None:
-            where = dict(dtype=torch.int32, device=k_cache.device)
-            kv_len_out = torch.empty((B,), **where) if stream is None else _on(stream, torch.empty, (B,), **where)
+        if stream is not None:
+            kv_len_out = _on(stream, torch.empty, (B,), dtype=torch.int32, device=k_cache.device)
         else:
-            kv_len_out = torch.empty_like(kv_len)
+            kv_len_out = torch.empty((B,), dtype=torch.int32, device=k_cache.device) if kv_len is None else torch.empty_like(kv_len)
         len_out_ptr = kv_len_out.data_ptr()
     else:
         len_out_ptr = _index(kv_len_out, (B,), "kv_len_out")

@@ -1,7 +1,7 @@
 // Eviction from a KV cache by accumulated attention weight: of every (sequence, kv head), the first `sink` rows, the last
 // `recent` rows and the rows with the largest scores, `keep` in all, stay; their order stays too. Ties go to the lowest row.
 //
-// Two launches. (1) Which rows: a CTA or a cluster of them per (sequence, kv head) finds the keep-th largest key by a radix selection
+// Two launches, or one that does both for small calls. (1) Which rows: a CTA or a cluster of them per (sequence, kv head) finds the keep-th largest key by a radix selection
 // (digits of 11, 11 and 10 bits, a histogram in shared memory per CTA, summed over the cluster), then counts and writes the
 // kept rows in order. A score's key is its bit pattern mapped so that unsigned order is the order of the numbers (NaN below
 // everything, -0 = +0); always-kept rows carry the largest key. (2) The copy, bound by memory: kept K and V rows and scores are
@@ -11,11 +11,14 @@
 //
 // Graphs of calls: 16 ragged sequences of up to 4096 rows into caches of 1999 (8 kv heads of 128, 246 MB) 49.1 us, of which the
 // copy is 39 (6.2 TB/s) and the selection 6; one sequence of 131072 rows to 16384 39.3 us: copy 22, the rest the selection on 64 SMs (48.6
-// while every CTA read the others' histograms whole, 2 us a digit); 1024 rows to 256 9.2 us, all of it latency.
+// while every CTA read the others' histograms whole, 2 us a digit); 1024 rows to 256, one launch,
+// 6.2 us (two: 9.3), all of it latency.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
 #include "attn_internal.cuh"
 #include "ptx_sm100.cuh"
-
-#include <cooperative_groups.h>
 
 namespace b200 {
 namespace {
@@ -48,6 +51,7 @@ constexpr int kBins = 2048;
 constexpr int kGroups = kBins / 32;
 constexpr uint32_t kSelWords = 4 * kBins + 3 * kGroups + 2 * kSelWarps + 4;  // shared memory in front of the keys
 constexpr uint32_t kAlways = 0xffffffffu;
+constexpr uint64_t kOneLaunchBytes = 256 * 1024, kOneLaunchSmem = 200 * 1024;
 
 // Unsigned order of the keys = order of the scores; NaN gets 0, below -inf. No score maps to kAlways (that pattern would be a NaN).
 __device__ __forceinline__ uint32_t score_key(float x) {
@@ -61,10 +65,35 @@ __device__ __forceinline__ uint32_t score_key(float x) {
 // the same from either value.
 __device__ __forceinline__ uint32_t rows_of(const EvictParams& p, uint32_t b) { return min(p.kv_len ? p.kv_len[b] : p.rows, p.rows); }
 
+// This CTA's share, one of gridDim.x, of what a (sequence, kv head) keeps: K and V, scores, and the list itself.
+__device__ __forceinline__ void copy_share(const EvictParams& p, const uint32_t* kept, uint32_t b, uint32_t seg, uint32_t len) {
+    __syncthreads();  // the list is complete
+    const uint32_t h = seg - b * p.n_kv_heads, after = min(len, p.keep);
+    const uint32_t first = blockIdx.x * kSelThreads + threadIdx.x, step = gridDim.x * kSelThreads;
+    if (h == 0 && first == 0) p.kv_len_out[b] = after;
+    for (uint32_t j = first; j < p.out_rows; j += step) {
+        if (j < p.keep) p.kept[static_cast<size_t>(seg) * p.keep + j] = kept[j];
+        p.scores_out[seg * p.score_out_stride + j] = j < after ? p.scores[seg * p.score_stride + kept[j]] : 0.f;
+    }
+    const uint32_t D16 = p.head_dim / 8, total = after * D16;
+    const size_t in = b * p.batch_stride + static_cast<size_t>(h) * p.head_dim, out = b * p.out_batch_stride + static_cast<size_t>(h) * p.head_dim;
+#pragma unroll 2
+    for (uint32_t u = first; u < total; u += step) {
+        const uint32_t j = u / D16, c = (u - j * D16) * 8;
+        const uint64_t from = in + kept[j] * p.row_stride + c, to = out + j * p.out_row_stride + c;
+        const uint4 xk = __ldcs(reinterpret_cast<const uint4*>(p.k + from)), xv = __ldcs(reinterpret_cast<const uint4*>(p.v + from));
+        *reinterpret_cast<uint4*>(p.k_out + to) = xk;
+        *reinterpret_cast<uint4*>(p.v_out + to) = xv;
+    }
+}
+
 // One cluster of kCtas per (sequence, kv head) = blockIdx.y. A CTA keeps the keys of its rows in shared memory and goes through them four
 // at a time; rows beyond `staged` (more than 40960 rows a CTA) are read again from the scores.
-template <int kCtas>
+// kCopy, for small calls into other caches: one launch. The CTAs of a (sequence, kv head) do not form a cluster, each selects for itself and
+// then copies its share of the kept rows.
+template <int kCtas, bool kCopy = false>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_constant__ EvictParams p) {
+    static_assert(!kCopy || kCtas == 1);
     extern __shared__ __align__(16) uint32_t s_all[];
     uint32_t* s_hist = s_all;                   // [4][kBins]: two for the top digit (even and odd lanes: fewer meet in a bin), one for each other
     uint32_t* s_group = s_hist + 4 * kBins;     // [3][kGroups]: a digit's histogram in sums over 32 bins
@@ -78,17 +107,18 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_
         if constexpr (kCtas > 1) cluster.sync();
         else __syncthreads();
     };
-    const uint32_t rank = blockIdx.x;
+    const uint32_t rank = kCopy ? 0u : blockIdx.x;
     const uint32_t seg = blockIdx.y, b = seg / p.n_kv_heads;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     grid_dep_launch_dependents();
     for (int i = tid; i < 4 * kBins / 4; i += kSelThreads) reinterpret_cast<uint4*>(s_hist)[i] = make_uint4(0, 0, 0, 0);
     grid_dep_wait();
     const uint32_t len = rows_of(p, b);
-    uint32_t* kept = p.kept + static_cast<size_t>(seg) * p.keep;
-    if (rank == 0 && tid == 0 && p.kv_len && p.kv_len[b] > p.rows && p.status) atomicOr(p.status, ATTN_STATUS_BAD_SHAPE);
+    uint32_t* kept = kCopy ? s_keys + p.staged : p.kept + static_cast<size_t>(seg) * p.keep;
+    if (blockIdx.x == 0 && tid == 0 && p.kv_len && p.kv_len[b] > p.rows && p.status) atomicOr(p.status, ATTN_STATUS_BAD_SHAPE);
     if (len <= p.keep) {  // the same for the whole cluster
         for (uint32_t j = rank * kSelThreads + tid; j < p.keep; j += kCtas * kSelThreads) kept[j] = j < len ? j : 0xffffffffu;
+        if constexpr (kCopy) copy_share(p, kept, b, seg, len);
         return;
     }
     // this CTA's rows: a contiguous slice, cut into one contiguous piece per warp
@@ -302,6 +332,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_
         emit(i, i < we, i < n_staged ? s_keys[i] : i < we ? make_key(i, scores[i]) : 0u);
     }
     if constexpr (kCtas > 1) cluster.sync();  // no CTA leaves while another reads its counts
+    if constexpr (kCopy) copy_share(p, kept, b, seg, len);
 }
 
 // ---- (2a) into another cache: grid (tiles of kept rows, sequences)
@@ -485,12 +516,19 @@ extern "C" int attn_kv_evict(const AttnKvEvictArgs* a, void* stream_v) {
     const uint64_t slice = (a->rows + cl - 1) / cl + 128 * kSelWarps;
     p.scores_aligned = aligned16(a->scores) && p.score_stride % 4 == 0;
     p.staged = static_cast<uint32_t>(slice < 40 * 1024 ? slice : 40 * 1024);
+    // Small calls in one launch: CTAs that select for themselves and copy a share, as many as there are SMs. Measured up to 256 KB a CTA to
+    // copy, 8 kv heads of 128, for two launches: 1024 rows to 256 6.2 us for 9.3, 2 x 4096 to 2048 11.0 for 15.5, 8000 to 7000 18.8
+    // for 22.6. Not where the new lengths are written over the old ones, which another CTA may still have to read.
+    const uint64_t shares = std::max<uint64_t>(1, std::min<uint64_t>(dev.sm_count / segments, 16));
+    const bool one_launch = !p.in_place && cl == 1 && a->kv_len_out != a->kv_len && segments <= dev.sm_count &&
+                            static_cast<uint64_t>(std::min(a->keep, a->rows)) * a->head_dim * 4 <= shares * kOneLaunchBytes &&
+                            (kSelWords + p.staged + static_cast<uint64_t>(a->keep)) * sizeof(uint32_t) <= kOneLaunchSmem;
     auto select = [&](auto kernel) -> int {
         B200_CUDA_TRY(allow_max_smem(kernel));
         cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(cl, static_cast<uint32_t>(segments));
+        cfg.gridDim = dim3(one_launch ? static_cast<uint32_t>(shares) : cl, static_cast<uint32_t>(segments));
         cfg.blockDim = dim3(kSelThreads);
-        cfg.dynamicSmemBytes = (kSelWords + p.staged) * sizeof(uint32_t);
+        cfg.dynamicSmemBytes = (kSelWords + p.staged + (one_launch ? a->keep : 0)) * sizeof(uint32_t);
         cfg.stream = stream;
         cudaLaunchAttribute attr[2];
         attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -504,6 +542,7 @@ extern "C" int attn_kv_evict(const AttnKvEvictArgs* a, void* stream_v) {
         g_launch_count.fetch_add(1, std::memory_order_relaxed);
         return ATTN_OK;
     };
+    if (one_launch) return select(evict_select_kernel<1, true>);
     const int selected = cl == 1   ? select(evict_select_kernel<1>)
                          : cl == 2 ? select(evict_select_kernel<2>)
                          : cl == 4 ? select(evict_select_kernel<4>)

@@ -564,3 +564,34 @@ def test_memory_of_a_call_belongs_to_its_stream(ctx):
         assert torch.equal(a, b)
     for x in others:
         assert bool((x == 7).all())
+
+
+@pytest.mark.parametrize("B, T, keep, Hkv, D", ((1, 1024, 256, 8, 128), (5, 700, 699, 4, 64), (2, 8192, 1000, 8, 128), (3, 300, 17, 2, 72),
+                                                (1, 8192, 8192, 1, 64), (18, 129, 33, 8, 128)))
+def test_evict_in_one_launch_or_two(ctx, B, T, keep, Hkv, D):
+    """Small calls select and copy in one launch, except where the new lengths take the old ones' place: the same results."""
+    g = _gen(T + keep)
+    k, v = (torch.randn((B, T, Hkv, D), generator=g).half().cuda() for _ in range(2))
+    scores = torch.randint(0, 50, (B, Hkv, T), generator=g).float().cuda()  # many ties
+    lens = torch.randint(0, T + 1, (B,), generator=g, dtype=torch.int32).cuda()
+    lens[0] = T
+    results = []
+    for alias in (False, True):
+        outs = [torch.full((B, keep + 3, Hkv, D), 3.0, dtype=torch.float16, device="cuda") for _ in range(2)]
+        outs.append(torch.full((B, Hkv, keep + 3), 3.0, device="cuda"))
+        old = lens.clone()
+        launches = ctx._b.load().attn_kernel_launch_count()
+        kept, new = ctx.kv_evict(k, v, scores, old, keep, sink=4, recent=9, out=tuple(outs), kv_len_out=old if alias else None)
+        assert ctx._b.load().attn_kernel_launch_count() - launches == (2 if alias else 1)
+        assert torch.equal(new, lens.clamp(max=keep)) and (alias or torch.equal(old, lens))
+        results.append((kept, new, *outs))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    kept = results[0][0]
+    for b in range(B):  # and both copy what the list says
+        n = min(int(lens[b]), keep)
+        at = kept[b, :, :n].long()
+        for h in range(Hkv):
+            assert torch.equal(results[0][2][b, :n, h], k[b, at[h], h]) and torch.equal(results[0][3][b, :n, h], v[b, at[h], h])
+            assert torch.equal(results[0][4][b, h, :n], scores[b, h, at[h]])
+        assert bool((kept[b, :, n:] == -1).all()) and bool((results[0][4][b, :, n:] == 0).all()) and bool((results[0][2][b, n:] == 3).all())
