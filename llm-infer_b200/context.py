@@ -117,12 +117,23 @@ def _index(t, shape, what):
 
 
 def _score_stride(t: torch.Tensor, batch: int, kv_heads: int, rows: int) -> int:
-    """Distance of the (sequence, kv head) runs of a [batch, kv_heads, rows] tensor of weights; 0 where there is one."""
+    """Distance of the (sequence, kv head) runs of a [batch, kv_heads, rows] tensor of weights; 0 where there is one. (The library takes
+    a distance of 0 as that of dense runs: an expanded tensor, whose runs are one, would be read and written behind its end.)"""
     stride = t.stride()
+    apart = stride[1] if kv_heads > 1 else stride[0] if batch > 1 else rows
     if t.dtype != torch.float32 or t.shape != (batch, kv_heads, rows) or (rows > 1 and stride[2] != 1) or \
-            (batch > 1 and kv_heads > 1 and stride[0] != kv_heads * stride[1]):
-        raise ValueError("scores must be fp32 [B, Hkv, rows] with dense rows at one distance")
-    return stride[1] if kv_heads > 1 else stride[0] if batch > 1 else 0
+            (batch > 1 and kv_heads > 1 and stride[0] != kv_heads * stride[1]) or apart < rows:
+        raise ValueError("scores must be fp32 [B, Hkv, rows] with dense rows at one distance, memory of their own each (not expanded)")
+    return apart if kv_heads > 1 or batch > 1 else 0
+
+
+def _row_stride(stride: int, rows: int, width: int, what: str) -> int:
+    """Distance of the rows of a cache or prefix; 0, which the library takes as dense, where there is one."""
+    if rows < 2:
+        return 0
+    if stride < width:
+        raise ValueError(f"the rows of {what} must not share memory (expanded or overlapping rows)")
+    return stride
 
 
 def rope_positions(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -148,6 +159,7 @@ def rope_positions(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
     c_stride = k_cache.stride()
     if v_cache.stride() != c_stride or c_stride[3] != 1 or c_stride[2] != D:
         raise ValueError("the caches must be [B, row, kv_head, head_dim] with dense heads and share their strides")
+    row_stride = _row_stride(c_stride[1], T, Hkv * D, "the caches")
     if layout not in _LAYOUTS:
         raise ValueError(f"layout must be one of {sorted(_LAYOUTS)}")
     half = inv_freq.numel()
@@ -179,7 +191,7 @@ def rope_positions(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
         return q_out
     _enqueue("attn_rope_positions", index, stream, ROPE_ARGS.pack(
         q_out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), inv_freq.data_ptr(),
-        pos_ptr, row_ptr, seq_ptr, q_stride, k_stride, v_stride, out_stride, c_stride[1] if T > 1 else 0, c_stride[0] if B > 1 else 0,
+        pos_ptr, row_ptr, seq_ptr, q_stride, k_stride, v_stride, out_stride, row_stride, c_stride[0] if B > 1 else 0,
         N, H, Hkv, D, 2 * half, B, T, factor, _DTYPES[dtype], _dtype_code(q_out), _DTYPES[cache_dtype], _LAYOUTS[layout],
         0 if status is None else status.data_ptr()))
     return q_out
@@ -231,6 +243,7 @@ def attn_decode_shared(q: torch.Tensor, k_prefix, v_prefix, k_cache: torch.Tenso
     stride = k_cache.stride()
     if v_cache.stride() != stride or (T and (stride[3] != 1 or stride[2] != D)):
         raise ValueError("the caches must be [B, row, kv_head, head_dim] with dense heads and share their strides")
+    row_stride = _row_stride(stride[1], T, Hkv * D, "the caches")
     P = kp = vp = prefix_stride = 0
     if (k_prefix is None) != (v_prefix is None):
         raise ValueError("k_prefix without v_prefix")
@@ -244,7 +257,7 @@ def attn_decode_shared(q: torch.Tensor, k_prefix, v_prefix, k_cache: torch.Tenso
             p_stride = k_prefix.stride()
             if v_prefix.stride() != p_stride or p_stride[2] != 1 or p_stride[1] != D:
                 raise ValueError("the prefix must be [row, kv_head, head_dim] with dense heads; K and V share their strides")
-            kp, vp, prefix_stride = k_prefix.data_ptr(), v_prefix.data_ptr(), p_stride[0] if P > 1 else 0
+            kp, vp, prefix_stride = k_prefix.data_ptr(), v_prefix.data_ptr(), _row_stride(p_stride[0], P, Hkv * D, "the prefix")
     len_ptr, uniform = 0, T
     if isinstance(kv_len, int):
         if not 0 <= kv_len <= T:
@@ -282,7 +295,7 @@ def attn_decode_shared(q: torch.Tensor, k_prefix, v_prefix, k_cache: torch.Tenso
     _enqueue("attn_decode_shared", index, stream, SHARED_ARGS.pack(
         out.data_ptr(), q.data_ptr(), kp, vp, k_cache.data_ptr() if T else 0, v_cache.data_ptr() if T else 0,
         0 if lse is None else lse.data_ptr(), _DTYPES[o_dtype], _DTYPES[dtype], B, H, Hkv, D, P, T, len_ptr, uniform,
-        scale, prefix_stride, stride[1] if T > 1 else 0, stride[0] if B > 1 else 0, scores_ptr, scores_out_ptr, score_stride,
+        scale, prefix_stride, row_stride, stride[0] if B > 1 else 0, scores_ptr, scores_out_ptr, score_stride,
         score_out_stride, workspace.ptr, workspace.nbytes, workspace.status_ptr))
     return out
 
@@ -310,6 +323,7 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor,
         raise ValueError("the caches must be [B, row, kv_head, head_dim] with dense heads; K and V share their strides")
     if dtype not in _CACHE or not (v_cache.dtype == k_out.dtype == v_out.dtype == dtype):
         raise TypeError("the caches must be fp16 or bf16, of one type")
+    row_in, row_out = _row_stride(s_in[1], T, Hkv * D, "the caches"), _row_stride(s_out[1], T2, Hkv * D, "the output caches")
     score_stride, score_out_stride = _score_stride(scores, B, Hkv, T), _score_stride(scores_out, B, Hkv, T2)
     if keep < 1 or keep > T2 or sink < 0 or recent < 0 or sink + recent > keep:
         raise ValueError("keep must be at least 1, fit the output caches and hold the sink and the recent rows")
@@ -334,6 +348,6 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor,
     _enqueue("attn_kv_evict", index, stream, EVICT_ARGS.pack(
         k_cache.data_ptr(), v_cache.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), scores.data_ptr(), scores_out.data_ptr(), kept_ptr,
         len_ptr, len_out_ptr, B, Hkv, D, T, T2, keep, sink, recent,
-        s_in[1] if T > 1 else 0, s_out[1] if T2 > 1 else 0, s_in[0] if B > 1 else 0, s_out[0] if B > 1 else 0, score_stride,
+        row_in, row_out, s_in[0] if B > 1 else 0, s_out[0] if B > 1 else 0, score_stride,
         score_out_stride, 0 if status is None else status.data_ptr()))
     return kept, kv_len_out
