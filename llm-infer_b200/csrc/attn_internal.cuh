@@ -269,9 +269,9 @@ struct SharedPrefixParams {
     uint32_t q_sign;
     uint32_t* status;
     uint32_t bf16, residual;
+    uint32_t own_smem;   // bytes of shared memory of a CTA of the split pass, two of which share a CTA
 };
 constexpr uint32_t kPrefixBlock = 64, kPrefixRows = 256;  // keys of a block, query rows of a segment (half of them for fp32 outputs)
-int launch_shared_prefix(const SharedPrefixParams& p, cudaStream_t stream);
 // fp16-weight GEMV on the tensor cores (attn_gemv_f16mma.cu): batches and the fused forms of attn_gemv_f16.
 int launch_gemv_f16_mma(const AttnGemvArgs* a, cudaStream_t stream);
 

@@ -4,6 +4,10 @@
 // Mathematics: for every query row the softmax-normalised sum over a run of keys and its log-sum-exp; the merge pass of
 // attn_shared.cu joins the runs (and the rows of the sequences' own caches) by weights exp(lse_i - LSE).
 //
+// One launch for both: the first p.grid CTAs take the prefix, the others two CTAs each of the split pass over the own rows
+// (shared_split.cuh), which needs the same registers and half the shared memory. Two launches beside each other would need the second to
+// read what earlier launches wrote without having waited for them: a launch may only wait for the one in front of it.
+//
 // Work: a segment is a kv head and two tiles of 128 query rows that share one K/V stream (a batch of up to 128 rows has one tile);
 // a segment has ceil(P / 64) blocks of 64 keys. The blocks of all segments form one list that is dealt to one CTA per SM in equal
 // contiguous runs; a CTA's part of a segment is one piece. The CTA's warps work as in the causal prefill: two softmax
@@ -27,10 +31,7 @@
 
 #include <algorithm>
 
-#include "attn_internal.cuh"
-#include "ptx_sm100.cuh"
-#include "tcgen05_sm100.cuh"
-#include "tma_tile.cuh"
+#include "shared_split.cuh"
 
 namespace b200 {
 namespace {
@@ -68,6 +69,7 @@ constexpr uint32_t kStageTileBytes = 128 * 128;
 constexpr uint32_t kSmemBars = kSmemStage + 2 * kStageTileBytes;
 constexpr uint32_t kSmemTmemPtr = kSmemBars + BAR_COUNT * 8;
 constexpr uint32_t kSmemAlloc = kSmemTmemPtr + 16 + 1024;  // slack to align the base to 1024 bytes
+static_assert(kThreads == 2 * kSplitThreads && 2 * kSplitSmem <= kMaxDynamicSmem && kSmemAlloc <= kMaxDynamicSmem);
 
 __device__ __forceinline__ void report_timeout(uint32_t* status) {
     if (status) atomicOr(status, ATTN_STATUS_WAIT_TIMEOUT);
@@ -82,8 +84,17 @@ struct Item {
 template <bool BF16, bool RES, int HD>
 __global__ void __launch_bounds__(kThreads, 1)
 shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                     const __grid_constant__ CUtensorMap tm_o, const __grid_constant__ SharedPrefixParams p) {
+                     const __grid_constant__ CUtensorMap tm_o, const __grid_constant__ CUtensorMap tm_own_k, const __grid_constant__ CUtensorMap tm_own_v,
+                     const __grid_constant__ SharedPrefixParams p, const __grid_constant__ SharedParams own) {
     extern __shared__ unsigned char smem_raw[];
+    if (blockIdx.x >= p.grid) {  // two CTAs of the split pass, six warps each
+        const int half = threadIdx.x >= kSplitThreads;
+        const uint32_t cta = (blockIdx.x - p.grid) * 2 + half;
+        if (cta < own.ctas)
+            split_body<HD, BF16, RES>(tm_own_k, tm_own_v, tm_own_k, tm_own_v, own, smem_raw + half * p.own_smem, cta, threadIdx.x - half * kSplitThreads,
+                                      2 * half);
+        return;
+    }
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
     unsigned char* smem = smem_raw + (base - raw);
@@ -106,8 +117,8 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         t0 = seg * blocks + static_cast<uint32_t>(div_mostly_32(static_cast<uint64_t>(i) * blocks, p.ctas_per_seg));
         t1 = seg * blocks + static_cast<uint32_t>(div_mostly_32((i + 1ull) * blocks, p.ctas_per_seg));
     } else {
-        t0 = static_cast<uint32_t>(div_mostly_32(blockIdx.x * total, gridDim.x));
-        t1 = static_cast<uint32_t>(div_mostly_32((blockIdx.x + 1) * total, gridDim.x));
+        t0 = static_cast<uint32_t>(div_mostly_32(blockIdx.x * total, p.grid));
+        t1 = static_cast<uint32_t>(div_mostly_32((blockIdx.x + 1) * total, p.grid));
     }
     auto item_at = [&](uint32_t t, Item& w) {  // the item that starts at block t of the list; false behind the run
         if (t >= t1) return false;
@@ -164,9 +175,9 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         const int r = ((warp & 3) << 5) | lane;  // row inside the tile = tensor-memory lane
         const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) << 5) << 16;
         // which CTAs share each segment, for the merge pass
-        for (uint32_t s = blockIdx.x * 256 + tid; s < p.segments; s += gridDim.x * 256)
+        for (uint32_t s = blockIdx.x * 256 + tid; s < p.segments; s += p.grid * 256)
             p.seg_ctas[s] = p.ctas_per_seg ? (s * p.ctas_per_seg) | p.ctas_per_seg << 16
-                                           : segment_ctas(static_cast<uint64_t>(s) * blocks, (s + 1ull) * blocks, total, gridDim.x);
+                                           : segment_ctas(static_cast<uint64_t>(s) * blocks, (s + 1ull) * blocks, total, p.grid);
         const bool leader = (warp & 3) == 0 && lane == 0;
         bool ok = true;
         uint32_t g0 = 0;  // key blocks of this tile before the current item: buffer and barrier phases run on over the items
@@ -554,7 +565,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                 const uint32_t buf = (g0[t] + j) & 1;
                 const uint64_t va = v_desc + st * (kKvBytes / 16);
                 const uint32_t pa = tmem_s(t, buf);
-if constexpr (RES) {  // from zero, the small parts first
+                if constexpr (RES) {  // from zero, the small parts first
                     const uint32_t d = tmem_o(static_cast<int>(buf));
 #pragma unroll
                     for (int kc = 0; kc < BN / 16 && BF16; ++kc) mma_ts(d, tmem_third(buf) + kc * 8, va + kc * 128, idesc_pv, kc > 0);
@@ -651,7 +662,12 @@ int encode(CUtensorMap* map, CUtensorMapDataType type, uint32_t rank, const void
 
 }  // namespace
 
-int launch_shared_prefix(const SharedPrefixParams& p, cudaStream_t stream) {
+int launch_shared_prefix(const SharedPrefixParams& prefix, const SharedParams& own, const CUtensorMap& tm_own_k, const CUtensorMap& tm_own_v, size_t own_smem,
+                         cudaStream_t stream) {
+    SharedPrefixParams p = prefix;
+    p.own_smem = static_cast<uint32_t>((own_smem + 15) / 16 * 16);
+    const size_t smem = std::max<size_t>(kSmemAlloc, 2 * static_cast<size_t>(p.own_smem));
+    const uint32_t grid = p.grid + (own.ctas + 1) / 2;
     const CUtensorMapDataType type = p.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     // K, V [row][kv head][head_dim] as (dim, row, head): blocks of 64 elements x 64 rows of one head; rows behind the end read as zeros
     const cuuint64_t kv_dims[3] = {p.head_dim, p.prefix, p.n_kv_heads};
@@ -668,7 +684,7 @@ int launch_shared_prefix(const SharedPrefixParams& p, cudaStream_t stream) {
     if ((rc = encode(&tm_o, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, p.part, o_dims, o_strides, o_box)) != ATTN_OK) return rc;
     auto launch = [&](auto kernel) -> int {
         B200_CUDA_TRY(allow_max_smem(kernel));
-        B200_CUDA_TRY(launch_dependent(kernel, dim3(p.grid), dim3(kThreads), kSmemAlloc, stream, tm_k, tm_v, tm_o, p));
+        B200_CUDA_TRY(launch_dependent(kernel, dim3(grid), dim3(kThreads), smem, stream, tm_k, tm_v, tm_o, tm_own_k, tm_own_v, p, own));
         g_launch_count.fetch_add(1, std::memory_order_relaxed);
         return ATTN_OK;
     };
