@@ -16,8 +16,9 @@
 //   merge   folds the pieces of an output row, by a warp, a CTA, or a CTA per slice of the row; further CTAs turn the scaled scores that
 //           the split pass left in the workspace into weights (exp2(s - LSE)), sum them over the heads and add them to the accumulators.
 // The scores of own rows cost 4 bytes per query head and row each way through L2, next to 4 * head_dim bytes of K and V per kv head.
-// P enters the second product rounded once to the caches' type when the output is 16 bits wide too (an error below the
-// output's own rounding), and in two (fp16) or three (bf16) parts that hold its 24 bits for fp32 outputs.
+// P enters the second product rounded once to the caches' type when the output is 16 bits wide too, which adds about as much error as the
+// output's own rounding (1.4 times the error of that alone), and for fp32 outputs in three parts of bf16 (24 bits) or two of fp16 (23 bits, or 2^-32
+// of the row's maximum where p is small: fp16 probabilities are lifted by 2^7 over the end of its range).
 //
 // Bound by HBM where there is enough to read: 16 ragged caches of up to 4096 rows (168 MB, with weights) take 38.6 us in a graph of
 // calls, of which the streaming alone takes 30; 7 sequences over 131072 shared rows (543 MB) 95 us = 5.7 TB/s. Smaller calls are a chain

@@ -16,7 +16,7 @@
 // spaced (heads of one group, then the next sequence), so the softmax warps bring them into the swizzled tile.
 //
 // With fp32 outputs a segment is one tile, whose keys and output columns the two softmax warpgroups share; P enters the second product in
-// the two (fp16) or three (bf16) parts that hold its 24 bits, and a block's products start from zero and are added up in registers.
+// three parts (bf16: its 24 bits) or two (fp16: 23 bits, or 2^-32 of the row's maximum where p is small), and a block's products start from zero and are added up in registers.
 // 64 query rows of 128 dimensions x 65536 keys, 8 kv heads: 67 us (fp16) and 74 (bf16), for 58 with outputs of 16 bits, all of it the
 // further MMAs (a third block of scores in tensor memory changed nothing); errors 7e-7 and 5e-7 of the output, where sums left in tensor
 // memory and two parts were off by 9e-6.
@@ -225,7 +225,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         if constexpr (RES) {
             // ---- fp32 outputs: the warpgroups share a tile, each takes half of a block's keys and half of O's columns. A block's products start
             // from zero and are added up here: the tensor cores cut their sums off instead of rounding them, which over hundreds of
-            // instructions makes the result small by 8e-6 of it. P's parts hold its 24 bits.
+            // instructions makes the result small by 8e-6 of it.
             constexpr int kKeys = BN / 2, kCols = HD / 2;
             const uint32_t xch = base + kSmemStage + kStageTileBytes + r * 4;  // [block parity][warpgroup][row]: the other half's maximum, or sum
             auto exchange = [&](uint32_t slot, float x) {
@@ -298,9 +298,9 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                     mx = fmaxf(mx, exchange(buf, mx)) * p.scale_log2;
                     fence_after();  // both halves have been read: P may overwrite them
                     float factor = 1.f;
-                    if (mx > m_used + 8.f) {
-                        factor = fast_exp2(m_used - mx);
-                        m_used = mx;
+                    if (mx > m_used + (8.f + kLift<BF16>)) {
+                        factor = fast_exp2(m_used - (mx - kLift<BF16>));
+                        m_used = mx - kLift<BF16>;
                     }
                     const float m_safe = m_used == -INFINITY ? 0.f : m_used;
                     const f32x2 scale2 = pack_f32x2(p.scale_log2, p.scale_log2), m2 = pack_f32x2(-m_safe, -m_safe);
@@ -347,7 +347,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                 named_bar_sync(4, 256);  // (the exchanged values have been read)
                 const float inv = l > 0.f ? 1.f / l : 0.f;
                 const uint32_t rec_row = (blockIdx.x + w.seg) * kRows;
-                if (t == 0 && w.m0 + r < query_rows) p.lse[rec_row + r] = l > 0.f ? m_used + __log2f(l) : -INFINITY;
+                if (t == 0 && w.m0 + r < query_rows) p.lse[rec_row + r] = l > 0.f ? (m_used + kLift<BF16>) + __log2f(l * kUnlift<BF16>) : -INFINITY;
                 // through shared memory and the TMA engine, 32 columns at a time: the second query tile and the staging tiles are free
 #pragma unroll
                 for (int pass = 0; pass < kCols / 32; ++pass) {
@@ -382,7 +382,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             if (!brought) bring_rows();
             brought = false;
             rows_there();
-            float m_used = -INFINITY;  // maximum the stored probabilities are relative to (log2 units)
+            float m_used = -INFINITY;  // what the stored probabilities are relative to (log2 units): a maximum less the lift
             float l = 0.f;
             for (uint32_t j = 0; j < w.blocks && ok; ++j) {
                 const uint32_t g = g0 + j, buf = g & 1, par = (g >> 1) & 1;
@@ -413,11 +413,11 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 #pragma unroll
                 for (int c = 12 + (BN - 12) / 8 * 8; c < BN; ++c) mx = fmaxf(mx, s[c]);
                 mx *= p.scale_log2;
-                // Rescale only when the maximum grew by more than 8 (probabilities stay below 2^8).
+                // Rescale only when the maximum grew by more than 8 (probabilities stay below 2^8, with fp16's lift 2^15).
                 float factor = 1.f;
-                if (mx > m_used + 8.f) {
-                    factor = fast_exp2(m_used - mx);  // 0 on the first block (m_used = -inf)
-                    m_used = mx;
+                if (mx > m_used + (8.f + kLift<BF16>)) {
+                    factor = fast_exp2(m_used - (mx - kLift<BF16>));  // 0 on the first block (m_used = -inf)
+                    m_used = mx - kLift<BF16>;
                 }
                 if (g >= 2 && !mbar_wait(bar(BAR_O_DONE + 2 * t + buf), par ^ 1)) { report_timeout(p.status); ok = false; break; }
                 if (j > 0 && __any_sync(0xffffffffu, factor != 1.f)) {
@@ -472,7 +472,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             fence_after();
             const float inv = l > 0.f ? 1.f / l : 0.f;
             const uint32_t rec_row = (blockIdx.x + w.seg) * kRows + t * BM;
-            if (m < query_rows) p.lse[rec_row + r] = l > 0.f ? m_used + __log2f(l) : -INFINITY;
+            if (m < query_rows) p.lse[rec_row + r] = l > 0.f ? (m_used + kLift<BF16>) + __log2f(l * kUnlift<BF16>) : -INFINITY;
             // The tile leaves through shared memory and the TMA engine, 128 bytes of every row at a time: the query tile, which nothing
             // reads any more, holds the first two passes, the staging tile the third, so that only the fourth waits for a store. (Each pass
             // behind the previous one's store in a single staging tile: 3 us more per piece.)

@@ -378,8 +378,8 @@ __device__ __forceinline__ void split_body(const CUtensorMap& tm_k, const CUtens
                         }
                     }
                 }
-                // The maximum that the probabilities are relative to moves only when it grew by more than 2^8: the true sum
-                // normalises at the end, and probabilities stay below 2^8.
+                // What the probabilities are relative to, the maximum less the lift, moves only when the maximum grew by more than 2^8: the
+                // true sum normalises at the end, and probabilities stay below 2^8 (2^15 with fp16's lift).
                 float mx[2];
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
@@ -390,11 +390,12 @@ __device__ __forceinline__ void split_body(const CUtensorMap& tm_k, const CUtens
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
                     mx[half] = x * p.scale_log2;
                 }
-                const bool grow0 = mx[0] > m[0] + 8.f, grow1 = mx[1] > m[1] + 8.f;
+                constexpr float kLift = tc::kLift<BF16>;
+                const bool grow0 = mx[0] > m[0] + (8.f + kLift), grow1 = mx[1] > m[1] + (8.f + kLift);
                 if (__any_sync(0xffffffffu, grow0 || grow1)) {
-                    const float f0 = grow0 ? tc::fast_exp2(m[0] - mx[0]) : 1.f, f1 = grow1 ? tc::fast_exp2(m[1] - mx[1]) : 1.f;
-                    if (grow0) m[0] = mx[0];
-                    if (grow1) m[1] = mx[1];
+                    const float m0 = mx[0] - kLift, m1 = mx[1] - kLift, f0 = grow0 ? tc::fast_exp2(m[0] - m0) : 1.f, f1 = grow1 ? tc::fast_exp2(m[1] - m1) : 1.f;
+                    if (grow0) m[0] = m0;
+                    if (grow1) m[1] = m1;
                     l[0] *= f0;
                     l[1] *= f1;
 #pragma unroll
@@ -425,7 +426,8 @@ __device__ __forceinline__ void split_body(const CUtensorMap& tm_k, const CUtens
                 }
                 const uint32_t vrow = vbase + (key0 + ((lane >> 3) & 1) * 8 + (lane & 7)) * 128;
                 if constexpr (RES) {
-                    // P in as many parts as hold its 24 bits. A matrix instruction cuts its sum off instead of rounding it, which makes long sums
+                    // P in three parts of bf16, which hold its 24 bits, or two of fp16, which hold 23 of a lifted p above 2^-2 (p above 2^-9 of the
+                    // running maximum) and 2^-32 of that maximum below. A matrix instruction cuts its sum off instead of rounding it, which makes long sums
                     // small (4e-6 of them after 440 instructions): each starts from zero here and is added to the rest by an addition.
                     constexpr int kTerms = BF16 ? 3 : 2;
                     uint32_t pa[NB][kTerms][4];
@@ -511,7 +513,7 @@ __device__ __forceinline__ void split_body(const CUtensorMap& tm_k, const CUtens
 #pragma unroll
                         for (int i = 0; i < D / 8; ++i)
                             *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[i][2 * half] * inv, o[i][2 * half + 1] * inv);
-                        if ((lane & 3) == 0) pl[rec * sh.rec_rows + r] = sum > 0.f ? m[half] + __log2f(sum) : -INFINITY;
+                        if ((lane & 3) == 0) pl[rec * sh.rec_rows + r] = sum > 0.f ? (m[half] + tc::kLift<BF16>) + __log2f(sum * tc::kUnlift<BF16>) : -INFINITY;
                     }
                 }
                 fresh = true;

@@ -222,6 +222,15 @@ __device__ __forceinline__ float fast_exp2(float x) {
     return y;
 }
 
+// Probabilities relative to a running maximum that lags by up to 2^8 are at most 2^8. In fp16, whose range ends at 2^16, they are lifted by 2^7: its
+// smallest spacing, 2^-24, is then 2^-31 of a probability, where 2^-24 lost those below e^-17 and most bits of those below e^-8. bf16 has
+// fp32's range. The lift comes off what the exponents are relative to, which is rounded once and the same everywhere. Its exponent, and the factor
+// that takes it out of a sum again:
+template <bool BF16>
+constexpr float kLift = BF16 ? 0.f : 7.f;
+template <bool BF16>
+constexpr float kUnlift = BF16 ? 1.f : 0.0078125f;
+
 // Two fp32 operations per instruction.
 using f32x2 = unsigned long long;
 __device__ __forceinline__ f32x2 pack_f32x2(float a, float b) {
