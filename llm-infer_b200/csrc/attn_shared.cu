@@ -145,14 +145,14 @@ __global__ void __launch_bounds__(kThreads, !SCORED ? 1 : SLICE < D ? 8 : 6) sha
         }
         if constexpr (WARP_ROWS) {
             if (lane < kLanes) {
-                const float inv = l > 0.f ? 1.f / l : 0.f;
+                const float inv = l == 0.f ? 0.f : 1.f / l;  // no row at all: zeros; NaN stays NaN
                 const size_t at = static_cast<size_t>(row) * D + lane * 4;
                 acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
                 if (p.o_dtype == ATTN_DTYPE_F32) *reinterpret_cast<float4*>(static_cast<float*>(p.o) + at) = acc;
                 else if (p.o_dtype == ATTN_DTYPE_F16) *reinterpret_cast<uint2*>(static_cast<__half*>(p.o) + at) = make_uint2(pack2<false>(acc.x, acc.y), pack2<false>(acc.z, acc.w));
                 else *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.o) + at) = make_uint2(pack2<true>(acc.x, acc.y), pack2<true>(acc.z, acc.w));
             }
-            if (lane == 0 && p.lse) p.lse[row] = l > 0.f ? (m + __log2f(l)) * 0.69314718055994531f : -INFINITY;
+            if (lane == 0 && p.lse) p.lse[row] = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
             return;
         }
         if (lane < kLanes) *reinterpret_cast<float4*>(&s_o[warp][lane * 4]) = acc;
@@ -171,12 +171,12 @@ __global__ void __launch_bounds__(kThreads, !SCORED ? 1 : SLICE < D ? 8 : 6) sha
                 sum += f * s_ml[w][1];
                 val += f * s_o[w][tid];
             }
-            val = sum > 0.f ? val / sum : 0.f;
+            val = sum == 0.f ? 0.f : val / sum;
             const size_t at = static_cast<size_t>(row) * D + slice * SLICE + tid;
             if (p.o_dtype == ATTN_DTYPE_F32) static_cast<float*>(p.o)[at] = val;
             else if (p.o_dtype == ATTN_DTYPE_F16) static_cast<__half*>(p.o)[at] = __float2half_rn(val);
             else static_cast<__nv_bfloat16*>(p.o)[at] = __float2bfloat16_rn(val);
-            if (tid == 0 && slice == 0 && p.lse) p.lse[row] = sum > 0.f ? (mm + __log2f(sum)) * 0.69314718055994531f : -INFINITY;
+            if (tid == 0 && slice == 0 && p.lse) p.lse[row] = sum == 0.f ? -INFINITY : (mm + __log2f(sum)) * 0.69314718055994531f;
         }
         return;
     }

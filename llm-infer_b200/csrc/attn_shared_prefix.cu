@@ -345,9 +345,9 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                 // ---- the piece: O / l and log-sum-exp (log2 units)
                 l += exchange(g0 & 1, l);
                 named_bar_sync(4, 256);  // (the exchanged values have been read)
-                const float inv = l > 0.f ? 1.f / l : 0.f;
+                const float inv = l == 0.f ? 0.f : 1.f / l;  // (a sum of NaN stays one)
                 const uint32_t rec_row = (blockIdx.x + w.seg) * kRows;
-                if (t == 0 && w.m0 + r < query_rows) p.lse[rec_row + r] = l > 0.f ? (m_used + kLift<BF16>) + __log2f(l * kUnlift<BF16>) : -INFINITY;
+                if (t == 0 && w.m0 + r < query_rows) p.lse[rec_row + r] = l == 0.f ? -INFINITY : (m_used + kLift<BF16>) + __log2f(l * kUnlift<BF16>);
                 // through shared memory and the TMA engine, 32 columns at a time: the second query tile and the staging tiles are free
 #pragma unroll
                 for (int pass = 0; pass < kCols / 32; ++pass) {
@@ -470,9 +470,9 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                 break;
             }
             fence_after();
-            const float inv = l > 0.f ? 1.f / l : 0.f;
+            const float inv = l == 0.f ? 0.f : 1.f / l;  // (a sum of NaN stays one)
             const uint32_t rec_row = (blockIdx.x + w.seg) * kRows + t * BM;
-            if (m < query_rows) p.lse[rec_row + r] = l > 0.f ? (m_used + kLift<BF16>) + __log2f(l * kUnlift<BF16>) : -INFINITY;
+            if (m < query_rows) p.lse[rec_row + r] = l == 0.f ? -INFINITY : (m_used + kLift<BF16>) + __log2f(l * kUnlift<BF16>);
             // The tile leaves through shared memory and the TMA engine, 128 bytes of every row at a time: the query tile, which nothing
             // reads any more, holds the first two passes, the staging tile the third, so that only the fourth waits for a store. (Each pass
             // behind the previous one's store in a single staging tile: 3 us more per piece.)

@@ -505,7 +505,7 @@ __device__ __forceinline__ void split_body(const CUtensorMap& tm_k, const CUtens
                     float sum = l[half];
                     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+                    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // (a sum of NaN stays one)
                     const uint32_t r = wr * 16 + half * 8 + lane / 4;
                     const bool there = cur.own ? r < p.group : cur.rb * sh.wm * 16 + r < p.batch * p.group;
                     if (there) {
@@ -513,7 +513,7 @@ __device__ __forceinline__ void split_body(const CUtensorMap& tm_k, const CUtens
 #pragma unroll
                         for (int i = 0; i < D / 8; ++i)
                             *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[i][2 * half] * inv, o[i][2 * half + 1] * inv);
-                        if ((lane & 3) == 0) pl[rec * sh.rec_rows + r] = sum > 0.f ? (m[half] + tc::kLift<BF16>) + __log2f(sum * tc::kUnlift<BF16>) : -INFINITY;
+                        if ((lane & 3) == 0) pl[rec * sh.rec_rows + r] = sum == 0.f ? -INFINITY : (m[half] + tc::kLift<BF16>) + __log2f(sum * tc::kUnlift<BF16>);
                     }
                 }
                 fresh = true;
