@@ -550,7 +550,7 @@ int attn_decode_shared(const AttnDecodeSharedArgs* args, void* stream);
  * stay: the first `sink`, the last `recent`, and of the others those with the largest scores, `keep` in all; among equal scores the
  * lowest rows (NaN counts as less than any number). Kept rows keep their order and move to rows 0, 1, ...; shorter sequences keep
  * all. Into other caches, or in place when k_out == k, v_out == v and scores_out == scores (same strides, out_rows == rows);
- * any other overlap is refused. */
+ * any other operands that share a byte are refused, and operands of different strides whose extents overlap. */
 typedef struct AttnKvEvictArgs {
     const void* k;        /* in : 16-bit caches of any type, sequence b at + b*kv_batch_stride, row t at + t*kv_row_stride */
     const void* v;

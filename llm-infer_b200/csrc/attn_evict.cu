@@ -436,10 +436,47 @@ __global__ void __launch_bounds__(kMoveThreads) evict_compact_kernel(const __gri
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// Whether two regions of `an` and `bn` bytes share a byte.
-bool overlap(const void* a, uint64_t an, const void* b, uint64_t bn) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return x < y + bn && y < x + an;
+// n1 runs, s1 bytes apart, of n2 runs, s2 bytes apart, of `width` bytes each.
+struct Runs {
+    const void* base;
+    uint64_t n1, s1, n2, s2, width;
+};
+using wide = __int128;  // (strides are the caller's and unchecked)
+wide floor_div(wide a, wide b) { return a / b - (a % b < 0 ? 1 : 0); }
+// Whether two operands share a byte: exactly where their strides are the same (interleaved halves, layers, K and V of one buffer do
+// not), by the whole extent of the levels whose strides differ otherwise.
+bool share_memory(Runs a, Runs b) {
+    const wide apart = static_cast<wide>(reinterpret_cast<uintptr_t>(b.base)) - static_cast<wide>(reinterpret_cast<uintptr_t>(a.base));
+    auto extent = [](const Runs& x) { return static_cast<wide>(x.n1 - 1) * x.s1 + static_cast<wide>(x.n2 - 1) * x.s2 + x.width; };
+    if (apart >= extent(a) || -apart >= extent(b)) return false;
+    if (a.n1 == 1) a.s1 = b.s1;  // a level of one run has any stride
+    if (b.n1 == 1) b.s1 = a.s1;
+    if (a.n2 == 1) a.s2 = b.s2;
+    if (b.n2 == 1) b.s2 = a.s2;
+    if (a.s1 != b.s1) return true;
+    wide aw = a.width, bw = b.width;
+    if (a.s2 != b.s2) {
+        aw += static_cast<wide>(a.n2 - 1) * a.s2;
+        bw += static_cast<wide>(b.n2 - 1) * b.s2;
+        a.n2 = b.n2 = 1;
+    }
+    // Some run of a, i1 and i2, and some of b, j1 and j2: apart + (j1 - i1) s1 + (j2 - i2) s2 in (-bw, aw)?
+    auto steps = [](wide low, wide high, wide stride, uint64_t an, uint64_t bn, wide* first, wide* last) {  // j - i with low < (j - i) stride < high
+        *first = -static_cast<wide>(an - 1);
+        *last = bn - 1;
+        if (stride == 0) return;
+        *first = std::max(*first, floor_div(low, stride) + 1);
+        *last = std::min(*last, -floor_div(-high, stride) - 1);
+    };
+    wide f1, l1, f2, l2;
+    steps(-bw - static_cast<wide>(b.n2 - 1) * b.s2 - apart, aw + static_cast<wide>(a.n2 - 1) * a.s2 - apart, a.s1, a.n1, b.n1, &f1, &l1);
+    if (l1 - f1 > 64) return true;  // (not looked at one by one)
+    for (wide k = f1; k <= l1; ++k) {
+        const wide at = apart + k * a.s1;
+        steps(-bw - at, aw - at, a.s2, a.n2, b.n2, &f2, &l2);
+        if (f2 <= l2 && (a.s2 != 0 || (at > -bw && at < aw))) return true;
+    }
+    return false;
 }
 
 }  // namespace
@@ -466,7 +503,10 @@ extern "C" int attn_kv_evict(const AttnKvEvictArgs* a, void* stream_v) {
     p.score_out_stride = a->score_out_stride ? a->score_out_stride : a->out_rows;
     if (p.row_stride < width || p.out_row_stride < width || p.score_stride < a->rows || p.score_out_stride < a->out_rows)
         return ATTN_ERR_INVALID_ARG;
-    if (a->batch > 1 && (p.batch_stride == 0 || p.out_batch_stride < (a->out_rows - 1) * p.out_row_stride + width)) return ATTN_ERR_INVALID_ARG;
+    // output sequences must not share memory: one behind the other, or row by row beside each other
+    if (a->batch > 1 && (p.batch_stride == 0 || (p.out_batch_stride < (a->out_rows - 1) * p.out_row_stride + width &&
+                                                 (p.out_batch_stride < width || p.out_row_stride < (a->batch - 1) * p.out_batch_stride + width))))
+        return ATTN_ERR_INVALID_ARG;
     if (!aligned16(a->k) || !aligned16(a->v) || !aligned16(a->k_out) || !aligned16(a->v_out) ||
         (p.row_stride | p.batch_stride | p.out_row_stride | p.out_batch_stride) % 8 != 0)
         return ATTN_ERR_ALIGNMENT;
@@ -478,12 +518,11 @@ extern "C" int attn_kv_evict(const AttnKvEvictArgs* a, void* stream_v) {
             a->out_rows != a->rows)
             return ATTN_ERR_INVALID_ARG;
     } else {
-        const uint64_t in_bytes = 2 * ((a->batch - 1) * p.batch_stride + (a->rows - 1) * p.row_stride + width);
-        const uint64_t out_bytes = 2 * ((a->batch - 1) * p.out_batch_stride + (a->out_rows - 1) * p.out_row_stride + width);
-        const uint64_t s_in = 4 * ((segments - 1) * p.score_stride + a->rows), s_out = 4 * ((segments - 1) * p.score_out_stride + a->out_rows);
-        if (overlap(a->k, in_bytes, a->k_out, out_bytes) || overlap(a->v, in_bytes, a->v_out, out_bytes) ||
-            overlap(a->k, in_bytes, a->v_out, out_bytes) || overlap(a->v, in_bytes, a->k_out, out_bytes) ||
-            overlap(a->scores, s_in, a->scores_out, s_out))
+        auto in = [&](const void* base) { return Runs{base, a->batch, 2 * p.batch_stride, a->rows, 2 * p.row_stride, 2 * width}; };
+        auto out = [&](const void* base) { return Runs{base, a->batch, 2 * p.out_batch_stride, a->out_rows, 2 * p.out_row_stride, 2 * width}; };
+        if (share_memory(in(a->k), out(a->k_out)) || share_memory(in(a->v), out(a->v_out)) || share_memory(in(a->k), out(a->v_out)) ||
+            share_memory(in(a->v), out(a->k_out)) ||
+            share_memory({a->scores, segments, 4 * p.score_stride, 1, 0, 4ull * a->rows}, {a->scores_out, segments, 4 * p.score_out_stride, 1, 0, 4ull * a->out_rows}))
             return ATTN_ERR_INVALID_ARG;
     }
     DeviceInfo dev{};
