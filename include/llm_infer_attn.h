@@ -549,8 +549,9 @@ int attn_decode_shared(const AttnDecodeSharedArgs* args, void* stream);
 /* Eviction from the caches by accumulated attention weight. Of every (sequence, kv head) with more than `keep` rows these
  * stay: the first `sink`, the last `recent`, and of the others those with the largest scores, `keep` in all; among equal scores the
  * lowest rows (NaN counts as less than any number). Kept rows keep their order and move to rows 0, 1, ...; shorter sequences keep
- * all. Into other caches, or in place when k_out == k, v_out == v and scores_out == scores (same strides, out_rows == rows);
- * any other operands that share a byte are refused, and operands of different strides whose extents overlap. */
+ * all. Into other caches, or in place when k_out == k, v_out == v and scores_out == scores (same strides, out_rows == rows).
+ * Anything else that is written and shares a byte with an input or another output is refused (of different strides: whose extent does), but for
+ * kv_len_out == kv_len. */
 typedef struct AttnKvEvictArgs {
     const void* k;        /* in : 16-bit caches of any type, sequence b at + b*kv_batch_stride, row t at + t*kv_row_stride */
     const void* v;

@@ -436,19 +436,21 @@ __global__ void __launch_bounds__(kMoveThreads) evict_compact_kernel(const __gri
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+using wide = __int128;  // (strides are the caller's and unchecked)
 // n1 runs, s1 bytes apart, of n2 runs, s2 bytes apart, of `width` bytes each.
 struct Runs {
-    const void* base;
+    wide base;
     uint64_t n1, s1, n2, s2, width;
+    wide extent;
+    Runs(const void* p, uint64_t n1, uint64_t s1, uint64_t n2, uint64_t s2, uint64_t width)
+        : base(reinterpret_cast<uintptr_t>(p)), n1(n1), s1(s1), n2(n2), s2(s2), width(width),
+          extent(static_cast<wide>(n1 - 1) * s1 + static_cast<wide>(n2 - 1) * s2 + width) {}
 };
-using wide = __int128;  // (strides are the caller's and unchecked)
 wide floor_div(wide a, wide b) { return a / b - (a % b < 0 ? 1 : 0); }
 // Whether two operands share a byte: exactly where their strides are the same (interleaved halves, layers, K and V of one buffer do
 // not), by the whole extent of the levels whose strides differ otherwise.
-bool share_memory(Runs a, Runs b) {
-    const wide apart = static_cast<wide>(reinterpret_cast<uintptr_t>(b.base)) - static_cast<wide>(reinterpret_cast<uintptr_t>(a.base));
-    auto extent = [](const Runs& x) { return static_cast<wide>(x.n1 - 1) * x.s1 + static_cast<wide>(x.n2 - 1) * x.s2 + x.width; };
-    if (apart >= extent(a) || -apart >= extent(b)) return false;
+bool share_bytes(Runs a, Runs b) {
+    const wide apart = b.base - a.base;
     if (a.n1 == 1) a.s1 = b.s1;  // a level of one run has any stride
     if (b.n1 == 1) b.s1 = a.s1;
     if (a.n2 == 1) a.s2 = b.s2;
@@ -478,6 +480,7 @@ bool share_memory(Runs a, Runs b) {
     }
     return false;
 }
+bool share_memory(const Runs& a, const Runs& b) { return a.base < b.base + b.extent && b.base < a.base + a.extent && share_bytes(a, b); }
 
 }  // namespace
 }  // namespace b200
@@ -510,20 +513,27 @@ extern "C" int attn_kv_evict(const AttnKvEvictArgs* a, void* stream_v) {
     if (!aligned16(a->k) || !aligned16(a->v) || !aligned16(a->k_out) || !aligned16(a->v_out) ||
         (p.row_stride | p.batch_stride | p.out_row_stride | p.out_batch_stride) % 8 != 0)
         return ATTN_ERR_ALIGNMENT;
-    // In place means all three: the same caches with the same strides, and the same scores. Any other overlap would be read
-    // after it was overwritten.
+    // In place means all three: the same caches with the same strides, and the same scores. Anything else that is written must share no
+    // memory with what is read or with what else is written, but for new lengths in the place of the old ones: the CTAs run in any order.
     p.in_place = a->k == a->k_out && a->v == a->v_out && a->scores == a->scores_out;
     if (p.in_place) {
         if (p.row_stride != p.out_row_stride || p.batch_stride != p.out_batch_stride || p.score_stride != p.score_out_stride ||
             a->out_rows != a->rows)
             return ATTN_ERR_INVALID_ARG;
-    } else {
-        auto in = [&](const void* base) { return Runs{base, a->batch, 2 * p.batch_stride, a->rows, 2 * p.row_stride, 2 * width}; };
-        auto out = [&](const void* base) { return Runs{base, a->batch, 2 * p.out_batch_stride, a->out_rows, 2 * p.out_row_stride, 2 * width}; };
-        if (share_memory(in(a->k), out(a->k_out)) || share_memory(in(a->v), out(a->v_out)) || share_memory(in(a->k), out(a->v_out)) ||
-            share_memory(in(a->v), out(a->k_out)) ||
-            share_memory({a->scores, segments, 4 * p.score_stride, 1, 0, 4ull * a->rows}, {a->scores_out, segments, 4 * p.score_out_stride, 1, 0, 4ull * a->out_rows}))
-            return ATTN_ERR_INVALID_ARG;
+    }
+    auto in = [&](const void* base) { return Runs{base, a->batch, 2 * p.batch_stride, a->rows, 2 * p.row_stride, 2 * width}; };
+    auto out = [&](const void* base) { return Runs{base, a->batch, 2 * p.out_batch_stride, a->out_rows, 2 * p.out_row_stride, 2 * width}; };
+    auto dense = [&](const void* base, uint64_t words) { return Runs{base, 1, 0, 1, 0, 4 * words}; };
+    const Runs read[] = {in(a->k), in(a->v), {a->scores, segments, 4 * p.score_stride, 1, 0, 4ull * a->rows}, dense(a->kv_len, a->batch)};
+    const Runs written[] = {out(a->k_out), out(a->v_out), {a->scores_out, segments, 4 * p.score_out_stride, 1, 0, 4ull * a->out_rows},
+                            dense(a->kept, segments * a->keep), dense(a->kv_len_out, a->batch)};
+    for (int i = 0; i < 5; ++i) {
+        for (int j = 0; j < (a->kv_len ? 4 : 3); ++j) {
+            const bool in_its_place = (p.in_place && i == j) || (i == 4 && j == 3 && a->kv_len_out == a->kv_len);
+            if (!in_its_place && share_memory(read[j], written[i])) return ATTN_ERR_INVALID_ARG;
+        }
+        for (int j = 0; j < i; ++j)
+            if (share_memory(written[j], written[i])) return ATTN_ERR_INVALID_ARG;
     }
     DeviceInfo dev{};
     const int rc = current_device_info(&dev);

@@ -61,9 +61,41 @@ def test_caches_are_refused_exactly_when_they_share_bytes(built_lib, pkg, seed):
 
 @no_device
 def test_scores_of_one_buffer_may_interleave(built_lib, pkg):
-    b, at = pkg.binding, 9 << 20
+    b, at = pkg.binding, 19 << 20
     both = dict(score_stride=10, score_out_stride=10)
     assert _code(built_lib, _args(b, scores=at, scores_out=at + 4 * 6, **both)) != INVALID
     assert _code(built_lib, _args(b, scores=at, scores_out=at + 4 * 5, **both)) == INVALID
     assert _code(built_lib, _args(b, scores=at, scores_out=at + 4 * 7, **both)) == INVALID  # its fourth column is the next run's first
     assert _code(built_lib, _args(b, scores=at + 4 * 4, scores_out=at, **both)) != INVALID
+
+
+@no_device
+def test_outputs_may_not_share_memory_with_each_other_or_with_what_is_read(built_lib, pkg):
+    """A CTA would read or write what another one writes."""
+    b = pkg.binding
+    cache, scores, kept, lens = 2 * 4 * 16 * 2, 2 * 2 * 4 * 4, 2 * 2 * 4 * 4, 2 * 4  # bytes of the outputs
+    assert _code(built_lib, _args(b)) != INVALID
+    at = lambda name: (NAMES.index(name) + 1) << 20  # noqa: E731
+    sizes = dict(k=2 * 6 * 16 * 2, v=2 * 6 * 16 * 2, scores=2 * 2 * 6 * 4, kv_len=lens, k_out=cache, v_out=cache, scores_out=scores, kept=kept, kv_len_out=lens)
+    written = ["k_out", "v_out", "scores_out", "kept", "kv_len_out"]
+    for i, x in enumerate(written):
+        step = 16 if x in ("k_out", "v_out") else 4
+        for y in ["k", "v", "scores", "kv_len"] + written[:i]:
+            other = at(y) - at(y) % 16
+            for where in (other - sizes[x] + step, other, -(-(other + sizes[y] - step) // step) * step):
+                if (x, y) == ("kv_len_out", "kv_len") and where == other:
+                    continue  # the new lengths may take the old ones' place
+                assert _code(built_lib, _args(b, **{x: where})) == INVALID, (x, y, where - other)
+            assert _code(built_lib, _args(b, **{x: other + (sizes[y] + 15) // 16 * 16})) != INVALID, (x, y)
+    assert _code(built_lib, _args(b, kv_len_out=at("kv_len"))) != INVALID
+
+
+@no_device
+def test_keys_that_are_their_own_values_cannot_be_compacted_in_place(built_lib, pkg):
+    """k == v in place: two CTAs would move the same rows."""
+    b, at = pkg.binding, 1 << 20
+    place = dict(rows=6, out_rows=6, kv_batch_stride=6 * 16, out_batch_stride=6 * 16, scores=9 << 20, scores_out=9 << 20)
+    names = dict(kept=11 << 20, kv_len=12 << 20, kv_len_out=13 << 20)
+    assert _code(built_lib, _args(b, k=at, v=at, k_out=at, v_out=at, **place, **names)) == INVALID
+    assert _code(built_lib, _args(b, k=at, v=2 << 20, k_out=at, v_out=2 << 20, **place, **names)) != INVALID
+    assert _code(built_lib, _args(b, k=at, v=at)) != INVALID  # read twice, written apart
