@@ -476,11 +476,22 @@ class Llama:
         q16 = torch.empty((B, c.n_heads, c.head_dim), dtype=torch.float16, device=dev)
         att = torch.empty((B, c.n_heads, c.head_dim), dtype=torch.float32, device=dev)
 
+        # The capacity that a call states chooses its kernels and the order of its sums. It follows the rows that the step's caches hold, in
+        # powers of two (the choice takes lengths to lie in the upper part of the capacity), and so not the number of tokens asked for.
+        limit = c.max_seq_len if budget <= 0 else min(c.max_seq_len, budget + evict_every)
+        seen = []  # each layer's rows and weights as the step's calls see them
+
+        def look(longest_cache):
+            n = min(limit, max(64, 1 << (longest_cache - 1).bit_length()))
+            if not seen or seen[0][0].shape[1] != n:
+                seen[:] = [(self.k_cache[l, :, :n], self.v_cache[l, :, :n], None if scores is None else scores[l, :, :, :n])
+                           for l in range(c.n_layers)]
+
         def attend(l):
             X.rope_positions(self.q, self.k, self.v, kc[l], vc[l], self.pos, self.kv_pos, inv_freq=self._inv_freq,
                              factor=self._rope_factor, layout=self._rope_layout, q_out=q16, status=self.status)
-            return X.attn_decode_shared(q16, kp[l], vp[l], kc[l], vc[l], self.kv_len, out=att,
-                                        scores=None if scores is None else scores[l], workspace=workspace)
+            k, v, weights = seen[l]
+            return X.attn_decode_shared(q16, kp[l], vp[l], k, v, self.kv_len, out=att, scores=weights, workspace=workspace)
 
         delay = [longest - len(p) for p in prompts]  # sequences start late, so that all prompts end at the same step
         held = [0] * B                               # rows of each cache
@@ -500,6 +511,7 @@ class Llama:
             positions = torch.tensor([[P + a for a in at], held, [n + 1 for n in held]], dtype=torch.int32).pin_memory()
             self._positions.copy_(positions, non_blocking=True)
             held = [n + 1 for n in held]
+            look(max(held))
             if step < longest:
                 self.tokens.copy_(torch.tensor([p[a] for p, a in zip(prompts, at)], dtype=torch.int32).pin_memory(), non_blocking=True)
             self._launch_step(0, step + 1 >= longest, attend)
