@@ -107,6 +107,7 @@ class Llama:
         self._own_rope = rope_layout != "interleaved" or rope_scaling is not None
         if self._own_rope and c.qkv_clip > 0:
             raise ValueError("scaled or half-paired positions have no clamp of q, k and v in the prompt phase")
+        self._shared_rope = not c.qkv_clip > 0  # (rope_positions does not clamp)
         q8 = weight_type == "q8_0"
         self._gemv = A.gemv_q8_0 if q8 else A.gemv_f16
         self._embed = A.embed_q8_0 if q8 else A.embed_f16
@@ -276,7 +277,7 @@ class Llama:
         if len(prompts) != self.batch or not self.can_prefill(prompts):
             raise ValueError("prefill() needs one prompt per sequence, head_dim 64 or 128 and prompts that fit the cache")
         w, c = self.w, self.cfg
-        x, last_rows = self._prompt_rows(prompts, self.k_cache, self.v_cache, exact)
+        x, last_rows = self._prompt_rows(prompts, self.k_cache, self.v_cache, exact, self._own_rope)
         # the last token of every prompt: final norm, classifier, greedy pick (the decode step's own kernels)
         A.gather_rows(x, last_rows, out=self.x)
         A.rmsnorm(self.x, w["rms_final"], c.norm_eps, out=self.xb)
@@ -284,9 +285,10 @@ class Llama:
         A.argmax(self.logits, out=self.next_token)
         self.tokens.copy_(self.next_token)
 
-    def _prompt_rows(self, prompts, k_cache: torch.Tensor, v_cache: torch.Tensor, exact: bool):
+    def _prompt_rows(self, prompts, k_cache: torch.Tensor, v_cache: torch.Tensor, exact: bool, own_rope: bool):
         """All layers over the tokens of ``prompts``, whose keys and values go into rows 0, 1, ... of k_cache, v_cache [layers,
-        len(prompts), rows, Hkv, D]. Returns the tokens' last hidden rows and the row of each prompt's last token."""
+        len(prompts), rows, Hkv, D]; with ``own_rope`` turned by context.rope_positions, else by the engine's kernel. Returns the
+        tokens' last hidden rows and the row of each prompt's last token."""
         import numpy as np
         c, w, B, dev = self.cfg, self.w, len(prompts), self.device
         q8 = self.weight_type == "q8_0"
@@ -334,7 +336,7 @@ class Llama:
         for l in range(c.n_layers):
             A.rmsnorm_pair(x, w["rms_att"][l], c.norm_eps, out=pair_d)
             project(pair_d, w["wqkv"][l], qkv)
-            if self._own_rope:
+            if own_rope:
                 heads = qkv.view(T, H + 2 * c.n_kv_heads, D)
                 X.rope_positions(heads[:, :H], heads[:, H:H + c.n_kv_heads], heads[:, H + c.n_kv_heads:], k_cache[l], v_cache[l],
                                  token_pos, token_pos, seq=token_seq, inv_freq=self._inv_freq, factor=self._rope_factor,
@@ -442,20 +444,22 @@ class Llama:
 
     def encode_prefix(self, tokens, exact: bool = True):
         """Keys and values of a prefix that sequences will share: (k, v) fp16 [layers, P, Hkv, D], computed once by the prompt
-        phase (prefill)."""
+        phase (prefill), with the angles of generate_shared."""
         c = self.cfg
         P = len(tokens)
         if not self.can_prefill([tokens[:1]]) or P == 0:
             raise ValueError("a prefix needs at least one token and a model that prefill() takes")
         k = torch.empty((c.n_layers, 1, P, c.n_kv_heads, c.head_dim), dtype=torch.float16, device=self.device)
         v = torch.empty_like(k)
-        self._prompt_rows([list(tokens)], k, v, exact)
+        self._prompt_rows([list(tokens)], k, v, exact, self._shared_rope)
         return k[:, 0], v[:, 0]
 
     def generate_shared(self, prefix, prompts, n_new: int, *, budget: int = 0, sink: int = KV_SINK, recent: int = 0,
                         evict_every: int = 32, want_logits: bool = False):
         """Greedy generation of a ragged batch behind a shared prefix: what generate() gives for prefix + prompt of every sequence, with
-        the prefix computed and kept once. ``prefix`` is a list of token ids or what encode_prefix() returned for one. The own caches
+        the prefix computed and kept once. Two roundings differ: queries enter the attention as fp16, and the angles of all rows are
+        context.rope_positions' (the engine's, whose products are rounded to fp32, are off by 4e-3 at position 100000) unless the model
+        clamps q, k and v, which the prompt phase does in the engine's kernel. ``prefix`` is a list of token ids or what encode_prefix() returned for one. The own caches
         hold the prompts' and the generated tokens' rows only; the prompts are fed one token per step.
         ``budget`` > 0 bounds them: whenever a cache holds budget + evict_every rows, every layer and kv head keeps budget of them -
         the first ``sink``, the last ``recent`` (0: half of the budget) and those that received the most attention weight so far
@@ -488,8 +492,12 @@ class Llama:
                            for l in range(c.n_layers)]
 
         def attend(l):
-            X.rope_positions(self.q, self.k, self.v, kc[l], vc[l], self.pos, self.kv_pos, inv_freq=self._inv_freq,
-                             factor=self._rope_factor, layout=self._rope_layout, q_out=q16, status=self.status)
+            if self._shared_rope:
+                X.rope_positions(self.q, self.k, self.v, kc[l], vc[l], self.pos, self.kv_pos, inv_freq=self._inv_freq,
+                                 factor=self._rope_factor, layout=self._rope_layout, q_out=q16, status=self.status)
+            else:
+                A.rope_kv_insert(self.q, self.k, self.v, kc[l], vc[l], self.pos, self.kv_pos, theta=c.rope_theta, rotary_dim=c.rotary_dim,
+                                 q_out=q16)
             k, v, weights = seen[l]
             return X.attn_decode_shared(q16, kp[l], vp[l], k, v, self.kv_len, out=att, scores=weights, workspace=workspace)
 

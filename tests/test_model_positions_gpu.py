@@ -1,4 +1,4 @@
-"""Generation behind a shared prefix: what its results must not depend on."""
+"""Generation behind a shared prefix: what its results must not depend on, and the angles of its rows."""
 import numpy as np
 import pytest
 import torch
@@ -32,3 +32,48 @@ def test_results_do_not_depend_on_how_many_tokens_are_asked_for(M, P, B, n_heads
     for n in (1, 3, 12, 50):
         few, few_logits = llama.generate_shared(prefix, prompts, n, **kw)
         assert torch.equal(few, tokens[:, :n]) and torch.equal(few_logits, logits[:, :n])
+
+
+@pytest.mark.parametrize("scaling", [None, {"type": "linear", "factor": 4.0}])
+def test_keys_of_a_long_prefix_are_turned_by_the_angles_of_the_own_rows(M, scaling):
+    """Late positions of layer 0 against 64-bit angles: fp16 rounding of the keys (2^-11) and what the projection's sums of 512 products may
+    be off by, 64 instructions that cut off 2^-23 of the products' magnitudes each. An angle whose product was rounded to fp32 is off
+    by up to 2^-8 here."""
+    cfg = _config(M, n_layers=1)
+    w = M.random_weights(cfg, 9)
+    from llm_infer_b200 import context
+    P = 65536 + 3
+    tokens = np.random.default_rng(3).integers(0, cfg.vocab_size, P)
+    llama = M.Llama(cfg, w, batch=1, rope_scaling=scaling)
+    k, _ = llama.encode_prefix(tokens.tolist())
+    f, factor = context.rope_frequencies(cfg.head_dim, cfg.rope_theta, scaling)
+    at = torch.arange(P - 2000, P)
+    x = w["embed"].cpu().double()[torch.from_numpy(tokens)[at]]
+    x = x / torch.sqrt((x * x).mean(1, keepdim=True) + cfg.norm_eps) * w["rms_att"][0].cpu().double()
+    wk = w["wk"][0].cpu().double().T
+    y, size = ((p @ q).view(len(at), cfg.n_kv_heads, cfg.head_dim // 2, 2) for p, q in ((x, wk), (x.abs(), wk.abs())))
+    a = at.double()[:, None] * f.double()[None]
+    c, s = (torch.cos(a) * factor)[:, None], (torch.sin(a) * factor)[:, None]
+    want = torch.stack([y[..., 0] * c - y[..., 1] * s, y[..., 0] * s + y[..., 1] * c], -1)
+    size = size.sum(-1, keepdim=True) * factor
+    got = k[0, at.to(k.device)].double().cpu().view(want.shape)
+    assert bool(((got - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -17 * size).all())
+
+
+def test_models_that_clamp_q_k_and_v_agree_with_the_ordinary_path(M):
+    cfg = _config(M, qkv_clip=0.75)
+    w = M.random_weights(cfg, 4)
+    rng = np.random.default_rng(8)
+    prefix = rng.integers(0, cfg.vocab_size, 40).tolist()
+    prompts = [rng.integers(0, cfg.vocab_size, 6).tolist() for _ in range(2)]
+    llama = M.Llama(cfg, w, batch=2)
+    tokens, logits = llama.generate_shared(prefix, prompts, 5, want_logits=True)
+    want_tokens, want = llama.generate([prefix + p for p in prompts], 5, want_logits=True)
+    for b in range(2):
+        for i in range(5):
+            bound = 2e-3 + 1e-2 * float(want[b, i].pow(2).mean().sqrt())
+            assert float((logits[b, i] - want[b, i]).abs().max()) <= bound
+            if int(tokens[b, i]) != int(want_tokens[b, i]):
+                top = torch.sort(want[b, i]).values
+                assert float(top[-1] - top[-2]) <= 2 * bound
+                break
