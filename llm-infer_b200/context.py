@@ -17,6 +17,7 @@ from . import binding as _b
 from .attention import _DTYPES, _dense, _dtype_code
 
 _LAYOUTS = {"interleaved": _b.ROPE_INTERLEAVED, "half": _b.ROPE_HALF}
+ROPE_LAYOUTS = tuple(sorted(_LAYOUTS))
 _INDEX = (torch.int32, torch.uint32)
 _CACHE = (torch.float16, torch.bfloat16)
 
@@ -161,7 +162,7 @@ def rope_positions(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
         raise ValueError("the caches must be [B, row, kv_head, head_dim] with dense heads and share their strides")
     row_stride = _row_stride(c_stride[1], T, Hkv * D, "the caches")
     if layout not in _LAYOUTS:
-        raise ValueError(f"layout must be one of {sorted(_LAYOUTS)}")
+        raise ValueError(f"layout must be one of {ROPE_LAYOUTS}")
     half = inv_freq.numel()
     if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or not 0 < 2 * half <= D:
         raise ValueError("inv_freq must be a dense fp32 tensor of rotary_dim / 2 values, rotary_dim <= head_dim")

@@ -20,6 +20,7 @@ import torch
 from . import attention as A
 from . import context as X
 
+_NO_SLIDE = "scaled or half-paired positions do not slide past max_seq_len"
 KV_SINK = 4  # attention-sink rows of the sliding window (include/model/model.hpp)
 
 
@@ -98,6 +99,8 @@ class Llama:
         self.cfg, self.batch, self.device = cfg, batch, dev
         c = cfg
         self.w = {}
+        if rope_layout not in X.ROPE_LAYOUTS:
+            raise ValueError(f"the rotary layout must be one of {X.ROPE_LAYOUTS}")
         if weight_type not in ("f16", "q8_0"):
             raise ValueError("weight_type must be 'f16' (the engine's) or 'q8_0'")
         self.weight_type = weight_type
@@ -195,6 +198,8 @@ class Llama:
         if any(over) and not all(over):
             raise ValueError("sequences inside and outside the sliding window cannot share a step")
         kv_sink = KV_SINK if all(over) and over else 0
+        if kv_sink and self._own_rope:
+            raise ValueError(_NO_SLIDE)
         kv_pos = [kv_sink + ((p - kv_sink) % (c.max_seq_len - kv_sink)) for p in pos]
         kv_len = [c.max_seq_len if p >= c.max_seq_len else p + 1 for p in pos]
         host = torch.tensor([pos, kv_pos, kv_len], dtype=torch.int32).pin_memory()
@@ -205,8 +210,6 @@ class Llama:
         """Positions, cache insert and attention of layer ``l`` over every sequence's own cache."""
         c = self.cfg
         if self._own_rope:
-            if kv_sink:
-                raise ValueError("scaled or half-paired positions do not slide past max_seq_len")
             X.rope_positions(self.q, self.k, self.v, self.k_cache[l], self.v_cache[l], self.pos, self.kv_pos, inv_freq=self._inv_freq,
                              factor=self._rope_factor, layout=self._rope_layout, q_out=self.q, status=self.status)
         else:
@@ -409,6 +412,8 @@ class Llama:
         longest = max(len(p) for p in prompts)
         if longest + n_new > self.cfg.max_seq_len and any(len(p) != longest for p in prompts):
             raise ValueError("only prompts of one length may run past max_seq_len (one sink setting per step)")
+        if self._own_rope and longest + n_new - 1 > self.cfg.max_seq_len:
+            raise ValueError(_NO_SLIDE)
         delay = [longest - len(p) for p in prompts]
         out = torch.zeros((B, n_new), dtype=torch.int32, device=self.device)
         out_logits = torch.zeros((B, n_new, self.cfg.vocab_size), device=self.device) if want_logits else None

@@ -1,4 +1,6 @@
 """Generation behind a shared prefix: what its results must not depend on, and the angles of its rows."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -77,3 +79,20 @@ def test_models_that_clamp_q_k_and_v_agree_with_the_ordinary_path(M):
                 top = torch.sort(want[b, i]).values
                 assert float(top[-1] - top[-2]) <= 2 * bound
                 break
+
+
+def test_scaled_positions_past_the_cache_are_refused_before_anything_runs(M):
+    cfg = _config(M)
+    w = M.random_weights(cfg, 5)
+    with pytest.raises(ValueError, match="layout"):
+        M.Llama(cfg, w, batch=1, rope_layout="halves")
+    for mode in ("token", "batched"):
+        llama = M.Llama(cfg, w, batch=1, rope_layout="half")
+        launches = M.X._b.load().attn_kernel_launch_count()
+        with pytest.raises(ValueError, match="slide"):
+            llama.generate([[1, 2, 3]], cfg.max_seq_len - 1, prompt_mode=mode)  # the last token's position is max_seq_len
+        with pytest.raises(ValueError, match="slide"):
+            llama.forward(torch.tensor([1], dtype=torch.int32), cfg.max_seq_len)
+        assert M.X._b.load().attn_kernel_launch_count() == launches
+    assert llama.generate([[1, 2, 3]], cfg.max_seq_len - 2, prompt_mode="token").shape == (1, cfg.max_seq_len - 2)
+    assert math.isfinite(float(llama.logits.sum()))
