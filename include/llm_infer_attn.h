@@ -486,7 +486,7 @@ typedef struct AttnRopePositionsArgs {
     void* k_cache;         /* kv_dtype, sequence s at + s*kv_batch_stride, row t at + t*kv_row_stride (elements) */
     void* v_cache;
     const float* inv_freq; /* device [rotary_dim/2]: radians per position of each pair, scaled as the model wants */
-    const uint32_t* pos;   /* device [tokens]: position (rotation angle) */
+    const uint32_t* pos;   /* device [tokens]: position (rotation angle), unsigned */
     const uint32_t* row;   /* device [tokens]: cache row; one that does not exist (>= cache_rows, or seq >= n_seqs) is not
                               written, and ATTN_STATUS_BAD_SHAPE is ORed into *status. No two tokens share a row. */
     const uint32_t* seq;   /* device [tokens]: sequence; NULL = token i belongs to sequence i */
@@ -507,8 +507,10 @@ int attn_rope_positions(const AttnRopePositionsArgs* args, void* stream);
 
 /* Single-token attention of a batch over a prefix that all sequences share (one copy of its K and V) and each sequence's
  * own rows: what attn_decode would give over caches that each hold the prefix's rows followed by the own ones, reading the
- * prefix once for the batch. With scores_out, the weight (softmax probability, summed over the query heads of a kv head) that
- * each own row received is added to an accumulator, which attn_kv_evict reads. No own rows and no prefix: zeros. */
+ * prefix once for the batch. (For outputs of dtype the probabilities are rounded once to dtype, where attn_decode carries their
+ * residual: about 1.4 times the error of the output's own rounding. fp32 outputs have no such term.) With scores_out, the weight
+ * (softmax probability, summed over the query heads of a kv head) that each own row received is added to an accumulator, which
+ * attn_kv_evict reads. No own rows and no prefix: zeros. NaN in a query or a valid row is NaN in the outputs that it belongs to. */
 typedef struct AttnDecodeSharedArgs {
     void* o;              /* out: [batch][n_heads][head_dim], o_dtype */
     const void* q;        /* in : [batch][n_heads][head_dim], dtype */
@@ -523,7 +525,8 @@ typedef struct AttnDecodeSharedArgs {
     uint32_t batch, n_heads, n_kv_heads;
     uint32_t head_dim;       /* 64 or 128; at most 64 query heads per kv head, 1024 in all, 2048 sequences */
     uint32_t prefix_len;
-    uint32_t kv_capacity;    /* rows an own cache holds; 0 = no own rows */
+    uint32_t kv_capacity;    /* rows an own cache holds; 0 = no own rows. With the other dimensions it chooses the kernels and the order
+                                of the sums: the last bits of a result go by it */
     const uint32_t* kv_len;  /* device [batch], valid own rows; NULL = kv_len_uniform. A length beyond the capacity is clamped and
                                 ATTN_STATUS_BAD_SHAPE is ORed into *status */
     uint32_t kv_len_uniform;

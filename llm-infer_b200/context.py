@@ -143,8 +143,8 @@ def rope_positions(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
     """Rotates every token's q and k by ``pos * inv_freq`` and writes k and v into row ``row`` of sequence ``seq``'s caches.
 
     q [N, H, D], k / v [N, Hkv, D] fp32 / fp16 / bf16 (one type; views into a stacked projection are taken as they are);
-    k_cache / v_cache fp16 / bf16 [B, T, Hkv, D]; pos, row, seq int32 CUDA tensors [N] (seq None: token i is of sequence i);
-    inv_freq fp32 [rotary_dim / 2] on the device and factor as rope_frequencies gives them, values behind rotary_dim are copied.
+    k_cache / v_cache fp16 / bf16 [B, T, Hkv, D]; pos, row, seq int32 CUDA tensors [N], not negative (seq None: token i is of sequence
+    i); inv_freq fp32 [rotary_dim / 2] on the device and factor (0: 1) as rope_frequencies gives them, values behind rotary_dim are copied.
     layout "interleaved" pairs (2i, 2i + 1), "half" pairs (i, i + rotary_dim / 2). Returns the rotated q [N, H, D] (``q_out``, or a
     new tensor of q_out_dtype, default q's). A row that does not exist is not written and sets ATTN_STATUS_BAD_SHAPE in status."""
     index = _one_device(q, k, v, k_cache, v_cache, pos, row, inv_freq, seq, q_out, status)
@@ -226,8 +226,8 @@ def attn_decode_shared(q: torch.Tensor, k_prefix, v_prefix, k_cache: torch.Tenso
     k_prefix   [P, Hkv, D]      q's type, or None (no prefix); rows may be strided. v_prefix the same
     k_cache    [B, T, Hkv, D]   q's type; rows and sequences may be strided (T may be 0). v_cache the same
     kv_len     None (all T rows), an int, or an int32 CUDA tensor [B] of valid own rows (0 is allowed)
-    scores     [B, Hkv, T] fp32 accumulated weights, rows dense; scores_out receives scores + this token's weights of the valid
-               rows (default: scores itself, in place). scores_out alone starts from zero
+    scores     [B, Hkv, T] fp32 accumulated weights, rows dense, each in memory of its own (not expanded); scores_out receives
+               scores + this token's weights of the valid rows (default: scores itself, in place). scores_out alone starts from zero
     returns    out [B, H, D] in out_dtype (q's type, the default, or fp32); fills ``lse`` [B, H] (fp32) when given
     """
     index = _one_device(q, k_prefix, v_prefix, k_cache, v_cache, kv_len if isinstance(kv_len, torch.Tensor) else None, out, lse, scores,
@@ -307,8 +307,8 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor,
     ``keep`` rows, in their order.
 
     k_cache, v_cache [B, T, Hkv, D] 16-bit, scores [B, Hkv, T] fp32 with dense rows, kv_len an int32 CUDA tensor [B] or None (T).
-    out  None: in place; or (k_out, v_out, scores_out) with [B, T2, Hkv, D] and [B, Hkv, T2], T2 >= keep, sharing no memory with
-         the inputs. K and V rows behind a new length are left alone, scores there become 0.
+    out  None: in place; or (k_out, v_out, scores_out) with [B, T2, Hkv, D] and [B, Hkv, T2], T2 >= keep, sharing no byte with
+         the inputs or each other. K and V rows behind a new length are left alone, scores there become 0.
     Returns (kept [B, Hkv, keep] int32: the source row of each kept row, -1 behind the new length; kv_len_out [B] int32:
     min(length, keep); it may be given as kv_len itself)."""
     k_out, v_out, scores_out = (k_cache, v_cache, scores) if out is None else out

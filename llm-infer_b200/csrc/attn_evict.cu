@@ -1,8 +1,8 @@
 // Eviction from a KV cache by accumulated attention weight: of every (sequence, kv head), the first `sink` rows, the last
 // `recent` rows and the rows with the largest scores, `keep` in all, stay; their order stays too. Ties go to the lowest row.
 //
-// Two launches, or one that does both for small calls. (1) Which rows: a CTA or a cluster of them per (sequence, kv head) finds the keep-th largest key by a radix selection
-// (digits of 11, 11 and 10 bits, a histogram in shared memory per CTA, summed over the cluster), then counts and writes the
+// Two launches, or one that does both for small calls. (1) Which rows: a CTA or a cluster of them per (sequence, kv head) finds the
+// keep-th largest key by a radix selection (digits of 11, 11 and 10 bits, a histogram in shared memory per CTA, summed over the cluster), then counts and writes the
 // kept rows in order. A score's key is its bit pattern mapped so that unsigned order is the order of the numbers (NaN below
 // everything, -0 = +0); always-kept rows carry the largest key. (2) The copy, bound by memory: kept K and V rows and scores are
 // read once and written once. Into another cache it is a plain gather with as many blocks as it has work for. In place, a row only
@@ -12,7 +12,8 @@
 // Graphs of calls: 16 ragged sequences of up to 4096 rows into caches of 1999 (8 kv heads of 128, 246 MB) 49.1 us, of which the
 // copy is 39 (6.2 TB/s) and the selection 6; one sequence of 131072 rows to 16384 39.3 us: copy 22, the rest the selection on 64 SMs (48.6
 // while every CTA read the others' histograms whole, 2 us a digit); 1024 rows to 256, one launch,
-// 6.2 us (two: 9.3), all of it latency.
+// 6.2 us (two: 9.3), all of it latency. In place: 16 sequences of 2080 rows back to 2048 (268 MB) 91 us, of 4096 to 1999 76, one of
+// 131072 to 16384 117: 2.9, 3.5 and 1.1 TB/s, a CTA per (head, slice) going through its rows one batch behind the other.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -244,7 +245,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_
         // (the next write of s_pick comes behind another meeting, and each digit has a histogram of its own)
     }
     // every key above `prefix` stays, and the first `need` rows of those equal to it
-    // ---- counts per warp, in order: keys above in the low half of a word, equal ones in the high half (a lane's at most 2^16)
+    // ---- counts per warp, in order: keys above, and equal ones
     const uint32_t wb = min(n, warp * per_warp), we = min(n, wb + per_warp);
     auto tally = [&](uint32_t i, const uint4& k, uint32_t (&gt)[4], uint32_t (&eq)[4]) {
         const uint32_t key[4] = {k.x, k.y, k.z, k.w};

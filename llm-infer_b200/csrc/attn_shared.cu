@@ -17,11 +17,12 @@
 //           the split pass left in the workspace into weights (exp2(s - LSE)), sum them over the heads and add them to the accumulators.
 // The scores of own rows cost 4 bytes per query head and row each way through L2, next to 4 * head_dim bytes of K and V per kv head.
 // P enters the second product rounded once to the caches' type when the output is 16 bits wide too, which adds about as much error as the
-// output's own rounding (1.4 times the error of that alone), and for fp32 outputs in three parts of bf16 (24 bits) or two of fp16 (23 bits, or 2^-32
-// of the row's maximum where p is small: fp16 probabilities are lifted by 2^7 over the end of its range).
+// output's own rounding (together 1.4 times the error of that alone; the residual would be a second product), and for fp32 outputs in three
+// parts of bf16 (24 bits) or two of fp16 (23 bits, or 2^-32 of the row's maximum where p is small: fp16 probabilities are lifted by 2^7, to
+// the upper end of fp16's range).
 //
-// Bound by HBM where there is enough to read: 16 ragged caches of up to 4096 rows (168 MB, with weights) take 38.6 us in a graph of
-// calls, of which the streaming alone takes 30; 7 sequences over 131072 shared rows (543 MB) 95 us = 5.7 TB/s. Smaller calls are a chain
+// Bound by HBM where there is enough to read: 16 ragged caches of up to 4096 rows (168 MB, with weights) take 38.9 us in a graph of
+// calls, of which the streaming alone takes 30; 7 sequences over 131072 shared rows (543 MB) 96 us = 5.6 TB/s. Smaller calls are a chain
 // of latencies: lengths and dealing 1.1 us, query rows and first tile 2.5, a tile 1.2 us from barrier to barrier, pieces and merge 4.
 // What that taught: query rows requested behind the tiles' 28 MB came 3 to 5 us late, a chain of eight dependent MMAs and divisions by
 // variables show, and a tile in two slots (K is handed back before the softmax) keeps the stream going.
@@ -345,7 +346,8 @@ int tile_map(CUtensorMap* map, const void* cache, bool bf16, uint32_t head_dim, 
 
 // Which kernel takes the prefix, and how the SMs are shared. The split pass can take it along with the own rows in one launch; the
 // tensor-core kernel does many query rows or long prefixes faster, but starts and ends more slowly. Where it takes fewer CTAs than there
-// are SMs, the split pass of the same launch runs beside it on the others, else as its CTAs end. Times in us, measured on shapes of 64- and 128-dimension heads (graphs of calls).
+// are SMs, the split pass of the same launch runs beside it on the others, else as its CTAs end. Times in us, measured on shapes of 64-
+// and 128-dimension heads (graphs of calls).
 struct PrefixChoice {
     bool tensor;
     uint32_t prefix_ctas, split_ctas;

@@ -16,16 +16,17 @@
 // spaced (heads of one group, then the next sequence), so the softmax warps bring them into the swizzled tile.
 //
 // With fp32 outputs a segment is one tile, whose keys and output columns the two softmax warpgroups share; P enters the second product in
-// three parts (bf16: its 24 bits) or two (fp16: 23 bits, or 2^-32 of the row's maximum where p is small), and a block's products start from zero and are added up in registers.
-// 64 query rows of 128 dimensions x 65536 keys, 8 kv heads: 67 us (fp16) and 74 (bf16), for 58 with outputs of 16 bits, all of it the
+// three parts (bf16: its 24 bits) or two (fp16: 23 bits, or 2^-32 of the row's maximum where p is small), and a block's products start
+// from zero and are added up in registers.
+// 64 query rows of 128 dimensions x 65536 keys, 8 kv heads: 71 us (fp16) and 79 (bf16), for 58 with outputs of 16 bits, all of it the
 // further MMAs (a third block of scores in tensor memory changed nothing); errors 7e-7 and 5e-7 of the output, where sums left in tensor
 // memory and two parts were off by 9e-6.
 //
 // Bound by the K/V stream up to 128 rows: a block takes 0.80 us of a CTA (32 KB, 0.72 us of an SM's share of HBM). With two tiles it
 // takes 1.1 us, in which the special-function units are busy for 0.55 and the tensor pipe for 0.6: the chain from scores to
 // probabilities of one block. A launch costs 10 us around its blocks (query rows 2, first block 2, piece and exit 4), which is why
-// short prefixes stay in the split pass of attn_shared.cu. 256 query rows x 65536 keys, 8 kv heads of 128, fp16: 79 us in all
-// (in the split pass: 355); 128 rows: 56 (185); 20 rows: 52 (51).
+// short prefixes stay in the split pass of attn_shared.cu. 256 query rows x 65536 keys, 8 kv heads of 128, fp16: 80 us in all
+// (in the split pass: 355); 128 rows: 59 (185); 20 rows: 53 (51).
 // Every wait is bounded; on expiry the role records ATTN_STATUS_WAIT_TIMEOUT, stops, and the CTA still runs its common exit.
 #include <cuda.h>
 
@@ -371,143 +372,143 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                 staged = true;
             }
         } else {
-        for (uint32_t at = t0; ok && item_at(at, w); at += w.blocks) {
-            if (!w.tile[t]) continue;
-            // ---- the query rows into the tile (the previous item's MMAs are over, its result has left)
-            const uint32_t m = w.m0 + t * BM + r;
-            if (staged) {
-                if (leader) tma_store_wait_read();
-                named_bar_sync(1 + t, 128);
-            }
-            if (!brought) bring_rows();
-            brought = false;
-            rows_there();
-            float m_used = -INFINITY;  // what the stored probabilities are relative to (log2 units): a maximum less the lift
-            float l = 0.f;
-            for (uint32_t j = 0; j < w.blocks && ok; ++j) {
-                const uint32_t g = g0 + j, buf = g & 1, par = (g >> 1) & 1;
-                const uint32_t s_tmem = tmem_s(t, buf) + lane_addr;
-                if (!mbar_wait(bar(BAR_S_FULL + 2 * t + buf), par)) { report_timeout(p.status); ok = false; break; }
-                fence_after();
-                float s[BN];
-#pragma unroll
-                for (int c = 0; c < BN / 32; ++c) tmem_ld32(s_tmem + c * 32, *reinterpret_cast<float(*)[32]>(&s[c * 32]));
-                tmem_wait_ld();
-                const uint32_t left = p.prefix - (w.block + j) * BN;  // keys from this block on
-                if (left < BN) {
-#pragma unroll
-                    for (int c = 0; c < BN; ++c) {
-                        if (c >= left) s[c] = -INFINITY;
-                    }
-                }
-                // four independent chains of three-input maxima
-                float mx4[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) mx4[i] = max3(s[i], s[4 + i], s[8 + i]);
-#pragma unroll
-                for (int c = 12; c + 8 <= BN; c += 8) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) mx4[i] = max3(mx4[i], s[c + i], s[c + 4 + i]);
-                }
-                float mx = max3(fmaxf(mx4[0], mx4[1]), mx4[2], mx4[3]);
-#pragma unroll
-                for (int c = 12 + (BN - 12) / 8 * 8; c < BN; ++c) mx = fmaxf(mx, s[c]);
-                mx *= p.scale_log2;
-                // Rescale only when the maximum grew by more than 8 (probabilities stay below 2^8, with fp16's lift 2^15).
-                float factor = 1.f;
-                if (mx > m_used + (8.f + kLift<BF16>)) {
-                    factor = fast_exp2(m_used - (mx - kLift<BF16>));  // 0 on the first block (m_used = -inf)
-                    m_used = mx - kLift<BF16>;
-                }
-                if (g >= 2 && !mbar_wait(bar(BAR_O_DONE + 2 * t + buf), par ^ 1)) { report_timeout(p.status); ok = false; break; }
-                if (j > 0 && __any_sync(0xffffffffu, factor != 1.f)) {
-                    if (!mbar_wait(bar(BAR_O_DONE + 2 * t + (buf ^ 1)), ((g - 1) >> 1) & 1)) { report_timeout(p.status); ok = false; break; }
-                    fence_after();
-#pragma unroll
-                    for (int c = 0; c < HD / 32; ++c) {
-                        float o[32];
-                        tmem_ld32(tmem_o(t) + lane_addr + c * 32, o);
-                        tmem_wait_ld();
-                        uint32_t u[32];
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(o[i] * factor);
-                        tmem_st32(tmem_o(t) + lane_addr + c * 32, u);
-                    }
-                }
-                l *= factor;
-                // probabilities; P overwrites S in place
-                const float m_safe = m_used == -INFINITY ? 0.f : m_used;
-                const f32x2 scale2 = pack_f32x2(p.scale_log2, p.scale_log2), m2 = pack_f32x2(-m_safe, -m_safe);
-                f32x2 sum2[2] = {pack_f32x2(0.f, 0.f), pack_f32x2(0.f, 0.f)};
-#pragma unroll
-                for (int c = 0; c < BN / 32; ++c) {
-                    uint32_t hi[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        float p0, p1;
-                        unpack_f32x2(fma_f32x2(pack_f32x2(s[c * 32 + 2 * i], s[c * 32 + 2 * i + 1]), scale2, m2), p0, p1);
-                        p0 = fast_exp2(p0);
-                        p1 = fast_exp2(p1);
-                        const f32x2 pp = pack_f32x2(p0, p1);
-                        sum2[i & 1] = add_f32x2(sum2[i & 1], pp);
-                        hi[i] = pack2<BF16>(p0, p1);
-                    }
-                    tmem_st16(s_tmem + c * 16, hi);  // 32 keys -> 16 packed columns
-                }
-                float s0, s1;
-                unpack_f32x2(add_f32x2(sum2[0], sum2[1]), s0, s1);
-                l += s0 + s1;
-                tmem_wait_st();
-                fence_before();
-                mbar_arrive(bar(BAR_P_FULL + 2 * t + buf));
-            }
-            g0 += w.blocks;
-            if (!ok) break;
-            // ---- the piece: O / l and log-sum-exp (log2 units)
-            if (!mbar_wait(bar(BAR_O_DONE + 2 * t + ((g0 - 1) & 1)), ((g0 - 1) >> 1) & 1)) {
-                report_timeout(p.status);
-                ok = false;
-                break;
-            }
-            fence_after();
-            const float inv = l == 0.f ? 0.f : 1.f / l;  // (a sum of NaN stays one)
-            const uint32_t rec_row = (blockIdx.x + w.seg) * kRows + t * BM;
-            if (m < query_rows) p.lse[rec_row + r] = l == 0.f ? -INFINITY : (m_used + kLift<BF16>) + __log2f(l * kUnlift<BF16>);
-            // The tile leaves through shared memory and the TMA engine, 128 bytes of every row at a time: the query tile, which nothing
-            // reads any more, holds the first two passes, the staging tile the third, so that only the fourth waits for a store. (Each pass
-            // behind the previous one's store in a single staging tile: 3 us more per piece.)
-            auto put = [&](int pass, uint32_t stage) {
-                float o[32];
-                tmem_ld32(tmem_o(t) + lane_addr + pass * 32, o);
-                tmem_wait_ld();
-#pragma unroll
-                for (int c = 0; c < 8; ++c)
-                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(stage + r * 128 + ((c ^ (r & 7)) << 4)),
-                                 "r"(__float_as_uint(o[c * 4] * inv)), "r"(__float_as_uint(o[c * 4 + 1] * inv)),
-                                 "r"(__float_as_uint(o[c * 4 + 2] * inv)), "r"(__float_as_uint(o[c * 4 + 3] * inv))
-                                 : "memory");
-            };
-            constexpr int kPasses = HD / 32;
-#pragma unroll 1
-            for (int pass = 0; pass < kPasses; ++pass) {
-                const uint32_t stage = pass == 2   ? base + kSmemStage + t * kStageTileBytes
-                                       : pass == 1 ? base + kSmemQ + t * kTileBytes + kSubTileBytes
-                                                   : base + kSmemQ + t * kTileBytes;
-                if (pass == 3) {  // the first pass's store has been read
-                    if (leader) asm volatile("cp.async.bulk.wait_group.read 2;" ::: "memory");
+            for (uint32_t at = t0; ok && item_at(at, w); at += w.blocks) {
+                if (!w.tile[t]) continue;
+                // ---- the query rows into the tile (the previous item's MMAs are over, its result has left)
+                const uint32_t m = w.m0 + t * BM + r;
+                if (staged) {
+                    if (leader) tma_store_wait_read();
                     named_bar_sync(1 + t, 128);
                 }
-                put(pass, stage);
-                fence_async_smem();
-                named_bar_sync(1 + t, 128);
-                if (leader) {
-                    tma_store_2d(&tm_o, stage, pass * 32, rec_row);
-                    tma_store_commit();
+                if (!brought) bring_rows();
+                brought = false;
+                rows_there();
+                float m_used = -INFINITY;  // what the stored probabilities are relative to (log2 units): a maximum less the lift
+                float l = 0.f;
+                for (uint32_t j = 0; j < w.blocks && ok; ++j) {
+                    const uint32_t g = g0 + j, buf = g & 1, par = (g >> 1) & 1;
+                    const uint32_t s_tmem = tmem_s(t, buf) + lane_addr;
+                    if (!mbar_wait(bar(BAR_S_FULL + 2 * t + buf), par)) { report_timeout(p.status); ok = false; break; }
+                    fence_after();
+                    float s[BN];
+#pragma unroll
+                    for (int c = 0; c < BN / 32; ++c) tmem_ld32(s_tmem + c * 32, *reinterpret_cast<float(*)[32]>(&s[c * 32]));
+                    tmem_wait_ld();
+                    const uint32_t left = p.prefix - (w.block + j) * BN;  // keys from this block on
+                    if (left < BN) {
+#pragma unroll
+                        for (int c = 0; c < BN; ++c) {
+                            if (c >= left) s[c] = -INFINITY;
+                        }
+                    }
+                    // four independent chains of three-input maxima
+                    float mx4[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mx4[i] = max3(s[i], s[4 + i], s[8 + i]);
+#pragma unroll
+                    for (int c = 12; c + 8 <= BN; c += 8) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) mx4[i] = max3(mx4[i], s[c + i], s[c + 4 + i]);
+                    }
+                    float mx = max3(fmaxf(mx4[0], mx4[1]), mx4[2], mx4[3]);
+#pragma unroll
+                    for (int c = 12 + (BN - 12) / 8 * 8; c < BN; ++c) mx = fmaxf(mx, s[c]);
+                    mx *= p.scale_log2;
+                    // Rescale only when the maximum grew by more than 8 (probabilities stay below 2^8, with fp16's lift 2^15).
+                    float factor = 1.f;
+                    if (mx > m_used + (8.f + kLift<BF16>)) {
+                        factor = fast_exp2(m_used - (mx - kLift<BF16>));  // 0 on the first block (m_used = -inf)
+                        m_used = mx - kLift<BF16>;
+                    }
+                    if (g >= 2 && !mbar_wait(bar(BAR_O_DONE + 2 * t + buf), par ^ 1)) { report_timeout(p.status); ok = false; break; }
+                    if (j > 0 && __any_sync(0xffffffffu, factor != 1.f)) {
+                        if (!mbar_wait(bar(BAR_O_DONE + 2 * t + (buf ^ 1)), ((g - 1) >> 1) & 1)) { report_timeout(p.status); ok = false; break; }
+                        fence_after();
+#pragma unroll
+                        for (int c = 0; c < HD / 32; ++c) {
+                            float o[32];
+                            tmem_ld32(tmem_o(t) + lane_addr + c * 32, o);
+                            tmem_wait_ld();
+                            uint32_t u[32];
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(o[i] * factor);
+                            tmem_st32(tmem_o(t) + lane_addr + c * 32, u);
+                        }
+                    }
+                    l *= factor;
+                    // probabilities; P overwrites S in place
+                    const float m_safe = m_used == -INFINITY ? 0.f : m_used;
+                    const f32x2 scale2 = pack_f32x2(p.scale_log2, p.scale_log2), m2 = pack_f32x2(-m_safe, -m_safe);
+                    f32x2 sum2[2] = {pack_f32x2(0.f, 0.f), pack_f32x2(0.f, 0.f)};
+#pragma unroll
+                    for (int c = 0; c < BN / 32; ++c) {
+                        uint32_t hi[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            float p0, p1;
+                            unpack_f32x2(fma_f32x2(pack_f32x2(s[c * 32 + 2 * i], s[c * 32 + 2 * i + 1]), scale2, m2), p0, p1);
+                            p0 = fast_exp2(p0);
+                            p1 = fast_exp2(p1);
+                            const f32x2 pp = pack_f32x2(p0, p1);
+                            sum2[i & 1] = add_f32x2(sum2[i & 1], pp);
+                            hi[i] = pack2<BF16>(p0, p1);
+                        }
+                        tmem_st16(s_tmem + c * 16, hi);  // 32 keys -> 16 packed columns
+                    }
+                    float s0, s1;
+                    unpack_f32x2(add_f32x2(sum2[0], sum2[1]), s0, s1);
+                    l += s0 + s1;
+                    tmem_wait_st();
+                    fence_before();
+                    mbar_arrive(bar(BAR_P_FULL + 2 * t + buf));
                 }
+                g0 += w.blocks;
+                if (!ok) break;
+                // ---- the piece: O / l and log-sum-exp (log2 units)
+                if (!mbar_wait(bar(BAR_O_DONE + 2 * t + ((g0 - 1) & 1)), ((g0 - 1) >> 1) & 1)) {
+                    report_timeout(p.status);
+                    ok = false;
+                    break;
+                }
+                fence_after();
+                const float inv = l == 0.f ? 0.f : 1.f / l;  // (a sum of NaN stays one)
+                const uint32_t rec_row = (blockIdx.x + w.seg) * kRows + t * BM;
+                if (m < query_rows) p.lse[rec_row + r] = l == 0.f ? -INFINITY : (m_used + kLift<BF16>) + __log2f(l * kUnlift<BF16>);
+                // The tile leaves through shared memory and the TMA engine, 128 bytes of every row at a time: the query tile, which nothing
+                // reads any more, holds the first two passes, the staging tile the third, so that only the fourth waits for a store. (Each pass
+                // behind the previous one's store in a single staging tile: 3 us more per piece.)
+                auto put = [&](int pass, uint32_t stage) {
+                    float o[32];
+                    tmem_ld32(tmem_o(t) + lane_addr + pass * 32, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(stage + r * 128 + ((c ^ (r & 7)) << 4)),
+                                     "r"(__float_as_uint(o[c * 4] * inv)), "r"(__float_as_uint(o[c * 4 + 1] * inv)),
+                                     "r"(__float_as_uint(o[c * 4 + 2] * inv)), "r"(__float_as_uint(o[c * 4 + 3] * inv))
+                                     : "memory");
+                };
+                constexpr int kPasses = HD / 32;
+#pragma unroll 1
+                for (int pass = 0; pass < kPasses; ++pass) {
+                    const uint32_t stage = pass == 2   ? base + kSmemStage + t * kStageTileBytes
+                                           : pass == 1 ? base + kSmemQ + t * kTileBytes + kSubTileBytes
+                                                       : base + kSmemQ + t * kTileBytes;
+                    if (pass == 3) {  // the first pass's store has been read
+                        if (leader) asm volatile("cp.async.bulk.wait_group.read 2;" ::: "memory");
+                        named_bar_sync(1 + t, 128);
+                    }
+                    put(pass, stage);
+                    fence_async_smem();
+                    named_bar_sync(1 + t, 128);
+                    if (leader) {
+                        tma_store_2d(&tm_o, stage, pass * 32, rec_row);
+                        tma_store_commit();
+                    }
+                }
+                staged = true;
+                fence_before();  // the next item's first product overwrites O; its P_FULL arrival orders it behind these loads
             }
-            staged = true;
-            fence_before();  // the next item's first product overwrites O; its P_FULL arrival orders it behind these loads
-        }
         }
         if (leader) tma_store_wait_all();
     } else {

@@ -188,7 +188,7 @@ __device__ __forceinline__ float round16(float x) {
     }
 }
 
-// Requests the 32 bytes that hold *p into L1 by a load whose value nobody waits for.
+// Requests the 32 bytes that hold *p into the caches by a load whose value nobody waits for.
 __device__ __forceinline__ void touch(const void* p) {
     uint32_t unused;
     asm volatile("ld.global.u32 %0, [%1];" : "=r"(unused) : "l"(p) : "memory");

@@ -301,7 +301,7 @@ __device__ __forceinline__ void split_body(const CUtensorMap& tm_k, const CUtens
                 __syncwarp();
                 const uint32_t r = lane & 15;
                 q_lane = r < n ? my_q + r * (D * 2) : q_zero;
-                // the next segment's rows, on their way into L1 (rows of the list's own segments follow one another in q)
+                // the next segment's rows, requested into L2, from where cp.async takes them (rows of the list's own segments follow one another in q)
                 if (cur.own && cur.unit + (cur.tiles - cur.tile) < u1) {
                     const uint64_t next = static_cast<uint64_t>(cur.b) * p.n_heads + (kvh + sh.hpc) * p.group + row0;
                     for (uint32_t i = lane; i < n * kParts * 4; i += 32)  // 32 bytes each
