@@ -576,6 +576,56 @@ typedef struct AttnKvEvictArgs {
 } AttnKvEvictArgs;
 int attn_kv_evict(const AttnKvEvictArgs* args, void* stream);
 
+/* ---- Layers in 8-bit integers ---------------------------------------------------------------------------------------
+ * The projections of a layer as products of 8-bit integers, a scale per token and a scale per channel (output row of the weight
+ * matrix): a row of x stands as whole numbers q in -127 .. 127 and one fp32 scale, x[i] ~ scale * q[i] with scale = max|x| / 127. The
+ * engine has no counterpart. Rows of q are `stride` bytes apart, a multiple of 16; bytes behind a row's end are never used.
+ *   attn_rmsnorm_i8    residual's addition, RMSNorm and quantisation of rows (in front of the Q/K/V and gate/up projections)
+ *   attn_quantize_i8   quantisation of rows (in front of the output and down projections; a weight matrix's channels at load time)
+ *   attn_gemm_i8       the product, with SwiGLU as its epilogue where asked, for one token or many */
+
+/* Per row: h = x + delta (fp32), x_out = h rounded to x's type, y = h / sqrt(mean(h^2) + eps) * weight (attn_quantize_i8: y = x),
+ * scale = max|y| / 127, q = y / scale rounded to the nearest whole number, ties to the even one. The norm's factor is the same for the
+ * whole row and so belongs to the scale alone: q is round(z * (127 / max|z|)) of z = h * weight, each operation rounded to fp32, and
+ * depends on no sum's order. A row of zeros: scale 0. A row that holds NaN or an infinity (or whose z passes fp32's range):
+ * q = 0 and scale = NaN, so that every product with it is NaN. */
+typedef struct AttnRowsI8Args {
+    int8_t* q;           /* out: [rows][dim], row r at q + r*q_stride, 16-byte aligned */
+    float* scale;        /* out: [rows] */
+    void* x_out;         /* out: x + delta, x_dtype; NULL: not written. May be x, with the same stride. Needs delta */
+    const void* x;       /* in : [rows][dim], x_dtype */
+    const void* delta;   /* optional in: [rows][dim], delta_dtype (attn_quantize_i8: NULL) */
+    const float* weight; /* in : [dim] (attn_quantize_i8: NULL) */
+    uint64_t q_stride;   /* bytes, a multiple of 16; 0 = dim rounded up to a multiple of 16 */
+    uint64_t x_stride, delta_stride, x_out_stride; /* elements; 0 = dim */
+    uint32_t rows, dim;
+    float eps;           /* at least 2^-126 (attn_quantize_i8: not used) */
+    int32_t x_dtype, delta_dtype; /* ATTN_DTYPE_F32 | F16 | BF16 */
+} AttnRowsI8Args;
+/* Nothing that is written may share memory with anything else that is read or written, but for x_out in the place of x. */
+int attn_rmsnorm_i8(const AttnRowsI8Args* args, void* stream);
+int attn_quantize_i8(const AttnRowsI8Args* args, void* stream);
+
+/* out[t][j] = a_scale[t] * w_scale[j] * sum_i a[t][i] * w[j][i], t < m tokens, j < n_out, i < k. The sum is exact (32-bit integers,
+ * k up to 131071), two fp32 products scale it and the result is rounded once to out's type: the same bits for every m and every
+ * stride. With swiglu != 0 the matrix holds n_out gate rows followed by n_out up rows, and out = silu(gate) * up, computed in fp32
+ * (src/model/block.cpp:206-210). */
+typedef struct AttnGemmI8Args {
+    void* out;            /* [m][n_out], out_dtype, row t at out + t*ldc elements */
+    const int8_t* a;      /* [m][k], row t at a + t*a_stride, 16-byte aligned */
+    const float* a_scale; /* [m] */
+    const int8_t* w;      /* [n_out][k] (swiglu: [2 n_out][k]), row j at w + j*w_stride, 16-byte aligned */
+    const float* w_scale; /* [n_out] (swiglu: [2 n_out]) */
+    uint64_t a_stride, w_stride; /* bytes, multiples of 16; 0 = k rounded up to a multiple of 16 */
+    uint64_t ldc;         /* 0 = n_out */
+    uint32_t m, n_out, k;
+    int32_t out_dtype;    /* ATTN_DTYPE_F32 | F16 | BF16 */
+    int32_t swiglu;
+    uint32_t* status;     /* optional device word for ATTN_STATUS_* bits */
+} AttnGemmI8Args;
+/* out may not share memory with an operand. */
+int attn_gemm_i8(const AttnGemmI8Args* args, void* stream);
+
 /* Human-readable text for an ATTN_ERR_* code. */
 const char* attn_status_string(int code);
 
@@ -588,7 +638,8 @@ uint64_t attn_kernel_launch_count(void);
 /* sizeof() of an argument structure as this library was compiled, so that a foreign-function binding can check its own
  * mirror of the layout: 0 AttnDecodeArgs, 1 AttnDecodeShardedArgs, 2 AttnPrefillArgs, 3 AttnRopeInsertArgs,
  * 4 AttnGemvArgs, 5 AttnMergeArgs, 6 AttnGemmArgs, 7 AttnRopePromptArgs,
- * 8 AttnGemmPairArgs, 9 AttnGemmQ8Args, 10 AttnRopePositionsArgs, 11 AttnDecodeSharedArgs, 12 AttnKvEvictArgs; 0 for any
+ * 8 AttnGemmPairArgs, 9 AttnGemmQ8Args, 10 AttnRopePositionsArgs, 11 AttnDecodeSharedArgs, 12 AttnKvEvictArgs,
+ * 13 AttnRowsI8Args, 14 AttnGemmI8Args; 0 for any
  * other index. */
 size_t attn_abi_struct_size(int which);
 

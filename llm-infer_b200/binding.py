@@ -58,6 +58,9 @@ EXPORTED_SYMBOLS = (
     "attn_decode_shared_workspace_bytes",
     "attn_decode_shared",
     "attn_kv_evict",
+    "attn_rmsnorm_i8",
+    "attn_quantize_i8",
+    "attn_gemm_i8",
     "attn_status_string",
     "attn_last_cuda_error",
     "attn_kernel_launch_count",
@@ -394,6 +397,45 @@ class AttnKvEvictArgs(C.Structure):
     ]
 
 
+class AttnRowsI8Args(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("scale", C.c_void_p),
+        ("x_out", C.c_void_p),
+        ("x", C.c_void_p),
+        ("delta", C.c_void_p),
+        ("weight", C.c_void_p),
+        ("q_stride", C.c_uint64),
+        ("x_stride", C.c_uint64),
+        ("delta_stride", C.c_uint64),
+        ("x_out_stride", C.c_uint64),
+        ("rows", C.c_uint32),
+        ("dim", C.c_uint32),
+        ("eps", C.c_float),
+        ("x_dtype", C.c_int32),
+        ("delta_dtype", C.c_int32),
+    ]
+
+
+class AttnGemmI8Args(C.Structure):
+    _fields_ = [
+        ("out", C.c_void_p),
+        ("a", C.c_void_p),
+        ("a_scale", C.c_void_p),
+        ("w", C.c_void_p),
+        ("w_scale", C.c_void_p),
+        ("a_stride", C.c_uint64),
+        ("w_stride", C.c_uint64),
+        ("ldc", C.c_uint64),
+        ("m", C.c_uint32),
+        ("n_out", C.c_uint32),
+        ("k", C.c_uint32),
+        ("out_dtype", C.c_int32),
+        ("swiglu", C.c_int32),
+        ("status", C.c_void_p),
+    ]
+
+
 class AttnError(RuntimeError):
     def __init__(self, code: int, what: str, cuda_error: int = 0):
         self.code = code
@@ -488,6 +530,12 @@ def load() -> C.CDLL:
     lib.attn_decode_shared.argtypes = [C.c_void_p, C.c_void_p]  # AttnDecodeSharedArgs, by reference or packed
     lib.attn_kv_evict.restype = C.c_int
     lib.attn_kv_evict.argtypes = [C.c_void_p, C.c_void_p]  # AttnKvEvictArgs, by reference or packed
+    lib.attn_rmsnorm_i8.restype = C.c_int
+    lib.attn_rmsnorm_i8.argtypes = [C.c_void_p, C.c_void_p]  # AttnRowsI8Args, by reference or packed
+    lib.attn_quantize_i8.restype = C.c_int
+    lib.attn_quantize_i8.argtypes = lib.attn_rmsnorm_i8.argtypes
+    lib.attn_gemm_i8.restype = C.c_int
+    lib.attn_gemm_i8.argtypes = [C.c_void_p, C.c_void_p]  # AttnGemmI8Args, by reference or packed
     lib.attn_status_string.restype = C.c_char_p
     lib.attn_status_string.argtypes = [C.c_int]
     lib.attn_last_cuda_error.restype = C.c_int
@@ -496,7 +544,7 @@ def load() -> C.CDLL:
     lib.attn_abi_struct_size.argtypes = [C.c_int]
     mirrors = (AttnDecodeArgs, AttnDecodeShardedArgs, AttnPrefillArgs, AttnRopeInsertArgs, AttnGemvArgs, AttnMergeArgs,
                AttnGemmArgs, AttnRopePromptArgs, AttnGemmPairArgs, AttnGemmQ8Args, AttnRopePositionsArgs, AttnDecodeSharedArgs,
-               AttnKvEvictArgs)
+               AttnKvEvictArgs, AttnRowsI8Args, AttnGemmI8Args)
     for index, mirror in enumerate(mirrors):
         if lib.attn_abi_struct_size(index) != C.sizeof(mirror):
             raise RuntimeError(f"{mirror.__name__}: the ctypes mirror ({C.sizeof(mirror)} bytes) does not match the "

@@ -305,6 +305,8 @@ size_t attn_abi_struct_size(int which) {
         case 10: return sizeof(AttnRopePositionsArgs);
         case 11: return sizeof(AttnDecodeSharedArgs);
         case 12: return sizeof(AttnKvEvictArgs);
+        case 13: return sizeof(AttnRowsI8Args);
+        case 14: return sizeof(AttnGemmI8Args);
         default: return 0;
     }
 }
