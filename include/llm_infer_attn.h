@@ -622,6 +622,9 @@ typedef struct AttnGemmI8Args {
     int32_t out_dtype;    /* ATTN_DTYPE_F32 | F16 | BF16 */
     int32_t swiglu;
     uint32_t* status;     /* optional device word for ATTN_STATUS_* bits */
+    int32_t w_early;      /* != 0: the caller vouches that w was in place before the previous kernel of the stream was launched (true
+                             of a loaded model's weights): with few tokens the kernel then fills its pipeline with weights while that
+                             kernel may still be running. No other operand is read early. 0 = wait first */
 } AttnGemmI8Args;
 /* out may not share memory with an operand. */
 int attn_gemm_i8(const AttnGemmI8Args* args, void* stream);

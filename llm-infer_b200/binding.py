@@ -433,6 +433,7 @@ class AttnGemmI8Args(C.Structure):
         ("out_dtype", C.c_int32),
         ("swiglu", C.c_int32),
         ("status", C.c_void_p),
+        ("w_early", C.c_int32),
     ]
 
 

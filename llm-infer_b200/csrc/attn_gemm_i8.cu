@@ -32,6 +32,7 @@ struct GemmI8Params {
     uint32_t k_steps;
     uint32_t stages;
     int32_t out_dtype;
+    uint32_t w_early;
     uint32_t* status;
 };
 
@@ -47,6 +48,15 @@ __device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_
         ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(acc)
         : "memory");
 }
+// The same over a pair of CTAs: A rows 0-127 and half of B's rows in the leader's shared memory, the others at the same offsets in
+// its partner.
+__device__ __forceinline__ void mma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(acc)
+        : "memory");
+}
 // 16 columns of this thread's tensor-memory lane.
 __device__ __forceinline__ void ld16(uint32_t taddr, uint32_t (&r)[16]) {
     tmem_ld16(taddr, reinterpret_cast<float(&)[16]>(r));
@@ -56,6 +66,12 @@ __device__ __forceinline__ void wait_ld(uint32_t (&r)[16]) {
     tmem_wait_ld();
 #pragma unroll
     for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(r[i]));
+}
+
+__device__ __forceinline__ int4 ld_cluster_i4(uint32_t addr) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
 }
 
 __device__ __forceinline__ float silu(float x) { return __fdiv_rn(x, 1.0f + expf(-x)); }
@@ -84,6 +100,7 @@ __device__ __forceinline__ void with_out_type(int32_t dtype, F f) {
 // shared memory over the cluster. Four warps: warp 0 requests the tiles by TMA, warp 1 issues the MMAs, all of them finish the tile.
 enum { S_FULL = 0, kStreamMaxStages = 8, S_EMPTY = S_FULL + kStreamMaxStages, S_ACC = S_EMPTY + kStreamMaxStages, S_BARS };
 constexpr int kStreamThreads = 128;
+constexpr uint32_t kMaxSlices = 8;  // CTAs of a cluster
 
 template <int PARTS, int N>
 constexpr uint32_t stream_stage_bytes() { return PARTS * kWTile + N * kStepK; }
@@ -110,15 +127,42 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
     const uint32_t ks0 = static_cast<uint32_t>(static_cast<uint64_t>(p.k_steps) * slice / slices);
     const uint32_t ks1 = static_cast<uint32_t>(static_cast<uint64_t>(p.k_steps) * (slice + 1) / slices);
 
-    if (tid == 0) {
-        for (uint32_t s = 0; s < p.stages; ++s) {
-            mbar_init(bar(S_FULL + s), 1);
-            mbar_init(bar(S_EMPTY + s), 1);
+    auto gave_up = [&]() {
+        if (p.status) atomicOr(p.status, ATTN_STATUS_WAIT_TIMEOUT);
+    };
+    // a stage's bytes are announced, its weights requested
+    auto load_w = [&](uint32_t ks, uint32_t s) {
+        mbar_arrive_expect_tx(bar(S_FULL + s), kStageBytes);
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part)
+            tma_load_2d(base + s * kStageBytes + part * kWTile, &tm_w, bar(S_FULL + s), static_cast<int>(ks * kStepK),
+                        static_cast<int>(row0 + part * p.n_out));
+    };
+    const uint32_t early = p.w_early ? min(ks1 - ks0, p.stages) : 0u;
+    if (warp == 0) {
+        if (elect_one()) {
+            prefetch_tensor_map(&tm_w);
+            prefetch_tensor_map(&tm_a);
+            for (uint32_t s = 0; s < p.stages; ++s) {
+                mbar_init(bar(S_FULL + s), 1);
+                mbar_init(bar(S_EMPTY + s), 1);
+            }
+            mbar_init(bar(S_ACC), 1);
+            mbar_init_fence();
+            // While the previous kernel of the stream may still be running: the first weights come as far as L2. (What that kernel
+            // writes to them still arrives: L2 is where both meet.) With w_early they go into the ring.
+            for (uint32_t i = 0; i < min(ks1 - ks0, p.stages); ++i) {
+                if (p.w_early) {
+                    load_w(ks0 + i, i);
+                } else {
+#pragma unroll
+                    for (int part = 0; part < PARTS; ++part)
+                        tma_prefetch_2d(&tm_w, static_cast<int>((ks0 + i) * kStepK), static_cast<int>(row0 + part * p.n_out));
+                }
+            }
         }
-        mbar_init(bar(S_ACC), 1);
-        mbar_init_fence();
-    }
-    if (warp == 1) {
+        __syncwarp();
+    } else if (warp == 1) {
         tmem_alloc(smem_u32(const_cast<uint32_t*>(s_tmem)), kCols);
         tmem_relinquish();
     }
@@ -129,11 +173,18 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
 
     grid_dep_launch_dependents();
     grid_dep_wait();
-    if (tid < N) s_scale[tid] = tok0 + tid < p.m ? p.a_scale[tok0 + tid] : 0.f;
 
-    auto gave_up = [&]() {
-        if (p.status) atomicOr(p.status, ATTN_STATUS_WAIT_TIMEOUT);
-    };
+    // Channels of this thread: one, its tensor-memory lane; where slices' sums meet, four neighbouring ones.
+    const bool meet = slices > 1;
+    const uint32_t col = row0 + (meet ? 4 * lane : tid), width = meet ? 4 : 1;
+    float ws[PARTS][4];
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ws[part][i] = i < width && col + i < p.n_out ? p.w_scale[part * p.n_out + col + i] : 0.f;
+    if (warp >= 2)  // (warp 0 has tiles to request)
+        for (uint32_t t = tid - 64; t < N; t += 64) s_scale[t] = tok0 + t < p.m ? p.a_scale[tok0 + t] : 0.f;
+
     if (warp == 0) {
         if (elect_one()) {
             uint32_t s = 0, phase = 0, issued = 0;
@@ -142,13 +193,8 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
                     gave_up();
                     break;
                 }
-                const uint32_t dst = base + s * kStageBytes, full = bar(S_FULL + s);
-                const int kc = static_cast<int>(ks * kStepK);
-                mbar_arrive_expect_tx(full, kStageBytes);
-#pragma unroll
-                for (int part = 0; part < PARTS; ++part)
-                    tma_load_2d(dst + part * kWTile, &tm_w, full, kc, static_cast<int>(row0 + part * p.n_out));
-                tma_load_2d(dst + PARTS * kWTile, &tm_a, full, kc, static_cast<int>(tok0));
+                if (issued >= early) load_w(ks, s);
+                tma_load_2d(base + s * kStageBytes + PARTS * kWTile, &tm_a, bar(S_FULL + s), static_cast<int>(ks * kStepK), static_cast<int>(tok0));
                 if (++s == p.stages) s = 0, phase ^= 1;
             }
             // no copy is in flight when the block ends, whatever became of the MMAs
@@ -185,39 +231,38 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
     // (a vote, so that a warp reads tensor memory as one)
     if (!__all_sync(0xffffffffu, mbar_wait(bar(S_ACC), 0)) && lane == 0) gave_up();
     fence_after();
-    __syncthreads();  // s_scale
+    __syncthreads();  // the tokens' scales; the copies of a block that gave up
 
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(warp * 32) << 16);
-    const uint32_t col = row0 + tid;  // channel of this thread
     const uint32_t tokens = min(static_cast<uint32_t>(N), p.m - tok0);
-    const bool live = col < p.n_out;
-    const float w0 = live ? p.w_scale[col] : 0.f;
-    const float w1 = PARTS == 2 && live ? p.w_scale[p.n_out + col] : 0.f;
-    auto finish = [&](auto type, uint32_t t, int32_t s0, int32_t s1) {
-        using T = decltype(type);
-        float y = scaled(s0, w0, s_scale[t]);
-        if constexpr (PARTS == 2) y = __fmul_rn(silu(y), scaled(s1, w1, s_scale[t]));
-        static_cast<T*>(p.out)[(tok0 + t) * p.ldc + col] = to_out<T>(y);
+    auto value = [&](uint32_t t, int i, int32_t s0, int32_t s1) {
+        float y = scaled(s0, ws[0][i], s_scale[t]);
+        if constexpr (PARTS == 2) y = __fmul_rn(silu(y), scaled(s1, ws[1][i], s_scale[t]));
+        return y;
     };
-    if (slices == 1) {
+    if (!meet) {
+        with_out_type(p.out_dtype, [&](auto type) {
+            using T = decltype(type);
+            T* dst = static_cast<T*>(p.out) + static_cast<size_t>(tok0) * p.ldc + col;
 #pragma unroll 1
-        for (uint32_t c = 0; c < N; c += 16) {
-            uint32_t r[PARTS][16];
+            for (uint32_t c = 0; c < tokens; c += 16) {
+                uint32_t r[PARTS][16];
 #pragma unroll
-            for (int part = 0; part < PARTS; ++part) ld16(lane_addr + part * N + c, r[part]);
+                for (int part = 0; part < PARTS; ++part) ld16(lane_addr + part * N + c, r[part]);
 #pragma unroll
-            for (int part = 0; part < PARTS; ++part) wait_ld(r[part]);
-            with_out_type(p.out_dtype, [&](auto type) {
+                for (int part = 0; part < PARTS; ++part) wait_ld(r[part]);
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (live && c + i < tokens) finish(type, c + i, r[0][i], r[PARTS - 1][i]);
-            });
-        }
+                    if (col < p.n_out && c + i < tokens)
+                        dst[(c + i) * p.ldc] = to_out<T>(value(c + i, 0, r[0][i], r[PARTS - 1][i]));
+                __syncwarp();
+            }
+        });
     } else {
         // this slice's sums, [part][token][channel], where the tiles were
         uint32_t* sums = reinterpret_cast<uint32_t*>(smem);
 #pragma unroll 1
-        for (uint32_t c = 0; c < N; c += 16) {
+        for (uint32_t c = 0; c < tokens; c += 16) {
 #pragma unroll
             for (int part = 0; part < PARTS; ++part) {
                 uint32_t r[16];
@@ -227,17 +272,26 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
                 for (int i = 0; i < 16; ++i) sums[(part * N + c + i) * kRowsM + tid] = r[i];
             }
         }
-        __syncwarp();
         cluster_sync();
+        // each CTA finishes every slices-th token: a warp one of them, a thread four channels, all slices' sums on their way at once
         with_out_type(p.out_dtype, [&](auto type) {
-            for (uint32_t t = slice; t < tokens; t += slices) {
-                int32_t s[2] = {0, 0};
+            using T = decltype(type);
+            T* dst = static_cast<T*>(p.out) + static_cast<size_t>(tok0) * p.ldc + col;
+            for (uint32_t t = slice + slices * warp; t < tokens; t += slices * 4) {
+                int32_t sum[PARTS][4];
 #pragma unroll
                 for (int part = 0; part < PARTS; ++part) {
-                    const uint32_t at = base + ((part * N + t) * kRowsM + tid) * 4;
-                    for (uint32_t r = 0; r < slices; ++r) s[part] += static_cast<int32_t>(ld_cluster_u32(cluster_address(at, r)));
+                    const uint32_t at = base + ((part * N + t) * kRowsM + 4 * lane) * 4;
+                    int4 v[kMaxSlices];
+#pragma unroll
+                    for (uint32_t r = 0; r < kMaxSlices; ++r) v[r] = r < slices ? ld_cluster_i4(cluster_address(at, r)) : make_int4(0, 0, 0, 0);
+#pragma unroll
+                    for (uint32_t r = 1; r < kMaxSlices; ++r) v[0].x += v[r].x, v[0].y += v[r].y, v[0].z += v[r].z, v[0].w += v[r].w;
+                    sum[part][0] = v[0].x, sum[part][1] = v[0].y, sum[part][2] = v[0].z, sum[part][3] = v[0].w;
                 }
-                if (live) finish(type, t, s[0], s[PARTS - 1]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (col + i < p.n_out) dst[t * p.ldc + i] = to_out<T>(value(t, i, sum[0][i], sum[PARTS - 1][i]));
             }
         });
         __syncwarp();
@@ -248,6 +302,239 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
     if (warp == 1) {
         fence_after();
         tmem_dealloc(tmem, kCols);
+    }
+}
+
+// ---- many tokens: pairs of CTAs -------------------------------------------------------------------------------------
+// Persistent. Two CTAs (cta_group::2, M 256) share a tile of 256 weight rows x N tokens: each loads its own 128 weight rows and half
+// of the tokens, and its tensor memory receives its own rows of the product. With SwiGLU a CTA's 128 rows are 64 gate rows and the
+// matching 64 up rows, so that a tile moves no more bytes than without. Ten warps: warp 0 requests the tiles by TMA, warp 1 issues the
+// MMAs into one of two accumulators, warps 2-9 scale, round and store the other one; a warpgroup has half of the tokens.
+constexpr int kEpiWarps = 8, kPairThreads = (2 + kEpiWarps) * 32;
+constexpr uint32_t kPairMaxStages = 8;
+enum { P_FULL = 0, P_EMPTY = P_FULL + kPairMaxStages, P_ACC_FULL = P_EMPTY + kPairMaxStages, P_ACC_EMPTY = P_ACC_FULL + 2,
+       P_BARS = P_ACC_EMPTY + 2 };
+constexpr uint32_t kHalfRows = kRowsM / 2;  // of a weight tile: gate or up rows with SwiGLU
+// SwiGLU: what gate and up warps hand each other, per warpgroup two slots of 8 tokens x 64 channels either way
+constexpr uint32_t kSlot = 8 * kHalfRows, kExchangeBytes = 2 * 2 * 2 * kSlot * 4;
+template <int N>
+constexpr uint32_t pair_stage_bytes() { return kWTile + N / 2 * kStepK; }
+constexpr uint32_t kPairTail = 1024 + 256 + kEpiWarps * 128 * 4;  // alignment of the base; barriers, tensor-memory address; scales
+
+// Whether `yes` holds in all threads of some warps of the block, which meet here.
+__device__ __forceinline__ bool block_all(int id, int threads, bool yes) {
+    uint32_t all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\tbarrier.cta.red.and.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(all)
+        : "r"(id), "r"(threads), "r"(static_cast<uint32_t>(yes))
+        : "memory");
+    return all != 0;
+}
+
+struct PairTiles {
+    uint32_t t_tiles, r_tiles, band;
+};
+// Tile t of the flat list: bands of `band` token tiles, inside a band the token tile varies fastest.
+__device__ __forceinline__ void tile_of(const PairTiles& p, uint32_t t, uint32_t& tt, uint32_t& rt) {
+    const uint32_t per_band = p.band * p.r_tiles;
+    const uint32_t b = t / per_band, r = t - b * per_band;
+    const uint32_t rows = min(p.band, p.t_tiles - b * p.band);
+    rt = r / rows;
+    tt = b * p.band + (r - rt * rows);
+}
+
+template <bool SWIGLU, int N>
+__global__ void __launch_bounds__(kPairThreads, 1)
+gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a,
+                    const __grid_constant__ GemmI8Params p, const __grid_constant__ PairTiles tl) {
+    constexpr uint32_t kStageBytes = pair_stage_bytes<N>();
+    constexpr uint32_t kTok = N / 2;                               // tokens that a CTA loads, and that a warpgroup finishes
+    constexpr uint32_t kChannels = SWIGLU ? kHalfRows : kRowsM;    // of a CTA's tile
+    extern __shared__ unsigned char smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;  // swizzled tiles want 1024-byte alignment
+    unsigned char* smem = smem_raw + (base - raw);
+    const uint32_t bars_at = p.stages * kStageBytes;
+    auto bar = [&](int i) { return base + bars_at + 8u * i; };
+    volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(smem + bars_at + P_BARS * 8);
+    float* s_scales = reinterpret_cast<float*>(smem + bars_at + 256);
+    float* s_exchange = s_scales + kEpiWarps * 128;
+
+    const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
+    const uint32_t rank = cluster_rank();
+    const uint32_t worker = blockIdx.x / 2, workers = gridDim.x / 2;
+    const uint32_t tiles = tl.t_tiles * tl.r_tiles;
+
+    if (tid == 0) {
+        prefetch_tensor_map(&tm_w);
+        prefetch_tensor_map(&tm_a);
+        for (uint32_t s = 0; s < p.stages; ++s) {
+            mbar_init(bar(P_FULL + s), 1);
+            mbar_init(bar(P_EMPTY + s), 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(bar(P_ACC_FULL + a), 1);
+            mbar_init(bar(P_ACC_EMPTY + a), kEpiWarps * 2);  // one arrival per finishing warp of the pair
+        }
+        mbar_init_fence();
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(s_tmem)), 512);
+        tmem_relinquish_pair();
+    }
+    fence_before();
+    __syncthreads();
+    cluster_sync();  // the partner's barriers exist before anything is counted on them
+    fence_after();
+    const uint32_t tmem = *s_tmem;
+
+    grid_dep_launch_dependents();
+    grid_dep_wait();
+
+    auto gave_up = [&]() {
+        if (p.status) atomicOr(p.status, ATTN_STATUS_WAIT_TIMEOUT);
+    };
+    if (warp == 0) {
+        if (elect_one()) {
+            uint32_t s = 0, phase = 0, issued = 0;
+            bool ok = true;
+            for (uint32_t t = worker; t < tiles && ok; t += workers) {
+                uint32_t tt, rt;
+                tile_of(tl, t, tt, rt);
+                const uint32_t row = (rt * 2 + rank) * kChannels;
+                const int w0 = static_cast<int>(row), w1 = static_cast<int>(SWIGLU ? p.n_out + row : row + kHalfRows);
+                const int tok = static_cast<int>(tt * N + rank * kTok);
+                for (uint32_t ks = 0; ks < p.k_steps; ++ks, ++issued) {
+                    if (issued >= p.stages && !mbar_wait(bar(P_EMPTY + s), phase ^ 1)) {
+                        gave_up();
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t dst = base + s * kStageBytes, full = bar(P_FULL + s);
+                    const int kc = static_cast<int>(ks * kStepK);
+                    if (rank == 0) mbar_arrive_expect_tx(full, 2 * kStageBytes);
+                    tma_load_2d_pair(dst, &tm_w, full, kc, w0);
+                    tma_load_2d_pair(dst + kWTile / 2, &tm_w, full, kc, w1);
+                    tma_load_2d_pair(dst + kWTile, &tm_a, full, kc, tok);
+                    if (++s == p.stages) s = 0, phase ^= 1;
+                }
+            }
+            // No copy is in flight when the pair ends, whatever became of the MMAs: the leader's barriers count both CTAs' bytes,
+            // and the CTAs meet at the end.
+            if (rank == 0)
+                for (uint32_t i = issued > p.stages ? issued - p.stages : 0; i < issued; ++i)
+                    mbar_wait(bar(P_FULL + i % p.stages), i / p.stages & 1);
+        }
+    } else if (warp == 1) {
+        if (rank == 0 && elect_one()) {
+            constexpr uint32_t idesc = instr_desc_i8(2 * kRowsM, N);
+            const uint64_t desc0 = smem_desc(base, 16, 1024);
+            uint32_t s = 0, phase = 0, local = 0;
+            bool ok = true;
+            for (uint32_t t = worker; t < tiles && ok; t += workers, ++local) {
+                const uint32_t buf = local & 1;
+                if (local >= 2 && !mbar_wait(bar(P_ACC_EMPTY + buf), (local / 2 - 1) & 1)) {
+                    gave_up();
+                    break;
+                }
+                fence_after();
+                const uint32_t d = tmem + buf * 256;
+                for (uint32_t ks = 0; ks < p.k_steps; ++ks) {
+                    if (!mbar_wait(bar(P_FULL + s), phase)) {
+                        gave_up();
+                        ok = false;
+                        break;
+                    }
+                    fence_after();
+                    // K-major operands, 128-byte swizzle: 32 bytes per k-step of 32, 8-row groups 1024 bytes apart
+                    const uint64_t w = desc0 + s * (kStageBytes / 16), a = w + kWTile / 16;
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) mma_i8_pair(d, w + 2 * kk, a + 2 * kk, idesc, ks | kk);
+                    commit_pair(bar(P_EMPTY + s));  // the stage may be refilled once these MMAs have read it
+                    if (++s == p.stages) s = 0, phase ^= 1;
+                }
+                commit_pair(bar(P_ACC_FULL + buf));
+            }
+        }
+    } else {
+        const uint32_t quarter = warp & 3;       // the tensor-memory lanes that this warp may read
+        const uint32_t group = (warp - 2) >> 2;  // its half of the tokens
+        const uint32_t lane_addr = tmem + ((quarter * 32) << 16) + group * kTok;
+        float* s_scale = s_scales + (warp - 2) * 128;
+        const uint32_t empty0 = cluster_address(bar(P_ACC_EMPTY), 0);  // the leader's, also for its partner
+        // SwiGLU: quarters 0 and 1 hold the gate rows, 2 and 3 the up rows of the same 64 channels
+        const bool is_up = SWIGLU && quarter >= 2;
+        const uint32_t in_tile = SWIGLU ? (quarter & 1) * 32 + lane : quarter * 32 + lane;
+        uint32_t local = 0, slot = 0;
+        for (uint32_t t = worker; t < tiles; t += workers, ++local) {
+            uint32_t tt, rt;
+            tile_of(tl, t, tt, rt);
+            const uint32_t buf = local & 1, tok0 = tt * N + group * kTok;
+            const uint32_t col = (rt * 2 + rank) * kChannels + in_tile;
+            const bool live = col < p.n_out;
+            const float ws = live ? p.w_scale[is_up ? p.n_out + col : col] : 0.f;
+#pragma unroll
+            for (uint32_t i = lane; i < kTok; i += 32) s_scale[i] = tok0 + i < p.m ? p.a_scale[tok0 + i] : 0.f;
+            __syncwarp();
+            const uint32_t tokens = tok0 < p.m ? min(kTok, p.m - tok0) : 0u;
+            // (a vote, so that the warp, with SwiGLU the warpgroup, gives up or goes on as one)
+            const bool there = mbar_wait(bar(P_ACC_FULL + buf), (local / 2) & 1);
+            if (!(SWIGLU ? block_all(1 + group, 128, there) : __all_sync(0xffffffffu, there))) {
+                if (lane == 0) gave_up();
+                break;
+            }
+            fence_after();
+            with_out_type(p.out_dtype, [&](auto type) {
+                using T = decltype(type);
+                T* dst = static_cast<T*>(p.out) + static_cast<size_t>(tok0) * p.ldc + col;
+#pragma unroll 1
+                for (uint32_t c = 0; c < kTok; c += 16) {
+                    uint32_t r[16];
+                    ld16(lane_addr + buf * 256 + c, r);
+                    wait_ld(r);
+                    if (c + 16 == kTok) {  // the accumulator is read: hand it back
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster_relaxed(empty0 + 8 * buf);
+                    }
+                    float y[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) y[i] = scaled(static_cast<int32_t>(r[i]), ws, s_scale[c + i]);
+                    if constexpr (SWIGLU) {
+                        // gate warps finish the chunk's first 8 tokens and up warps the last 8
+                        float* to = s_exchange + ((group * 2 + slot) * 2 + is_up) * kSlot + in_tile;
+                        const float* from = s_exchange + ((group * 2 + slot) * 2 + !is_up) * kSlot + in_tile;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) to[i * kHalfRows] = is_up ? y[i] : y[8 + i];
+                        named_bar_sync(1 + group, 128);
+                        slot ^= 1;  // (whoever writes a slot again has passed the barrier behind its last reads)
+                        const uint32_t c0 = c + (is_up ? 8 : 0);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float other = from[i * kHalfRows];
+                            const float gate = is_up ? other : y[i], up = is_up ? y[8 + i] : other;
+                            if (live && c0 + i < tokens) dst[(c0 + i) * p.ldc] = to_out<T>(__fmul_rn(silu(gate), up));
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (live && c + i < tokens) dst[(c + i) * p.ldc] = to_out<T>(y[i]);
+                    }
+                    __syncwarp();
+                }
+            });
+        }
+    }
+
+    // ---- common exit: everybody (of both CTAs) meets, then the allocating warp releases tensor memory ----
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    cluster_sync();
+    if (warp == 1) {
+        fence_after();
+        tmem_dealloc_pair(tmem, 512);
     }
 }
 
@@ -288,7 +575,7 @@ int launch_stream(Operands& o) {
     p.stages = std::min<uint32_t>(kStreamMaxStages, (kMaxDynamicSmem / 2 - 2048 - kStreamTail) / stage);
     const uint64_t tiles = static_cast<uint64_t>(row_tiles) * tok_tiles;
     uint32_t slices = 1;
-    while (slices < 8 && slices < p.k_steps && tiles * (slices + 1) <= 2ull * o.dev.sm_count) ++slices;
+    while (slices < kMaxSlices && 2 * slices <= p.k_steps && tiles * slices * 2 <= 2ull * o.dev.sm_count) slices *= 2;
     if (slices > 1 && p.stages * stage < PARTS * N * kRowsM * 4) slices = 1;  // (the slices' sums lie where the tiles were)
     const uint32_t smem = p.stages * stage + kStreamTail;
     CUtensorMap tm_w, tm_a;
@@ -316,9 +603,58 @@ int launch_stream(Operands& o) {
     return ATTN_OK;
 }
 
+template <bool SWIGLU, int N>
+int launch_pair(Operands& o) {
+    GemmI8Params& p = o.p;
+    constexpr uint32_t stage = pair_stage_bytes<N>(), span = SWIGLU ? kRowsM : 2 * kRowsM;
+    const uint32_t fixed = kPairTail + (SWIGLU ? kExchangeBytes : 0);
+    p.stages = std::min<uint32_t>(kPairMaxStages, (kMaxDynamicSmem - fixed) / stage);
+    PairTiles tl{};
+    tl.t_tiles = (p.m + N - 1) / N;
+    tl.r_tiles = (p.n_out + span - 1) / span;
+    if (static_cast<uint64_t>(tl.t_tiles) * tl.r_tiles > 0x7fffffffu) return ATTN_ERR_UNSUPPORTED;
+    // token tiles of a band: a wave of 74 tiles is then about as many tokens as channels, the least to read (9184 x 4096 x 28672 with
+    // SwiGLU: bands of 4, 8, 16, 36 tiles 749, 708, 786, 784 us; 9184 x 14336 x 4096 326, 322, 331, 354)
+    tl.band = std::min<uint32_t>(tl.t_tiles, 8);
+    CUtensorMap tm_w, tm_a;
+    int rc;
+    if ((rc = make_map(&tm_w, o.a->w, o.w_rows, o.a->k, o.w_stride, kHalfRows)) != ATTN_OK) return rc;
+    if ((rc = make_map(&tm_a, o.a->a, p.m, o.a->k, o.a_stride, N / 2)) != ATTN_OK) return rc;
+    auto kernel = gemm_i8_pair_kernel<SWIGLU, N>;
+    B200_CUDA_TRY(allow_max_smem(kernel));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(2 * std::min(tl.t_tiles * tl.r_tiles, static_cast<uint32_t>(o.dev.sm_count) / 2));
+    cfg.blockDim = dim3(kPairThreads);
+    cfg.dynamicSmemBytes = p.stages * stage + fixed;
+    cfg.stream = o.stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, tm_w, tm_a, p, tl));
+    g_launch_count.fetch_add(1, std::memory_order_relaxed);
+    return ATTN_OK;
+}
+
 template <int PARTS>
 int launch_gemm(Operands& o) {
-    return o.p.m <= 16 ? launch_stream<PARTS, 16>(o) : o.p.m <= 32 ? launch_stream<PARTS, 32>(o) : o.p.m <= 64 ? launch_stream<PARTS, 64>(o) : launch_stream<PARTS, 128>(o);
+    constexpr bool kSwiglu = PARTS == 2;
+    const uint32_t m = o.p.m;
+    if (m <= 16) return launch_stream<PARTS, 16>(o);
+    if (m <= 32) return launch_stream<PARTS, 32>(o);
+    if (m <= 64) return launch_stream<PARTS, 64>(o);
+    // Tiles of 256 tokens or of 128: the fewer waves of pairs, a wave of the smaller ones being half as long. What fits one wave
+    // of the larger ones is better spread (1003 x 14336 x 4096: 45.3 us for 49.3, 300 x 14336 x 4096 23.2 for 37.9), what does not has
+    // less to move with them (9184 x 14336 x 4096: 322 for 361, 2048 x 4096 x 28672 with SwiGLU 167 for 182).
+    const uint64_t pairs = o.dev.sm_count / 2, r_tiles = (o.p.n_out + (kSwiglu ? kRowsM : 2 * kRowsM) - 1) / (kSwiglu ? kRowsM : 2 * kRowsM);
+    auto waves = [&](uint32_t n) { return ((m + n - 1) / n * r_tiles + pairs - 1) / pairs; };
+    const uint64_t wide = waves(256) * 100, narrow = waves(128) * (waves(256) == 1 ? 48 : 54);
+    return wide <= narrow ? launch_pair<kSwiglu, 256>(o) : launch_pair<kSwiglu, 128>(o);
 }
 
 }  // namespace
@@ -358,6 +694,7 @@ extern "C" int attn_gemm_i8(const AttnGemmI8Args* a, void* stream_v) {
     p.n_out = a->n_out;
     p.k_steps = (a->k + kStepK - 1) / kStepK;
     p.out_dtype = a->out_dtype;
+    p.w_early = a->w_early ? 1u : 0u;
     p.status = a->status;
     o.stream = static_cast<cudaStream_t>(stream_v);
     return a->swiglu ? launch_gemm<2>(o) : launch_gemm<1>(o);

@@ -6,13 +6,17 @@
 // yields both reductions, and q, made of single fp32 operations on single elements, does not depend on the order of any sum. The largest
 // |z| is found on the bits without their sign, which order as the numbers do and put infinity and NaN on top.
 //
-// Bound by memory: every value is read once and written once. A row stays in the registers of its threads between the reductions and
-// the rounding (CHUNKS runs of VEC values a thread; CHUNKS 0, for rows longer than that: read twice, the second time from L2).
+// Bound by memory: every value is read once and written once (norm of 9184 x 4096 fp32 with its delta 74.1 us = 6.6 TB/s, quantisation of
+// 9184 x 4096 fp32 28.3 us = 6.6 TB/s, of 9184 x 14336 bf16 65.7 us = 6.0 TB/s; one row 1.9 - 2.1 us in a graph). A row stays in the
+// registers of its threads between the reductions and the rounding. Close behind memory come the instructions, ~ 10 a value: sums,
+// products and maxima take two values at a time, whole numbers come out of the low bits of a sum, 16-bit rows are searched without
+// widening them (bf16, 14336 wide: 87 -> 66 us).
 #include <algorithm>
 
 #include "attn_internal.cuh"
 #include "operand_memory.cuh"
 #include "ptx_sm100.cuh"
+#include "tcgen05_sm100.cuh"
 
 namespace b200 {
 namespace {
@@ -27,12 +31,14 @@ struct RowsParams {
     uint64_t q_stride, x_stride, delta_stride, x_out_stride;
     uint32_t rows, dim;
     uint32_t row_threads;  // of a row: 32 (a block serves several rows) or the whole block
+    uint32_t whole16;      // rows are a multiple of 16 bytes long
     float eps;
     int32_t delta_dtype;
 };
 
 constexpr uint32_t kMaxThreads = 1024, kWarpRows = 4;  // threads of a block, rows of one whose rows are a warp's
 constexpr uint32_t kInf = 0x7f800000u;
+constexpr float kLiftTiny = 18446744073709551616.f;  // 2^64
 // (four runs of eight values of x, delta and weight beside each other do not fit the 64 registers that 1024 threads have each)
 constexpr uint32_t max_threads(bool norm, int vec, uint32_t chunks) { return norm && vec == 8 && chunks == 4 ? 512 : kMaxThreads; }
 
@@ -41,12 +47,12 @@ template <int VEC>
 struct Raw {
     uint32_t w[VEC];
 };
-// `n` of the VEC values from element i on; ALIGNED: p + i may be read in runs of VEC values.
+// `n` of the VEC values from element i on. ALIGNED: all of them, in one run.
 template <int VEC, bool ALIGNED>
 __device__ __forceinline__ void load(Raw<VEC>& r, const void* p, size_t i, bool wide32, uint32_t n) {
     if (wide32) {
         const uint32_t* s = static_cast<const uint32_t*>(p) + i;
-        if (ALIGNED && n >= VEC) {
+        if constexpr (ALIGNED) {
 #pragma unroll
             for (int k = 0; k < VEC; k += 4) *reinterpret_cast<uint4*>(&r.w[k]) = *reinterpret_cast<const uint4*>(s + k);
         } else {
@@ -55,7 +61,7 @@ __device__ __forceinline__ void load(Raw<VEC>& r, const void* p, size_t i, bool 
         }
     } else {
         const unsigned short* s = static_cast<const unsigned short*>(p) + i;
-        if (ALIGNED && n >= VEC) {
+        if constexpr (ALIGNED) {
             if constexpr (VEC == 8) *reinterpret_cast<uint4*>(&r.w[0]) = *reinterpret_cast<const uint4*>(s);
             else *reinterpret_cast<uint2*>(&r.w[0]) = *reinterpret_cast<const uint2*>(s);
         } else {
@@ -88,7 +94,7 @@ template <int VEC, int DT, bool ALIGNED>
 __device__ __forceinline__ void store(void* p, size_t i, const float (&v)[VEC], uint32_t n) {
     if constexpr (DT == ATTN_DTYPE_F32) {
         float* d = static_cast<float*>(p) + i;
-        if (ALIGNED && n >= VEC) {
+        if constexpr (ALIGNED) {
 #pragma unroll
             for (int k = 0; k < VEC; k += 4) *reinterpret_cast<float4*>(d + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
         } else {
@@ -101,7 +107,7 @@ __device__ __forceinline__ void store(void* p, size_t i, const float (&v)[VEC], 
         uint32_t u[VEC / 2];
 #pragma unroll
         for (int k = 0; k < VEC; k += 2) u[k / 2] = pack2<DT == ATTN_DTYPE_BF16>(v[k], v[k + 1]);
-        if (ALIGNED && n >= VEC) {
+        if constexpr (ALIGNED) {
             if constexpr (VEC == 8) *reinterpret_cast<uint4*>(d) = make_uint4(u[0], u[1], u[2], u[3]);
             else *reinterpret_cast<uint2*>(d) = make_uint2(u[0], u[1]);
         } else {
@@ -112,29 +118,174 @@ __device__ __forceinline__ void store(void* p, size_t i, const float (&v)[VEC], 
     }
 }
 
-// A row's reductions, the same in all its threads: the largest bits and the sum.
-__device__ __forceinline__ void reduce_row(uint32_t& top, float& sum, bool whole_block) {
-    top = __reduce_max_sync(0xffffffffu, top);
+using tc::f32x2;
+
+// h and z of VEC values as they were read, two at a time; the weight is the same for every row, and comes from L1.
+template <int DT, bool NORM, bool DELTA, int VEC, bool ALIGNED>
+__device__ __forceinline__ void combine(const RowsParams& p, uint32_t i, const Raw<VEC>& rx, const Raw<VEC>& rd, float (&h)[VEC], float (&z)[VEC]) {
+    Raw<VEC> rw;
+    if constexpr (NORM) load<VEC, ALIGNED>(rw, p.weight, i, true, p.dim - i);
+    widen<VEC>(h, rx, DT);
+    float d[VEC];
+    if constexpr (DELTA) widen<VEC>(d, rd, p.delta_dtype);
 #pragma unroll
-    for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    for (int k = 0; k < VEC; k += 2) {
+        f32x2 v = tc::pack_f32x2(h[k], h[k + 1]);
+        if constexpr (DELTA) {
+            v = tc::add_f32x2(v, tc::pack_f32x2(d[k], d[k + 1]));
+            tc::unpack_f32x2(v, h[k], h[k + 1]);
+        }
+        if constexpr (NORM) v = tc::mul_f32x2(v, tc::pack_f32x2(__uint_as_float(rw.w[k]), __uint_as_float(rw.w[k + 1])));
+        tc::unpack_f32x2(v, z[k], z[k + 1]);
+    }
+}
+
+// The largest |z| so far and two sums of h^2. NaN counts as more than any number.
+struct Found {
+    float top = 0.f;
+    f32x2 sum = 0;  // (two zeros)
+    uint32_t top16 = 0;  // of 16-bit rows as they are: two largest ones, side by side
+};
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+    float d;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+template <bool NORM, int VEC>
+__device__ __forceinline__ void count(const float (&h)[VEC], const float (&z)[VEC], Found& f) {
+#pragma unroll
+    for (int k = 0; k < VEC; k += 2) {
+        f.top = max_abs(f.top, z[k], z[k + 1]);
+        if constexpr (NORM) {
+            const f32x2 v = tc::pack_f32x2(h[k], h[k + 1]);
+            f.sum = tc::fma_f32x2(v, v, f.sum);
+        }
+    }
+}
+// The same of 16-bit values that nothing is done to, without widening them.
+template <int DT, int VEC>
+__device__ __forceinline__ void count16(const Raw<VEC>& r, Found& f) {
+#pragma unroll
+    for (int k = 0; k < VEC / 2; ++k) {
+        const uint32_t v = r.w[k] & 0x7fff7fffu;
+        if constexpr (DT == ATTN_DTYPE_BF16) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(f.top16) : "r"(v));
+        else asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(f.top16) : "r"(v));
+    }
+}
+
+// A row's reductions, the same in all its threads: the largest bits and the sum. s_top, s_sum: a value per warp, in other places for the
+// block's next row.
+template <int DT, bool NORM>
+__device__ __forceinline__ void reduce_row(const Found& f, uint32_t& top, float& sum, bool whole_block, uint32_t* s_top, float* s_sum) {
+    top = __float_as_uint(f.top);
+    if constexpr (!NORM && DT != ATTN_DTYPE_F32) {
+        float lo, hi;
+        tc::unpack2<DT == ATTN_DTYPE_BF16>(f.top16, lo, hi);
+        top = max(top, max(__float_as_uint(lo), __float_as_uint(hi)));
+    }
+    float odd;
+    tc::unpack_f32x2(f.sum, sum, odd);
+    sum += odd;
+    top = __reduce_max_sync(0xffffffffu, top);
+    if constexpr (NORM) {
+#pragma unroll
+        for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    }
     if (!whole_block) return;
-    __shared__ uint32_t s_top[kMaxThreads / 32];
-    __shared__ float s_sum[kMaxThreads / 32];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (lane == 0) s_top[warp] = top, s_sum[warp] = sum;
     __syncthreads();
     const bool there = lane < blockDim.x / 32;
     top = __reduce_max_sync(0xffffffffu, there ? s_top[lane] : 0u);
-    sum = there ? s_sum[lane] : 0.f;
+    if constexpr (NORM) {
+        sum = there ? s_sum[lane] : 0.f;
 #pragma unroll
-    for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    }
 }
 
-// DT: type of x. NORM: weight, and the norm's factor in the scale. ALIGNED: rows may be read and written in runs of VEC values.
+// What turns a row's z into whole numbers.
+struct Rounding {
+    float inverse;  // 127 / A, A lifted where tiny
+    bool tiny;      // 127 / A leaves fp32's range below 2^-121: such rows are lifted first, which is exact
+    bool bad;
+};
+// ... and its scale, which thread `first` writes.
+template <bool NORM>
+__device__ __forceinline__ Rounding finish_row(const RowsParams& p, uint32_t row, uint32_t top, float sum, bool first) {
+    Rounding r;
+    const float a = __uint_as_float(top);
+    r.tiny = top < 0x03000000u;
+    r.bad = top >= kInf || (NORM && !(sum < __uint_as_float(kInf)));
+    r.inverse = top == 0 || r.bad ? 0.f : __fdiv_rn(127.f, r.tiny ? a * kLiftTiny : a);
+    if (first) {
+        float scale = a;
+        if constexpr (NORM) scale *= __frcp_rn(sqrtf(sum / static_cast<float>(p.dim) + p.eps));
+        p.scale[row] = r.bad ? __uint_as_float(0x7fc00000u) : __fdiv_rn(scale, 127.f);
+    }
+    return r;
+}
+// `n` of VEC whole numbers.
+template <int VEC, bool ALIGNED>
+__device__ __forceinline__ void put(int8_t* q, const float (&z)[VEC], const Rounding& r, uint32_t n) {
+    uint32_t u[VEC / 4];
+    // 1.5 * 2^23 puts the whole number next to a value of at most 2^22 (ties to the even one) into the low bits of the sum
+    const f32x2 magic = tc::pack_f32x2(12582912.f, 12582912.f);
+    const bool special = r.tiny || r.bad;
+#pragma unroll
+    for (int k = 0; k < VEC; k += 4) {
+        float b[4];
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+            float v0 = z[k + e], v1 = z[k + e + 1];
+            if (special) v0 = r.bad ? 0.f : v0 * kLiftTiny, v1 = r.bad ? 0.f : v1 * kLiftTiny;
+            // (the products one by one: a packed product and the packed sum behind it came out as if fused, rounded once)
+            tc::unpack_f32x2(tc::add_f32x2(tc::pack_f32x2(__fmul_rn(v0, r.inverse), __fmul_rn(v1, r.inverse)), magic), b[e], b[e + 1]);
+        }
+        u[k / 4] = __byte_perm(__byte_perm(__float_as_uint(b[0]), __float_as_uint(b[1]), 0x0040),
+                               __byte_perm(__float_as_uint(b[2]), __float_as_uint(b[3]), 0x0040), 0x5410);
+    }
+    if (ALIGNED || n >= VEC) {
+        if constexpr (VEC == 8) *reinterpret_cast<uint2*>(q) = make_uint2(u[0], u[1]);
+        else *reinterpret_cast<uint32_t*>(q) = u[0];
+    } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+            if (k < n) q[k] = static_cast<int8_t>(u[k / 4] >> (8 * (k & 3)));
+    }
+}
+
+// A row between its reductions and its rounding: z, or 16-bit values that nothing is done to as they are, in half the registers.
+template <int DT, bool NORM, int VEC, int CHUNKS>
+struct Kept {
+    static constexpr bool kRaw = !NORM && DT != ATTN_DTYPE_F32;
+    uint32_t raw[kRaw ? CHUNKS : 1][VEC / 2];
+    float z[kRaw ? 1 : CHUNKS][VEC];
+    __device__ __forceinline__ void keep(int c, const Raw<VEC>& r) {
+#pragma unroll
+        for (int k = 0; k < VEC / 2; ++k) raw[c][k] = r.w[k];
+    }
+    __device__ __forceinline__ const float (&values(int c))[VEC] {
+        if constexpr (kRaw) {
+            Raw<VEC> r;
+#pragma unroll
+            for (int k = 0; k < VEC / 2; ++k) r.w[k] = raw[c][k];
+            widen<VEC>(z[0], r, DT);
+            return z[0];
+        } else {
+            return z[c];
+        }
+    }
+};
+
+// A row per block, or per warp. DT: type of x. NORM: weight, and the norm's factor in the scale. ALIGNED: rows may be read and written
+// in runs of VEC values. CHUNKS runs a thread, or 0: a row longer than that, read twice.
 template <int DT, bool NORM, bool DELTA, int VEC, int CHUNKS, bool ALIGNED>
 __global__ void __launch_bounds__(max_threads(NORM, VEC, CHUNKS)) rows_i8_kernel(const __grid_constant__ RowsParams p) {
     grid_dep_launch_dependents();
     grid_dep_wait();
+    __shared__ uint32_t s_top[kMaxThreads / 32];
+    __shared__ float s_sum[kMaxThreads / 32];
     const bool whole_block = p.row_threads != 32;
     const uint32_t row = whole_block ? blockIdx.x : blockIdx.x * kWarpRows + (threadIdx.x >> 5);
     const uint32_t t = whole_block ? threadIdx.x : threadIdx.x & 31;
@@ -142,113 +293,138 @@ __global__ void __launch_bounds__(max_threads(NORM, VEC, CHUNKS)) rows_i8_kernel
     const size_t x_row = row * p.x_stride, d_row = row * p.delta_stride, o_row = row * p.x_out_stride;
     const bool wide_delta = p.delta_dtype == ATTN_DTYPE_F32;
     int8_t* q = p.q + row * p.q_stride;
-
-    auto fetch = [&](uint32_t i, Raw<VEC>& rx, Raw<VEC>& rd, Raw<VEC>& rw) {
-        const uint32_t n = p.dim - i;
+    // Without a branch, so that a thread's loads are requested one behind the other: past the row's end its last values again, or none.
+    // (Branches around them had the compiler wait for one run before it asked for the next: 9184 x 4096 fp32 31 -> 49 us.)
+    auto fetch = [&](uint32_t i, Raw<VEC>& rx, Raw<VEC>& rd) {
+        const uint32_t n = i < p.dim ? p.dim - i : 0u;
+        if constexpr (ALIGNED) i = min(i, p.dim - VEC);
         load<VEC, ALIGNED>(rx, p.x, x_row + i, DT == ATTN_DTYPE_F32, n);
         if constexpr (DELTA) load<VEC, ALIGNED>(rd, p.delta, d_row + i, wide_delta, n);
-        if constexpr (NORM) load<VEC, ALIGNED>(rw, p.weight, i, true, n);
     };
-    auto combine = [&](const Raw<VEC>& rx, const Raw<VEC>& rd, const Raw<VEC>& rw, float (&h)[VEC], float (&z)[VEC]) {
-        widen<VEC>(h, rx, DT);
-        if constexpr (DELTA) {
-            float d[VEC];
-            widen<VEC>(d, rd, p.delta_dtype);
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) h[k] = __fadd_rn(h[k], d[k]);
-        }
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) z[k] = NORM ? __fmul_rn(h[k], __uint_as_float(rw.w[k])) : h[k];
-    };
-    auto count = [&](const float (&h)[VEC], const float (&z)[VEC], uint32_t& top, float& sum) {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-            top = max(top, __float_as_uint(z[k]) & 0x7fffffffu);
-            if constexpr (NORM) sum = fmaf(h[k], h[k], sum);
-        }
-    };
-    float inverse, lift;
-    auto scale_of = [&](uint32_t top, float sum) {
-        const float a = __uint_as_float(top);
-        // (127 / A leaves fp32's range below 2^-121: such rows are lifted first, which is exact)
-        lift = top < 0x03000000u ? 18446744073709551616.f : 1.f;
-        inverse = top == 0 ? 0.f : __fdiv_rn(127.f, __fmul_rn(a, lift));
-        float scale = a;
-        if constexpr (NORM) scale *= __frcp_rn(sqrtf(sum / static_cast<float>(p.dim) + p.eps));
-        scale = __fdiv_rn(scale, 127.f);
-        const bool bad = top >= kInf || (NORM && !(sum < __uint_as_float(kInf)));
-        if (bad) inverse = 0.f, scale = __uint_as_float(0x7fc00000u);
-        if (t == 0) p.scale[row] = scale;
-        return bad;
-    };
-    auto put = [&](uint32_t i, const float (&z)[VEC], bool bad) {
-        const uint32_t n = p.dim - i;
-        uint32_t u[VEC / 4];
-#pragma unroll
-        for (int k = 0; k < VEC; k += 4) {
-            uint32_t b[4];
-#pragma unroll
-            // 1.5 * 2^23 puts the whole number next to a value of at most 2^22 (ties to the even one) into the low bits of the sum
-            for (int e = 0; e < 4; ++e)
-                b[e] = __float_as_uint(__fadd_rn(__fmul_rn(__fmul_rn(z[k + e], lift), inverse), 12582912.f));
-            u[k / 4] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-            if (bad) u[k / 4] = 0u;
-        }
-        if (n >= VEC) {
-            if constexpr (VEC == 8) *reinterpret_cast<uint2*>(q + i) = make_uint2(u[0], u[1]);
-            else *reinterpret_cast<uint32_t*>(q + i) = u[0];
-        } else {
-#pragma unroll
-            for (int k = 0; k < VEC; ++k)
-                if (k < n) q[i + k] = static_cast<int8_t>(u[k / 4] >> (8 * (k & 3)));
-        }
-    };
-
-    uint32_t top = 0;
-    float sum = 0.f;
+    Found found;
+    uint32_t top;
+    float sum;
     if constexpr (CHUNKS > 0) {
-        Raw<VEC> rx[CHUNKS], rd[CHUNKS], rw[CHUNKS];
-        float z[CHUNKS][VEC];
+        Raw<VEC> rx[CHUNKS], rd[CHUNKS];
+        Kept<DT, NORM, VEC, CHUNKS> kept;
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-            const uint32_t i = (c * p.row_threads + t) * VEC;
-            if (i < p.dim) fetch(i, rx[c], rd[c], rw[c]);
-        }
+        for (int c = 0; c < CHUNKS; ++c) fetch((c * p.row_threads + t) * VEC, rx[c], rd[c]);
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             const uint32_t i = (c * p.row_threads + t) * VEC;
             if (i < p.dim) {
-                float h[VEC];
-                combine(rx[c], rd[c], rw[c], h, z[c]);
-                count(h, z[c], top, sum);
-                if constexpr (DELTA)
-                    if (p.x_out) store<VEC, DT, ALIGNED>(p.x_out, o_row + i, h, p.dim - i);
+                if constexpr (kept.kRaw) {
+                    count16<DT, VEC>(rx[c], found);
+                    kept.keep(c, rx[c]);
+                } else {
+                    float h[VEC];
+                    combine<DT, NORM, DELTA, VEC, ALIGNED>(p, i, rx[c], rd[c], h, kept.z[c]);
+                    count<NORM, VEC>(h, kept.z[c], found);
+                    if constexpr (DELTA)
+                        if (p.x_out) store<VEC, DT, ALIGNED>(p.x_out, o_row + i, h, p.dim - i);
+                }
             }
         }
-        reduce_row(top, sum, whole_block);
-        const bool bad = scale_of(top, sum);
+        reduce_row<DT, NORM>(found, top, sum, whole_block, s_top, s_sum);
+        const Rounding r = finish_row<NORM>(p, row, top, sum, t == 0);
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             const uint32_t i = (c * p.row_threads + t) * VEC;
-            if (i < p.dim) put(i, z[c], bad);
+            if (i < p.dim) put<VEC, ALIGNED>(q + i, kept.values(c), r, p.dim - i);
         }
     } else {
-        Raw<VEC> rx, rd, rw;
+        Raw<VEC> rx, rd;
         float h[VEC], z[VEC];
         for (uint32_t i = t * VEC; i < p.dim; i += p.row_threads * VEC) {
-            fetch(i, rx, rd, rw);
-            combine(rx, rd, rw, h, z);
-            count(h, z, top, sum);
+            fetch(i, rx, rd);
+            combine<DT, NORM, DELTA, VEC, ALIGNED>(p, i, rx, rd, h, z);
+            count<NORM, VEC>(h, z, found);
         }
-        reduce_row(top, sum, whole_block);
-        const bool bad = scale_of(top, sum);
-        for (uint32_t i = t * VEC; i < p.dim; i += p.row_threads * VEC) {  // (x_out may be x: nothing was written before)
-            fetch(i, rx, rd, rw);
-            combine(rx, rd, rw, h, z);
+        reduce_row<DT, NORM>(found, top, sum, whole_block, s_top, s_sum);
+        const Rounding r = finish_row<NORM>(p, row, top, sum, t == 0);
+        for (uint32_t i = t * VEC; i < p.dim; i += p.row_threads * VEC) {  // (x_out may be x: nothing of the row was written before)
+            fetch(i, rx, rd);
+            combine<DT, NORM, DELTA, VEC, ALIGNED>(p, i, rx, rd, h, z);
             if constexpr (DELTA)
                 if (p.x_out) store<VEC, DT, ALIGNED>(p.x_out, o_row + i, h, p.dim - i);
-            put(i, z, bad);
+            put<VEC, ALIGNED>(q + i, z, r, p.dim - i);
         }
+    }
+}
+
+// Many rows: a block takes every grid-th one, through a ring of whole rows in shared memory that bulk copies fill, so that reads go on
+// while rows are reduced, rounded and stored. Rows lie on 16-byte boundaries and are a multiple of 16 bytes long.
+constexpr uint32_t kSlots = 2;
+constexpr uint32_t kRingTail = 16 * kMaxThreads / 32 + 64, kRingBytes = kMaxDynamicSmem - kRingTail;  // two turns' reductions, barriers; the rest
+template <int DT, bool NORM, bool DELTA, int VEC, int CHUNKS>
+__global__ void __launch_bounds__(kMaxThreads) rows_i8_ring_kernel(const __grid_constant__ RowsParams p) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    uint32_t* s_top = reinterpret_cast<uint32_t*>(smem);  // [2][warps]: a thread is past the barrier of the row between before it
+                                                          // writes where another may still have read
+    float* s_sum = reinterpret_cast<float*>(s_top + 2 * (kMaxThreads / 32));
+    const uint32_t full = smem_u32(smem) + 16 * (kMaxThreads / 32);
+    unsigned char* ring = smem + kRingTail;  // [kSlots]{x, delta}
+    const uint32_t x_bytes = p.dim * (DT == ATTN_DTYPE_F32 ? 4 : 2), d_bytes = DELTA ? p.dim * (p.delta_dtype == ATTN_DTYPE_F32 ? 4 : 2) : 0;
+    const uint32_t slot_bytes = x_bytes + d_bytes;
+    const uint32_t t = threadIdx.x;
+    if (t == 0) {
+        for (uint32_t s = 0; s < kSlots; ++s) mbar_init(full + 8 * s, 1);
+        mbar_init_fence();
+    }
+    __syncthreads();
+    grid_dep_launch_dependents();
+    grid_dep_wait();
+    const uint64_t policy = l2_policy_evict_first();
+    auto request = [&](uint32_t row, uint32_t slot) {  // thread 0
+        const uint32_t dst = smem_u32(ring) + slot * slot_bytes, bar = full + 8 * slot;
+        mbar_arrive_expect_tx(bar, slot_bytes);
+        bulk_g2s(dst, static_cast<const unsigned char*>(p.x) + row * p.x_stride * (DT == ATTN_DTYPE_F32 ? 4 : 2), x_bytes, bar, policy);
+        if constexpr (DELTA)
+            bulk_g2s(dst + x_bytes, static_cast<const unsigned char*>(p.delta) + row * p.delta_stride * (p.delta_dtype == ATTN_DTYPE_F32 ? 4 : 2),
+                     d_bytes, bar, policy);
+    };
+    const uint32_t mine = (p.rows - blockIdx.x + gridDim.x - 1) / gridDim.x;  // rows of this block
+    if (t == 0)
+        for (uint32_t s = 0; s < min(kSlots, mine); ++s) request(blockIdx.x + s * gridDim.x, s);
+    uint32_t slot = 0, phase = 0;
+    for (uint32_t n = 0; n < mine; ++n) {
+        const uint32_t row = blockIdx.x + n * gridDim.x;
+        // a wait that runs out makes the row one of NaN
+        Found found;
+        if (!mbar_wait(full + 8 * slot, phase)) found.top = __uint_as_float(0x7fffffffu);
+        const unsigned char* x = ring + slot * slot_bytes;
+        Kept<DT, NORM, VEC, CHUNKS> kept;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            const uint32_t i = (c * blockDim.x + t) * VEC;
+            if (i < p.dim) {
+                Raw<VEC> rx, rd;
+                load<VEC, true>(rx, x, i, DT == ATTN_DTYPE_F32, p.dim - i);
+                if constexpr (kept.kRaw) {
+                    count16<DT, VEC>(rx, found);
+                    kept.keep(c, rx);
+                } else {
+                    float h[VEC];
+                    if constexpr (DELTA) load<VEC, true>(rd, x + x_bytes, i, p.delta_dtype == ATTN_DTYPE_F32, p.dim - i);
+                    combine<DT, NORM, DELTA, VEC, true>(p, i, rx, rd, h, kept.z[c]);
+                    count<NORM, VEC>(h, kept.z[c], found);
+                    if constexpr (DELTA)
+                        if (p.x_out) store<VEC, DT, true>(p.x_out, row * p.x_out_stride + i, h, p.dim - i);
+                }
+            }
+        }
+        uint32_t top;
+        float sum;
+        reduce_row<DT, NORM>(found, top, sum, true, s_top + (n & 1) * (kMaxThreads / 32), s_sum + (n & 1) * (kMaxThreads / 32));
+        if (t == 0 && n + kSlots < mine) request(row + kSlots * gridDim.x, slot);  // (behind the barrier: all have read the slot)
+        const Rounding r = finish_row<NORM>(p, row, top, sum, t == 0);
+        int8_t* q = p.q + row * p.q_stride;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            const uint32_t i = (c * blockDim.x + t) * VEC;
+            if (i < p.dim) put<VEC, true>(q + i, kept.values(c), r, p.dim - i);
+        }
+        if (++slot == kSlots) slot = 0, phase ^= 1;
     }
 }
 
@@ -260,6 +436,24 @@ int launch_rows(RowsParams& p, bool aligned, const DeviceInfo& dev, cudaStream_t
     constexpr int kWide = DT == ATTN_DTYPE_F32 ? 4 : 8;
     const uint32_t vec = aligned ? kWide : 4;
     auto threads = [&](uint32_t chunks) { return ((p.dim + vec * chunks - 1) / (vec * chunks) + 31) / 32 * 32; };
+    const uint32_t row_bytes = p.dim * size_of(DT) + (DELTA ? p.dim * size_of(p.delta_dtype) : 0);
+    // Long rows in number: where few blocks of a row's threads fit an SM, the ring keeps the reads going. Quantisation of 9184 x 14336 bf16
+    // 78.7 -> 65.7 us, 5500 x 14336 fp32 87 -> 63, 4000 x 28672 fp16 77 -> 56, the norm of 2000 x 16384 bf16 with an fp32 delta 57 -> 53. Blocks
+    // of fewer threads do better without (quantisation of 9184 x 8192 bf16 36.6 for 51.3, of 4000 x 11008 25.1 for 30.5, the norm of 4096 x
+    // 8192 fp32 67.0 for 79.1, bf16 40.6 for 42.4).
+    constexpr uint32_t kRingFrom = !NORM ? 416 : DT == ATTN_DTYPE_F32 ? 544 : 512;
+    constexpr uint32_t kRingChunks = NORM && DT != ATTN_DTYPE_F32 ? 2 : 4;
+    const uint64_t slot = static_cast<uint64_t>(p.dim) * size_of(DT) + (DELTA ? static_cast<uint64_t>(p.dim) * size_of(p.delta_dtype) : 0);
+    if (aligned && p.whole16 && threads(4) >= kRingFrom && threads(kRingChunks) <= kMaxThreads && 2 * slot <= kRingBytes &&
+        p.rows > 2u * dev.sm_count) {
+        p.row_threads = threads(kRingChunks);
+        const uint32_t blocks = p.row_threads <= kMaxThreads / 2 && 2 * (kRingTail + kSlots * slot + 1024) <= 228 * 1024 ? 2 : 1;
+        auto kernel = rows_i8_ring_kernel<DT, NORM, DELTA, kWide, kRingChunks>;
+        B200_CUDA_TRY(allow_max_smem(kernel));
+        B200_CUDA_TRY(launch_dependent(kernel, dim3(blocks * dev.sm_count), dim3(p.row_threads), kRingTail + kSlots * slot, stream, p));
+        g_launch_count.fetch_add(1, std::memory_order_relaxed);
+        return ATTN_OK;
+    }
     uint32_t chunks = 4;
     if (aligned)  // few rows: more threads for each
         while (chunks > 1 && static_cast<uint64_t>(p.rows) * threads(chunks) < static_cast<uint64_t>(dev.sm_count) * 1024 &&
@@ -335,10 +529,13 @@ int rows_i8(const AttnRowsI8Args* a, bool norm, void* stream_v) {
     const uint64_t rows_apart = n > 1 ? ~0ull : 0ull;
     bool aligned = (at(a->x) | ((xs * p.x_stride) & rows_apart) | at(a->x_out) | (a->x_out ? (xs * p.x_out_stride) & rows_apart : 0) |
                     at(a->weight)) % 16 == 0;
+    const uint32_t vec = a->x_dtype == ATTN_DTYPE_F32 ? 4 : 8;
+    aligned = aligned && d % vec == 0;
     if (a->delta) {
-        const uint32_t vec = a->x_dtype == ATTN_DTYPE_F32 ? 4 : 8, run = std::min<uint32_t>(16, vec * ds);
+        const uint32_t run = std::min<uint32_t>(16, vec * ds);
         aligned = aligned && (at(a->delta) | ((ds * p.delta_stride) & rows_apart)) % run == 0;
     }
+    p.whole16 = (xs * d | (a->delta ? ds * d : 0)) % 16 == 0 && (!a->delta || (at(a->delta) | (ds * p.delta_stride & rows_apart)) % 16 == 0);
     cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
     if (!norm) return launch_rows_of<false, false>(a->x_dtype, p, aligned, dev, stream);
     return a->delta ? launch_rows_of<true, true>(a->x_dtype, p, aligned, dev, stream)

@@ -18,23 +18,23 @@ from . import binding as _b
 from .attention import _DTYPES
 from .context import _enqueue, _on, _one_device
 
-_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+_F32, _I8 = torch.float32, torch.int8
+_FLOATS = {t: _DTYPES[t] for t in (torch.float32, torch.float16, torch.bfloat16)}
 MAX_K = 131071  # longest inner dimension of gemm_i8: 32-bit sums of products of 8 bits stay exact
 
 # The argument structures as the library lays them out (packed: see context).
 ROWS_ARGS = struct.Struct("@6P4Q2If2i0P")
-GEMM_ARGS = struct.Struct("@5P3Q3I2iP")
+GEMM_ARGS = struct.Struct("@5P3Q3I2iPi0P")
 
 
 def rows_i8(rows: int, k: int, device=None) -> torch.Tensor:
     """An int8 tensor [rows, k] laid out as the operators take it: rows k rounded up to a multiple of 16 bytes apart."""
-    return torch.empty((rows, (k + 15) // 16 * 16), dtype=torch.int8, device="cuda" if device is None else device)[:, :k]
+    return torch.empty_strided((rows, k), ((k + 15) & ~15, 1), dtype=torch.int8, device="cuda" if device is None else device)
 
 
-def _matrix(t: torch.Tensor, rows: int, dim: int, what: str) -> int:
+# (A call's checks are part of the microseconds that a small one takes: what is dense is asked first, the rest is looked at here.)
+def _row_stride(t: torch.Tensor, rows: int, dim: int, what: str) -> int:
     """Distance of the rows of a [rows, dim] tensor; 0, which the library takes as dense, where there is one."""
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != dim:
-        raise ValueError(f"{what} must be [{rows}, {dim}]")
     stride = t.stride()
     if dim > 1 and stride[1] != 1:
         raise ValueError(f"the rows of {what} must be dense")
@@ -45,64 +45,57 @@ def _matrix(t: torch.Tensor, rows: int, dim: int, what: str) -> int:
     return stride[0]
 
 
-def _bytes(q: torch.Tensor, rows: int, k: int, what: str) -> int:
-    """Distance of the rows of an 8-bit matrix in bytes."""
-    if q.dtype != torch.int8:
-        raise TypeError(f"{what} must be int8")
-    stride = _matrix(q, rows, k, what)
+def _byte_stride(q: torch.Tensor, rows: int, k: int, what: str) -> int:
+    """The same for an 8-bit matrix, whose rows are a multiple of 16 bytes apart (0: k rounded up to one)."""
+    stride = _row_stride(q, rows, k, what)
     if stride % 16:
         raise ValueError(f"the rows of {what} must be a multiple of 16 bytes apart (rows_i8 lays them out so)")
-    return stride or (k + 15) // 16 * 16
-
-
-def _scales(s: torch.Tensor, rows: int, what: str) -> int:
-    if s.dtype != torch.float32 or s.dim() != 1 or s.shape[0] != rows or (rows > 1 and s.stride(0) != 1):
-        raise ValueError(f"{what} must be a dense fp32 tensor [{rows}]")
-    return s.data_ptr()
+    return stride
 
 
 def _rows(entry: str, x, weight, eps: float, delta, x_out, out, scale, stream):
     index = _one_device(x, weight, delta, x_out, out, scale)
-    if x.dim() != 2:
-        raise ValueError("x must be [N, D]")
-    N, D = x.shape
-    x_dtype = x.dtype
-    if x_dtype not in _FLOATS:
+    shape, x_dtype = x.shape, x.dtype
+    if len(shape) != 2 or shape[1] == 0:
+        raise ValueError("x must be [N, D], its rows not empty")
+    N, D = shape
+    x_code = _FLOATS.get(x_dtype)
+    if x_code is None:
         raise TypeError("x must be fp32, fp16 or bf16")
-    x_stride = _matrix(x, N, D, "x")
+    x_stride = 0 if x.is_contiguous() else _row_stride(x, N, D, "x")
     weight_ptr = delta_ptr = delta_stride = delta_code = x_out_ptr = x_out_stride = 0
     if weight is not None:
-        if weight.dtype != torch.float32 or weight.dim() != 1 or weight.shape[0] != D or not weight.is_contiguous():
+        if weight.dtype is not _F32 or weight.shape != (D,) or not weight.is_contiguous():
             raise ValueError(f"weight must be a dense fp32 tensor [{D}]")
         weight_ptr = weight.data_ptr()
     if delta is not None:
-        if delta.dtype not in _FLOATS:
+        delta_code = _FLOATS.get(delta.dtype)
+        if delta_code is None:
             raise TypeError("delta must be fp32, fp16 or bf16")
-        delta_ptr, delta_stride, delta_code = delta.data_ptr(), _matrix(delta, N, D, "delta"), _DTYPES[delta.dtype]
         if x_out is None:
             x_out = x
-        if x_out.dtype != x_dtype:
-            raise TypeError("x_out must have x's type")
-        x_out_ptr, x_out_stride = x_out.data_ptr(), _matrix(x_out, N, D, "x_out")
+        if delta.shape != shape or x_out.shape != shape or x_out.dtype != x_dtype:
+            raise ValueError("delta and x_out must have x's shape, x_out its type")
+        delta_ptr, delta_stride = delta.data_ptr(), 0 if delta.is_contiguous() else _row_stride(delta, N, D, "delta")
+        x_out_ptr, x_out_stride = x_out.data_ptr(), 0 if x_out.is_contiguous() else _row_stride(x_out, N, D, "x_out")
     elif x_out is not None:
         raise ValueError("x_out without delta")
-    if D == 0:
-        raise ValueError("rows must not be empty")
+    q_stride = 0
     if out is None:
         out = rows_i8(N, D, x.device) if stream is None else _on(stream, rows_i8, N, D, x.device)
-        q_stride = out.stride(0) if N > 1 else (D + 15) // 16 * 16
     else:
-        q_stride = _bytes(out, N, D, "out")
+        if out.dtype is not _I8 or out.shape != shape:
+            raise ValueError("out must be int8, of x's shape")
+        q_stride = _byte_stride(out, N, D, "out")
     if scale is None:
-        scale = torch.empty((N,), dtype=torch.float32, device=x.device) if stream is None else \
-            _on(stream, torch.empty, (N,), dtype=torch.float32, device=x.device)
-        scale_ptr = scale.data_ptr()
-    else:
-        scale_ptr = _scales(scale, N, "scale")
+        scale = torch.empty_strided((N,), (1,), dtype=torch.float32, device=x.device) if stream is None else \
+            _on(stream, torch.empty_strided, (N,), (1,), dtype=torch.float32, device=x.device)
+    elif scale.dtype is not _F32 or scale.shape != (N,) or not scale.is_contiguous():
+        raise ValueError(f"scale must be a dense fp32 tensor [{N}]")
     if N:
         _enqueue(entry, index, stream, ROWS_ARGS.pack(
-            out.data_ptr(), scale_ptr, x_out_ptr, x.data_ptr(), delta_ptr, weight_ptr, q_stride, x_stride, delta_stride, x_out_stride,
-            N, D, eps, _DTYPES[x_dtype], delta_code))
+            out.data_ptr(), scale.data_ptr(), x_out_ptr, x.data_ptr(), delta_ptr, weight_ptr, q_stride, x_stride, delta_stride,
+            x_out_stride, N, D, eps, x_code, delta_code))
     return out, scale
 
 
@@ -124,35 +117,49 @@ def quantize_i8(x: torch.Tensor, *, out=None, scale=None, stream=None):
 
 
 def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *, out=None, out_dtype=torch.float32,
-            swiglu: bool = False, status=None, stream=None) -> torch.Tensor:
+            swiglu: bool = False, status=None, w_early: bool = False, stream=None) -> torch.Tensor:
     """out[t, j] = a_scale[t] * w_scale[j] * sum_i a[t, i] * w[j, i]: the sum exact, rounded once to out's type.
 
     a       int8 [m, k], a_scale fp32 [m]; w int8 [n, k], w_scale fp32 [n]; rows a multiple of 16 bytes apart, k up to 131071
     swiglu  w holds n_out gate rows, then n_out up rows: out = silu(gate) * up [m, n_out]
     out     fp32 / fp16 / bf16 [m, n_out], rows may be strided (default: a new tensor of out_dtype); no operand's memory
+    w_early the caller vouches that w was in place before the previous kernel of the stream was launched: its first tiles are then read
+            while that kernel may still be running (a loaded model's weights)
     The same bits for a token whatever else is in the batch."""
     index = _one_device(a, a_scale, w, w_scale, out, status)
-    if a.dim() != 2 or w.dim() != 2:
+    a_shape, w_shape = a.shape, w.shape
+    if len(a_shape) != 2 or len(w_shape) != 2 or a_shape[1] != w_shape[1]:
         raise ValueError("a must be [m, k] and w [n, k]")
-    m, k = a.shape
-    w_rows = w.shape[0]
-    if swiglu and w_rows % 2:
-        raise ValueError("swiglu needs as many gate rows as up rows")
-    n = w_rows // 2 if swiglu else w_rows
-    a_stride, w_stride = _bytes(a, m, k, "a"), _bytes(w, w_rows, k, "w")
-    a_scale_ptr, w_scale_ptr = _scales(a_scale, m, "a_scale"), _scales(w_scale, w_rows, "w_scale")
-    if k > MAX_K or k == 0:
+    m, k = a_shape
+    n = rows = w_shape[0]
+    if not 0 < k <= MAX_K:
         raise ValueError(f"the inner dimension must be 1 to {MAX_K}")
+    if swiglu:
+        if rows % 2:
+            raise ValueError("swiglu needs as many gate rows as up rows")
+        n //= 2
+    if a.dtype is not _I8 or w.dtype is not _I8:
+        raise TypeError("a and w must be int8")
+    packed = k % 16 == 0
+    a_stride = 0 if packed and a.is_contiguous() else _byte_stride(a, m, k, "a")
+    w_stride = 0 if packed and w.is_contiguous() else _byte_stride(w, rows, k, "w")
+    if a_scale.dtype is not _F32 or w_scale.dtype is not _F32 or a_scale.shape != (m,) or w_scale.shape != (rows,) or \
+            not (a_scale.is_contiguous() and w_scale.is_contiguous()):
+        raise ValueError(f"a_scale and w_scale must be dense fp32 tensors [{m}] and [{rows}]")
+    ldc = 0
     if out is None:
-        ldc = 0
-        out = torch.empty((m, n), dtype=out_dtype, device=a.device) if stream is None else \
-            _on(stream, torch.empty, (m, n), dtype=out_dtype, device=a.device)
+        out = torch.empty_strided((m, n), (n, 1), dtype=out_dtype, device=a.device) if stream is None else \
+            _on(stream, torch.empty_strided, (m, n), (n, 1), dtype=out_dtype, device=a.device)
     else:
-        ldc = _matrix(out, m, n, "out")
-    if out.dtype not in _FLOATS:
+        if out.shape != (m, n):
+            raise ValueError(f"out must be [{m}, {n}]")
+        if not out.is_contiguous():
+            ldc = _row_stride(out, m, n, "out")
+    out_code = _FLOATS.get(out.dtype)
+    if out_code is None:
         raise TypeError("out must be fp32, fp16 or bf16")
     if m and n:
         _enqueue("attn_gemm_i8", index, stream, GEMM_ARGS.pack(
-            out.data_ptr(), a.data_ptr(), a_scale_ptr, w.data_ptr(), w_scale_ptr, a_stride, w_stride, ldc, m, n, k,
-            _DTYPES[out.dtype], 1 if swiglu else 0, 0 if status is None else status.data_ptr()))
+            out.data_ptr(), a.data_ptr(), a_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), a_stride, w_stride, ldc, m, n, k,
+            out_code, 1 if swiglu else 0, 0 if status is None else status.data_ptr(), 1 if w_early else 0))
     return out

@@ -48,7 +48,8 @@ def scale_tolerance(dim):
 
 
 ROWS = [(1, 1), (1, 4096), (2, 16), (3, 7), (5, 31), (4, 128), (7, 129), (33, 64), (64, 512), (9, 1000), (61, 5003), (2, 16384), (3, 16388),
-        (2, 28672), (1, 32768), (3, 33000), (1, 70001), (300, 1024), (1003, 96)]
+        (2, 28672), (1, 32768), (3, 33000), (1, 70001), (300, 1024), (1003, 96), (301, 8192), (700, 14336),
+        (450, 16384), (299, 28672)]
 
 
 @pytest.mark.parametrize("rows,dim", ROWS)
