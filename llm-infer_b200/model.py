@@ -19,8 +19,9 @@ import torch
 
 from . import attention as A
 from . import context as X
+from . import int8 as I
 
-_NO_SLIDE = "scaled or half-paired positions do not slide past max_seq_len"
+_NO_SLIDE = "scaled or half-paired positions, and those of 8-bit models, do not slide past max_seq_len"
 KV_SINK = 4  # attention-sink rows of the sliding window (include/model/model.hpp)
 
 
@@ -92,7 +93,10 @@ class Llama:
     def __init__(self, cfg: ModelConfig, weights: dict, batch: int, device=None, weight_type: str = "f16",
                  rope_layout: str = "interleaved", rope_scaling: dict | None = None):
         """``rope_layout`` and ``rope_scaling`` (context.rope_frequencies): positions of models that pair a head's halves, or whose
-        frequencies are scaled for long contexts. The defaults are the engine's positions and kernels."""
+        frequencies are scaled for long contexts. The defaults are the engine's positions and kernels.
+        ``weight_type`` "i8": the fp16 matrices of ``weights`` are brought to 8 bits with a scale per output channel, here and once, and
+        every projection multiplies 8-bit integers (module int8: activations get a scale per token on the way). One path for steps
+        of any batch and for prompts, positions by context.rope_positions, no clamp of q, k and v."""
         dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         if dev.type != "cuda":
             raise ValueError("the model runs on a CUDA device only (there is no CPU path)")
@@ -101,15 +105,16 @@ class Llama:
         self.w = {}
         if rope_layout not in X.ROPE_LAYOUTS:
             raise ValueError(f"the rotary layout must be one of {X.ROPE_LAYOUTS}")
-        if weight_type not in ("f16", "q8_0"):
-            raise ValueError("weight_type must be 'f16' (the engine's) or 'q8_0'")
+        if weight_type not in ("f16", "q8_0", "i8"):
+            raise ValueError("weight_type must be 'f16' (the engine's), 'q8_0' or 'i8'")
         self.weight_type = weight_type
         # the table of context.rope_positions, and whether every path has to use it
         inv_freq, self._rope_factor = X.rope_frequencies(c.rotary_dim or c.head_dim, c.rope_theta, rope_scaling)
         self._inv_freq, self._rope_layout = inv_freq.to(dev), rope_layout
-        self._own_rope = rope_layout != "interleaved" or rope_scaling is not None
+        i8 = weight_type == "i8"
+        self._own_rope = rope_layout != "interleaved" or rope_scaling is not None or i8
         if self._own_rope and c.qkv_clip > 0:
-            raise ValueError("scaled or half-paired positions have no clamp of q, k and v in the prompt phase")
+            raise ValueError("scaled or half-paired positions, and 8-bit models, have no clamp of q, k and v in the prompt phase")
         self._shared_rope = not c.qkv_clip > 0  # (rope_positions does not clamp)
         q8 = weight_type == "q8_0"
         self._gemv = A.gemv_q8_0 if q8 else A.gemv_f16
@@ -126,10 +131,13 @@ class Llama:
             if tuple(t.shape) != shape or t.dtype != want:
                 raise ValueError(f"weight {name}: expected {shape} {want}, got {tuple(t.shape)} {t.dtype}")
             self.w[name] = t.to(dev).contiguous()
-        # The GEMVs take stacked matrices: Q, K and V rows in one launch with three outputs, and gate (w1) rows
+        # The projections take stacked matrices: Q, K and V rows in one launch (the GEMVs with three outputs), and gate (w1) rows
         # followed by up (w3) rows with the SwiGLU product as its epilogue. Only the stacks are kept.
-        self.w["wqkv"] = torch.cat([self.w.pop("wq"), self.w.pop("wk"), self.w.pop("wv")], dim=1).contiguous()
-        self.w["w13"] = torch.cat([self.w.pop("w1"), self.w.pop("w3")], dim=1).contiguous()
+        if i8:
+            self._to_int8()
+        else:
+            self.w["wqkv"] = torch.cat([self.w.pop("wq"), self.w.pop("wk"), self.w.pop("wv")], dim=1).contiguous()
+            self.w["w13"] = torch.cat([self.w.pop("w1"), self.w.pop("w3")], dim=1).contiguous()
         # Weights as the decode step's GEMVs read them. Q8_0: a tiled copy of every matrix, made once here (same bytes,
         # same products bit for bit, streamed and unpacked faster: attn_repack_q8_0_tiled); the GGML blocks stay for the
         # embedding rows and for the whole-prompt path, which expands them to fp16.
@@ -148,9 +156,14 @@ class Llama:
         # residual), written by the producing kernel so that no GEMV CTA has to convert them again
         act = torch.int32 if q8 else f32
         self.xb = z(B, c.dim, dtype=act)
-        self.q, self.k, self.v = z(B, c.n_heads, c.head_dim), z(B, c.n_kv_heads, c.head_dim), z(B, c.n_kv_heads, c.head_dim)
+        if i8:  # one output of the stacked projection, and the buffers of its operands
+            self._rows8 = self._int8_rows(B)
+            self.q, self.k, self.v = self._heads(self._rows8["qkv"])
+        else:
+            self.q, self.k, self.v = z(B, c.n_heads, c.head_dim), z(B, c.n_kv_heads, c.head_dim), z(B, c.n_kv_heads, c.head_dim)
+        self.q_turned = z(B, c.n_heads, c.head_dim) if i8 else self.q  # (the attention wants dense queries)
         self.att = z(B, c.n_heads, c.head_dim, dtype=act)
-        self.hb = z(B, c.hidden_dim, dtype=act)
+        self.hb = z(B, 0 if i8 else c.hidden_dim, dtype=act)
         self.logits = z(B, c.vocab_size)
         self.next_token = z(B, dtype=torch.int32)
         self.tokens = z(B, dtype=torch.int32)   # the step's input tokens; a decode step writes its picks back here
@@ -171,7 +184,7 @@ class Llama:
         # The down projection of a batch: when the hidden activations of all sequences do not fit in shared memory next
         # to the weight ring, the inner dimension is split over sets of CTAs and the next RMSNorm adds the partial
         # products into x (same sum, fixed order).
-        chunks = c.hidden_dim // 256
+        chunks = 0 if i8 else c.hidden_dim // 256
         need = B * (c.hidden_dim * 4 + 64)
         k = max(1, -(-need // (140 * 1024)))
         while k <= chunks and chunks % k:
@@ -180,15 +193,70 @@ class Llama:
         self.partials = z(self._k_split, B, c.dim) if self._k_split > 1 else None
 
     @classmethod
-    def from_gguf(cls, path: str, batch: int, device=None) -> "Llama":
+    def from_gguf(cls, path: str, batch: int, device=None, int8: bool = False) -> "Llama":
         """Load a GGUF file (llama architecture, matrices all F16 or all Q8_0, F32 norms) as written by gguf.write_gguf
-        or by any writer of the engine's format (tensor names of src/model/model.cpp:25-38, block.cpp:18-69)."""
+        or by any writer of the engine's format (tensor names of src/model/model.cpp:25-38, block.cpp:18-69). ``int8``: the matrices
+        of an F16 file brought to 8 bits (weight_type "i8")."""
         import numpy as np
 
         from . import gguf
         cfg, w, weight_type = gguf.read_gguf(path)
+        if int8:
+            if weight_type != "f16":
+                raise ValueError("8-bit channels are made from F16 matrices")
+            weight_type = "i8"
         weights = {k: torch.from_numpy(np.array(v)) for k, v in w.items()}  # copies out of the read-only map
         return cls(cfg, weights, batch, device, weight_type=weight_type)
+
+    # -- 8-bit integers (weight_type "i8") --
+    def _to_int8(self) -> None:
+        """The fp16 matrices, stacked, become self.w8: name -> (8-bit rows, scales), a list of them over the layers."""
+        w = self.w
+        stacks = {"wqkv": ("wq", "wk", "wv"), "wo": ("wo",), "w13": ("w1", "w3"), "w2": ("w2",)}
+        self.w8 = {name: [I.quantize_i8(torch.cat([w[p][l] for p in parts])) for l in range(self.cfg.n_layers)]
+                   for name, parts in stacks.items()}
+        self.w8["wcls"] = I.quantize_i8(w["wcls"])
+        for name in ("wq", "wk", "wv", "wo", "w1", "w3", "w2", "wcls"):
+            del w[name]
+        torch.cuda.synchronize(self.device)  # (w_early: no kernel may still write them)
+
+    def _int8_rows(self, n: int) -> dict:
+        """Buffers of n tokens' way through the layers."""
+        c, dev = self.cfg, self.device
+        q_dim, e = c.n_heads * c.head_dim, torch.empty
+        return {"dim": I.rows_i8(n, c.dim, dev), "q_dim": I.rows_i8(n, q_dim, dev), "hidden": I.rows_i8(n, c.hidden_dim, dev),
+                "scale": e(n, device=dev), "qkv": e(n, q_dim + 2 * c.n_kv_heads * c.head_dim, device=dev), "delta": e(n, c.dim, device=dev),
+                "hb": e(n, c.hidden_dim, dtype=torch.bfloat16, device=dev)}
+
+    def _heads(self, qkv: torch.Tensor):
+        """q, k and v in the stacked projection's output."""
+        c = self.cfg
+        heads = qkv.view(qkv.shape[0], c.n_heads + 2 * c.n_kv_heads, c.head_dim)
+        return heads[:, :c.n_heads], heads[:, c.n_heads:c.n_heads + c.n_kv_heads], heads[:, c.n_heads + c.n_kv_heads:]
+
+    def _layers_i8(self, x: torch.Tensor, b: dict, attend):
+        """All layers over the rows of x in 8-bit products; ``attend(l)`` turns b["qkv"] into the attention's output. Returns what is
+        still to be added to x: the next norm does that, inside the layers and behind them."""
+        c, w, w8, status = self.cfg, self.w, self.w8, self.status
+        n, scale, delta = x.shape[0], b["scale"], None
+        for l in range(c.n_layers):
+            q, s = I.rmsnorm_i8(x, w["rms_att"][l], c.norm_eps, delta=delta, out=b["dim"], scale=scale)
+            I.gemm_i8(q, s, *w8["wqkv"][l], out=b["qkv"], status=status, w_early=True)
+            q, s = I.quantize_i8(attend(l).view(n, -1), out=b["q_dim"], scale=scale)
+            delta = I.gemm_i8(q, s, *w8["wo"][l], out=b["delta"], status=status, w_early=True)
+            q, s = I.rmsnorm_i8(x, w["rms_ffn"][l], c.norm_eps, delta=delta, out=b["dim"], scale=scale)  # x += Wo att
+            hb = I.gemm_i8(q, s, *w8["w13"][l], out=b["hb"], swiglu=True, status=status, w_early=True)
+            q, s = I.quantize_i8(hb, out=b["hidden"], scale=scale)
+            delta = I.gemm_i8(q, s, *w8["w2"][l], out=b["delta"], status=status, w_early=True)
+        return delta
+
+    def _classify_i8(self, delta: torch.Tensor) -> None:
+        """Final norm of x + delta, classifier and greedy pick of the batch."""
+        b = self._rows8
+        q, s = I.rmsnorm_i8(self.x, self.w["rms_final"], self.cfg.norm_eps, delta=delta, out=b["dim"], scale=b["scale"])
+        I.gemm_i8(q, s, *self.w8["wcls"], out=self.logits, status=self.status, w_early=True)
+        A.argmax(self.logits, out=self.next_token)
+        self.tokens.copy_(self.next_token)
 
     # -- positions: sliding-window arithmetic of src/model/model.cpp:66-68, per sequence --
     def _set_positions(self, pos) -> int:
@@ -211,14 +279,14 @@ class Llama:
         c = self.cfg
         if self._own_rope:
             X.rope_positions(self.q, self.k, self.v, self.k_cache[l], self.v_cache[l], self.pos, self.kv_pos, inv_freq=self._inv_freq,
-                             factor=self._rope_factor, layout=self._rope_layout, q_out=self.q, status=self.status)
+                             factor=self._rope_factor, layout=self._rope_layout, q_out=self.q_turned, status=self.status)
         else:
             A.rope_kv_insert(self.q, self.k, self.v, self.k_cache[l], self.v_cache[l], self.pos, self.kv_pos,
                              theta=c.rope_theta, rotary_dim=c.rotary_dim, kv_sink=kv_sink, q_out=self.q,
                              pos_early=True)   # positions are copied in before the step's first kernel
         # (two_pass: another order of the sums moves fp16 ties of the next layers' cache rows, so a step's results would
         # change with max_seq_len, which the choice of the form looks at)
-        A.attn_decode(self.q, self.k_cache[l], self.v_cache[l], self.kv_len, out=self.att,
+        A.attn_decode(self.q_turned, self.k_cache[l], self.v_cache[l], self.kv_len, out=self.att,
                       workspace=self.workspace, kv_early=self.kv_early and kv_sink == 0, two_pass=True)
         return self.att
 
@@ -227,6 +295,12 @@ class Llama:
         greedy pick (self.next_token) and feeds it back into self.tokens for the next step. ``attend(l)`` stands in for
         _attend: it reads self.q, self.k, self.v and returns the attention's output."""
         c, w, B = self.cfg, self.wg, self.batch
+        if self.weight_type == "i8":
+            A.embed_f16(w["embed"], self.tokens, out=self.x, status=self.status)
+            delta = self._layers_i8(self.x, self._rows8, attend or (lambda l: self._attend(l, kv_sink)))
+            if want_logits:
+                self._classify_i8(delta)
+            return
 
         def gemv(x, name, l=None, **kw):
             if name in self._rows:  # a tiled copy: its last row group may be padded
@@ -258,10 +332,11 @@ class Llama:
 
     def can_prefill(self, prompts, n_new: int = 0) -> bool:
         """Whether prefill() can take these prompts: head_dim 128 or 64 (the tensor-core attention kernel), inner
-        dimensions in multiples of 64, and every sequence inside its cache (no sliding window during the prompt or after
-        it)."""
+        dimensions in multiples of 64 (8-bit models: any), and every sequence inside its cache (no sliding window during
+        the prompt or after it)."""
         c = self.cfg
-        dims_ok = c.head_dim in (64, 128) and c.dim % 64 == 0 and c.hidden_dim % 64 == 0 and (c.n_heads * c.head_dim) % 64 == 0
+        dims_ok = c.head_dim in (64, 128) and (self.weight_type == "i8" or (
+            c.dim % 64 == 0 and c.hidden_dim % 64 == 0 and (c.n_heads * c.head_dim) % 64 == 0))
         return dims_ok and max(len(p) for p in prompts) + n_new <= c.max_seq_len
 
     def prefill(self, prompts, exact: bool = True) -> None:
@@ -274,13 +349,19 @@ class Llama:
         InferenceMode::Prefill for all but the last token of a prompt (src/model/model.cpp:74-76); the last tokens go
         through the final norm, classifier and greedy pick. Afterwards the caches hold rows 0 .. len-1 of every
         sequence and self.next_token / self.tokens / self.logits are what the token-at-a-time loop would have left.
+        8-bit models have one form, whose products are exact sums either way.
         ``exact`` = False drops the residual terms (activations and Q8_0 weights enter the tensor cores rounded once to
         fp16, one MMA instead of two or three): a third of the tensor work, results within about 1e-3 relative, no
         longer guaranteed to give the token-at-a-time path's greedy tokens."""
         if len(prompts) != self.batch or not self.can_prefill(prompts):
             raise ValueError("prefill() needs one prompt per sequence, head_dim 64 or 128 and prompts that fit the cache")
         w, c = self.w, self.cfg
-        x, last_rows = self._prompt_rows(prompts, self.k_cache, self.v_cache, exact, self._own_rope)
+        x, last_rows, delta = self._prompt_rows(prompts, self.k_cache, self.v_cache, exact, self._own_rope)
+        if self.weight_type == "i8":
+            A.gather_rows(x, last_rows, out=self.x)
+            A.gather_rows(delta, last_rows, out=self._rows8["delta"])
+            self._classify_i8(self._rows8["delta"])
+            return
         # the last token of every prompt: final norm, classifier, greedy pick (the decode step's own kernels)
         A.gather_rows(x, last_rows, out=self.x)
         A.rmsnorm(self.x, w["rms_final"], c.norm_eps, out=self.xb)
@@ -291,7 +372,8 @@ class Llama:
     def _prompt_rows(self, prompts, k_cache: torch.Tensor, v_cache: torch.Tensor, exact: bool, own_rope: bool):
         """All layers over the tokens of ``prompts``, whose keys and values go into rows 0, 1, ... of k_cache, v_cache [layers,
         len(prompts), rows, Hkv, D]; with ``own_rope`` turned by context.rope_positions, else by the engine's kernel. Returns the
-        tokens' last hidden rows and the row of each prompt's last token."""
+        tokens' last hidden rows, the row of each prompt's last token, and what is still to be added to the hidden rows (8-bit models;
+        None otherwise)."""
         import numpy as np
         c, w, B, dev = self.cfg, self.w, len(prompts), self.device
         q8 = self.weight_type == "q8_0"
@@ -307,12 +389,30 @@ class Llama:
         e = lambda *s, dtype=f32: torch.empty(*s, dtype=dtype, device=dev)  # noqa: E731
         q_dim, kv_dim, H, D = self._q_dim, self._kv_dim, c.n_heads, c.head_dim
         x = e(T, c.dim)
+        q16 = e(T, H, D, dtype=f16)
+        att = e(T, H, D)
+
+        def attend(l, qkv):
+            if own_rope:
+                X.rope_positions(*self._heads(qkv), k_cache[l], v_cache[l], token_pos, token_pos, seq=token_seq, inv_freq=self._inv_freq,
+                                 factor=self._rope_factor, layout=self._rope_layout, q_out=q16, status=self.status)
+            else:
+                A.rope_prompt(qkv, q16, k_cache[l], v_cache[l], token_seq, token_pos, n_heads=H,
+                              theta=c.rope_theta, rotary_dim=c.rotary_dim, qkv_clip=c.qkv_clip)
+            for b in range(B):
+                s0, s1, n = int(starts[b]), int(starts[b + 1]), lens[b]
+                A.attn_prefill_causal(q16[s0:s1].unsqueeze(0), k_cache[l, b, :n].unsqueeze(0),
+                                      v_cache[l, b, :n].unsqueeze(0), out=att[s0:s1].unsqueeze(0), status=self.status)
+            return att
+
+        if self.weight_type == "i8":
+            rows = self._int8_rows(T)
+            self._embed(w["embed"], tokens, out=x, status=self.status)
+            return x, last_rows, self._layers_i8(x, rows, lambda l: attend(l, rows["qkv"]))
         pair_d = (e(T, c.dim, dtype=f16), e(T, c.dim, dtype=f16))
         pair_q = pair_d if q_dim == c.dim else (e(T, q_dim, dtype=f16), e(T, q_dim, dtype=f16))
         pair_h = (e(T, c.hidden_dim, dtype=f16), e(T, c.hidden_dim, dtype=f16))
         qkv = e(T, q_dim + 2 * kv_dim)
-        q16 = e(T, H, D, dtype=f16)
-        att = e(T, H, D)
         if q8:  # room for the largest matrix of a layer: its int8 values as fp16 and its scales, or an fp16 pair
             shapes = [(w[k].shape[1], w[k].shape[2] // 34 * 32) for k in ("wqkv", "wo", "w13", "w2")]
             biggest = max(rows * n for rows, n in shapes)
@@ -339,24 +439,13 @@ class Llama:
         for l in range(c.n_layers):
             A.rmsnorm_pair(x, w["rms_att"][l], c.norm_eps, out=pair_d)
             project(pair_d, w["wqkv"][l], qkv)
-            if own_rope:
-                heads = qkv.view(T, H + 2 * c.n_kv_heads, D)
-                X.rope_positions(heads[:, :H], heads[:, H:H + c.n_kv_heads], heads[:, H + c.n_kv_heads:], k_cache[l], v_cache[l],
-                                 token_pos, token_pos, seq=token_seq, inv_freq=self._inv_freq, factor=self._rope_factor,
-                                 layout=self._rope_layout, q_out=q16, status=self.status)
-            else:
-                A.rope_prompt(qkv, q16, k_cache[l], v_cache[l], token_seq, token_pos, n_heads=H,
-                              theta=c.rope_theta, rotary_dim=c.rotary_dim, qkv_clip=c.qkv_clip)
-            for b in range(B):
-                s0, s1, n = int(starts[b]), int(starts[b + 1]), lens[b]
-                A.attn_prefill_causal(q16[s0:s1].unsqueeze(0), k_cache[l, b, :n].unsqueeze(0),
-                                      v_cache[l, b, :n].unsqueeze(0), out=att[s0:s1].unsqueeze(0), status=self.status)
+            attend(l, qkv)
             A.split_pair(att.view(T, q_dim), out=pair_q)
             project(pair_q, w["wo"][l], x, accumulate=True)               # x += Wo att
             A.rmsnorm_pair(x, w["rms_ffn"][l], c.norm_eps, out=pair_d)
             project(pair_d, w["w13"][l], pair_h, swiglu=True)             # silu(gate) * up
             project(pair_h, w["w2"][l], x, accumulate=True)               # x += W2 (silu(gate) * up)
-        return x, last_rows
+        return x, last_rows, None
 
     def capture(self) -> None:
         """Record the step once per mode (prefill: no classifier; decode: classifier + greedy pick + feedback) as CUDA
