@@ -5,6 +5,11 @@
 // The sum is exact: products of 8 bits, added in 32 (k up to 131071 keeps any sum below 2^31), so cutting k into slices and adding
 // them in any order gives the same bits. Weights are the M side of the MMA: a tensor-memory lane is a channel, which has its scale in
 // a register, and a warp stores 32 neighbouring channels of a token at a time.
+//
+// What bounds it: with few tokens the weights' way from memory (8 x 4096 x 128256 79 us = 6.7 TB/s, 8 x 4096 x 28672 20.5 us = 5.7 TB/s) and, where
+// they are few, some 4 us from a launch to its first and from its last tile (1 x 4096 x 6144 7.8 us in a graph for 3.9 of reading);
+// with many tokens the tensor cores (9184 x 4096 x 28672 with SwiGLU 654 us = 3.3 POP/s in a burst, twice the measured bf16 rate; in a long
+// loop the 1000 W cap holds it at 2.6 - 2.8 POP/s and 1.24 GHz, where the pipe is busy 92 % of the time).
 #include <algorithm>
 #include <type_traits>
 
@@ -74,10 +79,25 @@ __device__ __forceinline__ int4 ld_cluster_i4(uint32_t addr) {
     return v;
 }
 
-__device__ __forceinline__ float silu(float x) { return __fdiv_rn(x, 1.0f + expf(-x)); }
+// (expf is good to two units in the last place, the quotient to two more; the exact quotient takes a branch, behind which nothing of
+// the next value was begun: 7292 x 256 x 1536 30.9 -> 17.9 us)
+__device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.0f + expf(-x)); }
 // the scaled sum; the order of the two products is part of the result's bits
 __device__ __forceinline__ float scaled(int32_t sum, float w_scale, float a_scale) {
     return __fmul_rn(__fmul_rn(static_cast<float>(sum), w_scale), a_scale);
+}
+// The same of a channel's 16 tokens, two at a time; a_scale on a 16-byte boundary.
+__device__ __forceinline__ void scaled16(float (&y)[16], const uint32_t (&sum)[16], float w_scale, const float* a_scale) {
+    const f32x2 w2 = pack_f32x2(w_scale, w_scale);
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+        const float4 a = *reinterpret_cast<const float4*>(a_scale + i);
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+            const f32x2 s = pack_f32x2(static_cast<float>(static_cast<int32_t>(sum[i + e])), static_cast<float>(static_cast<int32_t>(sum[i + e + 1])));
+            unpack_f32x2(mul_f32x2(mul_f32x2(s, w2), e ? pack_f32x2(a.z, a.w) : pack_f32x2(a.x, a.y)), y[i + e], y[i + e + 1]);
+        }
+    }
 }
 template <typename T>
 __device__ __forceinline__ T to_out(float x);
@@ -87,6 +107,20 @@ template <>
 __device__ __forceinline__ __half to_out<__half>(float x) { return __float2half_rn(x); }
 template <>
 __device__ __forceinline__ __nv_bfloat16 to_out<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+// A channel's values of N tokens, of which there are `left`. Returns where the next token goes. (An address from the one before: with a
+// 64-bit product for each, 7292 x 256 x 1536 took 16.8 us for 12.0.)
+template <typename T, int N>
+__device__ __forceinline__ T* store_tokens(T* dst, uint64_t ldc, const float (&y)[N], uint32_t left) {
+    if (left >= N) {
+#pragma unroll
+        for (int i = 0; i < N; ++i, dst += ldc) *dst = to_out<T>(y[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i, dst += ldc)
+            if (i < left) *dst = to_out<T>(y[i]);
+    }
+    return dst;
+}
 // f with a value of the output's type
 template <typename F>
 __device__ __forceinline__ void with_out_type(int32_t dtype, F f) {
@@ -98,7 +132,7 @@ __device__ __forceinline__ void with_out_type(int32_t dtype, F f) {
 // ---- few tokens: the weights pass by once ---------------------------------------------------------------------------
 // A cluster of CTAs shares one tile of PARTS x 128 channels x N tokens; each CTA takes a slice of k, and the slices' sums meet in
 // shared memory over the cluster. Four warps: warp 0 requests the tiles by TMA, warp 1 issues the MMAs, all of them finish the tile.
-enum { S_FULL = 0, kStreamMaxStages = 8, S_EMPTY = S_FULL + kStreamMaxStages, S_ACC = S_EMPTY + kStreamMaxStages, S_BARS };
+enum { S_FULL = 0, kStreamMaxStages = 12, S_EMPTY = S_FULL + kStreamMaxStages, S_ACC = S_EMPTY + kStreamMaxStages, S_BARS };
 constexpr int kStreamThreads = 128;
 constexpr uint32_t kMaxSlices = 8;  // CTAs of a cluster
 
@@ -240,6 +274,41 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
         if constexpr (PARTS == 2) y = __fmul_rn(silu(y), scaled(s1, ws[1][i], s_scale[t]));
         return y;
     };
+    auto finish_slices = [&](auto type, auto count) {
+        using T = decltype(type);
+        constexpr uint32_t S = decltype(count)::value, kAtOnce = kMaxSlices / S;
+        for (uint32_t t0 = slice + S * kAtOnce * warp; t0 < tokens; t0 += S * kAtOnce * 4) {
+            int32_t sum[kAtOnce][PARTS][4];
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part) {
+                int4 v[kAtOnce][S];
+#pragma unroll
+                for (uint32_t u = 0; u < kAtOnce; ++u) {
+                    const uint32_t t = min(t0 + S * u, N - 1u);
+#pragma unroll
+                    for (uint32_t r = 0; r < S; ++r) v[u][r] = ld_cluster_i4(cluster_address(base + ((part * N + t) * kRowsM + 4 * lane) * 4, r));
+                }
+#pragma unroll
+                for (uint32_t u = 0; u < kAtOnce; ++u) {
+#pragma unroll
+                    for (uint32_t r = 1; r < S; ++r)
+                        v[u][0].x += v[u][r].x, v[u][0].y += v[u][r].y, v[u][0].z += v[u][r].z, v[u][0].w += v[u][r].w;
+                    sum[u][part][0] = v[u][0].x, sum[u][part][1] = v[u][0].y, sum[u][part][2] = v[u][0].z, sum[u][part][3] = v[u][0].w;
+                }
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < kAtOnce; ++u) {
+                const uint32_t t = t0 + S * u;
+                float y[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = value(min(t, N - 1u), i, sum[u][0][i], sum[u][PARTS - 1][i]);
+                T* dst = static_cast<T*>(p.out) + static_cast<size_t>(tok0 + t) * p.ldc + col;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (t < tokens && col + i < p.n_out) dst[i] = to_out<T>(y[i]);
+            }
+        }
+    };
     if (!meet) {
         with_out_type(p.out_dtype, [&](auto type) {
             using T = decltype(type);
@@ -251,10 +320,15 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
                 for (int part = 0; part < PARTS; ++part) ld16(lane_addr + part * N + c, r[part]);
 #pragma unroll
                 for (int part = 0; part < PARTS; ++part) wait_ld(r[part]);
+                float y[16];
+                scaled16(y, r[0], ws[0][0], s_scale + c);
+                if constexpr (PARTS == 2) {
+                    float up[16];
+                    scaled16(up, r[1], ws[1][0], s_scale + c);
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (col < p.n_out && c + i < tokens)
-                        dst[(c + i) * p.ldc] = to_out<T>(value(c + i, 0, r[0][i], r[PARTS - 1][i]));
+                    for (int i = 0; i < 16; ++i) y[i] = __fmul_rn(silu(y[i]), up[i]);
+                }
+                dst = store_tokens(dst, p.ldc, y, col < p.n_out ? tokens - c : 0u);
                 __syncwarp();
             }
         });
@@ -273,26 +347,12 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
             }
         }
         cluster_sync();
-        // each CTA finishes every slices-th token: a warp one of them, a thread four channels, all slices' sums on their way at once
+        // Each CTA finishes every slices-th token, a thread four channels of it. Eight reads are on their way at once: the slices' sums of
+        // as many tokens.
         with_out_type(p.out_dtype, [&](auto type) {
-            using T = decltype(type);
-            T* dst = static_cast<T*>(p.out) + static_cast<size_t>(tok0) * p.ldc + col;
-            for (uint32_t t = slice + slices * warp; t < tokens; t += slices * 4) {
-                int32_t sum[PARTS][4];
-#pragma unroll
-                for (int part = 0; part < PARTS; ++part) {
-                    const uint32_t at = base + ((part * N + t) * kRowsM + 4 * lane) * 4;
-                    int4 v[kMaxSlices];
-#pragma unroll
-                    for (uint32_t r = 0; r < kMaxSlices; ++r) v[r] = r < slices ? ld_cluster_i4(cluster_address(at, r)) : make_int4(0, 0, 0, 0);
-#pragma unroll
-                    for (uint32_t r = 1; r < kMaxSlices; ++r) v[0].x += v[r].x, v[0].y += v[r].y, v[0].z += v[r].z, v[0].w += v[r].w;
-                    sum[part][0] = v[0].x, sum[part][1] = v[0].y, sum[part][2] = v[0].z, sum[part][3] = v[0].w;
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (col + i < p.n_out) dst[t * p.ldc + i] = to_out<T>(value(t, i, sum[0][i], sum[PARTS - 1][i]));
-            }
+            if (slices == 2) finish_slices(type, std::integral_constant<int, 2>{});
+            else if (slices == 4) finish_slices(type, std::integral_constant<int, 4>{});
+            else finish_slices(type, std::integral_constant<int, 8>{});
         });
         __syncwarp();
         cluster_sync();  // (a CTA's sums are read by the others)
@@ -308,29 +368,17 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
 // ---- many tokens: pairs of CTAs -------------------------------------------------------------------------------------
 // Persistent. Two CTAs (cta_group::2, M 256) share a tile of 256 weight rows x N tokens: each loads its own 128 weight rows and half
 // of the tokens, and its tensor memory receives its own rows of the product. With SwiGLU a CTA's 128 rows are 64 gate rows and the
-// matching 64 up rows, so that a tile moves no more bytes than without. Ten warps: warp 0 requests the tiles by TMA, warp 1 issues the
+// matching 64 up rows, 16 and 16 in turn (a box of a three-dimensional map), so that a tile moves no more bytes than without and gate
+// and up of a channel lie 16 lanes apart in one warp. Ten warps: warp 0 requests the tiles by TMA, warp 1 issues the
 // MMAs into one of two accumulators, warps 2-9 scale, round and store the other one; a warpgroup has half of the tokens.
 constexpr int kEpiWarps = 8, kPairThreads = (2 + kEpiWarps) * 32;
 constexpr uint32_t kPairMaxStages = 8;
 enum { P_FULL = 0, P_EMPTY = P_FULL + kPairMaxStages, P_ACC_FULL = P_EMPTY + kPairMaxStages, P_ACC_EMPTY = P_ACC_FULL + 2,
        P_BARS = P_ACC_EMPTY + 2 };
 constexpr uint32_t kHalfRows = kRowsM / 2;  // of a weight tile: gate or up rows with SwiGLU
-// SwiGLU: what gate and up warps hand each other, per warpgroup two slots of 8 tokens x 64 channels either way
-constexpr uint32_t kSlot = 8 * kHalfRows, kExchangeBytes = 2 * 2 * 2 * kSlot * 4;
 template <int N>
 constexpr uint32_t pair_stage_bytes() { return kWTile + N / 2 * kStepK; }
 constexpr uint32_t kPairTail = 1024 + 256 + kEpiWarps * 128 * 4;  // alignment of the base; barriers, tensor-memory address; scales
-
-// Whether `yes` holds in all threads of some warps of the block, which meet here.
-__device__ __forceinline__ bool block_all(int id, int threads, bool yes) {
-    uint32_t all;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\tbarrier.cta.red.and.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-        : "=r"(all)
-        : "r"(id), "r"(threads), "r"(static_cast<uint32_t>(yes))
-        : "memory");
-    return all != 0;
-}
 
 struct PairTiles {
     uint32_t t_tiles, r_tiles, band;
@@ -359,7 +407,6 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     auto bar = [&](int i) { return base + bars_at + 8u * i; };
     volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(smem + bars_at + P_BARS * 8);
     float* s_scales = reinterpret_cast<float*>(smem + bars_at + 256);
-    float* s_exchange = s_scales + kEpiWarps * 128;
 
     const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
     const uint32_t rank = cluster_rank();
@@ -402,8 +449,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
             for (uint32_t t = worker; t < tiles && ok; t += workers) {
                 uint32_t tt, rt;
                 tile_of(tl, t, tt, rt);
-                const uint32_t row = (rt * 2 + rank) * kChannels;
-                const int w0 = static_cast<int>(row), w1 = static_cast<int>(SWIGLU ? p.n_out + row : row + kHalfRows);
+                const int row = static_cast<int>((rt * 2 + rank) * kChannels);
                 const int tok = static_cast<int>(tt * N + rank * kTok);
                 for (uint32_t ks = 0; ks < p.k_steps; ++ks, ++issued) {
                     if (issued >= p.stages && !mbar_wait(bar(P_EMPTY + s), phase ^ 1)) {
@@ -414,8 +460,12 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
                     const uint32_t dst = base + s * kStageBytes, full = bar(P_FULL + s);
                     const int kc = static_cast<int>(ks * kStepK);
                     if (rank == 0) mbar_arrive_expect_tx(full, 2 * kStageBytes);
-                    tma_load_2d_pair(dst, &tm_w, full, kc, w0);
-                    tma_load_2d_pair(dst + kWTile / 2, &tm_w, full, kc, w1);
+                    if constexpr (SWIGLU) {
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) tma_load_3d_pair(dst + g * (kWTile / 4), &tm_w, full, kc, row + 16 * g, 0);
+                    } else {
+                        tma_load_2d_pair(dst, &tm_w, full, kc, row);
+                    }
                     tma_load_2d_pair(dst + kWTile, &tm_a, full, kc, tok);
                     if (++s == p.stages) s = 0, phase ^= 1;
                 }
@@ -463,10 +513,10 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
         const uint32_t lane_addr = tmem + ((quarter * 32) << 16) + group * kTok;
         float* s_scale = s_scales + (warp - 2) * 128;
         const uint32_t empty0 = cluster_address(bar(P_ACC_EMPTY), 0);  // the leader's, also for its partner
-        // SwiGLU: quarters 0 and 1 hold the gate rows, 2 and 3 the up rows of the same 64 channels
-        const bool is_up = SWIGLU && quarter >= 2;
-        const uint32_t in_tile = SWIGLU ? (quarter & 1) * 32 + lane : quarter * 32 + lane;
-        uint32_t local = 0, slot = 0;
+        // SwiGLU: lanes 0-15 hold gate rows, lanes 16-31 the up rows of the same 16 channels
+        const bool is_up = SWIGLU && lane >= 16;
+        const uint32_t in_tile = SWIGLU ? quarter * 16 + (lane & 15) : quarter * 32 + lane;
+        uint32_t local = 0;
         for (uint32_t t = worker; t < tiles; t += workers, ++local) {
             uint32_t tt, rt;
             tile_of(tl, t, tt, rt);
@@ -478,20 +528,22 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
             for (uint32_t i = lane; i < kTok; i += 32) s_scale[i] = tok0 + i < p.m ? p.a_scale[tok0 + i] : 0.f;
             __syncwarp();
             const uint32_t tokens = tok0 < p.m ? min(kTok, p.m - tok0) : 0u;
-            // (a vote, so that the warp, with SwiGLU the warpgroup, gives up or goes on as one)
-            const bool there = mbar_wait(bar(P_ACC_FULL + buf), (local / 2) & 1);
-            if (!(SWIGLU ? block_all(1 + group, 128, there) : __all_sync(0xffffffffu, there))) {
+            // (a vote, so that the warp gives up or goes on as one)
+            if (!__all_sync(0xffffffffu, mbar_wait(bar(P_ACC_FULL + buf), (local / 2) & 1))) {
                 if (lane == 0) gave_up();
                 break;
             }
             fence_after();
+            const uint32_t acc = lane_addr + buf * 256;
             with_out_type(p.out_dtype, [&](auto type) {
                 using T = decltype(type);
-                T* dst = static_cast<T*>(p.out) + static_cast<size_t>(tok0) * p.ldc + col;
+                // (SwiGLU: gate lanes finish the first 8 of 16 tokens, up lanes the last 8)
+                uint32_t first = is_up ? 8 : 0;
+                T* dst = static_cast<T*>(p.out) + static_cast<size_t>(tok0 + first) * p.ldc + col;
 #pragma unroll 1
-                for (uint32_t c = 0; c < kTok; c += 16) {
+                for (uint32_t c = 0; c < kTok; c += 16, first += 16) {
                     uint32_t r[16];
-                    ld16(lane_addr + buf * 256 + c, r);
+                    ld16(acc + c, r);
                     wait_ld(r);
                     if (c + 16 == kTok) {  // the accumulator is read: hand it back
                         fence_before();
@@ -499,27 +551,18 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
                         if (lane == 0) mbar_arrive_cluster_relaxed(empty0 + 8 * buf);
                     }
                     float y[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) y[i] = scaled(static_cast<int32_t>(r[i]), ws, s_scale[c + i]);
+                    scaled16(y, r, ws, s_scale + c);
+                    const uint32_t left = live && first < tokens ? tokens - first : 0u;
                     if constexpr (SWIGLU) {
-                        // gate warps finish the chunk's first 8 tokens and up warps the last 8
-                        float* to = s_exchange + ((group * 2 + slot) * 2 + is_up) * kSlot + in_tile;
-                        const float* from = s_exchange + ((group * 2 + slot) * 2 + !is_up) * kSlot + in_tile;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) to[i * kHalfRows] = is_up ? y[i] : y[8 + i];
-                        named_bar_sync(1 + group, 128);
-                        slot ^= 1;  // (whoever writes a slot again has passed the barrier behind its last reads)
-                        const uint32_t c0 = c + (is_up ? 8 : 0);
+                        float z[8];
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            const float other = from[i * kHalfRows];
-                            const float gate = is_up ? other : y[i], up = is_up ? y[8 + i] : other;
-                            if (live && c0 + i < tokens) dst[(c0 + i) * p.ldc] = to_out<T>(__fmul_rn(silu(gate), up));
+                            const float other = __shfl_xor_sync(0xffffffffu, is_up ? y[i] : y[8 + i], 16);
+                            z[i] = __fmul_rn(silu(is_up ? other : y[i]), is_up ? y[8 + i] : other);
                         }
+                        dst = store_tokens(dst, p.ldc, z, left) + 8 * p.ldc;
                     } else {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (live && c + i < tokens) dst[(c + i) * p.ldc] = to_out<T>(y[i]);
+                        dst = store_tokens(dst, p.ldc, y, left);
                     }
                     __syncwarp();
                 }
@@ -538,15 +581,16 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     }
 }
 
-// [rows][k] bytes, rows `stride` apart; box = 128 bytes of k x box_rows rows, 128-byte swizzle. Past k and past the rows: zeros.
-int make_map(CUtensorMap* map, const void* ptr, uint64_t rows, uint64_t k, uint64_t stride, uint32_t box_rows) {
+// [rows][k] bytes, rows `stride` apart; box = 128 bytes of k x box_rows rows, 128-byte swizzle. Past k and past the rows: zeros. With
+// `parts` > 1 that many such matrices one behind the other, and box_rows rows of each in the box.
+int make_map(CUtensorMap* map, const void* ptr, uint64_t rows, uint64_t k, uint64_t stride, uint32_t box_rows, uint32_t parts = 1) {
     EncodeTiledFn enc = encode_tiled_fn();
     if (!enc) return ATTN_ERR_CUDA;
-    const cuuint64_t dims[2] = {k, rows};
-    const cuuint64_t strides[1] = {stride};
-    const cuuint32_t box[2] = {kStepK, box_rows};
-    const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+    const cuuint64_t dims[3] = {k, rows, parts};
+    const cuuint64_t strides[2] = {stride, rows * stride};
+    const cuuint32_t box[3] = {kStepK, box_rows, parts};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, parts > 1 ? 3 : 2, const_cast<void*>(ptr), dims, strides, box, estr,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
@@ -565,18 +609,21 @@ struct Operands {
     cudaStream_t stream;
 };
 
+// Shared memory of a stream CTA: all of an SM's where there are no more CTAs than SMs (clusters have to fit the groups of 16 SMs and
+// more that they are placed in), else half of it, so that one CTA streams while its neighbour starts or ends.
+uint32_t stream_smem(uint64_t ctas, uint32_t slices, uint32_t sms) {
+    const uint64_t fit = slices == 1 ? sms : slices == 2 ? sms - 4 : slices == 4 ? sms - 20 : 0;
+    return ctas <= fit ? kMaxDynamicSmem : kMaxDynamicSmem / 2 - 2048;
+}
+
 template <int PARTS, int N>
-int launch_stream(Operands& o) {
+int launch_stream(Operands& o, uint32_t slices) {
     GemmI8Params& p = o.p;
     constexpr uint32_t stage = stream_stage_bytes<PARTS, N>();
+    static_assert(2 * stage >= PARTS * N * kRowsM * 4, "the slices' sums lie where the tiles were");
     const uint32_t row_tiles = (p.n_out + kRowsM - 1) / kRowsM, tok_tiles = (p.m + N - 1) / N;
-    if (row_tiles > 65535 || tok_tiles > 65535) return ATTN_ERR_UNSUPPORTED;
-    // two CTAs on an SM, so that one of them streams while the other starts or ends
-    p.stages = std::min<uint32_t>(kStreamMaxStages, (kMaxDynamicSmem / 2 - 2048 - kStreamTail) / stage);
     const uint64_t tiles = static_cast<uint64_t>(row_tiles) * tok_tiles;
-    uint32_t slices = 1;
-    while (slices < kMaxSlices && 2 * slices <= p.k_steps && tiles * slices * 2 <= 2ull * o.dev.sm_count) slices *= 2;
-    if (slices > 1 && p.stages * stage < PARTS * N * kRowsM * 4) slices = 1;  // (the slices' sums lie where the tiles were)
+    p.stages = std::min<uint32_t>(kStreamMaxStages, (stream_smem(tiles * slices, slices, o.dev.sm_count) - kStreamTail) / stage);
     const uint32_t smem = p.stages * stage + kStreamTail;
     CUtensorMap tm_w, tm_a;
     int rc;
@@ -607,8 +654,7 @@ template <bool SWIGLU, int N>
 int launch_pair(Operands& o) {
     GemmI8Params& p = o.p;
     constexpr uint32_t stage = pair_stage_bytes<N>(), span = SWIGLU ? kRowsM : 2 * kRowsM;
-    const uint32_t fixed = kPairTail + (SWIGLU ? kExchangeBytes : 0);
-    p.stages = std::min<uint32_t>(kPairMaxStages, (kMaxDynamicSmem - fixed) / stage);
+    p.stages = std::min<uint32_t>(kPairMaxStages, (kMaxDynamicSmem - kPairTail) / stage);
     PairTiles tl{};
     tl.t_tiles = (p.m + N - 1) / N;
     tl.r_tiles = (p.n_out + span - 1) / span;
@@ -618,14 +664,16 @@ int launch_pair(Operands& o) {
     tl.band = std::min<uint32_t>(tl.t_tiles, 8);
     CUtensorMap tm_w, tm_a;
     int rc;
-    if ((rc = make_map(&tm_w, o.a->w, o.w_rows, o.a->k, o.w_stride, kHalfRows)) != ATTN_OK) return rc;
+    if (SWIGLU) rc = make_map(&tm_w, o.a->w, p.n_out, o.a->k, o.w_stride, 16, 2);
+    else rc = make_map(&tm_w, o.a->w, o.w_rows, o.a->k, o.w_stride, kRowsM);
+    if (rc != ATTN_OK) return rc;
     if ((rc = make_map(&tm_a, o.a->a, p.m, o.a->k, o.a_stride, N / 2)) != ATTN_OK) return rc;
     auto kernel = gemm_i8_pair_kernel<SWIGLU, N>;
     B200_CUDA_TRY(allow_max_smem(kernel));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(2 * std::min(tl.t_tiles * tl.r_tiles, static_cast<uint32_t>(o.dev.sm_count) / 2));
     cfg.blockDim = dim3(kPairThreads);
-    cfg.dynamicSmemBytes = p.stages * stage + fixed;
+    cfg.dynamicSmemBytes = p.stages * stage + kPairTail;
     cfg.stream = o.stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -644,17 +692,30 @@ int launch_pair(Operands& o) {
 template <int PARTS>
 int launch_gemm(Operands& o) {
     constexpr bool kSwiglu = PARTS == 2;
-    const uint32_t m = o.p.m;
-    if (m <= 16) return launch_stream<PARTS, 16>(o);
-    if (m <= 32) return launch_stream<PARTS, 32>(o);
-    if (m <= 64) return launch_stream<PARTS, 64>(o);
-    // Tiles of 256 tokens or of 128: the fewer waves of pairs, a wave of the smaller ones being half as long. What fits one wave
-    // of the larger ones is better spread (1003 x 14336 x 4096: 45.3 us for 49.3, 300 x 14336 x 4096 23.2 for 37.9), what does not has
-    // less to move with them (9184 x 14336 x 4096: 322 for 361, 2048 x 4096 x 28672 with SwiGLU 167 for 182).
-    const uint64_t pairs = o.dev.sm_count / 2, r_tiles = (o.p.n_out + (kSwiglu ? kRowsM : 2 * kRowsM) - 1) / (kSwiglu ? kRowsM : 2 * kRowsM);
-    auto waves = [&](uint32_t n) { return ((m + n - 1) / n * r_tiles + pairs - 1) / pairs; };
-    const uint64_t wide = waves(256) * 100, narrow = waves(128) * (waves(256) == 1 ? 48 : 54);
-    return wide <= narrow ? launch_pair<kSwiglu, 256>(o) : launch_pair<kSwiglu, 128>(o);
+    const uint64_t m = o.p.m, sms = o.dev.sm_count, r128 = (o.p.n_out + kRowsM - 1) / kRowsM;
+    const uint32_t n = m <= 16 ? 16 : m <= 32 ? 32 : 64;
+    const uint64_t tiles = (m + n - 1) / n * r128;
+    // Single CTAs for up to 64 tokens (a whole vocabulary of channels is left to pairs, which are persistent: 61 x 4096 x 128256 88.4 and 83.4
+    // us, 8 tokens 79.0 and 82.0), and for more where the tiles are half as many as SMs at most and slices of k make up for it:
+    // 105 x 12608 x 896 9.1 us in 8 slices, pairs 20.2; 400 x 14336 x 512 10.4 and 21; 128 x 4096 x 4096 8.9 and 9.5; but 256 x 4096 x 6144 13.8 and
+    // 10.8. With SwiGLU pairs lose against four slices of a long k only: 299 x 4728 x 864 8.7 and 10.1, 522 x 1712 x 1664 10.4 and 7.9.
+    const bool few = tiles <= sms / 2 && (!kSwiglu || (tiles <= 32 && o.p.k_steps >= 32));
+    if (m <= 64 ? r128 <= (m <= 32 ? 65535 : 4 * sms) : few) {
+        // Slices until they are 256 (of 64 tokens with SwiGLU, whose stages are large, 128), none shorter than its sums' way to their place is
+        // worth: a stage with up to 16 tokens (14 x 1744 x 1004 in 1, 2, 4, 8 slices 7.6, 6.3, 5.3, 4.8 us), eight with 64 (100 x 2000 x 2000 6.9,
+        // 6.3, 6.3, 6.8; 40 x 1024 x 1024 3.8, 4.0, 3.9, 4.1; 170 x 11328 x 1024 18.0, 12.1, 9.8, 9.6).
+        const uint32_t shortest = n == 16 ? 1 : n == 32 ? 3 : 8, most = PARTS * n > 64 ? 128 : 256;
+        uint32_t slices = 1;
+        while (2 * slices <= (PARTS * n > 64 ? 4 : kMaxSlices) && tiles <= sms / 2 && tiles * 2 * slices <= most && o.p.k_steps >= shortest * 2 * slices)
+            slices *= 2;
+        return n == 16 ? launch_stream<PARTS, 16>(o, slices) : n == 32 ? launch_stream<PARTS, 32>(o, slices) : launch_stream<PARTS, 64>(o, slices);
+    }
+    if (m <= 64) return launch_pair<kSwiglu, 64>(o);
+    // Tiles of 256 tokens or of 128: the fewer waves of pairs, one of the smaller ones being a little more than half as long. 1003 x 4096 x 4096
+    // 15.7 us in one wave of the larger, 16.8 in two; 9184 x 14336 x 4096 322 and 361; but 512 x 4096 x 4096, one wave either way, 14.8 and 10.6.
+    const uint64_t pairs = sms / 2, span = kSwiglu ? kRowsM : 2 * kRowsM, r_tiles = (o.p.n_out + span - 1) / span;
+    auto waves = [&](uint32_t tokens) { return ((m + tokens - 1) / tokens * r_tiles + pairs - 1) / pairs; };
+    return waves(256) * 10 <= waves(128) * 6 ? launch_pair<kSwiglu, 256>(o) : launch_pair<kSwiglu, 128>(o);
 }
 
 }  // namespace
@@ -679,7 +740,8 @@ extern "C" int attn_gemm_i8(const AttnGemmI8Args* a, void* stream_v) {
     auto at = [](const void* ptr) { return reinterpret_cast<uintptr_t>(ptr); };
     if ((at(a->a) | at(a->w) | o.a_stride | o.w_stride) % 16 || (at(a->a_scale) | at(a->w_scale)) % 4 || at(a->out) % size)
         return ATTN_ERR_ALIGNMENT;
-    if (o.a_stride >= 1ull << 40 || o.w_stride >= 1ull << 40) return ATTN_ERR_UNSUPPORTED;  // a tensor map's limit
+    // a tensor map's limits
+    if (o.a_stride >= 1ull << 40 || o.w_stride >= 1ull << 40 || (a->swiglu && o.w_stride >= (1ull << 40) / a->n_out)) return ATTN_ERR_UNSUPPORTED;
     const Runs out(a->out, 1, 0, a->m, size * p.ldc, static_cast<uint64_t>(size) * a->n_out);
     if (share_memory(out, Runs(a->a, 1, 0, a->m, o.a_stride, a->k)) || share_memory(out, Runs(a->w, 1, 0, o.w_rows, o.w_stride, a->k)) ||
         share_memory(out, Runs(a->a_scale, 1, 0, 1, 0, 4ull * a->m)) || share_memory(out, Runs(a->w_scale, 1, 0, 1, 0, 4 * o.w_rows)))

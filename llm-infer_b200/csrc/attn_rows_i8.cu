@@ -47,7 +47,7 @@ template <int VEC>
 struct Raw {
     uint32_t w[VEC];
 };
-// `n` of the VEC values from element i on. ALIGNED: all of them, in one run.
+// VEC values from element i on. ALIGNED: all of them, in one run; otherwise one by one, n of them.
 template <int VEC, bool ALIGNED>
 __device__ __forceinline__ void load(Raw<VEC>& r, const void* p, size_t i, bool wide32, uint32_t n) {
     if (wide32) {
@@ -57,7 +57,7 @@ __device__ __forceinline__ void load(Raw<VEC>& r, const void* p, size_t i, bool 
             for (int k = 0; k < VEC; k += 4) *reinterpret_cast<uint4*>(&r.w[k]) = *reinterpret_cast<const uint4*>(s + k);
         } else {
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) r.w[k] = k < n ? s[k] : 0u;
+            for (uint32_t k = 0; k < VEC; ++k) r.w[k] = k < n ? s[k] : 0u;
         }
     } else {
         const unsigned short* s = static_cast<const unsigned short*>(p) + i;
@@ -66,7 +66,7 @@ __device__ __forceinline__ void load(Raw<VEC>& r, const void* p, size_t i, bool 
             else *reinterpret_cast<uint2*>(&r.w[0]) = *reinterpret_cast<const uint2*>(s);
         } else {
 #pragma unroll
-            for (int k = 0; k < VEC; k += 2)
+            for (uint32_t k = 0; k < VEC; k += 2)
                 r.w[k / 2] = (k < n ? s[k] : 0u) | (k + 1 < n ? static_cast<uint32_t>(s[k + 1]) << 16 : 0u);
         }
     }
@@ -99,7 +99,7 @@ __device__ __forceinline__ void store(void* p, size_t i, const float (&v)[VEC], 
             for (int k = 0; k < VEC; k += 4) *reinterpret_cast<float4*>(d + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
         } else {
 #pragma unroll
-            for (int k = 0; k < VEC; ++k)
+            for (uint32_t k = 0; k < VEC; ++k)
                 if (k < n) d[k] = v[k];
         }
     } else {
@@ -112,7 +112,7 @@ __device__ __forceinline__ void store(void* p, size_t i, const float (&v)[VEC], 
             else *reinterpret_cast<uint2*>(d) = make_uint2(u[0], u[1]);
         } else {
 #pragma unroll
-            for (int k = 0; k < VEC; ++k)
+            for (uint32_t k = 0; k < VEC; ++k)
                 if (k < n) d[k] = static_cast<unsigned short>(u[k / 2] >> (16 * (k & 1)));
         }
     }
@@ -225,7 +225,7 @@ __device__ __forceinline__ Rounding finish_row(const RowsParams& p, uint32_t row
     }
     return r;
 }
-// `n` of VEC whole numbers.
+// VEC whole numbers, `n` of which there are.
 template <int VEC, bool ALIGNED>
 __device__ __forceinline__ void put(int8_t* q, const float (&z)[VEC], const Rounding& r, uint32_t n) {
     uint32_t u[VEC / 4];
@@ -250,7 +250,7 @@ __device__ __forceinline__ void put(int8_t* q, const float (&z)[VEC], const Roun
         else *reinterpret_cast<uint32_t*>(q) = u[0];
     } else {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k)
+        for (uint32_t k = 0; k < VEC; ++k)
             if (k < n) q[k] = static_cast<int8_t>(u[k / 4] >> (8 * (k & 3)));
     }
 }
@@ -301,6 +301,7 @@ __global__ void __launch_bounds__(max_threads(NORM, VEC, CHUNKS)) rows_i8_kernel
         load<VEC, ALIGNED>(rx, p.x, x_row + i, DT == ATTN_DTYPE_F32, n);
         if constexpr (DELTA) load<VEC, ALIGNED>(rd, p.delta, d_row + i, wide_delta, n);
     };
+    auto index = [&](uint32_t c) { return (c * p.row_threads + t) * VEC; };  // of run c
     Found found;
     uint32_t top;
     float sum;
@@ -308,10 +309,10 @@ __global__ void __launch_bounds__(max_threads(NORM, VEC, CHUNKS)) rows_i8_kernel
         Raw<VEC> rx[CHUNKS], rd[CHUNKS];
         Kept<DT, NORM, VEC, CHUNKS> kept;
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) fetch((c * p.row_threads + t) * VEC, rx[c], rd[c]);
+        for (int c = 0; c < CHUNKS; ++c) fetch(index(c), rx[c], rd[c]);
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-            const uint32_t i = (c * p.row_threads + t) * VEC;
+            const uint32_t i = index(c);
             if (i < p.dim) {
                 if constexpr (kept.kRaw) {
                     count16<DT, VEC>(rx[c], found);
@@ -329,20 +330,20 @@ __global__ void __launch_bounds__(max_threads(NORM, VEC, CHUNKS)) rows_i8_kernel
         const Rounding r = finish_row<NORM>(p, row, top, sum, t == 0);
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-            const uint32_t i = (c * p.row_threads + t) * VEC;
+            const uint32_t i = index(c);
             if (i < p.dim) put<VEC, ALIGNED>(q + i, kept.values(c), r, p.dim - i);
         }
     } else {
         Raw<VEC> rx, rd;
         float h[VEC], z[VEC];
-        for (uint32_t i = t * VEC; i < p.dim; i += p.row_threads * VEC) {
+        for (uint32_t i = index(0); i < p.dim; i += p.row_threads * VEC) {
             fetch(i, rx, rd);
             combine<DT, NORM, DELTA, VEC, ALIGNED>(p, i, rx, rd, h, z);
             count<NORM, VEC>(h, z, found);
         }
         reduce_row<DT, NORM>(found, top, sum, whole_block, s_top, s_sum);
         const Rounding r = finish_row<NORM>(p, row, top, sum, t == 0);
-        for (uint32_t i = t * VEC; i < p.dim; i += p.row_threads * VEC) {  // (x_out may be x: nothing of the row was written before)
+        for (uint32_t i = index(0); i < p.dim; i += p.row_threads * VEC) {  // (x_out may be x: nothing of the row was written before)
             fetch(i, rx, rd);
             combine<DT, NORM, DELTA, VEC, ALIGNED>(p, i, rx, rd, h, z);
             if constexpr (DELTA)
@@ -399,17 +400,17 @@ __global__ void __launch_bounds__(kMaxThreads) rows_i8_ring_kernel(const __grid_
             const uint32_t i = (c * blockDim.x + t) * VEC;
             if (i < p.dim) {
                 Raw<VEC> rx, rd;
-                load<VEC, true>(rx, x, i, DT == ATTN_DTYPE_F32, p.dim - i);
+                load<VEC, true>(rx, x, i, DT == ATTN_DTYPE_F32, VEC);
                 if constexpr (kept.kRaw) {
                     count16<DT, VEC>(rx, found);
                     kept.keep(c, rx);
                 } else {
                     float h[VEC];
-                    if constexpr (DELTA) load<VEC, true>(rd, x + x_bytes, i, p.delta_dtype == ATTN_DTYPE_F32, p.dim - i);
+                    if constexpr (DELTA) load<VEC, true>(rd, x + x_bytes, i, p.delta_dtype == ATTN_DTYPE_F32, VEC);
                     combine<DT, NORM, DELTA, VEC, true>(p, i, rx, rd, h, kept.z[c]);
                     count<NORM, VEC>(h, kept.z[c], found);
                     if constexpr (DELTA)
-                        if (p.x_out) store<VEC, DT, true>(p.x_out, row * p.x_out_stride + i, h, p.dim - i);
+                        if (p.x_out) store<VEC, DT, true>(p.x_out, row * p.x_out_stride + i, h, VEC);
                 }
             }
         }
@@ -422,7 +423,7 @@ __global__ void __launch_bounds__(kMaxThreads) rows_i8_ring_kernel(const __grid_
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             const uint32_t i = (c * blockDim.x + t) * VEC;
-            if (i < p.dim) put<VEC, true>(q + i, kept.values(c), r, p.dim - i);
+            if (i < p.dim) put<VEC, true>(q + i, kept.values(c), r, VEC);
         }
         if (++slot == kSlots) slot = 0, phase ^= 1;
     }
@@ -432,8 +433,9 @@ uint32_t size_of(int32_t dtype) { return dtype == ATTN_DTYPE_F32 ? 4 : 2; }
 bool is_float(int32_t d) { return d == ATTN_DTYPE_F32 || d == ATTN_DTYPE_F16 || d == ATTN_DTYPE_BF16; }
 
 template <int DT, bool NORM, bool DELTA>
-int launch_rows(RowsParams& p, bool aligned, const DeviceInfo& dev, cudaStream_t stream) {
+int launch_rows(RowsParams& p, uint32_t run, const DeviceInfo& dev, cudaStream_t stream) {
     constexpr int kWide = DT == ATTN_DTYPE_F32 ? 4 : 8;
+    const bool aligned = run == kWide;
     const uint32_t vec = aligned ? kWide : 4;
     auto threads = [&](uint32_t chunks) { return ((p.dim + vec * chunks - 1) / (vec * chunks) + 31) / 32 * 32; };
     const uint32_t row_bytes = p.dim * size_of(DT) + (DELTA ? p.dim * size_of(p.delta_dtype) : 0);
@@ -464,7 +466,8 @@ int launch_rows(RowsParams& p, bool aligned, const DeviceInfo& dev, cudaStream_t
     const bool warps = p.row_threads == 32;
     const uint32_t block = warps ? 32 * kWarpRows : p.row_threads;
     const uint32_t grid = warps ? (p.rows + kWarpRows - 1) / kWarpRows : p.rows;
-    void (*kernel)(RowsParams) = !aligned ? (chunks ? rows_i8_kernel<DT, NORM, DELTA, 4, 4, false> : rows_i8_kernel<DT, NORM, DELTA, 4, 0, false>)
+    void (*kernel)(RowsParams) = run == 1 ? (chunks ? rows_i8_kernel<DT, NORM, DELTA, 4, 4, false> : rows_i8_kernel<DT, NORM, DELTA, 4, 0, false>)
+                                 : !aligned ? (chunks ? rows_i8_kernel<DT, NORM, DELTA, 4, 4, true> : rows_i8_kernel<DT, NORM, DELTA, 4, 0, true>)
                                  : chunks == 4 ? rows_i8_kernel<DT, NORM, DELTA, kWide, 4, true>
                                  : chunks == 2 ? rows_i8_kernel<DT, NORM, DELTA, kWide, 2, true>
                                  : chunks == 1 ? rows_i8_kernel<DT, NORM, DELTA, kWide, 1, true>
@@ -475,10 +478,10 @@ int launch_rows(RowsParams& p, bool aligned, const DeviceInfo& dev, cudaStream_t
 }
 
 template <bool NORM, bool DELTA>
-int launch_rows_of(int32_t dtype, RowsParams& p, bool aligned, const DeviceInfo& dev, cudaStream_t stream) {
-    return dtype == ATTN_DTYPE_F32   ? launch_rows<ATTN_DTYPE_F32, NORM, DELTA>(p, aligned, dev, stream)
-           : dtype == ATTN_DTYPE_F16 ? launch_rows<ATTN_DTYPE_F16, NORM, DELTA>(p, aligned, dev, stream)
-                                     : launch_rows<ATTN_DTYPE_BF16, NORM, DELTA>(p, aligned, dev, stream);
+int launch_rows_of(int32_t dtype, RowsParams& p, uint32_t run, const DeviceInfo& dev, cudaStream_t stream) {
+    return dtype == ATTN_DTYPE_F32   ? launch_rows<ATTN_DTYPE_F32, NORM, DELTA>(p, run, dev, stream)
+           : dtype == ATTN_DTYPE_F16 ? launch_rows<ATTN_DTYPE_F16, NORM, DELTA>(p, run, dev, stream)
+                                     : launch_rows<ATTN_DTYPE_BF16, NORM, DELTA>(p, run, dev, stream);
 }
 
 int rows_i8(const AttnRowsI8Args* a, bool norm, void* stream_v) {
@@ -525,21 +528,25 @@ int rows_i8(const AttnRowsI8Args* a, bool norm, void* stream_v) {
     p.dim = a->dim;
     p.eps = a->eps;
     p.delta_dtype = a->delta_dtype;
-    // runs of VEC values: 16 bytes of 16-bit values, 32 bytes (two accesses of 16) of fp32 beside them
-    const uint64_t rows_apart = n > 1 ? ~0ull : 0ull;
-    bool aligned = (at(a->x) | ((xs * p.x_stride) & rows_apart) | at(a->x_out) | (a->x_out ? (xs * p.x_out_stride) & rows_apart : 0) |
-                    at(a->weight)) % 16 == 0;
-    const uint32_t vec = a->x_dtype == ATTN_DTYPE_F32 ? 4 : 8;
-    aligned = aligned && d % vec == 0;
-    if (a->delta) {
-        const uint32_t run = std::min<uint32_t>(16, vec * ds);
-        aligned = aligned && (at(a->delta) | ((ds * p.delta_stride) & rows_apart)) % run == 0;
-    }
-    p.whole16 = (xs * d | (a->delta ? ds * d : 0)) % 16 == 0 && (!a->delta || (at(a->delta) | (ds * p.delta_stride & rows_apart)) % 16 == 0);
+    // Runs that a thread reads and writes at once: 8 values of 16 bits, 4 of any type, or single ones, as the rows' length, places and distances
+    // allow. (9184 x 14335 bf16, one by one: 126 us;
+    // of 14336: 65.7. Neighbouring values to neighbouring threads instead, whole numbers in single bytes then: 254.)
+    const uint64_t apart = n > 1 ? ~0ull : 0ull;
+    auto fits = [&](uint64_t ptr, uint64_t stride, uint32_t size, uint32_t values) {
+        return (ptr | (stride * size & apart)) % std::min<uint32_t>(16, size * values) == 0;
+    };
+    auto run_fits = [&](uint32_t values) {
+        return d % values == 0 && fits(at(a->x), p.x_stride, xs, values) && at(a->weight) % 16 == 0 &&
+               (!a->x_out || fits(at(a->x_out), p.x_out_stride, xs, values)) && (!a->delta || fits(at(a->delta), p.delta_stride, ds, values));
+    };
+    const uint32_t run = xs == 2 && run_fits(8) ? 8 : run_fits(4) ? 4 : 1;
+    // whole rows by bulk copies
+    p.whole16 = (xs * d | (a->delta ? ds * d : 0)) % 16 == 0 && (at(a->x) | (xs * p.x_stride & apart)) % 16 == 0 &&
+                (!a->delta || (at(a->delta) | (ds * p.delta_stride & apart)) % 16 == 0);
     cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
-    if (!norm) return launch_rows_of<false, false>(a->x_dtype, p, aligned, dev, stream);
-    return a->delta ? launch_rows_of<true, true>(a->x_dtype, p, aligned, dev, stream)
-                    : launch_rows_of<true, false>(a->x_dtype, p, aligned, dev, stream);
+    if (!norm) return launch_rows_of<false, false>(a->x_dtype, p, run, dev, stream);
+    return a->delta ? launch_rows_of<true, true>(a->x_dtype, p, run, dev, stream)
+                    : launch_rows_of<true, false>(a->x_dtype, p, run, dev, stream);
 }
 
 }  // namespace

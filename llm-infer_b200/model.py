@@ -276,17 +276,18 @@ class Llama:
 
     def _attend(self, l: int, kv_sink: int) -> torch.Tensor:
         """Positions, cache insert and attention of layer ``l`` over every sequence's own cache."""
-        c = self.cfg
+        c, q = self.cfg, self.q
         if self._own_rope:
+            q = self.q_turned
             X.rope_positions(self.q, self.k, self.v, self.k_cache[l], self.v_cache[l], self.pos, self.kv_pos, inv_freq=self._inv_freq,
-                             factor=self._rope_factor, layout=self._rope_layout, q_out=self.q_turned, status=self.status)
+                             factor=self._rope_factor, layout=self._rope_layout, q_out=q, status=self.status)
         else:
             A.rope_kv_insert(self.q, self.k, self.v, self.k_cache[l], self.v_cache[l], self.pos, self.kv_pos,
                              theta=c.rope_theta, rotary_dim=c.rotary_dim, kv_sink=kv_sink, q_out=self.q,
                              pos_early=True)   # positions are copied in before the step's first kernel
         # (two_pass: another order of the sums moves fp16 ties of the next layers' cache rows, so a step's results would
         # change with max_seq_len, which the choice of the form looks at)
-        A.attn_decode(self.q_turned, self.k_cache[l], self.v_cache[l], self.kv_len, out=self.att,
+        A.attn_decode(q, self.k_cache[l], self.v_cache[l], self.kv_len, out=self.att,
                       workspace=self.workspace, kv_early=self.kv_early and kv_sink == 0, two_pass=True)
         return self.att
 

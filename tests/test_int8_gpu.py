@@ -143,8 +143,8 @@ def test_special_rows(i8, dim, dtype):
 
 def product(a, a_scale, w, w_scale, swiglu, dtype):
     """The definition: the exact sum, rounded to fp32, times the channel's and the token's scale, each product rounded. Second: a bound
-    on how far the result may be from the first. Without SwiGLU none: the same operations. With it: exp is good to two units (2^-22),
-    the sum, the quotient and the product round once each (2^-24), the result once to its type."""
+    on how far the result may be from the first. Without SwiGLU none: the same operations. With it: exp is good to two units (2^-22)
+    and so is the quotient, the sum and the product round once each (2^-24), the result once to its type."""
     sums = (a.double() @ w.double().t())
     y = sums.float() * w_scale * a_scale[:, None]
     if not swiglu:
@@ -155,7 +155,7 @@ def product(a, a_scale, w, w_scale, swiglu, dtype):
     step = 2.0 ** -24 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
     # (below the type's smallest normal number, 2^-14 in fp16, its values are a fixed distance apart, 2^-24: half of that is the rounding)
     least = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
-    return want, want.abs() * (2.0 ** -22 + 3 * 2.0 ** -24 + step) * 1.01 + least + 1e-37
+    return want, want.abs() * (2 * 2.0 ** -22 + 2 * 2.0 ** -24 + step) * 1.01 + least + 1e-37
 
 
 def _eight_bits(i8, g, rows, k, lowest=-127):
