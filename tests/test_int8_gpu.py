@@ -309,6 +309,73 @@ def test_a_layers_calls_one_behind_the_other(i8, m, dim, hidden):
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
 
 
+@pytest.mark.parametrize("m,k,n,swiglu", [(1, 4096, 4096, False), (1, 100, 130, False), (9, 5000, 640, True), (40, 2048, 3000, False), (64, 4096, 200, True),
+                                          (130, 6000, 300, False), (500, 1000, 1200, False)])
+def test_weights_requested_early(i8, m, k, n, swiglu):
+    """w_early: weights that nothing writes are read while the kernels in front still run; what those write is waited for. Chains of
+    quantisation and product, each reading what the one before it wrote, in a row and in a graph."""
+    g, steps = _gen(m + n), 12
+    rows = 2 * n if swiglu else n
+    w, ws = i8.quantize_i8(_rand(g, rows, k))
+    x = [_rand(g, m, k) for _ in range(steps)]
+    q, s = i8.rows_i8(m, k), torch.empty(m, device=DEV)
+    outs = [torch.zeros((m, n), device=DEV) for _ in range(steps)]
+    torch.cuda.synchronize()
+    want = [i8.gemm_i8(*i8.quantize_i8(y), w, ws, swiglu=swiglu) for y in x]
+    torch.cuda.synchronize()
+
+    def run():
+        for y, out in zip(x, outs):
+            i8.quantize_i8(y, out=q, scale=s)
+            i8.gemm_i8(q, s, w, ws, out=out, swiglu=swiglu, w_early=True)
+
+    run()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for _ in range(3):
+        for out in outs:
+            out.zero_()
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_offsets_that_pass_32_bits(i8):
+    """More than 2^32 values in an output, and in the rows that are quantised; rows of an operand further than 2^32 bytes behind its first."""
+    g = _gen(12)
+    m, n, k = 66000, 66000, 16
+    a, w = _eight_bits(i8, g, m, k), _eight_bits(i8, g, n, k)
+    one = torch.ones(m, device=DEV)
+    out = i8.gemm_i8(a, one, w, one, out_dtype=torch.float16)
+    for t in (0, 1, 32767, 65076, 65999):
+        assert torch.equal(out[t], (a[t:t + 1].double() @ w.double().t()).half()[0])
+    del out
+    rows, dim = 140000, 32768
+    x = torch.empty((rows, dim), dtype=torch.float16, device=DEV)
+    for lo in range(0, rows, 20000):
+        x[lo:lo + 20000] = _rand(g, min(20000, rows - lo), dim, dtype=torch.float16)
+    q, scale = i8.quantize_i8(x)
+    for t in (0, 131071, 131072, 139999):
+        assert torch.equal(q[t:t + 1], whole_numbers(x[t:t + 1].float())) and abs(float(scale[t]) * 127 / float(x[t].abs().max()) - 1) < 2.0 ** -22
+    # the last rows as an operand of the product, reached from the first row's address
+    far = q[::1000, :2048]
+    assert far.stride(0) * (far.shape[0] - 1) > 2 ** 32
+    for m in (far.shape[0], 3):
+        b, bs = far[-m:], scale[::1000][-m:].contiguous()
+        got = i8.gemm_i8(far, scale[::1000].contiguous(), b, bs)
+        assert torch.equal(got, (far.double() @ b.double().t()).float() * bs * scale[::1000][:, None])
+    torch.cuda.synchronize()
+
+
+def test_a_matrix_with_itself(i8):
+    q, s = i8.quantize_i8(_rand(_gen(13), 200, 1000))
+    out = i8.gemm_i8(q, s, q, s)
+    assert torch.equal(out, (q.double() @ q.double().t()).float() * s * s[:, None])
+
+
 def test_empty_calls_and_refusals(i8):
     g = _gen(9)
     x, weight = _rand(g, 4, 64), torch.ones(64, device=DEV)
