@@ -30,7 +30,11 @@ GEMM_ARGS = struct.Struct("@5P3Q3I2iPi0P")
 def rows_i8(rows: int, k: int, device=None) -> torch.Tensor:
     """An int8 tensor [rows, k] laid out as the operators take it: rows a multiple of 16 bytes apart, from k = 128 on a multiple of 128,
     which is what memory is read in (10525 x 2948 x 2048: 64.6 us with rows 2960 bytes apart, 51.1 so)."""
-    return torch.empty_strided((rows, k), ((k + 127) & ~127 if k >= 128 else (k + 15) & ~15, 1), dtype=torch.int8, device="cuda" if device is None else device)
+    return torch.empty_strided((rows, k), (_apart(k), 1), dtype=_I8, device="cuda" if device is None else device)
+
+
+def _apart(k: int) -> int:
+    return (k + 127) & ~127 if k >= 128 else (k + 15) & ~15
 
 
 # (A call's checks are part of the microseconds that a small one takes: what is dense is asked first, the rest is looked at here.)
@@ -83,9 +87,11 @@ def _rows(entry: str, x, weight, eps: float, delta, x_out, out, scale, stream):
         raise ValueError("x_out without delta")
     if out is None:
         out = rows_i8(N, D, x.device) if stream is None else _on(stream, rows_i8, N, D, x.device)
-    elif out.dtype is not _I8 or out.shape != shape:
-        raise ValueError("out must be int8, of x's shape")
-    q_stride = _byte_stride(out, N, D, "out")
+        q_stride = _apart(D)
+    else:
+        if out.dtype is not _I8 or out.shape != shape:
+            raise ValueError("out must be int8, of x's shape")
+        q_stride = _byte_stride(out, N, D, "out")
     if scale is None:
         scale = torch.empty_strided((N,), (1,), dtype=torch.float32, device=x.device) if stream is None else \
             _on(stream, torch.empty_strided, (N,), (1,), dtype=torch.float32, device=x.device)

@@ -36,7 +36,7 @@ def test_strides_of_rows(i8):
         assert (a.x_stride, a.delta_stride, a.x_out_stride) == strides and (a.rows, a.dim) == x.shape
         assert a.x == x.data_ptr() and a.q == q.data_ptr() and a.scale == s.data_ptr() and a.weight == w.data_ptr()
         assert a.delta == (0 if delta is None else delta.data_ptr()) or a.delta is None
-        assert a.q_stride == (48 if x.shape[0] > 1 else 0)
+        assert a.q_stride == 48
 
 
 def test_x_out_is_x_where_none_is_given(i8):
