@@ -3,8 +3,8 @@
 //
 // Mathematics: h = x + delta, z = h * weight, A = max|z|, r = 1 / sqrt(mean(h^2) + eps). The norm is y = r z, and the symmetric
 // 8-bit form has scale max|y| / 127 = r A / 127 and q = round(y / scale) = round(z * (127 / A)): r cancels. So one pass over the row
-// yields both reductions, and q, made of single fp32 operations on single elements, does not depend on the order of any sum. The largest
-// |z| is found on the bits without their sign, which order as the numbers do and put infinity and NaN on top.
+// yields both reductions, and q, made of single fp32 operations on single elements, does not depend on the order of any sum. The maxima
+// keep NaN, and a row's largest bits say whether it holds one or an infinity.
 //
 // Bound by memory: every value is read once and written once (norm of 9184 x 4096 fp32 with its delta 74.1 us = 6.6 TB/s, quantisation of
 // 9184 x 4096 fp32 28.3 us = 6.6 TB/s, of 9184 x 14336 bf16 65.7 us = 6.0 TB/s; one row 1.9 - 2.1 us in a graph). A row stays in the
@@ -278,7 +278,7 @@ struct Kept {
     }
 };
 
-// A row per block, or per warp. DT: type of x. NORM: weight, and the norm's factor in the scale. ALIGNED: rows may be read and written
+// A row per block, or per warp (narrow ones: no barrier). DT: type of x. NORM: weight, and the norm's factor in the scale. ALIGNED: rows may be read and written
 // in runs of VEC values. CHUNKS runs a thread, or 0: a row longer than that, read twice.
 template <int DT, bool NORM, bool DELTA, int VEC, int CHUNKS, bool ALIGNED>
 __global__ void __launch_bounds__(max_threads(NORM, VEC, CHUNKS)) rows_i8_kernel(const __grid_constant__ RowsParams p) {
@@ -438,7 +438,6 @@ int launch_rows(RowsParams& p, uint32_t run, const DeviceInfo& dev, cudaStream_t
     const bool aligned = run == kWide;
     const uint32_t vec = aligned ? kWide : 4;
     auto threads = [&](uint32_t chunks) { return ((p.dim + vec * chunks - 1) / (vec * chunks) + 31) / 32 * 32; };
-    const uint32_t row_bytes = p.dim * size_of(DT) + (DELTA ? p.dim * size_of(p.delta_dtype) : 0);
     // Long rows in number: where few blocks of a row's threads fit an SM, the ring keeps the reads going. Quantisation of 9184 x 14336 bf16
     // 78.7 -> 65.7 us, 5500 x 14336 fp32 87 -> 63, 4000 x 28672 fp16 77 -> 56, the norm of 2000 x 16384 bf16 with an fp32 delta 57 -> 53. Blocks
     // of fewer threads do better without (quantisation of 9184 x 8192 bf16 36.6 for 51.3, of 4000 x 11008 25.1 for 30.5, the norm of 4096 x
@@ -529,8 +528,8 @@ int rows_i8(const AttnRowsI8Args* a, bool norm, void* stream_v) {
     p.eps = a->eps;
     p.delta_dtype = a->delta_dtype;
     // Runs that a thread reads and writes at once: 8 values of 16 bits, 4 of any type, or single ones, as the rows' length, places and distances
-    // allow. (9184 x 14335 bf16, one by one: 126 us;
-    // of 14336: 65.7. Neighbouring values to neighbouring threads instead, whole numbers in single bytes then: 254.)
+    // allow. (Quantisation of 9184 x 14336 bf16 65.7 us, of 14335, one by one, 126; neighbouring values to neighbouring threads, whole
+    // numbers in single bytes then, 254.)
     const uint64_t apart = n > 1 ? ~0ull : 0ull;
     auto fits = [&](uint64_t ptr, uint64_t stride, uint32_t size, uint32_t values) {
         return (ptr | (stride * size & apart)) % std::min<uint32_t>(16, size * values) == 0;
