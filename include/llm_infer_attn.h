@@ -21,6 +21,11 @@
  *     void* so that this header needs no CUDA include);
  *   - the caller owns every buffer, as the engine's Tensor<T> does
  *     (include/model/tensor.hpp:29-44);
+ *   - kernels of a stream overlap several deep: each may start before the one in front of it has ended, which may itself
+ *     have started early. All but what a *_early argument names is waited for. Where one asks that an operand was "in
+ *     place before the previous kernel of the stream was launched", whatever wrote it must have COMPLETED by then: the host
+ *     has waited for it (cudaStreamSynchronize, an event), or a copy enqueued between the two keeps them apart. An earlier
+ *     place in the stream alone does not suffice;
  *   - K/V caches keep the engine's layout: 16-bit elements,
  *     [row][kv_head][head_dim], one cache per sequence
  *     (include/model/block.hpp:66-67, src/model/block.cpp:71-74);
@@ -622,9 +627,10 @@ typedef struct AttnGemmI8Args {
     int32_t out_dtype;    /* ATTN_DTYPE_F32 | F16 | BF16 */
     int32_t swiglu;
     uint32_t* status;     /* optional device word for ATTN_STATUS_* bits */
-    int32_t w_early;      /* != 0: the caller vouches that w was in place before the previous kernel of the stream was launched (true
-                             of a loaded model's weights): with few tokens the kernel then fills its pipeline with weights while that
-                             kernel may still be running. No other operand is read early. 0 = wait first */
+    int32_t w_early;      /* != 0: the caller vouches that what wrote w had completed, the host having waited for it, before the previous
+                             kernel of the stream was enqueued (true of a loaded model's weights; an earlier place in the stream
+                             does not suffice, see the conventions). With few tokens the kernel then fills its pipeline with weights while that kernel, and
+                             those in front of it, may still be running. No other operand is read early. 0 = wait first */
 } AttnGemmI8Args;
 /* out may not share memory with an operand. */
 int attn_gemm_i8(const AttnGemmI8Args* args, void* stream);

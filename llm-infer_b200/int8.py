@@ -128,8 +128,9 @@ def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: to
     a       int8 [m, k], a_scale fp32 [m]; w int8 [n, k], w_scale fp32 [n]; rows a multiple of 16 bytes apart, k up to 131071
     swiglu  w holds n_out gate rows, then n_out up rows: out = silu(gate) * up [m, n_out]
     out     fp32 / fp16 / bf16 [m, n_out], rows may be strided (default: a new tensor of out_dtype); no operand's memory
-    w_early the caller vouches that w was in place before the previous kernel of the stream was launched: its first tiles are then read
-            while that kernel may still be running (a loaded model's weights)
+    w_early the caller vouches that what wrote w had completed, the host having waited for it (torch.cuda.synchronize), before the
+            previous kernel of the stream was enqueued, as for a loaded model's weights: its first tiles are then read while that kernel,
+            and those in front of it, may still be running. A quantize_i8 of w further ahead in the stream is not waited for
     The same bits for a token whatever else is in the batch."""
     index = _one_device(a, a_scale, w, w_scale, out, status)
     a_shape, w_shape = a.shape, w.shape
