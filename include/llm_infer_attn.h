@@ -606,6 +606,8 @@ typedef struct AttnRowsI8Args {
     uint32_t rows, dim;
     float eps;           /* at least 2^-126 (attn_quantize_i8: not used) */
     int32_t x_dtype, delta_dtype; /* ATTN_DTYPE_F32 | F16 | BF16 */
+    uint32_t* status;    /* optional device word, ATTN_STATUS_* bits are ORed in; NULL to skip. ATTN_STATUS_WAIT_TIMEOUT: rows did not
+                            arrive; theirs are q = 0 and scale = NaN, and x_out is not written, or in part */
 } AttnRowsI8Args;
 /* Nothing that is written may share memory with anything else that is read or written, but for x_out in the place of x. */
 int attn_rmsnorm_i8(const AttnRowsI8Args* args, void* stream);

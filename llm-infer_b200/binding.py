@@ -414,6 +414,7 @@ class AttnRowsI8Args(C.Structure):
         ("eps", C.c_float),
         ("x_dtype", C.c_int32),
         ("delta_dtype", C.c_int32),
+        ("status", C.c_void_p),
     ]
 
 

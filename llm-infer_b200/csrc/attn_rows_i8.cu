@@ -16,6 +16,7 @@
 #include "attn_internal.cuh"
 #include "operand_memory.cuh"
 #include "ptx_sm100.cuh"
+#include "rows_ring.cuh"
 #include "tcgen05_sm100.cuh"
 
 namespace b200 {
@@ -34,10 +35,12 @@ struct RowsParams {
     uint32_t whole16;      // rows are a multiple of 16 bytes long
     float eps;
     int32_t delta_dtype;
+    uint32_t* status;
 };
 
 constexpr uint32_t kMaxThreads = 1024, kWarpRows = 4;  // threads of a block, rows of one whose rows are a warp's
 constexpr uint32_t kInf = 0x7f800000u;
+constexpr uint32_t kLost = 0xffffffffu;  // among rows' largest bits: a row that did not arrive
 constexpr float kLiftTiny = 18446744073709551616.f;  // 2^64
 // (four runs of eight values of x, delta and weight beside each other do not fit the 64 registers that 1024 threads have each)
 constexpr uint32_t max_threads(bool norm, int vec, uint32_t chunks) { return norm && vec == 8 && chunks == 4 ? 512 : kMaxThreads; }
@@ -173,11 +176,12 @@ __device__ __forceinline__ void count16(const Raw<VEC>& r, Found& f) {
     }
 }
 
-// A row's reductions, the same in all its threads: the largest bits and the sum. s_top, s_sum: a value per warp, in other places for the
-// block's next row.
+// A row's reductions, the same in all its threads: the largest bits, among them a thread's `floor`, and the sum. s_top, s_sum: a value per
+// warp, in other places for the block's next row.
 template <int DT, bool NORM>
-__device__ __forceinline__ void reduce_row(const Found& f, uint32_t& top, float& sum, bool whole_block, uint32_t* s_top, float* s_sum) {
-    top = __float_as_uint(f.top);
+__device__ __forceinline__ void reduce_row(const Found& f, uint32_t floor, uint32_t& top, float& sum, bool whole_block, uint32_t* s_top,
+                                           float* s_sum) {
+    top = max(__float_as_uint(f.top), floor);
     if constexpr (!NORM && DT != ATTN_DTYPE_F32) {
         float lo, hi;
         tc::unpack2<DT == ATTN_DTYPE_BF16>(f.top16, lo, hi);
@@ -326,7 +330,7 @@ __global__ void __launch_bounds__(max_threads(NORM, VEC, CHUNKS)) rows_i8_kernel
                 }
             }
         }
-        reduce_row<DT, NORM>(found, top, sum, whole_block, s_top, s_sum);
+        reduce_row<DT, NORM>(found, 0u, top, sum, whole_block, s_top, s_sum);
         const Rounding r = finish_row<NORM>(p, row, top, sum, t == 0);
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
@@ -341,7 +345,7 @@ __global__ void __launch_bounds__(max_threads(NORM, VEC, CHUNKS)) rows_i8_kernel
             combine<DT, NORM, DELTA, VEC, ALIGNED>(p, i, rx, rd, h, z);
             count<NORM, VEC>(h, z, found);
         }
-        reduce_row<DT, NORM>(found, top, sum, whole_block, s_top, s_sum);
+        reduce_row<DT, NORM>(found, 0u, top, sum, whole_block, s_top, s_sum);
         const Rounding r = finish_row<NORM>(p, row, top, sum, t == 0);
         for (uint32_t i = index(0); i < p.dim; i += p.row_threads * VEC) {  // (x_out may be x: nothing of the row was written before)
             fetch(i, rx, rd);
@@ -376,25 +380,24 @@ __global__ void __launch_bounds__(kMaxThreads) rows_i8_ring_kernel(const __grid_
     grid_dep_launch_dependents();
     grid_dep_wait();
     const uint64_t policy = l2_policy_evict_first();
-    auto request = [&](uint32_t row, uint32_t slot) {  // thread 0
-        const uint32_t dst = smem_u32(ring) + slot * slot_bytes, bar = full + 8 * slot;
+    auto request = [&](uint32_t n, uint32_t slot) {  // row n of this block
+        if (t != 0) return;
+        const uint32_t row = blockIdx.x + n * gridDim.x, dst = smem_u32(ring) + slot * slot_bytes, bar = full + 8 * slot;
         mbar_arrive_expect_tx(bar, slot_bytes);
         bulk_g2s(dst, static_cast<const unsigned char*>(p.x) + row * p.x_stride * (DT == ATTN_DTYPE_F32 ? 4 : 2), x_bytes, bar, policy);
         if constexpr (DELTA)
             bulk_g2s(dst + x_bytes, static_cast<const unsigned char*>(p.delta) + row * p.delta_stride * (p.delta_dtype == ATTN_DTYPE_F32 ? 4 : 2),
                      d_bytes, bar, policy);
     };
+    auto wait = [&](uint32_t slot, uint32_t phase) { return mbar_wait(full + 8 * slot, phase); };
     const uint32_t mine = (p.rows - blockIdx.x + gridDim.x - 1) / gridDim.x;  // rows of this block
-    if (t == 0)
-        for (uint32_t s = 0; s < min(kSlots, mine); ++s) request(blockIdx.x + s * gridDim.x, s);
-    uint32_t slot = 0, phase = 0;
-    for (uint32_t n = 0; n < mine; ++n) {
+    Kept<DT, NORM, VEC, CHUNKS> kept;
+    uint32_t top;
+    float sum;
+    auto reduce = [&](uint32_t n, uint32_t slot, bool there) {
         const uint32_t row = blockIdx.x + n * gridDim.x;
-        // a wait that runs out makes the row one of NaN
-        Found found;
-        if (!mbar_wait(full + 8 * slot, phase)) found.top = __uint_as_float(0x7fffffffu);
         const unsigned char* x = ring + slot * slot_bytes;
-        Kept<DT, NORM, VEC, CHUNKS> kept;
+        Found found;
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             const uint32_t i = (c * blockDim.x + t) * VEC;
@@ -410,14 +413,15 @@ __global__ void __launch_bounds__(kMaxThreads) rows_i8_ring_kernel(const __grid_
                     combine<DT, NORM, DELTA, VEC, true>(p, i, rx, rd, h, kept.z[c]);
                     count<NORM, VEC>(h, kept.z[c], found);
                     if constexpr (DELTA)
-                        if (p.x_out) store<VEC, DT, true>(p.x_out, row * p.x_out_stride + i, h, VEC);
+                        if (p.x_out && there) store<VEC, DT, true>(p.x_out, row * p.x_out_stride + i, h, VEC);
                 }
             }
         }
-        uint32_t top;
-        float sum;
-        reduce_row<DT, NORM>(found, top, sum, true, s_top + (n & 1) * (kMaxThreads / 32), s_sum + (n & 1) * (kMaxThreads / 32));
-        if (t == 0 && n + kSlots < mine) request(row + kSlots * gridDim.x, slot);  // (behind the barrier: all have read the slot)
+        reduce_row<DT, NORM>(found, there ? 0u : kLost, top, sum, true, s_top + (n & 1) * (kMaxThreads / 32), s_sum + (n & 1) * (kMaxThreads / 32));
+        return top != kLost;
+    };
+    auto finish = [&](uint32_t n) {
+        const uint32_t row = blockIdx.x + n * gridDim.x;
         const Rounding r = finish_row<NORM>(p, row, top, sum, t == 0);
         int8_t* q = p.q + row * p.q_stride;
 #pragma unroll
@@ -425,8 +429,19 @@ __global__ void __launch_bounds__(kMaxThreads) rows_i8_ring_kernel(const __grid_
             const uint32_t i = (c * blockDim.x + t) * VEC;
             if (i < p.dim) put<VEC, true>(q + i, kept.values(c), r, VEC);
         }
-        if (++slot == kSlots) slot = 0, phase ^= 1;
-    }
+    };
+    // A copy that did not arrive within the limit: the block's rows from there on become rows of NaN.
+    auto lose = [&](uint32_t n) {
+        if (t == 0 && p.status) atomicOr(p.status, ATTN_STATUS_WAIT_TIMEOUT);
+        const float none[VEC] = {};
+        for (; n < mine; ++n) {
+            const uint32_t row = blockIdx.x + n * gridDim.x;
+            const Rounding r = finish_row<NORM>(p, row, kLost, 0.f, t == 0);
+#pragma unroll 1
+            for (uint32_t i = t * VEC; i < p.dim; i += blockDim.x * VEC) put<VEC, true>(p.q + row * p.q_stride + i, none, r, VEC);
+        }
+    };
+    run_ring<kSlots>(mine, request, wait, reduce, finish, lose);
 }
 
 uint32_t size_of(int32_t dtype) { return dtype == ATTN_DTYPE_F32 ? 4 : 2; }
@@ -527,6 +542,7 @@ int rows_i8(const AttnRowsI8Args* a, bool norm, void* stream_v) {
     p.dim = a->dim;
     p.eps = a->eps;
     p.delta_dtype = a->delta_dtype;
+    p.status = a->status;
     // Runs that a thread reads and writes at once: 8 values of 16 bits, 4 of any type, or single ones, as the rows' length, places and distances
     // allow. (Quantisation of 9184 x 14336 bf16 65.7 us, of 14335, one by one, 126; neighbouring values to neighbouring threads, whole
     // numbers in single bytes then, 254.)

@@ -23,7 +23,7 @@ _FLOATS = {t: _DTYPES[t] for t in (torch.float32, torch.float16, torch.bfloat16)
 MAX_K = 131071  # longest inner dimension of gemm_i8: 32-bit sums of products of 8 bits stay exact
 
 # The argument structures as the library lays them out (packed: see context).
-ROWS_ARGS = struct.Struct("@6P4Q2If2i0P")
+ROWS_ARGS = struct.Struct("@6P4Q2If2iP")
 GEMM_ARGS = struct.Struct("@5P3Q3I2iPi0P")
 
 
@@ -58,8 +58,8 @@ def _byte_stride(q: torch.Tensor, rows: int, k: int, what: str) -> int:
     return stride
 
 
-def _rows(entry: str, x, weight, eps: float, delta, x_out, out, scale, stream):
-    index = _one_device(x, weight, delta, x_out, out, scale)
+def _rows(entry: str, x, weight, eps: float, delta, x_out, out, scale, status, stream):
+    index = _one_device(x, weight, delta, x_out, out, scale, status)
     shape, x_dtype = x.shape, x.dtype
     if len(shape) != 2 or shape[1] == 0:
         raise ValueError("x must be [N, D], its rows not empty")
@@ -100,25 +100,27 @@ def _rows(entry: str, x, weight, eps: float, delta, x_out, out, scale, stream):
     if N:
         _enqueue(entry, index, stream, ROWS_ARGS.pack(
             out.data_ptr(), scale.data_ptr(), x_out_ptr, x.data_ptr(), delta_ptr, weight_ptr, q_stride, x_stride, delta_stride,
-            x_out_stride, N, D, eps, x_code, delta_code))
+            x_out_stride, N, D, eps, x_code, delta_code, 0 if status is None else status.data_ptr()))
     return out, scale
 
 
-def rmsnorm_i8(x: torch.Tensor, weight: torch.Tensor, eps: float, *, delta=None, x_out=None, out=None, scale=None, stream=None):
+def rmsnorm_i8(x: torch.Tensor, weight: torch.Tensor, eps: float, *, delta=None, x_out=None, out=None, scale=None, status=None,
+               stream=None):
     """(q, scale) of y = h / sqrt(mean(h^2) + eps) * weight, h = x + delta, per row: scale = max|y| / 127, q = round(y / scale).
 
     x       [N, D] fp32 / fp16 / bf16, rows may be strided; weight fp32 [D]; eps at least 2^-126
     delta   [N, D] of any of these types: the residual's addition. h is written to ``x_out`` (x's type; default: x itself)
     out     int8 [N, D] (rows_i8), scale fp32 [N]; new tensors by default
+    status  optional device word for ATTN_STATUS_* bits: rows that did not arrive have q = 0 and scale NaN, and x_out is not written, or in part
     A row of zeros has scale 0; one with NaN or an infinity q = 0 and scale NaN. Nothing that is written may share memory with
     another operand, but for x_out in the place of x."""
-    return _rows("attn_rmsnorm_i8", x, weight, eps, delta, x_out, out, scale, stream)
+    return _rows("attn_rmsnorm_i8", x, weight, eps, delta, x_out, out, scale, status, stream)
 
 
-def quantize_i8(x: torch.Tensor, *, out=None, scale=None, stream=None):
+def quantize_i8(x: torch.Tensor, *, out=None, scale=None, status=None, stream=None):
     """(q, scale) of the rows of x [N, D] fp32 / fp16 / bf16: scale = max|x| / 127, q = round(x / scale), ties to even. Of a weight
     matrix [n_out, k] the rows are the channels that gemm_i8 wants. Special rows and memory as rmsnorm_i8."""
-    return _rows("attn_quantize_i8", x, None, 0.0, None, None, out, scale, stream)
+    return _rows("attn_quantize_i8", x, None, 0.0, None, None, out, scale, status, stream)
 
 
 def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *, out=None, out_dtype=torch.float32,

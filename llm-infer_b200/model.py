@@ -240,20 +240,20 @@ class Llama:
         c, w, w8, status = self.cfg, self.w, self.w8, self.status
         n, scale, delta = x.shape[0], b["scale"], None
         for l in range(c.n_layers):
-            q, s = I.rmsnorm_i8(x, w["rms_att"][l], c.norm_eps, delta=delta, out=b["dim"], scale=scale)
+            q, s = I.rmsnorm_i8(x, w["rms_att"][l], c.norm_eps, delta=delta, out=b["dim"], scale=scale, status=status)
             I.gemm_i8(q, s, *w8["wqkv"][l], out=b["qkv"], status=status, w_early=True)
-            q, s = I.quantize_i8(attend(l).view(n, -1), out=b["q_dim"], scale=scale)
+            q, s = I.quantize_i8(attend(l).view(n, -1), out=b["q_dim"], scale=scale, status=status)
             delta = I.gemm_i8(q, s, *w8["wo"][l], out=b["delta"], status=status, w_early=True)
-            q, s = I.rmsnorm_i8(x, w["rms_ffn"][l], c.norm_eps, delta=delta, out=b["dim"], scale=scale)  # x += Wo att
+            q, s = I.rmsnorm_i8(x, w["rms_ffn"][l], c.norm_eps, delta=delta, out=b["dim"], scale=scale, status=status)  # x += Wo att
             hb = I.gemm_i8(q, s, *w8["w13"][l], out=b["hb"], swiglu=True, status=status, w_early=True)
-            q, s = I.quantize_i8(hb, out=b["hidden"], scale=scale)
+            q, s = I.quantize_i8(hb, out=b["hidden"], scale=scale, status=status)
             delta = I.gemm_i8(q, s, *w8["w2"][l], out=b["delta"], status=status, w_early=True)
         return delta
 
     def _classify_i8(self, delta: torch.Tensor) -> None:
         """Final norm of x + delta, classifier and greedy pick of the batch."""
         b = self._rows8
-        q, s = I.rmsnorm_i8(self.x, self.w["rms_final"], self.cfg.norm_eps, delta=delta, out=b["dim"], scale=b["scale"])
+        q, s = I.rmsnorm_i8(self.x, self.w["rms_final"], self.cfg.norm_eps, delta=delta, out=b["dim"], scale=b["scale"], status=self.status)
         I.gemm_i8(q, s, *self.w8["wcls"], out=self.logits, status=self.status, w_early=True)
         A.argmax(self.logits, out=self.next_token)
         self.tokens.copy_(self.next_token)
