@@ -16,7 +16,7 @@ import torch
 
 from . import binding as _b
 from .attention import _DTYPES
-from .context import _enqueue, _on, _one_device
+from .context import _INDEX, _enqueue, _on, _one_device
 
 _F32, _I8 = torch.float32, torch.int8
 _FLOATS = {t: _DTYPES[t] for t in (torch.float32, torch.float16, torch.bfloat16)}
@@ -56,6 +56,15 @@ def _byte_stride(q: torch.Tensor, rows: int, k: int, what: str) -> int:
     if stride % 16:
         raise ValueError(f"the rows of {what} must be a multiple of 16 bytes apart (rows_i8 lays them out so)")
     return stride
+
+
+def _status(t: torch.Tensor | None) -> int:
+    """The address of a status word; 0 without one."""
+    if t is None:
+        return 0
+    if t.dtype not in _INDEX or t.numel() == 0:
+        raise ValueError("status must be a tensor of 32-bit integers, its first element the word")
+    return t.data_ptr()
 
 
 def _rows(entry: str, x, weight, eps: float, delta, x_out, out, scale, status, stream):
@@ -100,7 +109,7 @@ def _rows(entry: str, x, weight, eps: float, delta, x_out, out, scale, status, s
     if N:
         _enqueue(entry, index, stream, ROWS_ARGS.pack(
             out.data_ptr(), scale.data_ptr(), x_out_ptr, x.data_ptr(), delta_ptr, weight_ptr, q_stride, x_stride, delta_stride,
-            x_out_stride, N, D, eps, x_code, delta_code, 0 if status is None else status.data_ptr()))
+            x_out_stride, N, D, eps, x_code, delta_code, _status(status)))
     return out, scale
 
 
@@ -169,5 +178,5 @@ def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: to
     if m and n:
         _enqueue("attn_gemm_i8", index, stream, GEMM_ARGS.pack(
             out.data_ptr(), a.data_ptr(), a_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), a_stride, w_stride, ldc, m, n, k,
-            out_code, 1 if swiglu else 0, 0 if status is None else status.data_ptr(), 1 if w_early else 0))
+            out_code, 1 if swiglu else 0, _status(status), 1 if w_early else 0))
     return out
