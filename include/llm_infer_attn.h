@@ -592,8 +592,9 @@ int attn_kv_evict(const AttnKvEvictArgs* args, void* stream);
 /* Per row: h = x + delta (fp32), x_out = h rounded to x's type, y = h / sqrt(mean(h^2) + eps) * weight (attn_quantize_i8: y = x),
  * scale = max|y| / 127, q = y / scale rounded to the nearest whole number, ties to the even one. The norm's factor is the same for the
  * whole row and so belongs to the scale alone: q is round(z * (127 / max|z|)) of z = h * weight, each operation rounded to fp32, and
- * depends on no sum's order. A row of zeros: scale 0. A row that holds NaN or an infinity (or whose z passes fp32's range):
- * q = 0 and scale = NaN, so that every product with it is NaN. */
+ * depends on no sum's order. A row of zeros: scale 0. A row that holds NaN or an infinity, or whose z passes fp32's range, or
+ * (attn_rmsnorm_i8) whose sum of h^2 does, for which |h| of 1.8e19 / sqrt(dim) throughout is enough: q = 0 and scale = NaN, so that every
+ * product with it is NaN. */
 typedef struct AttnRowsI8Args {
     int8_t* q;           /* out: [rows][dim], row r at q + r*q_stride, 16-byte aligned */
     float* scale;        /* out: [rows] */
@@ -609,14 +610,15 @@ typedef struct AttnRowsI8Args {
     uint32_t* status;    /* optional device word, ATTN_STATUS_* bits are ORed in; NULL to skip. ATTN_STATUS_WAIT_TIMEOUT: rows did not
                             arrive; theirs are q = 0 and scale = NaN, and x_out is not written, or in part */
 } AttnRowsI8Args;
-/* Nothing that is written may share memory with anything else that is read or written, but for x_out in the place of x. */
+/* Nothing that is written may share memory with anything else that is read or written, but for x_out in the place of x. Rows that lie
+ * between another operand's rows at the same distance share none; at another distance their whole extents may not meet. */
 int attn_rmsnorm_i8(const AttnRowsI8Args* args, void* stream);
 int attn_quantize_i8(const AttnRowsI8Args* args, void* stream);
 
 /* out[t][j] = a_scale[t] * w_scale[j] * sum_i a[t][i] * w[j][i], t < m tokens, j < n_out, i < k. The sum is exact (32-bit integers,
- * k up to 131071), two fp32 products scale it and the result is rounded once to out's type: the same bits for every m and every
- * stride. With swiglu != 0 the matrix holds n_out gate rows followed by n_out up rows, and out = silu(gate) * up, computed in fp32
- * (src/model/block.cpp:206-210). */
+ * k up to 131071). It is converted to fp32, which rounds it beyond 2^24, multiplied by w_scale[j], then by a_scale[t], each product rounded
+ * to fp32, and rounded to out's type: the same bits for every m and every stride. With swiglu != 0 the matrix holds n_out gate rows
+ * followed by n_out up rows, and out = silu(gate) * up, computed in fp32 (src/model/block.cpp:206-210). */
 typedef struct AttnGemmI8Args {
     void* out;            /* [m][n_out], out_dtype, row t at out + t*ldc elements */
     const int8_t* a;      /* [m][k], row t at a + t*a_stride, 16-byte aligned */
@@ -631,10 +633,11 @@ typedef struct AttnGemmI8Args {
     uint32_t* status;     /* optional device word for ATTN_STATUS_* bits */
     int32_t w_early;      /* != 0: the caller vouches that what wrote w had completed, the host having waited for it, before the previous
                              kernel of the stream was enqueued (true of a loaded model's weights; an earlier place in the stream
-                             does not suffice, see the conventions). With few tokens the kernel then fills its pipeline with weights while that kernel, and
-                             those in front of it, may still be running. No other operand is read early. 0 = wait first */
+                             does not suffice, see the conventions). With few tokens the kernel then fills its pipeline with weights
+                             while that kernel, and those in front of it, may still be running. No other operand is read early.
+                             0 = wait first */
 } AttnGemmI8Args;
-/* out may not share memory with an operand. */
+/* out may not share memory with an operand (rows between rows: as above). */
 int attn_gemm_i8(const AttnGemmI8Args* args, void* stream);
 
 /* Human-readable text for an ATTN_ERR_* code. */

@@ -121,8 +121,9 @@ def rmsnorm_i8(x: torch.Tensor, weight: torch.Tensor, eps: float, *, delta=None,
     delta   [N, D] of any of these types: the residual's addition. h is written to ``x_out`` (x's type; default: x itself)
     out     int8 [N, D] (rows_i8), scale fp32 [N]; new tensors by default
     status  optional device word for ATTN_STATUS_* bits: rows that did not arrive have q = 0 and scale NaN, and x_out is not written, or in part
-    A row of zeros has scale 0; one with NaN or an infinity q = 0 and scale NaN. Nothing that is written may share memory with
-    another operand, but for x_out in the place of x."""
+    A row of zeros has scale 0; one with NaN or an infinity, or whose h * weight or sum of h^2 passes fp32's range (|h| of 1.8e19 / sqrt(D)
+    throughout), q = 0 and scale NaN. Nothing that is written may share memory with another operand, but for x_out in the place of x;
+    rows between another operand's rows, at the same distance, share none."""
     return _rows("attn_rmsnorm_i8", x, weight, eps, delta, x_out, out, scale, status, stream)
 
 
@@ -134,7 +135,8 @@ def quantize_i8(x: torch.Tensor, *, out=None, scale=None, status=None, stream=No
 
 def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *, out=None, out_dtype=torch.float32,
             swiglu: bool = False, status=None, w_early: bool = False, stream=None) -> torch.Tensor:
-    """out[t, j] = a_scale[t] * w_scale[j] * sum_i a[t, i] * w[j, i]: the sum exact, rounded once to out's type.
+    """out[t, j] = a_scale[t] * w_scale[j] * sum_i a[t, i] * w[j, i]: the sum exact in 32-bit integers, then converted to
+    fp32 (rounded beyond 2^24), times w_scale[j], times a_scale[t], each rounded to fp32, and rounded to out's type.
 
     a       int8 [m, k], a_scale fp32 [m]; w int8 [n, k], w_scale fp32 [n]; rows a multiple of 16 bytes apart, k up to 131071
     swiglu  w holds n_out gate rows, then n_out up rows: out = silu(gate) * up [m, n_out]

@@ -95,7 +95,8 @@ class Llama:
         """``rope_layout`` and ``rope_scaling`` (context.rope_frequencies): positions of models that pair a head's halves, or whose
         frequencies are scaled for long contexts. The defaults are the engine's positions and kernels.
         ``weight_type`` "i8": the fp16 matrices of ``weights`` are brought to 8 bits with a scale per output channel, here and once, and
-        every projection multiplies 8-bit integers (module int8: activations get a scale per token on the way). One path for steps
+        every projection multiplies 8-bit integers (module int8: activations get a scale per token on the way, and the
+        gated hidden ones are held in bf16 ahead of their 8 bits). One path for steps
         of any batch and for prompts, positions by context.rope_positions, no clamp of q, k and v."""
         dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         if dev.type != "cuda":
@@ -225,6 +226,8 @@ class Llama:
         c, dev = self.cfg, self.device
         q_dim, e = c.n_heads * c.head_dim, torch.empty
         return {"dim": I.rows_i8(n, c.dim, dev), "q_dim": I.rows_i8(n, q_dim, dev), "hidden": I.rows_i8(n, c.hidden_dim, dev),
+                # (hb in bf16: its rounding, up to a quarter of an 8-bit step on a row's largest values, comes on top of the half step
+                # of quantize_i8, which reads half the bytes so; fp16 would overflow where bf16 does not)
                 "scale": e(n, device=dev), "qkv": e(n, q_dim + 2 * c.n_kv_heads * c.head_dim, device=dev), "delta": e(n, c.dim, device=dev),
                 "hb": e(n, c.hidden_dim, dtype=torch.bfloat16, device=dev)}
 
