@@ -58,10 +58,8 @@ def _byte_stride(q: torch.Tensor, rows: int, k: int, what: str) -> int:
     return stride
 
 
-def _status(t: torch.Tensor | None) -> int:
-    """The address of a status word; 0 without one."""
-    if t is None:
-        return 0
+def _status(t: torch.Tensor) -> int:
+    """The address of a status word."""
     if t.dtype not in _INDEX or t.numel() == 0:
         raise ValueError("status must be a tensor of 32-bit integers, its first element the word")
     return t.data_ptr()
@@ -109,7 +107,7 @@ def _rows(entry: str, x, weight, eps: float, delta, x_out, out, scale, status, s
     if N:
         _enqueue(entry, index, stream, ROWS_ARGS.pack(
             out.data_ptr(), scale.data_ptr(), x_out_ptr, x.data_ptr(), delta_ptr, weight_ptr, q_stride, x_stride, delta_stride,
-            x_out_stride, N, D, eps, x_code, delta_code, _status(status)))
+            x_out_stride, N, D, eps, x_code, delta_code, 0 if status is None else _status(status)))
     return out, scale
 
 
@@ -180,5 +178,5 @@ def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: to
     if m and n:
         _enqueue("attn_gemm_i8", index, stream, GEMM_ARGS.pack(
             out.data_ptr(), a.data_ptr(), a_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), a_stride, w_stride, ldc, m, n, k,
-            out_code, 1 if swiglu else 0, _status(status), 1 if w_early else 0))
+            out_code, 1 if swiglu else 0, 0 if status is None else _status(status), 1 if w_early else 0))
     return out
