@@ -6,10 +6,10 @@
 // them in any order gives the same bits. Weights are the M side of the MMA: a tensor-memory lane is a channel, which has its scale in
 // a register, and a warp stores 32 neighbouring channels of a token at a time.
 //
-// What bounds it: with few tokens the weights' way from memory (8 x 4096 x 128256 79 us = 6.7 TB/s, 8 x 4096 x 28672 20.4 us = 5.8 TB/s) and, where
-// they are few, some 4 us from a launch to its first and from its last tile (1 x 4096 x 6144 7.8 us in a graph for 3.9 of reading);
+// What bounds it: with few tokens the weights' way from memory (8 x 4096 x 128256 79 us = 6.7 TB/s, 8 x 4096 x 28672 20.4 - 20.9 us = 5.6 - 5.8 TB/s) and, where
+// they are few, some 4 us from a launch to its first and from its last tile (1 x 4096 x 6144 7.5 us in a graph for 3.8 of reading);
 // with many tokens the tensor cores (9184 x 4096 x 28672 with SwiGLU 634 - 654 us = 3.3 - 3.4 POP/s in a burst, twice the measured bf16
-// rate; in a long loop the 1000 W cap holds it at 2.9 POP/s and 1.24 GHz, where the pipe does 95 % of what it can).
+// rate; in a long loop the 1000 W cap holds it at 2.8 - 2.9 POP/s and 1.24 - 1.26 GHz, where the pipe does 93 - 95 % of what it can).
 #include <algorithm>
 #include <type_traits>
 

@@ -7,7 +7,7 @@
 // keep NaN, and a row's largest bits say whether it holds one or an infinity.
 //
 // Bound by memory: every value is read once and written once (norm of 9184 x 4096 fp32 with its delta 74.1 us = 6.6 TB/s, quantisation of
-// 9184 x 4096 fp32 28.3 us = 6.6 TB/s, of 9184 x 14336 bf16 65.7 us = 6.0 TB/s; one row 1.9 - 2.1 us in a graph). A row stays in the
+// 9184 x 4096 fp32 28.3 us = 6.6 TB/s, of 9184 x 14336 bf16 65 - 67 us = 5.9 - 6.1 TB/s; one row 1.8 - 2.1 us in a graph). A row stays in the
 // registers of its threads between the reductions and the rounding. Close behind memory come the instructions, ~ 10 a value: sums,
 // products and maxima take two values at a time, whole numbers come out of the low bits of a sum, 16-bit rows are searched without
 // widening them (bf16, 14336 wide: 87 -> 66 us).
@@ -454,7 +454,7 @@ int launch_rows(RowsParams& p, uint32_t run, const DeviceInfo& dev, cudaStream_t
     const uint32_t vec = aligned ? kWide : 4;
     auto threads = [&](uint32_t chunks) { return ((p.dim + vec * chunks - 1) / (vec * chunks) + 31) / 32 * 32; };
     // Long rows in number: where few blocks of a row's threads fit an SM, the ring keeps the reads going. Quantisation of 9184 x 14336 bf16
-    // 78.7 -> 65.7 us, 5500 x 14336 fp32 87 -> 63, 4000 x 28672 fp16 77 -> 56, the norm of 2000 x 16384 bf16 with an fp32 delta 57 -> 53. Blocks
+    // 78.7 -> 65.7 us, 5500 x 14336 fp32 87 -> 62, 4000 x 28672 fp16 77 -> 56, the norm of 2000 x 16384 bf16 with an fp32 delta 57 -> 53. Blocks
     // of fewer threads do better without (quantisation of 9184 x 8192 bf16 36.6 for 51.3, of 4000 x 11008 25.1 for 30.5, the norm of 4096 x
     // 8192 fp32 67.0 for 79.1, bf16 40.6 for 42.4).
     constexpr uint32_t kRingFrom = !NORM ? 416 : DT == ATTN_DTYPE_F32 ? 544 : 512;
