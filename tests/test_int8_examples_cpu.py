@@ -18,11 +18,13 @@ void example(int8_t* w8, float* w_scale, const void* w_fp16, int8_t* a8, float* 
 
 
 def _examples():
-    """The C++ blocks of the repository's documents that have weights read early."""
+    """The C++ blocks that have weights read early, of the documents that show how the header is used."""
     found = []
     for path in glob.glob(os.path.join(ROOT, "*.md")):
         with open(path) as f:
-            found += [b for b in re.findall(r"```cpp\n(.*?)```", f.read(), re.S) if re.search(r"w_early = 1", b)]
+            text = f.read()
+        if '#include "llm_infer_attn.h"' in text:
+            found += [b for b in re.findall(r"```cpp\n(.*?)```", text, re.S) if "w_early = 1" in b and "attn_gemm_i8(&" in b]
     return found
 
 
